@@ -323,6 +323,69 @@ int pp_masked_gate_bwd(const void* d_out, const void* inter, int dtype, const fl
                        const int32_t* expert_ids, const int32_t* perm, const int32_t* seg, int64_t n_rows,
                        int I, int E, void* d_inter, float* d_gates, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Rotary positions, and a paged cache of keys and values. No counterpart in the
+ * reference's own code (its attention is the model library's); the decoder around the
+ * MoE-MLP needs them to serve several sequences.
+ *
+ * Pair i of a head (of its first rotary_dim channels) turns by position * inv_freq[i]
+ * (float64 on the device, rotary_dim / 2 of them): y1 = mscale (x1 cos - x2 sin),
+ * y2 = mscale (x1 sin + x2 cos); the other channels are copied. layout: the pair is
+ * channels (i, rotary_dim / 2 + i) or (2 i, 2 i + 1). The angle is good to 2^-51 of
+ * itself, whatever the position.
+ * ------------------------------------------------------------------------- */
+#define PP_ROTARY_HALF 0
+#define PP_ROTARY_INTERLEAVED 1
+
+/* x [batch][length][heads][D] (dtype) -> y of the same dtype. x_strides, y_strides: host arrays of
+ * 3, the strides of batch, token and head in elements; channels are contiguous. positions
+ * [batch][length] int32 or int64 (pos64), pos_strides: host array of 2. Any alignment (16-byte
+ * vectors where every head starts on a 16-byte boundary, rotary_dim % 16 == 0 and D % 8 == 0).
+ * inverse: turn by the opposite angles (the transposed map: the gradient of x from that of y).
+ * y may be x itself with the same strides. */
+int pp_rotary(const void* x, int dtype, const int64_t* x_strides, const void* positions, int pos64,
+              const int64_t* pos_strides, int64_t batch, int64_t length, int heads, int D,
+              const double* inv_freq, int rotary_dim, int layout, float mscale, int inverse, void* y,
+              const int64_t* y_strides, void* stream);
+
+/* A ragged batch over a paged cache, as pp_kv_append and pp_paged_attention take it. n_tokens
+ * packed rows; sequence s has the new tokens cu_q[s] .. cu_q[s + 1] (n_seqs + 1 nondecreasing
+ * offsets, the first taken as 0, clamped to n_tokens) and kv_lens[s] tokens in the cache once they
+ * are appended: row i of it is at position kv_lens[s] - (new tokens) + i. Position p of it is at
+ * place p % page_size of page block_table[s][p / page_size] (int32 [n_seqs][max_pages]).
+ * k_pages [num_pages][Hkv][page_size][D], v_pages [num_pages][Hkv][D][page_size], bfloat16.
+ * An entry outside [0, num_pages), a position beyond the table and one below 0 hold no token: they
+ * are not written and not attended. D 64 or 128; page_size a power of two, 16 to 4096; Hq a
+ * multiple of Hkv; max_pages * page_size <= 2^30. All lengths are read on the device, so a
+ * captured call serves lengths that grow.
+ *
+ * pp_kv_append: k and v [n_tokens][Hkv][D] (dtype, strides of token and head in elements; heads on
+ * 16-byte boundaries) into the pages, k turned by its position (inv_freq NULL: as it is;
+ * rotary_dim % 16 == 0), both rounded to bfloat16. q (NULL: none) [n_tokens][Hq][D] of the same
+ * dtype is turned into q_out [n_tokens][Hq][D] bfloat16 (which may be q itself if q is bfloat16 and
+ * contiguous). Rows behind cu_q[n_seqs]: no cache place is written; their q_out is zeroed if
+ * zero_tail, else left as it is. Two tokens of one call must not have the same place. */
+int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                 const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs, const int32_t* cu_q,
+                 const int32_t* kv_lens, const int32_t* block_table, int max_pages, int num_pages,
+                 int page_size, int Hq, int Hkv, int D, const double* inv_freq, int rotary_dim, int layout,
+                 float mscale, void* k_pages, void* v_pages, void* q_out, int zero_tail, void* stream);
+
+/* Attention of the new tokens over the cache that holds them: the token at position p attends the
+ * positions 0 .. p, query head h the key head h / (Hq / Hkv). q [n_tokens][Hq][D] bfloat16 (strides
+ * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous. Scores, softmax and sums in float32. A
+ * row that attends nothing gives zeros; what a masked place holds, NaN and infinities too, does not
+ * reach a row. Rows behind cu_q[n_seqs] are zeroed if zero_tail, else left as they are. workspace:
+ * pp_paged_attention_workspace_bytes of the same sizes (0: none), no initialisation, 16-byte
+ * aligned; calls that may overlap need one each. The same bits on every call. */
+size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq,
+                                          int Hkv, int D);
+int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs,
+                       const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
+                       const void* k_pages, const void* v_pages, int num_pages, int page_size, int Hq, int Hkv,
+                       int D, float scale, void* out_bf16, int zero_tail, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,8 @@ PP_OK = 0
 PP_DTYPE_F32 = 0
 PP_DTYPE_BF16 = 1
 PP_MAX_EXPERTS = 256
+PP_ROTARY_HALF = 0
+PP_ROTARY_INTERLEAVED = 1
 
 _lib = None
 
@@ -73,6 +75,15 @@ SIGNATURES = {
                                    c_void_p]),
     "pp_masked_gate_bwd": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                    c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "pp_rotary": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_int,
+                          c_void_p, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p]),
+    "pp_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p,
+                             c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int,
+                             c_float, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "pp_paged_attention_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "pp_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                   c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p,
+                                   c_size_t, c_void_p]),
 }
 
 

@@ -1,0 +1,708 @@
+// Attention of the new tokens of a ragged batch over a paged cache.
+//
+//   o[i, h] = sum_t p_t v_t,  p = softmax_t(scale q[i, h] . k_t),  t = 0 .. position of token i
+//
+// in one pass over the cache: running maximum m, running sum l and the accumulated o of a row are
+// rescaled by exp(m_old - m_new) when m grows; all three in float32. The query heads of one key head
+// are rows of the same tile (row r of a sequence and key head = token r / group, head r % group of
+// the group), so the cache is read once for the whole group.
+//
+// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a row's scores, maximum, sum
+// and outputs then stay in one column of the MFMA results, i.e. in the lanes l % 16 (or l % 32) = row,
+// and the scores are the second product's right operand without leaving their lane, if the rows of
+// the K operand are taken in an order that gives every lane 8 consecutive tokens. The V pages keep a
+// channel's tokens next to each other ([page][head][channel][token]), so V^T operands are 16-byte
+// loads, like K's.
+//
+// A workgroup takes one tile of rows of one key head over one range of tokens. Where the tiles alone
+// do not fill the GPU, a tile's tokens are cut into ranges ("splits"); the ranges' (m, l, o) go to
+// the workspace and attn_join_kernel combines them in order. The cut depends on the tile's own tokens
+// and on the arguments alone, so a call gives the same bits every time.
+//
+// Masked places: their scores are replaced, not added to, and a step that has any multiplies the
+// finite part of V only; what is not finite in V goes to the rows that attend it by a second product
+// (attn_poison). So stale or foreign data in a page, and a later token's NaN, do not reach a row. A
+// row that attends nothing gives zeros.
+#include <algorithm>
+
+#include "paged.h"
+
+// 16 bytes in registers (a plain vector type: arrays of the struct type were kept in LDS)
+typedef uint32_t a_u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ a_u4 a_mk(uint32_t x, uint32_t y, uint32_t z, uint32_t w) { return a_u4{x, y, z, w}; }
+
+#define ATTN_THREADS 256
+#define ATTN_LOW -3.0e38f  // running maximum before the first score
+
+struct AttnArgs {
+  PagedSeqs seqs;
+  const bf16_t* q;
+  int64_t qs[2];  // strides of token and head, in elements
+  const bf16_t *k, *v;
+  int Hq, Hkv, group;
+  float c;        // scale * log2(e): scores in powers of two
+  bf16_t* out;
+  int zero_tail;
+  int splits, least;  // most ranges of a tile; fewest tokens of a range
+  float *po, *pml;    // workspace: [row][split][D], [row][split][2]
+  int* pns;           // workspace: splits of a row
+  int tiles;          // tiles of rows, of every sequence together
+};
+
+// What a workgroup works on.
+struct AttnTile {
+  int s;         // sequence
+  int c0;        // its first row on the token axis
+  int r0, nr;    // rows of the tile
+  int64_t p0;    // position of the sequence's first new token
+  int nt;        // tokens that the tile's last row attends
+  int lo, hi;    // tokens of this range
+  int ns;        // ranges of the tile (0: nothing is attended)
+};
+
+template <int R>
+__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int split) {
+  AttnTile w;
+  const int g = a.group;
+  auto first = [g](int c, int s) { return (int64_t)c * g / R + s; };
+  w.s = paged_seq_of(a.seqs, t, first);
+  w.c0 = a.seqs.start(w.s);
+  const int len = max(a.seqs.start(w.s + 1) - w.c0, 0);
+  const int64_t r0 = (t - first(w.c0, w.s)) * R;
+  w.nr = r0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)R, (int64_t)len * g - r0));  // < 0: offsets out of order
+  w.r0 = (int)max((int64_t)0, min(r0, (int64_t)len * g));
+  const bool tail = w.s == a.seqs.n_seqs;
+  w.p0 = tail ? -(int64_t)len : (int64_t)a.seqs.kv_lens[w.s] - len;
+  w.nt = (int)max((int64_t)0, min(w.p0 + (w.r0 + max(w.nr, 1) - 1) / g + 1, (int64_t)a.seqs.capacity()));
+  // equal ranges of whole steps, none of them empty
+  const int cut = max(1, min(a.splits, (w.nt + a.least - 1) / a.least));
+  const int per = ((w.nt + cut - 1) / cut + 127) / 128 * 128;
+  w.ns = w.nt > 0 ? (w.nt + per - 1) / per : 0;
+  w.lo = (int)min((int64_t)split * per, (int64_t)w.nt);
+  w.hi = min(w.nt, w.lo + per);
+  return w;
+}
+
+__device__ __forceinline__ int64_t attn_row(const AttnArgs& a, const AttnTile& w, int h, int r) {
+  const int i = (w.r0 + r) / a.group;
+  return (int64_t)(w.c0 + i) * a.Hq + h * a.group + (w.r0 + r - i * a.group);
+}
+
+// Last position that row r attends.
+__device__ __forceinline__ int attn_limit(const AttnArgs& a, const AttnTile& w, int r) {
+  return (int)min(w.p0 + (w.r0 + r) / a.group, (int64_t)a.seqs.capacity() - 1);
+}
+
+// Rows that attend nothing: zeros (rows of no sequence: only if the call owns the output).
+__device__ __forceinline__ void attn_zero(const AttnArgs& a, const AttnTile& w, int h, int D) {
+  const bool tail = w.s == a.seqs.n_seqs;
+  for (int k = threadIdx.x; k < w.nr * (D / 8); k += ATTN_THREADS) {
+    const int r = k / (D / 8), d = 8 * (k - r * (D / 8));
+    const int64_t row = attn_row(a, w, h, r);
+    if (!tail || a.zero_tail) *(a_u4*)(a.out + row * D + d) = a_mk(0, 0, 0, 0);
+    if (a.splits > 1 && d == 0) a.pns[row] = 0;
+  }
+}
+
+// ------------------------------------------------------------------ masked steps
+// Non-finite elements of a V operand (8 tokens of one channel).
+__device__ __forceinline__ bool attn_has_bad(const a_u4 v) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+__device__ __forceinline__ uint32_t attn_clean1(uint32_t x) { return (x & 0x7f80u) == 0x7f80u ? 0u : x; }
+__device__ __forceinline__ a_u4 attn_clean(a_u4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = attn_clean1(v[i] & 0xffffu) | (attn_clean1(v[i] >> 16) << 16);
+  return v;
+}
+// +inf, -inf and NaN as 1, 2^8 and 2^16 (everything else 0): a sum of up to 64 of them tells how many
+// of each there are, exactly, in float32.
+__device__ __forceinline__ uint32_t attn_code1(uint32_t x) {
+  if ((x & 0x7f80u) != 0x7f80u) return 0u;
+  return (x & 0x7fu) ? 0x4780u : (x & 0x8000u) ? 0x4380u : 0x3f80u;
+}
+__device__ __forceinline__ a_u4 attn_code(a_u4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = attn_code1(v[i] & 0xffffu) | (attn_code1(v[i] >> 16) << 16);
+  return v;
+}
+__device__ __forceinline__ float attn_poison(float o, float code) {
+  const uint32_t n = (uint32_t)code;
+  if (n == 0) return o;
+  const bool up = n & 0xffu, down = (n >> 8) & 0xffu;
+  if ((n >> 16) || (up && down)) return __uint_as_float(0x7fc00000u);
+  return o + __uint_as_float(up ? 0x7f800000u : 0xff800000u);
+}
+
+__device__ __forceinline__ uint32_t attn_pk(float a, float b) {
+  return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
+}
+
+__device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// v_mfma_f32_16x16x32_bf16: A lane l holds row l % 16, k = 8 (l / 16) .. + 7; B lane l column l % 16,
+// the same k; D lane l, element i is row 4 (l / 16) + i, column l % 16.
+__device__ __forceinline__ f32x4_t mfma16(const a_u4 a, const a_u4 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------ few rows
+// Up to 16 NB rows of one key head; the cache bounds it. The four waves take alternate steps of 32
+// tokens, each with its own m, l and o, and join them at the end through LDS. K and V operands come
+// straight from memory into registers, the next step's while the present one is computed; the page
+// numbers a step before that.
+// K operand row m of block b (16 tokens) is token 8 (m / 4) + 4 b + m % 4 of the step, which leaves
+// lane group g = lane / 16 with the scores of tokens 8 g .. 8 g + 7: its k of the second product.
+// P enters as a sum of two bf16 values (the rounded one and what is left, 2^-17 of it): the second
+// product costs nothing next to the loads.
+template <int D, int NB>
+struct AttnStep {
+  a_u4 k[2][D / 32], v[D / 16];
+  bool ok;  // the page of the lane's tokens 8 g .. 8 g + 7 is there
+};
+
+template <int D, int NB>
+__global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel(AttnArgs a) {
+  constexpr int R = 16 * NB, KS = D / 32, MB = D / 16, OS = D + 4;
+  __shared__ float o_s[4][R][OS];
+  __shared__ float ml_s[4][R][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x % a.splits;
+  const int item = blockIdx.x / a.splits, h = item % a.Hkv;
+  const AttnTile w = attn_tile<R>(a, item / a.Hkv, split);
+  if (w.nr <= 0) return;
+  if (w.ns == 0) {
+    if (split == 0) attn_zero(a, w, h, D);
+    return;
+  }
+  if (split >= w.ns) return;
+
+  a_u4 qf[NB][KS];
+  int limit[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int r = 16 * n + col;
+    const bool in = r < w.nr;
+    limit[n] = in ? attn_limit(a, w, r) : a.seqs.capacity();
+    const int i = (w.r0 + r) / a.group;
+    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[n][s] = in ? *(const a_u4*)(src + 32 * s + 8 * g) : a_mk(0, 0, 0, 0);
+  }
+  const int low = attn_limit(a, w, 0);  // every row attends the tokens up to here
+
+  f32x4_t o[NB][MB];
+  float m[NB], l[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    m[n] = ATTN_LOW, l[n] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < MB; ++b) o[n][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const int ps = 1 << a.seqs.lp;
+  const int gk = 8 * (col >> 2), gv = 8 * g;  // the lane's tokens of K and of V, within a step
+  int pk = -1, pv = -1;                       // their pages
+  auto pages = [&](int t) {
+    pk = t + gk < w.hi ? a.seqs.page(w.s, (t + gk) >> a.seqs.lp) : -1;
+    pv = t + gv < w.hi ? a.seqs.page(w.s, (t + gv) >> a.seqs.lp) : -1;
+  };
+  auto load = [&](AttnStep<D, NB>& x, int t) {  // places without a page read page 0, and are masked
+    x.ok = pv >= 0;
+    const bf16_t* kp = a.k + ((((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((t + gk) & (ps - 1)) + (col & 3)) * D + 8 * g;
+    const bf16_t* vp = a.v + ((((int64_t)max(pv, 0) * a.Hkv + h) * D + col) << a.seqs.lp) + ((t + gv) & (ps - 1));
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) x.k[b][s] = *(const a_u4*)(kp + 4 * b * D + 32 * s);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) x.v[b] = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+  };
+  auto compute = [&](AttnStep<D, NB>& x, int t) {
+    // whether a place of the step is masked for any row (wave-uniform)
+    const bool part = t + 31 > low || t + 32 > w.hi || __ballot(!x.ok) != 0;
+    bool bad = false;
+    if (part) {
+#pragma unroll
+      for (int b = 0; b < MB; ++b) bad |= attn_has_bad(x.v[b]);
+      bad = __ballot(bad) != 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      f32x4_t s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        s[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < KS; ++q) s[b] = mfma16(x.k[b][q], qf[n][q], s[b]);
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * a.c;
+      uint32_t seen = 0xffu;
+      if (part) {
+        seen = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = x.ok && t + gv + j <= limit[n] && t + gv + j < w.hi;
+          seen |= in ? 1u << j : 0u;
+          p[j] = in ? p[j] : -__builtin_inff();
+        }
+      }
+      float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+      top = fmaxf(top, pl_xor16f(top, lane));
+      top = fmaxf(top, pl_xor32f(top, lane));
+      const float mn = fmaxf(m[n], top), shrink = attn_exp2(m[n] - mn);
+      m[n] = mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = attn_exp2(p[j] - mn);
+        sum += p[j];
+      }
+      l[n] = __fmaf_rn(l[n], shrink, sum);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        hi[j] = attn_pk(p[2 * j], p[2 * j + 1]);
+        lo[j] = attn_pk(p[2 * j] - __uint_as_float(hi[j] << 16), p[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
+      }
+      const a_u4 ph = a_mk(hi[0], hi[1], hi[2], hi[3]), pl = a_mk(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        o[n][b] *= shrink;
+        const a_u4 v = bad ? attn_clean(x.v[b]) : x.v[b];
+        o[n][b] = mfma16(v, ph, o[n][b]);
+        o[n][b] = mfma16(v, pl, o[n][b]);
+      }
+      if (bad) {
+        uint32_t one[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          one[j] = ((seen >> (2 * j)) & 1 ? 0x3f80u : 0u) | ((seen >> (2 * j + 1)) & 1 ? 0x3f800000u : 0u);
+        const a_u4 on = a_mk(one[0], one[1], one[2], one[3]);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          const f32x4_t code = mfma16(attn_code(x.v[b]), on, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][b][i] = attn_poison(o[n][b][i], code[i]);
+        }
+      }
+    }
+  };
+
+  int t = w.lo + 32 * wave;
+  if (t < w.hi) {
+    AttnStep<D, NB> x, y;
+    pages(t);
+    load(x, t);
+    pages(t + 128);
+    while (true) {
+      const bool more = t + 128 < w.hi;
+      if (more) {
+        load(y, t + 128);
+        pages(t + 256);
+      }
+      compute(x, t);
+      if (!more) break;
+      t += 128;
+      const bool again = t + 128 < w.hi;
+      if (again) {
+        load(x, t + 128);
+        pages(t + 256);
+      }
+      compute(y, t);
+      if (!again) break;
+      t += 128;
+    }
+  }
+
+  // the four waves' rows joined
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    float sum = l[n];
+    sum += pl_xor16f(sum, lane);
+    sum += pl_xor32f(sum, lane);
+    const int r = 16 * n + col;
+    if (g == 0) ml_s[wave][r][0] = m[n], ml_s[wave][r][1] = sum;
+#pragma unroll
+    for (int b = 0; b < MB; ++b) *(f32x4_t*)&o_s[wave][r][16 * b + 4 * g] = o[n][b];
+  }
+  __syncthreads();
+  for (int k = tid; k < w.nr * (D / 8); k += ATTN_THREADS) {
+    const int r = k / (D / 8), d = 8 * (k - r * (D / 8));
+    float mm = ml_s[0][r][0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) mm = fmaxf(mm, ml_s[i][r][0]);
+    float sum = 0.0f, acc[8] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = attn_exp2(ml_s[i][r][0] - mm);
+      sum = __fmaf_rn(ml_s[i][r][1], f, sum);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = __fmaf_rn(o_s[i][r][d + j], f, acc[j]);
+    }
+    const int64_t row = attn_row(a, w, h, r);
+    if (w.ns == 1) {
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+      *(a_u4*)(a.out + row * D + d) = a_mk(attn_pk(acc[0] * inv, acc[1] * inv), attn_pk(acc[2] * inv, acc[3] * inv),
+                                                  attn_pk(acc[4] * inv, acc[5] * inv), attn_pk(acc[6] * inv, acc[7] * inv));
+    } else {
+      float* to = a.po + (row * a.splits + split) * D + d;
+      *(float4*)to = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *(float4*)(to + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (d == 0) *(float2*)(a.pml + (row * a.splits + split) * 2) = make_float2(mm, sum);
+    }
+    if (a.splits > 1 && split == 0 && d == 0) a.pns[row] = w.ns;
+  }
+}
+
+// ------------------------------------------------------------------ many rows
+// 128 rows of one key head, 32 to each of four waves; the matrix cores bound it. Steps of 64 tokens:
+// K [64][D] and V^T [D][64] go through registers into one of two LDS buffers, the next step's while
+// the present one is computed (one barrier a step). Row m of the K tile is the token whose number
+// within its 16 has bits 2 and 3 of m swapped, which leaves lane half e = lane / 32 with the scores of
+// tokens 16 b + 8 e .. + 7: its k of the second product. 16-byte chunk c of LDS row m sits at place
+// c ^ (m % 8) of its 128 bytes, so that 8 lanes on consecutive rows touch 8 different bank groups.
+#define ATTN_ROWS 128
+#define ATTN_KT 64
+
+template <int D>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) {
+  constexpr int KC = D / 8, NK = ATTN_KT * KC / ATTN_THREADS, NV = D * (ATTN_KT / 8) / ATTN_THREADS, MB = D / 32;
+  __shared__ a_u4 k_s[2][ATTN_KT * KC];
+  __shared__ a_u4 v_s[2][D * (ATTN_KT / 8)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, e = lane >> 5;
+  // workgroup b runs on XCD b % 8; an XCD's workgroups take consecutive items, so that the tiles of
+  // one key head share that XCD's L2
+  const int per = gridDim.x >> 3;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  // items are (head, tile, split); the last tiles, which attend most, come first
+  const int split = id % a.splits;
+  const int item = id / a.splits, h = item / a.tiles;
+  if (h >= a.Hkv) return;
+  const AttnTile w = attn_tile<ATTN_ROWS>(a, a.tiles - 1 - item % a.tiles, split);
+  if (w.nr <= 0) return;
+  if (w.ns == 0) {
+    if (split == 0) attn_zero(a, w, h, D);
+    return;
+  }
+  if (split >= w.ns) return;
+
+  const int r = 32 * wave + col;
+  const bool in = r < w.nr, busy = 32 * wave < w.nr;
+  const int limit = in ? attn_limit(a, w, r) : 0x7fffffff;
+  // tokens that every row of the wave attends, and that any does
+  const int low = busy ? attn_limit(a, w, 32 * wave) : 0, top = busy ? attn_limit(a, w, min(32 * wave + 31, w.nr - 1)) : -1;
+  a_u4 qf[D / 16];
+  {
+    const int i = (w.r0 + r) / a.group;
+    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1] + 8 * e;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = in ? *(const a_u4*)(src + 16 * s) : a_mk(0, 0, 0, 0);
+  }
+  f32x16_t o[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) o[b][q] = 0.0f;
+  float m = ATTN_LOW, l = 0.0f;
+
+  const int ps = 1 << a.seqs.lp;
+  const int krow = tid / KC, kc = tid % KC, vrow = tid / 8, vc = tid % 8;
+  const int ktok = (krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1);  // of its 16
+  int pg[4];  // pages of the next step's four groups of 16 tokens, -1: none
+  auto pages = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pg[j] = t + 16 * j < w.hi ? a.seqs.page(w.s, (t + 16 * j) >> a.seqs.lp) : -1;
+  };
+  a_u4 kst[NK], vst[NV];
+  int have = 0, next_have = 0;  // groups whose page is there
+  auto load = [&](int t) {  // places without a page read page 0, and are masked
+    next_have = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next_have |= pg[j] >= 0 ? 1 << j : 0;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int b16 = (i * (ATTN_THREADS / KC) + krow) >> 4;
+      const int p = KC == 16 ? pg[i & 3] : (b16 & 1) ? pg[(2 * i + 1) & 3] : pg[(2 * i) & 3];
+      kst[i] = *(const a_u4*)(a.k + ((((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((t + 16 * b16) & (ps - 1)) + ktok) * D + 8 * kc);
+    }
+    const int pv = (vc & 4) ? ((vc & 2) ? pg[3] : pg[2]) : ((vc & 2) ? pg[1] : pg[0]);
+    const bf16_t* vp = a.v + ((((int64_t)max(pv, 0) * a.Hkv + h) * D + vrow) << a.seqs.lp) + ((t + 8 * vc) & (ps - 1));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) vst[i] = *(const a_u4*)(vp + ((int64_t)(32 * i) << a.seqs.lp));
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int row = i * (ATTN_THREADS / KC) + krow;
+      k_s[buf][row * KC + (kc ^ (row & 7))] = kst[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v_s[buf][(32 * i + vrow) * 8 + (vc ^ (vrow & 7))] = vst[i];
+  };
+
+  int t = w.lo, buf = 0;
+  pages(t);
+  load(t);
+  pages(t + ATTN_KT);
+  put(0);
+  have = next_have;
+  __syncthreads();
+  while (true) {
+    const bool more = t + ATTN_KT < w.hi;
+    if (more) {
+      load(t + ATTN_KT);
+      pages(t + 2 * ATTN_KT);
+    }
+    if (t <= top) {
+      f32x16_t s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) s[b][q] = 0.0f;
+#pragma unroll
+      for (int q = 0; q < D / 16; ++q)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          s[b] = mfma32a(k_s[buf][(32 * b + col) * KC + ((2 * q + e) ^ (col & 7))], qf[q], s[b]);
+      const bool part = t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != 15;
+      uint32_t seen = ~0u;
+      float mx = ATTN_LOW;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) s[b][q] *= a.c;
+      if (part) {
+        seen = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const int g16 = 2 * b + (q >> 3), tok = t + 16 * g16 + 8 * e + (q & 7);
+            const bool on = tok <= limit && tok < w.hi && ((have >> g16) & 1);
+            seen |= on ? 1u << (16 * b + q) : 0u;
+            s[b][q] = on ? s[b][q] : -__builtin_inff();
+          }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) mx = fmaxf(mx, s[b][q]);
+      mx = fmaxf(mx, pl_xor32f(mx, lane));
+      const float mn = fmaxf(m, mx);
+      if (__ballot(mn != m)) {  // some row's maximum grew (or is NaN)
+        const float shrink = attn_exp2(m - mn);
+        l *= shrink;
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) o[b][q] *= shrink;
+        m = mn;
+      }
+      a_u4 pf[4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t p2[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = attn_exp2(s[kk >> 1][8 * (kk & 1) + 2 * j] - mn), y = attn_exp2(s[kk >> 1][8 * (kk & 1) + 2 * j + 1] - mn);
+          l += x + y;
+          p2[j] = attn_pk(x, y);
+        }
+        pf[kk] = a_mk(p2[0], p2[1], p2[2], p2[3]);
+      }
+      const a_u4* const vb = v_s[buf];
+      bool bad = false;
+      if (part) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int b = 0; b < MB; ++b) bad |= attn_has_bad(vb[(32 * b + col) * 8 + ((2 * kk + e) ^ (col & 7))]);
+        bad = __ballot(bad) != 0;
+      }
+      if (!bad) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int b = 0; b < MB; ++b) o[b] = mfma32a(vb[(32 * b + col) * 8 + ((2 * kk + e) ^ (col & 7))], pf[kk], o[b]);
+      } else {
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          f32x16_t code;
+#pragma unroll
+          for (int q = 0; q < 16; ++q) code[q] = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const a_u4 v = vb[(32 * b + col) * 8 + ((2 * kk + e) ^ (col & 7))];
+            uint32_t one[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              one[j] = ((seen >> (8 * kk + 2 * j)) & 1 ? 0x3f80u : 0u) | ((seen >> (8 * kk + 2 * j + 1)) & 1 ? 0x3f800000u : 0u);
+            o[b] = mfma32a(attn_clean(v), pf[kk], o[b]);
+            code = mfma32a(attn_code(v), a_mk(one[0], one[1], one[2], one[3]), code);
+          }
+#pragma unroll
+          for (int q = 0; q < 16; ++q) o[b][q] = attn_poison(o[b][q], code[q]);
+        }
+      }
+    }
+    if (!more) break;
+    put(buf ^ 1);
+    have = next_have;
+    __syncthreads();
+    buf ^= 1;
+    t += ATTN_KT;
+  }
+
+  l += pl_xor32f(l, lane);
+  if (!in) return;
+  const int64_t row = attn_row(a, w, h, r);
+  if (w.ns == 1) {
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    bf16_t* to = a.out + row * D + 4 * e;
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(uint2*)(to + 32 * b + 8 * q) = make_uint2(attn_pk(o[b][4 * q] * inv, o[b][4 * q + 1] * inv),
+                                                    attn_pk(o[b][4 * q + 2] * inv, o[b][4 * q + 3] * inv));
+  } else {
+    float* to = a.po + (row * a.splits + split) * D + 4 * e;
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(float4*)(to + 32 * b + 8 * q) = make_float4(o[b][4 * q], o[b][4 * q + 1], o[b][4 * q + 2], o[b][4 * q + 3]);
+    if (e == 0) *(float2*)(a.pml + (row * a.splits + split) * 2) = make_float2(m, l);
+  }
+  if (a.splits > 1 && split == 0 && e == 0) a.pns[row] = w.ns;
+}
+
+// ------------------------------------------------------------------ join
+// One workgroup per row (token and query head): lane i of a wave holds the weight of range i, the
+// waves take alternate ranges and are added in wave order.
+#define ATTN_MAX_SPLITS 64
+
+template <int D>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(AttnArgs a) {
+  constexpr int W = D / 64;
+  __shared__ float acc_s[4][D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const int ns = min(a.pns[row], a.splits);
+  if (ns <= 1) return;  // written already
+  float m = ATTN_LOW, l = 0.0f;
+  if (lane < ns) {
+    const float2 ml = *(const float2*)(a.pml + (row * a.splits + lane) * 2);
+    m = ml.x, l = ml.y;
+  }
+  const float top = wave_max(m);  // every lane takes part
+  const float f = lane < ns ? attn_exp2(m - top) : 0.0f;
+  const float sum = wave_sum(f * l);
+  float acc[W] = {};
+  const float* from = a.po + row * a.splits * D + lane * W;
+#pragma unroll 2
+  for (int i = wave; i < ns; i += 4) {
+    const float x = __shfl(f, i, PP_WAVE);
+#pragma unroll
+    for (int j = 0; j < W; ++j) acc[j] = __fmaf_rn(from[(int64_t)i * D + j], x, acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < W; ++j) acc_s[wave][lane * W + j] = acc[j];
+  __syncthreads();
+  const int d = 2 * threadIdx.x;
+  if (d >= D) return;
+  float x = acc_s[0][d], y = acc_s[0][d + 1];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) x += acc_s[i][d], y += acc_s[i][d + 1];
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  *(uint32_t*)(a.out + row * D + d) = attn_pk(x * inv, y * inv);
+}
+
+// ------------------------------------------------------------------ host
+struct AttnPlan {
+  int rows;    // per tile: 16, 32 or ATTN_ROWS
+  int splits, least;
+  int64_t tiles;
+};
+
+static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv) {
+  AttnPlan p;
+  const int64_t group = Hq / Hkv, rows = n_tokens * group, each = rows / std::max(n_seqs, 1);
+  p.rows = each <= 16 ? 16 : each <= 32 ? 32 : ATTN_ROWS;
+  p.tiles = rows / p.rows + n_seqs + 1;
+  p.least = p.rows == ATTN_ROWS ? 512 : 128;
+  const int64_t slots = 2 * pp_device_cus(), capacity = (int64_t)max_pages * page_size;
+  const int64_t items = std::max<int64_t>(1, (rows / p.rows + n_seqs) * Hkv);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ATTN_MAX_SPLITS, (2 * slots + items - 1) / items,
+                                                          (capacity + p.least - 1) / p.least}));
+  return p;
+}
+
+static size_t attn_ws_bytes(const AttnPlan& p, int64_t rows, int D) {
+  if (p.splits == 1) return 0;
+  return (size_t)rows * p.splits * (D + 2) * 4 + (size_t)rows * 4;
+}
+
+extern "C" size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size,
+                                                     int Hq, int Hkv, int D) {
+  if (n_tokens <= 0 || n_seqs < 0 || max_pages < 1 || page_size < 1 || Hkv < 1 || Hq < Hkv || D < 1) return 0;
+  return attn_ws_bytes(attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv), n_tokens * Hq, D);
+}
+
+extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs,
+                                  const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                                  int max_pages, const void* k_pages, const void* v_pages, int num_pages,
+                                  int page_size, int Hq, int Hkv, int D, float scale, void* out_bf16, int zero_tail,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* const what = "pp_paged_attention";
+  int rc = pp_paged_check(what, n_tokens, n_seqs, cu_q, kv_lens, block_table, max_pages, k_pages, v_pages, num_pages,
+                          page_size, Hq, Hkv, D);
+  if (rc) return rc;
+  PP_REQUIRE(Hq >= 1, PP_ERR_INVALID, "%s: no query heads", what);
+  if (n_tokens == 0) return PP_OK;
+  PP_REQUIRE(q && q_strides && out_bf16, PP_ERR_INVALID, "%s: null pointer", what);
+  PP_REQUIRE((((uintptr_t)q | (uintptr_t)out_bf16) & 15) == 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0,
+             PP_ERR_INVALID, "%s: every head of q and out must start on a 16-byte boundary", what);
+  const AttnPlan p = attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv);
+  const size_t need = attn_ws_bytes(p, n_tokens * Hq, D);
+  PP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PP_ERR_INVALID,
+             "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes, need);
+  AttnArgs a;
+  a.seqs = {cu_q, kv_lens, block_table, (int)n_tokens, n_seqs, max_pages, num_pages, paged_log2(page_size)};
+  a.q = (const bf16_t*)q, a.qs[0] = q_strides[0], a.qs[1] = q_strides[1];
+  a.k = (const bf16_t*)k_pages, a.v = (const bf16_t*)v_pages;
+  a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv;
+  a.c = scale * 1.4426950408889634f;
+  a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
+  a.splits = p.splits, a.least = p.least, a.tiles = (int)p.tiles;
+  a.po = (float*)workspace;
+  a.pml = a.po + n_tokens * Hq * p.splits * D;
+  a.pns = (int*)(a.pml + n_tokens * Hq * p.splits * 2);
+  const int64_t items = p.tiles * Hkv * p.splits;
+  PP_REQUIRE(items <= 0x7ffffff0, PP_ERR_UNSUPPORTED, "%s: too many sequences and heads", what);
+  hipStream_t st = (hipStream_t)stream;
+  const unsigned n = (unsigned)items, n8 = (n + 7) & ~7u;
+#define ATTN(D_)                                                                          \
+  do {                                                                                    \
+    if (p.rows == 16) attn_few_kernel<D_, 1><<<n, ATTN_THREADS, 0, st>>>(a);              \
+    else if (p.rows == 32) attn_few_kernel<D_, 2><<<n, ATTN_THREADS, 0, st>>>(a);         \
+    else attn_many_kernel<D_><<<n8, ATTN_THREADS, 0, st>>>(a);                            \
+    if (p.splits > 1)                                                                     \
+      attn_join_kernel<D_><<<(unsigned)(n_tokens * Hq), ATTN_THREADS, 0, st>>>(a);        \
+  } while (0)
+  if (D == 64) ATTN(64);
+  else ATTN(128);
+#undef ATTN
+  return pp_check_launch(what);
+}

@@ -1,0 +1,62 @@
+// What the paged-cache kernels share: the description of a ragged batch and its cache.
+//
+// n_seqs sequences; the rows cu_q[s] .. cu_q[s + 1] of the packed token axis are the new tokens of
+// sequence s, and kv_lens[s] tokens are in the cache once they are appended, so row i of the
+// sequence sits at position kv_lens[s] - (its new tokens) + i. Position p is in page
+// block_table[s][p / page_size], place p % page_size. An entry outside [0, num_pages) and a
+// position beyond the table (or below zero) hold no token: nothing is written there, nothing is
+// attended there. Rows behind cu_q[n_seqs] belong to no sequence; the kernels treat them as
+// sequence number n_seqs, of length 0.
+#pragma once
+#include "pp_common.h"
+
+struct PagedSeqs {
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  const int32_t* table;
+  int n_rows, n_seqs;
+  int max_pages, num_pages;
+  int lp;  // log2 of the page size
+  __device__ int start(int s) const {  // first row of sequence s, whatever the caller's array holds
+    if (s <= 0) return 0;
+    if (s > n_seqs) return n_rows;
+    return min(max(cu_q[s], 0), n_rows);
+  }
+  // page of table entry e of sequence s, -1 for none
+  __device__ int page(int s, int64_t e) const {
+    if (e < 0 || e >= max_pages) return -1;
+    const int id = table[(int64_t)s * max_pages + e];
+    return (unsigned)id < (unsigned)num_pages ? id : -1;
+  }
+  // positions that the table has room for
+  __device__ int capacity() const { return max_pages << lp; }  // at most 2^30 (checked by the host)
+};
+
+// The sequence that work item t belongs to, where sequence s has the items first(start(s), s)
+// and on: the last s with first(start(s), s) <= t. `first` grows with s, by at least the items that
+// the sequence has, so the item space needs no prefix sum. One load per 64 sequences; every wave
+// finds it for itself. A result in [0, n_seqs], also for offsets out of order.
+template <typename F>
+__device__ __forceinline__ int paged_seq_of(const PagedSeqs& q, int64_t t, F first) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int s0 = 0; s0 <= q.n_seqs; s0 += 64) {
+    const int s = s0 + lane;
+    const bool in = s <= q.n_seqs && first(q.start(s), s) <= t;
+    const uint64_t b = __ballot(in);
+    n += __popcll(b);
+    if (b != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(max(n - 1, 0));
+}
+
+static inline int paged_log2(int v) {
+  for (int b = 0; b < 31; ++b)
+    if ((1 << b) == v) return b;
+  return -1;
+}
+
+// Checks of the arguments that the append and the attention have in common.
+int pp_paged_check(const char* what, int64_t n_tokens, int n_seqs, const void* cu_q, const void* kv_lens,
+                   const void* block_table, int max_pages, const void* k_pages, const void* v_pages, int num_pages,
+                   int page_size, int Hq, int Hkv, int D);

@@ -19,6 +19,9 @@
 //   moe_prefill(_into)    TauSparseMoE.forward_prefill (:532-604)
 //   masked_gate(_bwd)     MoELayer.forward's expert gating and its backward
 //                         (src/MoEBlock_origin.py:205-212)
+//   rotary, kv_append(_q), paged_attention(_into)
+//                         no counterpart in the reference's own code: the attention side of a
+//                         decoder that serves several sequences
 #include <ATen/ATen.h>
 #include <algorithm>
 #include <c10/core/DeviceGuard.h>
@@ -461,6 +464,195 @@ std::tuple<Tensor, Tensor> masked_gate_bwd_meta(const Tensor&, const Tensor& int
   return {need_d_inter ? at::empty_like(inter) : at::empty({0}, inter.options()), at::empty_like(gates)};
 }
 
+// ------------------------------------------------------------------ rotary positions
+int rotary_layout(c10::string_view layout, const char* name) {
+  if (layout == "half") return PP_ROTARY_HALF;
+  TORCH_CHECK(layout == "interleaved", "prunepath.", name, ": layout must be 'half' or 'interleaved'");
+  return PP_ROTARY_INTERLEAVED;
+}
+
+void same_device(const char* name, const Tensor& ref, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) {
+    TORCH_CHECK(t->is_cuda(), "prunepath.", name, ": tensors must be on the GPU (got ", t->device(),
+                "); there is no CPU implementation");
+    TORCH_CHECK(t->device() == ref.device(), "prunepath.", name, ": tensors on different devices (", ref.device(), ", ",
+                t->device(), ")");
+  }
+}
+
+// x [..., heads, D] with positions [...] as (batch, length): the leading axes merged where their
+// strides allow it, at most two left.
+Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                  double mscale, bool inverse) {
+  const int lay = rotary_layout(layout, "rotary");
+  TORCH_CHECK(x.dim() == 3 || x.dim() == 4, "prunepath.rotary: x must be [N, heads, D] or [B, L, heads, D]");
+  TORCH_CHECK(positions.dim() == x.dim() - 2 && positions.sizes() == x.sizes().slice(0, x.dim() - 2),
+              "prunepath.rotary: positions must have x's leading shape");
+  TORCH_CHECK(positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt,
+              "prunepath.rotary: positions must be int32 or int64");
+  TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && inv_freq.is_contiguous(),
+              "prunepath.rotary: inv_freq must be contiguous float64 [rotary_dim / 2]");
+  same_device("rotary", x, {&x, &positions, &inv_freq});
+  const c10::DeviceGuard g(x.device());
+  const Tensor in = x.size(-1) > 1 && x.stride(-1) != 1 ? x.contiguous() : x;
+  Tensor out = at::empty_like(in);
+  if (out.size(-1) > 1 && out.stride(-1) != 1) out = at::empty(in.sizes(), in.options());
+  const int64_t d = in.dim();
+  const bool four = d == 4;
+  const int64_t xs[3] = {four ? in.stride(0) : 0, in.stride(d - 3), in.stride(d - 2)};
+  const int64_t ys[3] = {four ? out.stride(0) : 0, out.stride(d - 3), out.stride(d - 2)};
+  const int64_t ps[2] = {four ? positions.stride(0) : 0, positions.stride(d - 3)};
+  check_rc(pp_rotary(in.data_ptr(), x_code(in, "rotary"), xs, positions.data_ptr(),
+                     positions.scalar_type() == at::kLong, ps, four ? in.size(0) : 1, in.size(d - 3),
+                     (int)in.size(d - 2), (int)in.size(d - 1), inv_freq.data_ptr<double>(), (int)(2 * inv_freq.numel()),
+                     lay, (float)mscale, inverse, out.data_ptr(), ys, stream_of(in)),
+           "rotary");
+  return out;
+}
+
+Tensor rotary_meta(const Tensor& x, const Tensor&, const Tensor&, c10::string_view, double, bool) {
+  return at::empty_like(x);
+}
+
+// ------------------------------------------------------------------ paged cache
+struct Paged {
+  int64_t n, seqs, Hq, Hkv, D, pages, max_pages, page;
+};
+
+Paged paged_check(const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                  const Tensor& kv_lens, const Tensor& cu_q, int64_t n, int64_t Hq, int64_t D) {
+  TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
+                  v_pages.scalar_type() == at::kBFloat16,
+              "prunepath.", name, ": k_pages [pages, kv_heads, page, D] and v_pages [pages, kv_heads, D, page] bfloat16 required");
+  Paged p;
+  p.n = n, p.Hq = Hq, p.D = D;
+  p.pages = k_pages.size(0), p.Hkv = k_pages.size(1), p.page = k_pages.size(2);
+  TORCH_CHECK(k_pages.size(3) == D && v_pages.size(0) == p.pages && v_pages.size(1) == p.Hkv && v_pages.size(2) == D &&
+                  v_pages.size(3) == p.page,
+              "prunepath.", name, ": shapes of k_pages ", k_pages.sizes(), ", v_pages ", v_pages.sizes(),
+              " and head size ", D, " disagree");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && kv_lens.dim() == 1 &&
+                  kv_lens.scalar_type() == at::kInt && cu_q.dim() == 1 && cu_q.scalar_type() == at::kInt,
+              "prunepath.", name, ": block_table [seqs, max_pages], kv_lens [seqs] and cu_q [seqs + 1] must be int32");
+  p.seqs = kv_lens.size(0), p.max_pages = block_table.size(1);
+  TORCH_CHECK(block_table.size(0) == p.seqs && cu_q.size(0) == p.seqs + 1, "prunepath.", name, ": block_table ",
+              block_table.sizes(), ", kv_lens ", kv_lens.sizes(), " and cu_q ", cu_q.sizes(), " disagree");
+  TORCH_CHECK(p.pages <= 0x7fffffff && p.max_pages <= 0x7fffffff && p.page <= 0x7fffffff && p.Hkv <= 0x7fffffff &&
+                  p.seqs <= 0x7fffffff && Hq <= 0x7fffffff,
+              "prunepath.", name, ": a size beyond 2^31");
+  return p;
+}
+
+void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bool zero_tail, const Tensor& k,
+                    const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                    const Tensor& kv_lens, const Tensor& cu_q, const optional<Tensor>& inv_freq,
+                    c10::string_view layout, double mscale) {
+  const char* const name = "kv_append";
+  const int lay = rotary_layout(layout, name);
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
+              "prunepath.kv_append: k and v must be [N, kv_heads, D] of one dtype");
+  const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, k.size(0), q ? q->size(1) : 0, k.size(2));
+  TORCH_CHECK(k.size(1) == p.Hkv, "prunepath.kv_append: ", k.size(1), " heads for a cache of ", p.Hkv);
+  TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, "prunepath.kv_append: channels must be contiguous");
+  need_gpu(name, k, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, inv_freq ? &*inv_freq : nullptr});
+  same_device(name, k, {&k, &v});
+  if (inv_freq)
+    TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
+                "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
+  int64_t qs[2] = {0, 0};
+  if (q) {
+    TORCH_CHECK(q->dim() == 3 && q->size(0) == p.n && q->size(2) == p.D && q->scalar_type() == k.scalar_type() &&
+                    q->stride(2) == 1,
+                "prunepath.kv_append: q must be [N, heads, D] of k's dtype, channels contiguous");
+    TORCH_CHECK(q_out->scalar_type() == at::kBFloat16 && q_out->sizes() == q->sizes() && q_out->is_contiguous(),
+                "prunepath.kv_append: q_out must be contiguous bfloat16 of q's shape");
+    same_device(name, k, {&*q, &*q_out});
+    qs[0] = q->stride(0), qs[1] = q->stride(1);
+  }
+  const c10::DeviceGuard g(k.device());
+  const int64_t ks[2] = {k.stride(0), k.stride(1)}, vs[2] = {v.stride(0), v.stride(1)};
+  check_rc(pp_kv_append(q ? q->data_ptr() : nullptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, x_code(k, name), p.n,
+                        (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
+                        block_table.data_ptr<int32_t>(), (int)p.max_pages, (int)p.pages, (int)p.page, (int)p.Hq,
+                        (int)p.Hkv, (int)p.D, (const double*)ptr(inv_freq), inv_freq ? (int)(2 * inv_freq->numel()) : 0,
+                        lay, (float)mscale, k_pages.data_ptr(), v_pages.data_ptr(), q ? q_out->data_ptr() : nullptr,
+                        zero_tail, stream_of(k)),
+           name);
+}
+
+void kv_append_gpu(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                   const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                   const optional<Tensor>& inv_freq, c10::string_view layout, double mscale) {
+  kv_append_into(c10::nullopt, c10::nullopt, false, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq,
+                 layout, mscale);
+}
+
+Tensor kv_append_q_gpu(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                       const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                       const optional<Tensor>& inv_freq, c10::string_view layout, double mscale) {
+  Tensor out = at::empty(q.sizes(), q.options().dtype(at::kBFloat16));
+  kv_append_into(q, out, true, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale);
+  return out;
+}
+
+void kv_append_q_into_gpu(const Tensor& q, const Tensor& q_out, const Tensor& k, const Tensor& v, const Tensor& k_pages,
+                          const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                          const optional<Tensor>& inv_freq, c10::string_view layout, double mscale) {
+  kv_append_into(q, q_out, false, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale);
+}
+
+void kv_append_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                    const Tensor&, const optional<Tensor>&, c10::string_view, double) {}
+Tensor kv_append_q_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                        const Tensor&, const Tensor&, const optional<Tensor>&, c10::string_view, double) {
+  return at::empty_symint(q.sym_sizes(), q.options().dtype(at::kBFloat16));
+}
+void kv_append_q_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                           const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, c10::string_view,
+                           double) {}
+
+void attention_into(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                    const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out, bool zero_tail) {
+  const char* const name = "paged_attention";
+  TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.stride(2) == 1,
+              "prunepath.paged_attention: q must be bfloat16 [N, heads, D], channels contiguous");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.is_contiguous(),
+              "prunepath.paged_attention: out must be contiguous bfloat16 of q's shape");
+  const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, q.size(0), q.size(1), q.size(2));
+  need_gpu(name, q, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &out});
+  same_device(name, q, {&q});
+  const c10::DeviceGuard g(q.device());
+  const size_t need = pp_paged_attention_workspace_bytes(p.n, (int)p.seqs, (int)p.max_pages, (int)p.page, (int)p.Hq,
+                                                         (int)p.Hkv, (int)p.D);
+  Tensor ws;
+  if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+  const int64_t qs[2] = {q.stride(0), q.stride(1)};
+  check_rc(pp_paged_attention(q.data_ptr(), qs, p.n, (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
+                              block_table.data_ptr<int32_t>(), (int)p.max_pages, k_pages.data_ptr(), v_pages.data_ptr(),
+                              (int)p.pages, (int)p.page, (int)p.Hq, (int)p.Hkv, (int)p.D, (float)scale, out.data_ptr(),
+                              zero_tail, need ? ws.data_ptr() : nullptr, need, stream_of(q)),
+           name);
+}
+
+void paged_attention_into_gpu(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                              const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out) {
+  attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale, out, false);
+}
+
+Tensor paged_attention_gpu(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                           const Tensor& kv_lens, const Tensor& cu_q, double scale) {
+  Tensor out = at::empty(q.sizes(), q.options());
+  attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale, out, true);
+  return out;
+}
+
+Tensor paged_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                            double) {
+  return at::empty_symint(q.sym_sizes(), q.options());
+}
+void paged_attention_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                               double, const Tensor&) {}
+
 void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
   TORCH_CHECK(false, op.schema().name(), ": tensors must be on the GPU (got cpu); there is no CPU implementation");
 }
@@ -492,6 +684,19 @@ TORCH_LIBRARY(prunepath, m) {
   m.def("masked_gate(Tensor inter, Tensor gates, Tensor expert_ids, Tensor perm, Tensor seg) -> Tensor");
   m.def("masked_gate_bwd(Tensor d_out, Tensor inter, Tensor gates, Tensor expert_ids, Tensor perm, Tensor seg, "
         "bool need_d_inter=True) -> (Tensor d_inter, Tensor d_gates)");
+  m.def("rotary(Tensor x, Tensor positions, Tensor inv_freq, str layout='half', float mscale=1.0, bool inverse=False) "
+        "-> Tensor");
+  m.def("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor block_table, Tensor kv_lens, "
+        "Tensor cu_q, Tensor? inv_freq=None, str layout='half', float mscale=1.0) -> ()");
+  m.def("kv_append_q(Tensor q, Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor block_table, "
+        "Tensor kv_lens, Tensor cu_q, Tensor? inv_freq=None, str layout='half', float mscale=1.0) -> Tensor");
+  m.def("kv_append_q_into(Tensor q, Tensor(c!) q_out, Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+        "Tensor block_table, Tensor kv_lens, Tensor cu_q, Tensor? inv_freq=None, str layout='half', "
+        "float mscale=1.0) -> ()");
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor kv_lens, Tensor cu_q, "
+        "float scale) -> Tensor");
+  m.def("paged_attention_into(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor kv_lens, "
+        "Tensor cu_q, float scale, Tensor(a!) out) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CUDA, m) {
@@ -509,6 +714,12 @@ TORCH_LIBRARY_IMPL(prunepath, CUDA, m) {
   m.impl("moe_prefill_into", &prefill_into);
   m.impl("masked_gate", &masked_gate_gpu);
   m.impl("masked_gate_bwd", &masked_gate_bwd_gpu);
+  m.impl("rotary", &rotary_gpu);
+  m.impl("kv_append", &kv_append_gpu);
+  m.impl("kv_append_q", &kv_append_q_gpu);
+  m.impl("kv_append_q_into", &kv_append_q_into_gpu);
+  m.impl("paged_attention", &paged_attention_gpu);
+  m.impl("paged_attention_into", &paged_attention_into_gpu);
 }
 
 TORCH_LIBRARY_IMPL(prunepath, Meta, m) {
@@ -526,11 +737,18 @@ TORCH_LIBRARY_IMPL(prunepath, Meta, m) {
   m.impl("moe_prefill_into", &moe_prefill_into_meta);
   m.impl("masked_gate", &masked_gate_meta);
   m.impl("masked_gate_bwd", &masked_gate_bwd_meta);
+  m.impl("rotary", &rotary_meta);
+  m.impl("kv_append", &kv_append_meta);
+  m.impl("kv_append_q", &kv_append_q_meta);
+  m.impl("kv_append_q_into", &kv_append_q_into_meta);
+  m.impl("paged_attention", &paged_attention_meta);
+  m.impl("paged_attention_into", &paged_attention_into_meta);
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CPU, m) {
   for (const char* name : {"route", "route_logits", "bucket", "pack_experts", "pack_router", "decode_workspace_init",
                            "moe_decode", "moe_decode_into", "moe_decode_batch", "moe_decode_batch_into",
-                           "moe_prefill", "moe_prefill_into", "masked_gate", "masked_gate_bwd"})
+                           "moe_prefill", "moe_prefill_into", "masked_gate", "masked_gate_bwd", "rotary", "kv_append",
+                           "kv_append_q", "kv_append_q_into", "paged_attention", "paged_attention_into"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&refuse_cpu>());
 }

@@ -14,6 +14,7 @@ synchronises with the host, so the calls can be captured in a CUDA (HIP) graph.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -333,3 +334,133 @@ def masked_gate(inter: torch.Tensor, gates: torch.Tensor, layout) -> torch.Tenso
     x = inter.contiguous()
     _mg_dtype(x)
     return L.torch_ops().masked_gate(x, gates.float().contiguous(), eid, perm, seg)
+
+
+# ----------------------------------------------------------------------------- rotary positions
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: int = 4096, turns: Tuple[float, float] = (1.0, 32.0), device=None):
+    """(inv_freq float64 [dim / 2], mscale) for ``rotary`` and ``kv_append``: the angle per position
+    of each pair, base^(-2 i / dim), and the factor of cos and sin (1 unless stated). ``scaling`` for
+    contexts ``factor`` times longer than ``original_length``:
+
+    * None: as it is;
+    * "linear": every angle divided by factor;
+    * "ntk": base grows by factor^(dim / (dim - 2)), so that the slowest pair turns factor times
+      slower and the fastest as before;
+    * "yarn": pairs that make fewer than ``turns[0]`` turns over the original length are divided by
+      factor, those with more than ``turns[1]`` stay, a linear ramp between; mscale is
+      0.1 ln(factor) + 1."""
+    if dim < 2 or dim % 2:
+        raise ValueError(f"rotary_frequencies: dim must be an even number from 2 on (got {dim})")
+    if not (base > 0 and factor > 0):
+        raise ValueError("rotary_frequencies: base and factor must be positive")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    f, mscale = base ** (-2.0 * i / dim), 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ntk":
+        f = (base * factor ** (dim / (dim - 2)) if dim > 2 else base) ** (-2.0 * i / dim)
+    elif scaling == "yarn":
+        few, many = turns
+        if not many > few:
+            raise ValueError("rotary_frequencies: turns must be (fewer, more)")
+        keep = ((original_length * f / (2.0 * math.pi) - few) / (many - few)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        mscale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling is not None:
+        raise ValueError(f"rotary_frequencies: scaling must be None, 'linear', 'ntk' or 'yarn' (got {scaling!r})")
+    return f.to(device), mscale
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    _, positions, inv_freq, layout, mscale, inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+    ctx.how = (layout, mscale, inverse)
+
+
+def _rotary_backward(ctx, grad):
+    positions, inv_freq = ctx.saved_tensors
+    layout, mscale, inverse = ctx.how
+    return L.torch_ops().rotary(grad, positions, inv_freq, layout, mscale, not inverse), None, None, None, None, None
+
+
+_ROTARY_AUTOGRAD = False
+
+
+def _register_rotary_autograd() -> None:
+    global _ROTARY_AUTOGRAD
+    if not _ROTARY_AUTOGRAD:
+        L.torch_ops()
+        torch.library.register_autograd("prunepath::rotary", _rotary_backward, setup_context=_rotary_setup_context)
+        _ROTARY_AUTOGRAD = True
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, layout: str = "half",
+           mscale: float = 1.0) -> torch.Tensor:
+    """x [N, heads, D] or [B, L, heads, D] (fp32 or bf16, any strides) with every head's first
+    2 * len(inv_freq) channels turned by position * inv_freq (``torch.ops.prunepath.rotary``):
+    pairs (i, i + rotary_dim / 2) for layout "half", (2 i, 2 i + 1) for "interleaved"; cos and sin
+    times mscale; the other channels unchanged. positions int32 or int64 of x's leading shape,
+    inv_freq float64 (``rotary_frequencies``). A new tensor of x's dtype; differentiable in x (the
+    gradient is the turn by the opposite angles, exact at any order)."""
+    _register_rotary_autograd()
+    return L.torch_ops().rotary(x, positions, inv_freq, layout, mscale, False)
+
+
+# ----------------------------------------------------------------------------- paged cache
+def paged_cache(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device=None):
+    """(k_pages [num_pages, kv_heads, page_size, head_dim], v_pages [num_pages, kv_heads, head_dim,
+    page_size]) bfloat16 for ``kv_append`` and ``paged_attention``, uninitialised (nothing that was
+    not appended is ever attended). page_size a power of two from 16 on, head_dim 64 or 128."""
+    k = torch.empty(num_pages, kv_heads, page_size, head_dim, dtype=torch.bfloat16, device=device)
+    return k, torch.empty(num_pages, kv_heads, head_dim, page_size, dtype=torch.bfloat16, device=device)
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+              block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor,
+              inv_freq: Optional[torch.Tensor] = None, layout: str = "half", mscale: float = 1.0,
+              q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Appends the new tokens' k and v [N, kv_heads, D] (fp32 or bf16, rows may be parts of a joint
+    projection's) to the paged cache, k turned by its position (``rotary``; inv_freq None: as it
+    is), in one launch (``torch.ops.prunepath.kv_append`` and ``kv_append_q``).
+
+    The ragged batch: rows cu_q[s] .. cu_q[s + 1] (int32 [seqs + 1]) are sequence s, kv_lens [seqs]
+    int32 its length *with* them; position p is at place p % page_size of page
+    block_table[s, p // page_size] (int32 [seqs, max_pages]). An entry outside the cache (-1) holds
+    no token: what falls there is dropped. No two tokens of a call may have the same place.
+
+    q [N, heads, D]: turned as k is, returned as bf16 [N, heads, D] (in ``q_out``, which may be q
+    itself, if given). Rows behind cu_q[seqs] append nothing; in a new result they are zeros, in
+    q_out they stay. inference only: no gradient."""
+    ops = L.torch_ops()
+    with torch.no_grad():
+        if q is None:
+            if q_out is not None:
+                raise RuntimeError("prunepath.kv_append: q_out without q")
+            ops.kv_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+            return None
+        if q_out is None:
+            return ops.kv_append_q(q, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+        ops.kv_append_q_into(q, q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+        return q_out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    kv_lens: torch.Tensor, cu_q: torch.Tensor, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens (the ragged batch of ``kv_append``, appended before) over the
+    paged cache: the token at position p attends the positions 0 .. p of its sequence, query head h
+    the key head h // (heads / kv_heads). q bf16 [N, heads, D] -> bf16 [N, heads, D]
+    (``torch.ops.prunepath.paged_attention``, or ``paged_attention_into`` writing ``out``); scale
+    defaults to D^-0.5. Scores and softmax in fp32. A row that attends nothing is zero. Rows behind
+    cu_q[seqs] are zero in a new result and stay in ``out``. Single tokens, chunks and whole prompts,
+    in one call; lengths are read on the device, so a captured call serves lengths that grow.
+    Inference only: no gradient."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    ops = L.torch_ops()
+    with torch.no_grad():
+        if out is None:
+            return ops.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale))
+        ops.paged_attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), out)
+        return out
