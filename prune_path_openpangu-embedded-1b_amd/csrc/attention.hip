@@ -41,7 +41,8 @@ struct AttnArgs {
   int64_t qs[2];  // strides of token and head, in elements
   const bf16_t *k, *v;
   int Hq, Hkv, group;
-  float c;        // scale * log2(e): scores in powers of two
+  float c;        // |scale| * log2(e): scores in powers of two
+  uint32_t flip;  // the sign of scale, on both halves of a pair of q
   bf16_t* out;
   int zero_tail;
   int splits, least;  // most ranges of a tile; fewest tokens of a range
@@ -106,12 +107,10 @@ __device__ __forceinline__ void attn_zero(const AttnArgs& a, const AttnTile& w, 
 }
 
 // ------------------------------------------------------------------ masked steps
-// Non-finite elements of a V operand (8 tokens of one channel).
-__device__ __forceinline__ bool attn_has_bad(const a_u4 v) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
-  return bad;
+// Bits 15 and 31 of a word: whether its two elements are not finite (an exponent of ones carries).
+__device__ __forceinline__ uint32_t attn_bad2(uint32_t x) { return (x & 0x7f807f80u) + 0x00800080u; }
+__device__ __forceinline__ uint32_t attn_bad(const a_u4 v) {
+  return attn_bad2(v[0]) | attn_bad2(v[1]) | attn_bad2(v[2]) | attn_bad2(v[3]);
 }
 __device__ __forceinline__ uint32_t attn_clean1(uint32_t x) { return (x & 0x7f80u) == 0x7f80u ? 0u : x; }
 __device__ __forceinline__ a_u4 attn_clean(a_u4 v) {
@@ -138,6 +137,15 @@ __device__ __forceinline__ float attn_poison(float o, float code) {
   return o + __uint_as_float(up ? 0x7f800000u : 0xff800000u);
 }
 
+// 1 for every attended of 8 tokens (bits of `seen`), as an operand.
+__device__ __forceinline__ a_u4 attn_ones(uint32_t seen) {
+  a_u4 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = ((seen >> (2 * j)) & 1 ? 0x3f80u : 0u) | ((seen >> (2 * j + 1)) & 1 ? 0x3f800000u : 0u);
+  return v;
+}
+
 __device__ __forceinline__ uint32_t attn_pk(float a, float b) {
   return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
 }
@@ -157,20 +165,15 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // ------------------------------------------------------------------ few rows
 // Up to 16 NB rows of one key head; the cache bounds it. The four waves take alternate steps of 32
 // tokens, each with its own m, l and o, and join them at the end through LDS. K and V operands come
-// straight from memory into registers, the next step's while the present one is computed; the page
-// numbers a step before that.
+// straight from memory into registers. The next step's K is asked for once the present one's scores
+// are computed, its V after the second product, so a wave always has one of the two in flight with
+// one set of registers.
 // K operand row m of block b (16 tokens) is token 8 (m / 4) + 4 b + m % 4 of the step, which leaves
 // lane group g = lane / 16 with the scores of tokens 8 g .. 8 g + 7: its k of the second product.
 // P enters as a sum of two bf16 values (the rounded one and what is left, 2^-17 of it): the second
 // product costs nothing next to the loads.
 template <int D, int NB>
-struct AttnStep {
-  a_u4 k[2][D / 32], v[D / 16];
-  bool ok;  // the page of the lane's tokens 8 g .. 8 g + 7 is there
-};
-
-template <int D, int NB>
-__global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel(AttnArgs a) {
   constexpr int R = 16 * NB, KS = D / 32, MB = D / 16, OS = D + 4;
   __shared__ float o_s[4][R][OS];
   __shared__ float ml_s[4][R][2];
@@ -185,6 +188,38 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel
   }
   if (split >= w.ns) return;
 
+  const int ps = 1 << a.seqs.lp;
+  const int gk = 8 * (col >> 2), gv = 8 * g;  // the lane's tokens of K and of V, within a step
+  int pk, pv;                                 // their pages, -1: none
+  int pc;                                     // the present V's
+  a_u4 kf[2][KS], vf[MB];
+  auto pages = [&](int t) {
+    pk = t + gk < w.hi ? a.seqs.page(w.s, (t + gk) >> a.seqs.lp) : -1;
+    pv = t + gv < w.hi ? a.seqs.page(w.s, (t + gv) >> a.seqs.lp) : -1;
+  };
+  // places without a page read page 0, and are masked
+  auto load_k = [&](int t) {
+    const bf16_t* kp = a.k + ((((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((t + gk) & (ps - 1)) + (col & 3)) * D + 8 * g;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[b][s] = *(const a_u4*)(kp + 4 * b * D + 32 * s);
+  };
+  auto at_v = [&](int page, int t) {
+    return a.v + ((((int64_t)max(page, 0) * a.Hkv + h) * D + col) << a.seqs.lp) + ((t + gv) & (ps - 1));
+  };
+  auto load_v = [&](int t) {
+    pc = pv;
+    const bf16_t* vp = at_v(pv, t);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) vf[b] = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+  };
+  int t = w.lo + 32 * wave;
+  pages(t);
+  load_k(t);
+  load_v(t);
+  pages(t + 128);
+
   a_u4 qf[NB][KS];
   int limit[NB];
 #pragma unroll
@@ -195,7 +230,7 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel
     const int i = (w.r0 + r) / a.group;
     const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[n][s] = in ? *(const a_u4*)(src + 32 * s + 8 * g) : a_mk(0, 0, 0, 0);
+    for (int s = 0; s < KS; ++s) qf[n][s] = in ? *(const a_u4*)(src + 32 * s + 8 * g) ^ a.flip : a_mk(0, 0, 0, 0);
   }
   const int low = attn_limit(a, w, 0);  // every row attends the tokens up to here
 
@@ -208,51 +243,42 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel
     for (int b = 0; b < MB; ++b) o[n][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  const int ps = 1 << a.seqs.lp;
-  const int gk = 8 * (col >> 2), gv = 8 * g;  // the lane's tokens of K and of V, within a step
-  int pk = -1, pv = -1;                       // their pages
-  auto pages = [&](int t) {
-    pk = t + gk < w.hi ? a.seqs.page(w.s, (t + gk) >> a.seqs.lp) : -1;
-    pv = t + gv < w.hi ? a.seqs.page(w.s, (t + gv) >> a.seqs.lp) : -1;
-  };
-  auto load = [&](AttnStep<D, NB>& x, int t) {  // places without a page read page 0, and are masked
-    x.ok = pv >= 0;
-    const bf16_t* kp = a.k + ((((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((t + gk) & (ps - 1)) + (col & 3)) * D + 8 * g;
-    const bf16_t* vp = a.v + ((((int64_t)max(pv, 0) * a.Hkv + h) * D + col) << a.seqs.lp) + ((t + gv) & (ps - 1));
+  for (; t < w.hi; t += 128) {
+    f32x4_t s[NB][2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.k[b][s] = *(const a_u4*)(kp + 4 * b * D + 32 * s);
+      for (int b = 0; b < 2; ++b) {
+        s[n][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int b = 0; b < MB; ++b) x.v[b] = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
-  };
-  auto compute = [&](AttnStep<D, NB>& x, int t) {
+        for (int q = 0; q < KS; ++q) s[n][b] = mfma16(kf[b][q], qf[n][q], s[n][b]);
+      }
+    const bool more = t + 128 < w.hi;
+    if (more) load_k(t + 128);
     // whether a place of the step is masked for any row (wave-uniform)
-    const bool part = t + 31 > low || t + 32 > w.hi || __ballot(!x.ok) != 0;
+    const bool part = t + 31 > low || t + 32 > w.hi || __ballot(pc < 0) != 0;
     bool bad = false;
     if (part) {
+      uint32_t any = 0;
 #pragma unroll
-      for (int b = 0; b < MB; ++b) bad |= attn_has_bad(x.v[b]);
-      bad = __ballot(bad) != 0;
+      for (int b = 0; b < MB; ++b) any |= attn_bad(vf[b]);
+      bad = __ballot((any & 0x80008000u) != 0) != 0;
+      if (bad) {
+#pragma unroll
+        for (int b = 0; b < MB; ++b) vf[b] = attn_clean(vf[b]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      f32x4_t s[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        s[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int q = 0; q < KS; ++q) s[b] = mfma16(x.k[b][q], qf[n][q], s[b]);
-      }
       float p[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * a.c;
+      for (int j = 0; j < 8; ++j) p[j] = s[n][j >> 2][j & 3];
       uint32_t seen = 0xffu;
       if (part) {
         seen = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool in = x.ok && t + gv + j <= limit[n] && t + gv + j < w.hi;
+          const bool in = pc >= 0 && t + gv + j <= limit[n] && t + gv + j < w.hi;
           seen |= in ? 1u << j : 0u;
           p[j] = in ? p[j] : -__builtin_inff();
         }
@@ -260,12 +286,12 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel
       float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
       top = fmaxf(top, pl_xor16f(top, lane));
       top = fmaxf(top, pl_xor32f(top, lane));
-      const float mn = fmaxf(m[n], top), shrink = attn_exp2(m[n] - mn);
+      const float mn = fmaxf(m[n], top * a.c), shrink = attn_exp2(m[n] - mn);
       m[n] = mn;
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        p[j] = attn_exp2(p[j] - mn);
+        p[j] = attn_exp2(__fmaf_rn(p[j], a.c, -mn));
         sum += p[j];
       }
       l[n] = __fmaf_rn(l[n], shrink, sum);
@@ -279,49 +305,24 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 2 : 1) void attn_few_kernel
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
         o[n][b] *= shrink;
-        const a_u4 v = bad ? attn_clean(x.v[b]) : x.v[b];
-        o[n][b] = mfma16(v, ph, o[n][b]);
-        o[n][b] = mfma16(v, pl, o[n][b]);
+        o[n][b] = mfma16(vf[b], ph, o[n][b]);
+        o[n][b] = mfma16(vf[b], pl, o[n][b]);
       }
-      if (bad) {
-        uint32_t one[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          one[j] = ((seen >> (2 * j)) & 1 ? 0x3f80u : 0u) | ((seen >> (2 * j + 1)) & 1 ? 0x3f800000u : 0u);
-        const a_u4 on = a_mk(one[0], one[1], one[2], one[3]);
+      if (bad) {  // what was taken out of V, read again, for the rows that attend it
+        const a_u4 one = attn_ones(seen);
+        const bf16_t* vp = at_v(pc, t);
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
-          const f32x4_t code = mfma16(attn_code(x.v[b]), on, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+          const a_u4 x = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+          const f32x4_t code = mfma16(attn_code(x), one, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[n][b][i] = attn_poison(o[n][b][i], code[i]);
         }
       }
     }
-  };
-
-  int t = w.lo + 32 * wave;
-  if (t < w.hi) {
-    AttnStep<D, NB> x, y;
-    pages(t);
-    load(x, t);
-    pages(t + 128);
-    while (true) {
-      const bool more = t + 128 < w.hi;
-      if (more) {
-        load(y, t + 128);
-        pages(t + 256);
-      }
-      compute(x, t);
-      if (!more) break;
-      t += 128;
-      const bool again = t + 128 < w.hi;
-      if (again) {
-        load(x, t + 128);
-        pages(t + 256);
-      }
-      compute(y, t);
-      if (!again) break;
-      t += 128;
+    if (more) {
+      load_v(t + 128);
+      pages(t + 256);
     }
   }
 
@@ -380,6 +381,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   constexpr int KC = D / 8, NK = ATTN_KT * KC / ATTN_THREADS, NV = D * (ATTN_KT / 8) / ATTN_THREADS, MB = D / 32;
   __shared__ a_u4 k_s[2][ATTN_KT * KC];
   __shared__ a_u4 v_s[2][D * (ATTN_KT / 8)];
+  __shared__ int bad_s[2];  // first token of the buffer's step if V there was not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, e = lane >> 5;
   // workgroup b runs on XCD b % 8; an XCD's workgroups take consecutive items, so that the tiles of
   // one key head share that XCD's L2
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
     const int i = (w.r0 + r) / a.group;
     const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1] + 8 * e;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) qf[s] = in ? *(const a_u4*)(src + 16 * s) : a_mk(0, 0, 0, 0);
+    for (int s = 0; s < D / 16; ++s) qf[s] = in ? *(const a_u4*)(src + 16 * s) ^ a.flip : a_mk(0, 0, 0, 0);
   }
   f32x16_t o[MB];
 #pragma unroll
@@ -418,70 +420,95 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 
   const int ps = 1 << a.seqs.lp;
   const int krow = tid / KC, kc = tid % KC, vrow = tid / 8, vc = tid % 8;
-  const int ktok = (krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1);  // of its 16
-  int pg[4];  // pages of the next step's four groups of 16 tokens, -1: none
+  const int k16 = __builtin_amdgcn_readfirstlane(krow >> 4);  // 0, or at D = 64 the wave's group of 16 tokens
+  const uint32_t koff = (((krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1)) * D + 8 * kc) * 2;  // its row's token
+  int pg[4], pn[4];  // pages of the step's four groups of 16 tokens and of the next one's, -1: none
   auto pages = [&](int t) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pg[j] = t + 16 * j < w.hi ? a.seqs.page(w.s, (t + 16 * j) >> a.seqs.lp) : -1;
+    for (int j = 0; j < 4; ++j) pn[j] = t + 16 * j < w.hi ? a.seqs.page(w.s, (t + 16 * j) >> a.seqs.lp) : -1;
   };
-  a_u4 kst[NK], vst[NV];
-  int have = 0, next_have = 0;  // groups whose page is there
-  auto load = [&](int t) {  // places without a page read page 0, and are masked
-    next_have = 0;
+  auto turn = [&] {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) next_have |= pg[j] >= 0 ? 1 << j : 0;
+    for (int j = 0; j < 4; ++j) pg[j] = pn[j];
+  };
+  a_u4 st[NK > NV ? NK : NV];
+  auto load_k = [&](int t) {  // places without a page read page 0, and are masked
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int b16 = (i * (ATTN_THREADS / KC) + krow) >> 4;
-      const int p = KC == 16 ? pg[i & 3] : (b16 & 1) ? pg[(2 * i + 1) & 3] : pg[(2 * i) & 3];
-      kst[i] = *(const a_u4*)(a.k + ((((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((t + 16 * b16) & (ps - 1)) + ktok) * D + 8 * kc);
+      const int j = KC == 16 ? i : 2 * i + k16;  // its group of 16 tokens
+      const int p = KC == 16 ? pn[i & 3] : k16 ? pn[(2 * i + 1) & 3] : pn[(2 * i) & 3];
+      const bf16_t* base = a.k + ((((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((t + 16 * j) & (ps - 1))) * D;
+      st[i] = *(const a_u4*)((const char*)base + koff);
     }
-    const int pv = (vc & 4) ? ((vc & 2) ? pg[3] : pg[2]) : ((vc & 2) ? pg[1] : pg[0]);
+  };
+  auto load_v = [&](int t) {
+    const int pv = (vc & 4) ? ((vc & 2) ? pn[3] : pn[2]) : ((vc & 2) ? pn[1] : pn[0]);
     const bf16_t* vp = a.v + ((((int64_t)max(pv, 0) * a.Hkv + h) * D + vrow) << a.seqs.lp) + ((t + 8 * vc) & (ps - 1));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) vst[i] = *(const a_u4*)(vp + ((int64_t)(32 * i) << a.seqs.lp));
+    for (int i = 0; i < NV; ++i) st[i] = *(const a_u4*)(vp + ((int64_t)(32 * i) << a.seqs.lp));
   };
-  auto put = [&](int buf) {
+  auto put_k = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int row = i * (ATTN_THREADS / KC) + krow;
-      k_s[buf][row * KC + (kc ^ (row & 7))] = kst[i];
+      k_s[buf][row * KC + (kc ^ (row & 7))] = st[i];
+    }
+  };
+  const int low0 = attn_limit(a, w, 0);  // every row of the tile attends the tokens up to here
+  auto put_v = [&](int buf, int t) {
+    // a step with a masked place: only the finite part of V, and a mark where there is another (a
+    // mark by chance, before the first, costs a product of zeros)
+    if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || (pn[0] | pn[1] | pn[2] | pn[3]) < 0) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        any |= attn_bad(st[i]);
+        st[i] = attn_clean(st[i]);
+      }
+      if (any & 0x80008000u) bad_s[buf] = t;
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v_s[buf][(32 * i + vrow) * 8 + (vc ^ (vrow & 7))] = vst[i];
+    for (int i = 0; i < NV; ++i) v_s[buf][(32 * i + vrow) * 8 + (vc ^ (vrow & 7))] = st[i];
   };
+  const a_u4* const kb0 = &k_s[0][col * KC];
+  const a_u4* const vb0 = &v_s[0][col * 8];
+  const int sw = col & 7;
 
   int t = w.lo, buf = 0;
   pages(t);
-  load(t);
+  load_k(t);
+  put_k(0);
+  load_v(t);
+  put_v(0, t);
+  turn();
   pages(t + ATTN_KT);
-  put(0);
-  have = next_have;
   __syncthreads();
   while (true) {
     const bool more = t + ATTN_KT < w.hi;
-    if (more) {
-      load(t + ATTN_KT);
-      pages(t + 2 * ATTN_KT);
-    }
-    if (t <= top) {
-      f32x16_t s[2];
+    if (more) load_k(t + ATTN_KT);
+    const bool on = t <= top;  // some row of the wave attends the step
+    f32x16_t s[2];
+    if (on) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int q = 0; q < 16; ++q) s[b][q] = 0.0f;
+      const a_u4* const kb = kb0 + buf * (ATTN_KT * KC);
 #pragma unroll
-      for (int q = 0; q < D / 16; ++q)
+      for (int q = 0; q < D / 16; ++q) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          s[b] = mfma32a(k_s[buf][(32 * b + col) * KC + ((2 * q + e) ^ (col & 7))], qf[q], s[b]);
+        for (int b = 0; b < 2; ++b) s[b] = mfma32a(kb[32 * b * KC + ((2 * q + e) ^ sw)], qf[q], s[b]);
+        if (q & 1) __builtin_amdgcn_sched_barrier(0);  // four operands ahead are enough: the rest stays in LDS
+      }
+    }
+    if (more) {
+      put_k(buf ^ 1);
+      load_v(t + ATTN_KT);
+    }
+    if (on) {
+      const int have = (pg[0] >= 0 ? 1 : 0) | (pg[1] >= 0 ? 2 : 0) | (pg[2] >= 0 ? 4 : 0) | (pg[3] >= 0 ? 8 : 0);
       const bool part = t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != 15;
       uint32_t seen = ~0u;
-      float mx = ATTN_LOW;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) s[b][q] *= a.c;
       if (part) {
         seen = 0;
 #pragma unroll
@@ -489,18 +516,19 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 #pragma unroll
           for (int q = 0; q < 16; ++q) {
             const int g16 = 2 * b + (q >> 3), tok = t + 16 * g16 + 8 * e + (q & 7);
-            const bool on = tok <= limit && tok < w.hi && ((have >> g16) & 1);
-            seen |= on ? 1u << (16 * b + q) : 0u;
-            s[b][q] = on ? s[b][q] : -__builtin_inff();
+            const bool in = tok <= limit && tok < w.hi && ((have >> g16) & 1);
+            seen |= in ? 1u << (16 * b + q) : 0u;
+            s[b][q] = in ? s[b][q] : -__builtin_inff();
           }
       }
+      float mx = ATTN_LOW;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int q = 0; q < 16; ++q) mx = fmaxf(mx, s[b][q]);
       mx = fmaxf(mx, pl_xor32f(mx, lane));
-      const float mn = fmaxf(m, mx);
-      if (__ballot(mn != m)) {  // some row's maximum grew (or is NaN)
+      const float mn = fmaxf(m, mx * a.c);
+      if (__ballot(mn != m)) {  // some row's maximum grew
         const float shrink = attn_exp2(m - mn);
         l *= shrink;
 #pragma unroll
@@ -515,27 +543,21 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
         uint32_t p2[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x = attn_exp2(s[kk >> 1][8 * (kk & 1) + 2 * j] - mn), y = attn_exp2(s[kk >> 1][8 * (kk & 1) + 2 * j + 1] - mn);
+          const int q = 8 * (kk & 1) + 2 * j;
+          const float x = attn_exp2(__fmaf_rn(s[kk >> 1][q], a.c, -mn)), y = attn_exp2(__fmaf_rn(s[kk >> 1][q + 1], a.c, -mn));
           l += x + y;
           p2[j] = attn_pk(x, y);
         }
         pf[kk] = a_mk(p2[0], p2[1], p2[2], p2[3]);
       }
-      const a_u4* const vb = v_s[buf];
-      bool bad = false;
-      if (part) {
+      const a_u4* const vb = vb0 + buf * (D * 8);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+      for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
-          for (int b = 0; b < MB; ++b) bad |= attn_has_bad(vb[(32 * b + col) * 8 + ((2 * kk + e) ^ (col & 7))]);
-        bad = __ballot(bad) != 0;
+        for (int b = 0; b < MB; ++b) o[b] = mfma32a(vb[32 * b * 8 + ((2 * kk + e) ^ sw)], pf[kk], o[b]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (!bad) {
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-          for (int b = 0; b < MB; ++b) o[b] = mfma32a(vb[(32 * b + col) * 8 + ((2 * kk + e) ^ (col & 7))], pf[kk], o[b]);
-      } else {
+      if (bad_s[buf] == t) {  // what was taken out of V, read again, for the rows that attend it
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
           f32x16_t code;
@@ -543,22 +565,20 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
           for (int q = 0; q < 16; ++q) code[q] = 0.0f;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            const a_u4 v = vb[(32 * b + col) * 8 + ((2 * kk + e) ^ (col & 7))];
-            uint32_t one[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              one[j] = ((seen >> (8 * kk + 2 * j)) & 1 ? 0x3f80u : 0u) | ((seen >> (8 * kk + 2 * j + 1)) & 1 ? 0x3f800000u : 0u);
-            o[b] = mfma32a(attn_clean(v), pf[kk], o[b]);
-            code = mfma32a(attn_code(v), a_mk(one[0], one[1], one[2], one[3]), code);
+            const bf16_t* vp = a.v + ((((int64_t)max(pg[kk], 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
+                               ((t + 16 * kk) & (ps - 1)) + 8 * e;
+            code = mfma32a(attn_code(*(const a_u4*)vp), attn_ones(seen >> (8 * kk)), code);
           }
 #pragma unroll
           for (int q = 0; q < 16; ++q) o[b][q] = attn_poison(o[b][q], code[q]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
     if (!more) break;
-    put(buf ^ 1);
-    have = next_have;
+    put_v(buf ^ 1, t + ATTN_KT);
+    turn();
+    pages(t + 2 * ATTN_KT);
     __syncthreads();
     buf ^= 1;
     t += ATTN_KT;
@@ -683,7 +703,7 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.q = (const bf16_t*)q, a.qs[0] = q_strides[0], a.qs[1] = q_strides[1];
   a.k = (const bf16_t*)k_pages, a.v = (const bf16_t*)v_pages;
   a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv;
-  a.c = scale * 1.4426950408889634f;
+  a.c = fabsf(scale) * 1.4426950408889634f, a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
   a.splits = p.splits, a.least = p.least, a.tiles = (int)p.tiles;
   a.po = (float*)workspace;
