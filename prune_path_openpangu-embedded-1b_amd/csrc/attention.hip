@@ -146,10 +146,13 @@ __device__ __forceinline__ a_u4 attn_ones(uint32_t seen) {
   return v;
 }
 
-__device__ __forceinline__ uint32_t attn_pk(float a, float b) {
-  return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
-}
 
+// max(a, b, c) in one instruction (fmaxf first makes each operand a quiet value).
+__device__ __forceinline__ float attn_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // v_mfma_f32_16x16x32_bf16: A lane l holds row l % 16, k = 8 (l / 16) .. + 7; B lane l column l % 16,
@@ -177,7 +180,7 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
   constexpr int R = 16 * NB, KS = D / 32, MB = D / 16, OS = D + 4;
   __shared__ float o_s[4][R][OS];
   __shared__ float ml_s[4][R][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
   const int split = blockIdx.x % a.splits;
   const int item = blockIdx.x / a.splits, h = item % a.Hkv;
   const AttnTile w = attn_tile<R>(a, item / a.Hkv, split);
@@ -275,6 +278,7 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
       for (int j = 0; j < 8; ++j) p[j] = s[n][j >> 2][j & 3];
       uint32_t seen = 0xffu;
       if (part) {
+        asm volatile("");  // a branch: few steps have one
         seen = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -298,8 +302,8 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        hi[j] = attn_pk(p[2 * j], p[2 * j + 1]);
-        lo[j] = attn_pk(p[2 * j] - __uint_as_float(hi[j] << 16), p[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
+        hi[j] = f32_to_bf16x2(p[2 * j], p[2 * j + 1]);
+        lo[j] = f32_to_bf16x2(p[2 * j] - __uint_as_float(hi[j] << 16), p[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
       }
       const a_u4 ph = a_mk(hi[0], hi[1], hi[2], hi[3]), pl = a_mk(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
@@ -354,8 +358,8 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
     const int64_t row = attn_row(a, w, h, r);
     if (w.ns == 1) {
       const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-      *(a_u4*)(a.out + row * D + d) = a_mk(attn_pk(acc[0] * inv, acc[1] * inv), attn_pk(acc[2] * inv, acc[3] * inv),
-                                                  attn_pk(acc[4] * inv, acc[5] * inv), attn_pk(acc[6] * inv, acc[7] * inv));
+      *(a_u4*)(a.out + row * D + d) = a_mk(f32_to_bf16x2(acc[0] * inv, acc[1] * inv), f32_to_bf16x2(acc[2] * inv, acc[3] * inv),
+                                                  f32_to_bf16x2(acc[4] * inv, acc[5] * inv), f32_to_bf16x2(acc[6] * inv, acc[7] * inv));
     } else {
       float* to = a.po + (row * a.splits + split) * D + d;
       *(float4*)to = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -375,6 +379,7 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
 // c ^ (m % 8) of its 128 bytes, so that 8 lanes on consecutive rows touch 8 different bank groups.
 #define ATTN_ROWS 128
 #define ATTN_KT 64
+#define ATTN_SLACK 8.0f
 
 template <int D>
 __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) {
@@ -382,7 +387,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   __shared__ a_u4 k_s[2][ATTN_KT * KC];
   __shared__ a_u4 v_s[2][D * (ATTN_KT / 8)];
   __shared__ int bad_s[2];  // first token of the buffer's step if V there was not finite
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, e = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, e = lane >> 5;
   // workgroup b runs on XCD b % 8; an XCD's workgroups take consecutive items, so that the tiles of
   // one key head share that XCD's L2
   const int per = gridDim.x >> 3;
@@ -422,53 +427,50 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   const int krow = tid / KC, kc = tid % KC, vrow = tid / 8, vc = tid % 8;
   const int k16 = __builtin_amdgcn_readfirstlane(krow >> 4);  // 0, or at D = 64 the wave's group of 16 tokens
   const uint32_t koff = (((krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1)) * D + 8 * kc) * 2;  // its row's token
-  int pg[4], pn[4];  // pages of the step's four groups of 16 tokens and of the next one's, -1: none
+  // The page of the lane's group of 16 tokens, (lane % 8) / 2, of a step, -1: none: of the present
+  // step and the three after it. That is the group of the lane's V chunk; lane 2 j has group j's.
+  int pg, p1, p2, pn;
   auto pages = [&](int t) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) pn[j] = t + 16 * j < w.hi ? a.seqs.page(w.s, (t + 16 * j) >> a.seqs.lp) : -1;
+    const int at = t + 16 * (vc >> 1);
+    pn = at < w.hi ? a.seqs.page(w.s, at >> a.seqs.lp) : -1;
   };
-  auto turn = [&] {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) pg[j] = pn[j];
-  };
-  a_u4 st[NK > NV ? NK : NV];
+  a_u4 kst[NK], vst[NV];
   auto load_k = [&](int t) {  // places without a page read page 0, and are masked
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int j = KC == 16 ? i : 2 * i + k16;  // its group of 16 tokens
-      const int p = KC == 16 ? pn[i & 3] : k16 ? pn[(2 * i + 1) & 3] : pn[(2 * i) & 3];
+      const int p = __builtin_amdgcn_readlane(pn, 2 * j);
       const bf16_t* base = a.k + ((((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((t + 16 * j) & (ps - 1))) * D;
-      st[i] = *(const a_u4*)((const char*)base + koff);
+      kst[i] = *(const a_u4*)((const char*)base + koff);
     }
   };
   auto load_v = [&](int t) {
-    const int pv = (vc & 4) ? ((vc & 2) ? pn[3] : pn[2]) : ((vc & 2) ? pn[1] : pn[0]);
-    const bf16_t* vp = a.v + ((((int64_t)max(pv, 0) * a.Hkv + h) * D + vrow) << a.seqs.lp) + ((t + 8 * vc) & (ps - 1));
+    const bf16_t* vp = a.v + ((((int64_t)max(pn, 0) * a.Hkv + h) * D + vrow) << a.seqs.lp) + ((t + 8 * vc) & (ps - 1));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) st[i] = *(const a_u4*)(vp + ((int64_t)(32 * i) << a.seqs.lp));
+    for (int i = 0; i < NV; ++i) vst[i] = *(const a_u4*)(vp + ((int64_t)(32 * i) << a.seqs.lp));
   };
   auto put_k = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int row = i * (ATTN_THREADS / KC) + krow;
-      k_s[buf][row * KC + (kc ^ (row & 7))] = st[i];
+      k_s[buf][row * KC + (kc ^ (row & 7))] = kst[i];
     }
   };
   const int low0 = attn_limit(a, w, 0);  // every row of the tile attends the tokens up to here
-  auto put_v = [&](int buf, int t) {
+  auto put_v = [&](int buf, int t, int page) {
     // a step with a masked place: only the finite part of V, and a mark where there is another (a
     // mark by chance, before the first, costs a product of zeros)
-    if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || (pn[0] | pn[1] | pn[2] | pn[3]) < 0) {
+    if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(page < 0)) {
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        any |= attn_bad(st[i]);
-        st[i] = attn_clean(st[i]);
+        any |= attn_bad(vst[i]);
+        vst[i] = attn_clean(vst[i]);
       }
       if (any & 0x80008000u) bad_s[buf] = t;
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v_s[buf][(32 * i + vrow) * 8 + (vc ^ (vrow & 7))] = st[i];
+    for (int i = 0; i < NV; ++i) v_s[buf][(32 * i + vrow) * 8 + (vc ^ (vrow & 7))] = vst[i];
   };
   const a_u4* const kb0 = &k_s[0][col * KC];
   const a_u4* const vb0 = &v_s[0][col * 8];
@@ -477,15 +479,30 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   int t = w.lo, buf = 0;
   pages(t);
   load_k(t);
-  put_k(0);
   load_v(t);
-  put_v(0, t);
-  turn();
+  pg = pn;
   pages(t + ATTN_KT);
-  __syncthreads();
+  put_k(0);
+  put_v(0, t, pg);
+  if (t + ATTN_KT < w.hi) {
+    load_k(t + ATTN_KT);
+    load_v(t + ATTN_KT);
+  }
+  p1 = pn;
+  pages(t + 2 * ATTN_KT);
   while (true) {
+    __syncthreads();  // the present step is in its buffer, and every wave is done with the other one
     const bool more = t + ATTN_KT < w.hi;
-    if (more) load_k(t + ATTN_KT);
+    if (more) {
+      put_k(buf ^ 1);
+      put_v(buf ^ 1, t + ATTN_KT, p1);
+      if (t + 2 * ATTN_KT < w.hi) {
+        load_k(t + 2 * ATTN_KT);
+        load_v(t + 2 * ATTN_KT);
+        p2 = pn;
+        pages(t + 3 * ATTN_KT);
+      }
+    }
     const bool on = t <= top;  // some row of the wave attends the step
     f32x16_t s[2];
     if (on) {
@@ -501,22 +518,18 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
         if (q & 1) __builtin_amdgcn_sched_barrier(0);  // four operands ahead are enough: the rest stays in LDS
       }
     }
-    if (more) {
-      put_k(buf ^ 1);
-      load_v(t + ATTN_KT);
-    }
     if (on) {
-      const int have = (pg[0] >= 0 ? 1 : 0) | (pg[1] >= 0 ? 2 : 0) | (pg[2] >= 0 ? 4 : 0) | (pg[3] >= 0 ? 8 : 0);
-      const bool part = t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != 15;
+      const uint64_t have = __ballot(pg >= 0);  // bit 2 j: group j
       uint32_t seen = ~0u;
-      if (part) {
+      if (t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != ~0ull) {  // a masked place
+        asm volatile("");  // a branch: few steps have one
         seen = 0;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int q = 0; q < 16; ++q) {
             const int g16 = 2 * b + (q >> 3), tok = t + 16 * g16 + 8 * e + (q & 7);
-            const bool in = tok <= limit && tok < w.hi && ((have >> g16) & 1);
+            const bool in = tok <= limit && tok < w.hi && ((have >> (2 * g16)) & 1);
             seen |= in ? 1u << (16 * b + q) : 0u;
             s[b][q] = in ? s[b][q] : -__builtin_inff();
           }
@@ -525,11 +538,12 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) mx = fmaxf(mx, s[b][q]);
-      mx = fmaxf(mx, pl_xor32f(mx, lane));
-      const float mn = fmaxf(m, mx * a.c);
-      if (__ballot(mn != m)) {  // some row's maximum grew
-        const float shrink = attn_exp2(m - mn);
+        for (int q = 0; q < 16; q += 2) mx = attn_max3(mx, s[b][q], s[b][q + 1]);
+      mx = fmaxf(mx, pl_xor32f(mx, lane)) * a.c;
+      // m follows the maximum only where it has grown by more than ATTN_SLACK: p stays below
+      // 2^ATTN_SLACK, and most steps leave o and l as they are
+      if (__ballot(mx > m + ATTN_SLACK)) {
+        const float mn = fmaxf(m, mx), shrink = attn_exp2(m - mn);
         l *= shrink;
 #pragma unroll
         for (int b = 0; b < MB; ++b)
@@ -544,9 +558,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int q = 8 * (kk & 1) + 2 * j;
-          const float x = attn_exp2(__fmaf_rn(s[kk >> 1][q], a.c, -mn)), y = attn_exp2(__fmaf_rn(s[kk >> 1][q + 1], a.c, -mn));
+          const float x = attn_exp2(__fmaf_rn(s[kk >> 1][q], a.c, -m)), y = attn_exp2(__fmaf_rn(s[kk >> 1][q + 1], a.c, -m));
           l += x + y;
-          p2[j] = attn_pk(x, y);
+          p2[j] = f32_to_bf16x2(x, y);
         }
         pf[kk] = a_mk(p2[0], p2[1], p2[2], p2[3]);
       }
@@ -557,7 +571,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
         for (int b = 0; b < MB; ++b) o[b] = mfma32a(vb[32 * b * 8 + ((2 * kk + e) ^ sw)], pf[kk], o[b]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (bad_s[buf] == t) {  // what was taken out of V, read again, for the rows that attend it
+      if (__builtin_amdgcn_readfirstlane(bad_s[buf]) == t) {  // what was taken out of V, read again, for the rows that attend it
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
           f32x16_t code;
@@ -565,7 +579,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
           for (int q = 0; q < 16; ++q) code[q] = 0.0f;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            const bf16_t* vp = a.v + ((((int64_t)max(pg[kk], 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
+            const bf16_t* vp = a.v + ((((int64_t)max(__builtin_amdgcn_readlane(pg, 2 * kk), 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
                                ((t + 16 * kk) & (ps - 1)) + 8 * e;
             code = mfma32a(attn_code(*(const a_u4*)vp), attn_ones(seen >> (8 * kk)), code);
           }
@@ -576,10 +590,8 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
       }
     }
     if (!more) break;
-    put_v(buf ^ 1, t + ATTN_KT);
-    turn();
-    pages(t + 2 * ATTN_KT);
-    __syncthreads();
+    pg = p1;
+    p1 = p2;
     buf ^= 1;
     t += ATTN_KT;
   }
@@ -594,8 +606,8 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
     for (int b = 0; b < MB; ++b)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *(uint2*)(to + 32 * b + 8 * q) = make_uint2(attn_pk(o[b][4 * q] * inv, o[b][4 * q + 1] * inv),
-                                                    attn_pk(o[b][4 * q + 2] * inv, o[b][4 * q + 3] * inv));
+        *(uint2*)(to + 32 * b + 8 * q) = make_uint2(f32_to_bf16x2(o[b][4 * q] * inv, o[b][4 * q + 1] * inv),
+                                                    f32_to_bf16x2(o[b][4 * q + 2] * inv, o[b][4 * q + 3] * inv));
   } else {
     float* to = a.po + (row * a.splits + split) * D + 4 * e;
 #pragma unroll
@@ -646,7 +658,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int i = 1; i < 4; ++i) x += acc_s[i][d], y += acc_s[i][d + 1];
   const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-  *(uint32_t*)(a.out + row * D + d) = attn_pk(x * inv, y * inv);
+  *(uint32_t*)(a.out + row * D + d) = f32_to_bf16x2(x * inv, y * inv);
 }
 
 // ------------------------------------------------------------------ host

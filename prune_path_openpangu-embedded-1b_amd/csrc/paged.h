@@ -10,6 +10,13 @@
 #pragma once
 #include "pp_common.h"
 
+// Two floats rounded to bf16 and packed, a in the low half: one v_cvt_pk_bf16_f32.
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f32_to_bf16x2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), bf16x2_t));
+}
+
 struct PagedSeqs {
   const int32_t* cu_q;
   const int32_t* kv_lens;

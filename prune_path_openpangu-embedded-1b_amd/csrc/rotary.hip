@@ -49,7 +49,7 @@ struct RotVec<bf16_t, 8> {
   static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | ((uint32_t)f32_to_bf16(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16x2(v[2 * i], v[2 * i + 1]);
     *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
@@ -230,7 +230,7 @@ struct AppArgs {
 
 __device__ __forceinline__ uint32_t app_pair(const float* p) {
   const float2 f = *(const float2*)p;
-  return (uint32_t)f32_to_bf16(f.x) | ((uint32_t)f32_to_bf16(f.y) << 16);
+  return f32_to_bf16x2(f.x, f.y);
 }
 __device__ __forceinline__ uint32_t app_pair(const bf16_t* p) { return *(const uint32_t*)p; }
 

@@ -28,6 +28,7 @@
 #include <c10/hip/HIPStream.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/stack.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "../../include/prunepath_moe.h"
@@ -514,6 +515,44 @@ Tensor rotary_meta(const Tensor& x, const Tensor&, const Tensor&, c10::string_vi
   return at::empty_like(x);
 }
 
+// The op's gradient in x is the op with the opposite angles, which has a gradient in its turn.
+Tensor rotary_call(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                   double mscale, bool inverse) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("prunepath::rotary", "")
+                       .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, c10::string_view, double, bool)>();
+  return op.call(x, positions, inv_freq, layout, mscale, inverse);
+}
+
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& positions,
+                        const Tensor& inv_freq, c10::string_view layout, double mscale, bool inverse) {
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["layout"] = std::string(layout);
+    ctx->saved_data["mscale"] = mscale;
+    ctx->saved_data["inverse"] = inverse;
+    at::AutoDispatchBelowADInplaceOrView below;
+    return rotary_call(x, positions, inv_freq, layout, mscale, inverse);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor g;
+    if (grads[0].defined())
+      g = rotary_call(grads[0], saved[0], saved[1], ctx->saved_data["layout"].toStringRef(),
+                      ctx->saved_data["mscale"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    return {g, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                       double mscale, bool inverse) {
+  if (c10::GradMode::is_enabled() && x.requires_grad())
+    return RotaryFunction::apply(x, positions, inv_freq, layout, mscale, inverse);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rotary_call(x, positions, inv_freq, layout, mscale, inverse);
+}
+
 // ------------------------------------------------------------------ paged cache
 struct Paged {
   int64_t n, seqs, Hq, Hkv, D, pages, max_pages, page;
@@ -743,6 +782,13 @@ TORCH_LIBRARY_IMPL(prunepath, Meta, m) {
   m.impl("kv_append_q_into", &kv_append_q_into_meta);
   m.impl("paged_attention", &paged_attention_meta);
   m.impl("paged_attention_into", &paged_attention_into_meta);
+}
+
+TORCH_LIBRARY_IMPL(prunepath, Autograd, m) {
+  m.impl("rotary", &rotary_autograd);
+  // inference: no gradient is recorded
+  for (const char* name : {"kv_append", "kv_append_q", "kv_append_q_into", "paged_attention", "paged_attention_into"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CPU, m) {

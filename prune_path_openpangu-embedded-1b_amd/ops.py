@@ -372,29 +372,6 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
     return f.to(device), mscale
 
 
-def _rotary_setup_context(ctx, inputs, output):
-    _, positions, inv_freq, layout, mscale, inverse = inputs
-    ctx.save_for_backward(positions, inv_freq)
-    ctx.how = (layout, mscale, inverse)
-
-
-def _rotary_backward(ctx, grad):
-    positions, inv_freq = ctx.saved_tensors
-    layout, mscale, inverse = ctx.how
-    return L.torch_ops().rotary(grad, positions, inv_freq, layout, mscale, not inverse), None, None, None, None, None
-
-
-_ROTARY_AUTOGRAD = False
-
-
-def _register_rotary_autograd() -> None:
-    global _ROTARY_AUTOGRAD
-    if not _ROTARY_AUTOGRAD:
-        L.torch_ops()
-        torch.library.register_autograd("prunepath::rotary", _rotary_backward, setup_context=_rotary_setup_context)
-        _ROTARY_AUTOGRAD = True
-
-
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, layout: str = "half",
            mscale: float = 1.0) -> torch.Tensor:
     """x [N, heads, D] or [B, L, heads, D] (fp32 or bf16, any strides) with every head's first
@@ -403,7 +380,6 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
     times mscale; the other channels unchanged. positions int32 or int64 of x's leading shape,
     inv_freq float64 (``rotary_frequencies``). A new tensor of x's dtype; differentiable in x (the
     gradient is the turn by the opposite angles, exact at any order)."""
-    _register_rotary_autograd()
     return L.torch_ops().rotary(x, positions, inv_freq, layout, mscale, False)
 
 
@@ -433,16 +409,15 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     itself, if given). Rows behind cu_q[seqs] append nothing; in a new result they are zeros, in
     q_out they stay. inference only: no gradient."""
     ops = L.torch_ops()
-    with torch.no_grad():
-        if q is None:
-            if q_out is not None:
-                raise RuntimeError("prunepath.kv_append: q_out without q")
-            ops.kv_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
-            return None
-        if q_out is None:
-            return ops.kv_append_q(q, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
-        ops.kv_append_q_into(q, q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
-        return q_out
+    if q is None:
+        if q_out is not None:
+            raise RuntimeError("prunepath.kv_append: q_out without q")
+        ops.kv_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+        return None
+    if q_out is None:
+        return ops.kv_append_q(q, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+    ops.kv_append_q_into(q, q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+    return q_out
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -459,8 +434,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if scale is None:
         scale = q.shape[-1] ** -0.5
     ops = L.torch_ops()
-    with torch.no_grad():
-        if out is None:
-            return ops.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale))
-        ops.paged_attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), out)
-        return out
+    if out is None:
+        return ops.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale))
+    ops.paged_attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), out)
+    return out
