@@ -193,13 +193,15 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
 
   const int ps = 1 << a.seqs.lp;
   const int gk = 8 * (col >> 2), gv = 8 * g;  // the lane's tokens of K and of V, within a step
+  int ek, ev;                                 // their table entries
   int pk, pv;                                 // their pages, -1: none
   int pc;                                     // the present V's
   a_u4 kf[2][KS], vf[MB];
-  auto pages = [&](int t) {
-    pk = t + gk < w.hi ? a.seqs.page(w.s, (t + gk) >> a.seqs.lp) : -1;
-    pv = t + gv < w.hi ? a.seqs.page(w.s, (t + gv) >> a.seqs.lp) : -1;
+  auto entries = [&](int t) {
+    ek = t + gk < w.hi ? a.seqs.entry(w.s, (t + gk) >> a.seqs.lp) : -1;
+    ev = t + gv < w.hi ? a.seqs.entry(w.s, (t + gv) >> a.seqs.lp) : -1;
   };
+  auto pages = [&] { pk = a.seqs.page(ek), pv = a.seqs.page(ev); };
   // places without a page read page 0, and are masked
   auto load_k = [&](int t) {
     const bf16_t* kp = a.k + ((((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((t + gk) & (ps - 1)) + (col & 3)) * D + 8 * g;
@@ -218,10 +220,11 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
     for (int b = 0; b < MB; ++b) vf[b] = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
   };
   int t = w.lo + 32 * wave;
-  pages(t);
+  entries(t);
+  pages();
+  entries(t + 128);
   load_k(t);
   load_v(t);
-  pages(t + 128);
 
   a_u4 qf[NB][KS];
   int limit[NB];
@@ -247,6 +250,8 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
   }
 
   for (; t < w.hi; t += 128) {
+    pages();
+    entries(t + 256);
     f32x4_t s[NB][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -324,10 +329,7 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
         }
       }
     }
-    if (more) {
-      load_v(t + 128);
-      pages(t + 256);
-    }
+    if (more) load_v(t + 128);
   }
 
   // the four waves' rows joined
@@ -378,6 +380,17 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
 // tokens 16 b + 8 e .. + 7: its k of the second product. 16-byte chunk c of LDS row m sits at place
 // c ^ (m % 8) of its 128 bytes, so that 8 lanes on consecutive rows touch 8 different bank groups.
 #define ATTN_ROWS 128
+
+// 16 bytes per lane from memory into LDS at lds + 16 lane, by the copy path that does not pass through
+// registers. The compiler does not know of it: attn_landed() is what waits, for every copy that was
+// asked for, before the workgroup's barrier.
+typedef __attribute__((address_space(3))) void attn_lds_t;
+__device__ __forceinline__ uint32_t attn_lds(void* p) { return (uint32_t)(uintptr_t)(attn_lds_t*)p; }
+__device__ __forceinline__ void attn_copy(const void* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void attn_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 #define ATTN_KT 64
 #define ATTN_SLACK 8.0f
 
@@ -424,84 +437,63 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   float m = ATTN_LOW, l = 0.0f;
 
   const int ps = 1 << a.seqs.lp;
-  const int krow = tid / KC, kc = tid % KC, vrow = tid / 8, vc = tid % 8;
-  const int k16 = __builtin_amdgcn_readfirstlane(krow >> 4);  // 0, or at D = 64 the wave's group of 16 tokens
+  // the thread's 16-byte chunk of each K copy (row krow of its 16 or 32) and of each V copy (channel
+  // vrow of 32): its place in LDS is tid, so the swizzle is in what it reads
+  const int krow = tid / KC, kc = (tid % KC) ^ (krow & 7), vrow = tid / 8, vc = (tid % 8) ^ (vrow & 7);
+  const int k16 = KC == 16 ? 0 : wave >> 1;  // group of 16 rows, at D = 64
   const uint32_t koff = (((krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1)) * D + 8 * kc) * 2;  // its row's token
-  // The page of the lane's group of 16 tokens, (lane % 8) / 2, of a step, -1: none: of the present
-  // step and the three after it. That is the group of the lane's V chunk; lane 2 j has group j's.
-  int pg, p1, p2, pn;
-  auto pages = [&](int t) {
+  // The page of the lane's group of 16 tokens, vc / 2, of a step, -1: none: of the present step and the
+  // next. Lanes 0 .. 7 have vc = lane, so lane 2 j has group j's.
+  int pg, pn, en;  // en: the table entry of the step after the next
+  auto entry = [&](int t) {
     const int at = t + 16 * (vc >> 1);
-    pn = at < w.hi ? a.seqs.page(w.s, at >> a.seqs.lp) : -1;
+    en = at < w.hi ? a.seqs.entry(w.s, at >> a.seqs.lp) : -1;
   };
-  a_u4 kst[NK], vst[NV];
-  auto load_k = [&](int t) {  // places without a page read page 0, and are masked
+  const uint32_t k_lds = attn_lds(&k_s[0][64 * wave]), v_lds = attn_lds(&v_s[0][64 * wave]);
+  auto load = [&](int t, int buf) {  // places without a page read page 0, and are masked
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int j = KC == 16 ? i : 2 * i + k16;  // its group of 16 tokens
       const int p = __builtin_amdgcn_readlane(pn, 2 * j);
       const bf16_t* base = a.k + ((((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((t + 16 * j) & (ps - 1))) * D;
-      kst[i] = *(const a_u4*)((const char*)base + koff);
+      attn_copy((const char*)base + koff, k_lds + (buf * ATTN_KT * KC + i * ATTN_THREADS) * 16);
     }
-  };
-  auto load_v = [&](int t) {
     const bf16_t* vp = a.v + ((((int64_t)max(pn, 0) * a.Hkv + h) * D + vrow) << a.seqs.lp) + ((t + 8 * vc) & (ps - 1));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) vst[i] = *(const a_u4*)(vp + ((int64_t)(32 * i) << a.seqs.lp));
-  };
-  auto put_k = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int row = i * (ATTN_THREADS / KC) + krow;
-      k_s[buf][row * KC + (kc ^ (row & 7))] = kst[i];
-    }
+    for (int i = 0; i < NV; ++i)
+      attn_copy(vp + ((int64_t)(32 * i) << a.seqs.lp), v_lds + (buf * D * 8 + i * ATTN_THREADS) * 16);
   };
   const int low0 = attn_limit(a, w, 0);  // every row of the tile attends the tokens up to here
-  auto put_v = [&](int buf, int t, int page) {
-    // a step with a masked place: only the finite part of V, and a mark where there is another (a
-    // mark by chance, before the first, costs a product of zeros)
-    if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(page < 0)) {
-      uint32_t any = 0;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        any |= attn_bad(vst[i]);
-        vst[i] = attn_clean(vst[i]);
-      }
-      if (any & 0x80008000u) bad_s[buf] = t;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) v_s[buf][(32 * i + vrow) * 8 + (vc ^ (vrow & 7))] = vst[i];
-  };
   const a_u4* const kb0 = &k_s[0][col * KC];
   const a_u4* const vb0 = &v_s[0][col * 8];
   const int sw = col & 7;
 
   int t = w.lo, buf = 0;
-  pages(t);
-  load_k(t);
-  load_v(t);
-  pg = pn;
-  pages(t + ATTN_KT);
-  put_k(0);
-  put_v(0, t, pg);
-  if (t + ATTN_KT < w.hi) {
-    load_k(t + ATTN_KT);
-    load_v(t + ATTN_KT);
-  }
-  p1 = pn;
-  pages(t + 2 * ATTN_KT);
+  entry(t);
+  pn = a.seqs.page(en);
+  entry(t + ATTN_KT);
+  load(t, 0);
   while (true) {
-    __syncthreads();  // the present step is in its buffer, and every wave is done with the other one
+    attn_landed();  // the present step is in its buffer, and every wave is done with the other one
     const bool more = t + ATTN_KT < w.hi;
+    pg = pn;
     if (more) {
-      put_k(buf ^ 1);
-      put_v(buf ^ 1, t + ATTN_KT, p1);
-      if (t + 2 * ATTN_KT < w.hi) {
-        load_k(t + 2 * ATTN_KT);
-        load_v(t + 2 * ATTN_KT);
-        p2 = pn;
-        pages(t + 3 * ATTN_KT);
+      pn = a.seqs.page(en);
+      entry(t + 2 * ATTN_KT);
+      load(t + ATTN_KT, buf ^ 1);
+    }
+    // a step with a masked place: only the finite part of V, and a mark where there is another (a mark
+    // by chance, before the first, costs a product of zeros)
+    if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(pg < 0)) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const a_u4 v = v_s[buf][i * ATTN_THREADS + tid];
+        if (attn_bad(v) & 0x80008000u) {
+          v_s[buf][i * ATTN_THREADS + tid] = attn_clean(v);
+          bad_s[buf] = t;
+        }
       }
+      wg_lds_barrier();
     }
     const bool on = t <= top;  // some row of the wave attends the step
     f32x16_t s[2];
@@ -511,11 +503,20 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 #pragma unroll
         for (int q = 0; q < 16; ++q) s[b][q] = 0.0f;
       const a_u4* const kb = kb0 + buf * (ATTN_KT * KC);
+      // operands of two k steps at a time, the next two's on their way
+      a_u4 x[2][4];
+      auto get = [&](a_u4 (&f)[4], int q) {
 #pragma unroll
-      for (int q = 0; q < D / 16; ++q) {
+        for (int i = 0; i < 4; ++i) f[i] = kb[32 * (i & 1) * KC + ((2 * (q + (i >> 1)) + e) ^ sw)];
+      };
+      get(x[0], 0);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = mfma32a(kb[32 * b * KC + ((2 * q + e) ^ sw)], qf[q], s[b]);
-        if (q & 1) __builtin_amdgcn_sched_barrier(0);  // four operands ahead are enough: the rest stays in LDS
+      for (int q = 0; q < D / 16; q += 2) {
+        if (q + 2 < D / 16) get(x[((q >> 1) + 1) & 1], q + 2);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i & 1] = mfma32a(x[(q >> 1) & 1][i], qf[q + (i >> 1)], s[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (on) {
@@ -565,10 +566,18 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
         pf[kk] = a_mk(p2[0], p2[1], p2[2], p2[3]);
       }
       const a_u4* const vb = vb0 + buf * (D * 8);
+      a_u4 x[2][MB];
+      auto get = [&](a_u4 (&f)[MB], int kk) {
+#pragma unroll
+        for (int b = 0; b < MB; ++b) f[b] = vb[32 * b * 8 + ((2 * kk + e) ^ sw)];
+      };
+      get(x[0], 0);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
+        if (kk < 3) get(x[(kk + 1) & 1], kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) o[b] = mfma32a(vb[32 * b * 8 + ((2 * kk + e) ^ sw)], pf[kk], o[b]);
+        for (int b = 0; b < MB; ++b) o[b] = mfma32a(x[kk & 1][b], pf[kk], o[b]);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (__builtin_amdgcn_readfirstlane(bad_s[buf]) == t) {  // what was taken out of V, read again, for the rows that attend it
@@ -590,8 +599,6 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
       }
     }
     if (!more) break;
-    pg = p1;
-    p1 = p2;
     buf ^= 1;
     t += ATTN_KT;
   }

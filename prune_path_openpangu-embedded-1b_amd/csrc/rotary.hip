@@ -261,7 +261,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
   const int ps = 1 << a.seqs.lp;
   int page = -1;
   if (kind != 0) {
-    page = p0 < 0 ? -1 : a.seqs.page(s, p0 >> a.seqs.lp);
+    page = p0 < 0 ? -1 : a.seqs.page(a.seqs.entry(s, p0 >> a.seqs.lp));
     if (page < 0) return;
   }
   const int place = (int)(p0 & (ps - 1));
