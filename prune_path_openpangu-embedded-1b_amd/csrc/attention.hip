@@ -377,8 +377,9 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
 // K [64][D] and V^T [D][64] go through registers into one of two LDS buffers, the next step's while
 // the present one is computed (one barrier a step). Row m of the K tile is the token whose number
 // within its 16 has bits 2 and 3 of m swapped, which leaves lane half e = lane / 32 with the scores of
-// tokens 16 b + 8 e .. + 7: its k of the second product. 16-byte chunk c of LDS row m sits at place
-// c ^ (m % 8) of its 128 bytes, so that 8 lanes on consecutive rows touch 8 different bank groups.
+// tokens 16 b + 8 e .. + 7: its k of the second product. The 16-byte chunks of an LDS row are
+// permuted, so that the 16 lanes that read at a time, on 16 different rows, meet all 64 banks: in rows
+// of 256 bytes chunk c sits at place c ^ (row % 16), in rows of 128 at c ^ (row / 2 % 8).
 #define ATTN_ROWS 128
 
 // 16 bytes per lane from memory into LDS at lds + 16 lane, by the copy path that does not pass through
@@ -401,15 +402,11 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   __shared__ a_u4 v_s[2][D * (ATTN_KT / 8)];
   __shared__ int bad_s[2];  // first token of the buffer's step if V there was not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, e = lane >> 5;
-  // workgroup b runs on XCD b % 8; an XCD's workgroups take consecutive items, so that the tiles of
-  // one key head share that XCD's L2
-  const int per = gridDim.x >> 3;
-  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  // items are (head, tile, split); the last tiles, which attend most, come first
-  const int split = id % a.splits;
-  const int item = id / a.splits, h = item / a.tiles;
-  if (h >= a.Hkv) return;
-  const AttnTile w = attn_tile<ATTN_ROWS>(a, a.tiles - 1 - item % a.tiles, split);
+  // Items are (tile, split, head): the last tiles, which attend most, first, and the heads fastest.
+  // Workgroup b runs on XCD b % 8, so an XCD meets only the key heads of one remainder (of 8, or of
+  // what 8 and their number have in common), whose K and V its L2 then holds.
+  const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % a.splits;
+  const AttnTile w = attn_tile<ATTN_ROWS>(a, a.tiles - 1 - rest / a.splits, split);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
     if (split == 0) attn_zero(a, w, h, D);
@@ -439,11 +436,13 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   const int ps = 1 << a.seqs.lp;
   // the thread's 16-byte chunk of each K copy (row krow of its 16 or 32) and of each V copy (channel
   // vrow of 32): its place in LDS is tid, so the swizzle is in what it reads
-  const int krow = tid / KC, kc = (tid % KC) ^ (krow & 7), vrow = tid / 8, vc = (tid % 8) ^ (vrow & 7);
+  const int krow = tid / KC, vrow = tid / 8, vc = (tid % 8) ^ ((vrow >> 1) & 7);
+  const int kc = (tid % KC) ^ (KC == 16 ? krow & 15 : (krow >> 1) & 7);
   const int k16 = KC == 16 ? 0 : wave >> 1;  // group of 16 rows, at D = 64
   const uint32_t koff = (((krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1)) * D + 8 * kc) * 2;  // its row's token
   // The page of the lane's group of 16 tokens, vc / 2, of a step, -1: none: of the present step and the
-  // next. Lanes 0 .. 7 have vc = lane, so lane 2 j has group j's.
+  // next. Lanes 0 .. 7 have vc = lane ^ of_odd: lane 2 j ^ of_odd has group j's.
+  const int of_odd = 4 * (wave & 1);
   int pg, pn, en;  // en: the table entry of the step after the next
   auto entry = [&](int t) {
     const int at = t + 16 * (vc >> 1);
@@ -454,7 +453,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int j = KC == 16 ? i : 2 * i + k16;  // its group of 16 tokens
-      const int p = __builtin_amdgcn_readlane(pn, 2 * j);
+      const int p = __builtin_amdgcn_readlane(pn, (2 * j) ^ of_odd);
       const bf16_t* base = a.k + ((((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((t + 16 * j) & (ps - 1))) * D;
       attn_copy((const char*)base + koff, k_lds + (buf * ATTN_KT * KC + i * ATTN_THREADS) * 16);
     }
@@ -466,7 +465,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   const int low0 = attn_limit(a, w, 0);  // every row of the tile attends the tokens up to here
   const a_u4* const kb0 = &k_s[0][col * KC];
   const a_u4* const vb0 = &v_s[0][col * 8];
-  const int sw = col & 7;
+  const int ksw = KC == 16 ? col & 15 : (col >> 1) & 7, vsw = (col >> 1) & 7;
 
   int t = w.lo, buf = 0;
   entry(t);
@@ -507,7 +506,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
       a_u4 x[2][4];
       auto get = [&](a_u4 (&f)[4], int q) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = kb[32 * (i & 1) * KC + ((2 * (q + (i >> 1)) + e) ^ sw)];
+        for (int i = 0; i < 4; ++i) f[i] = kb[32 * (i & 1) * KC + ((2 * (q + (i >> 1)) + e) ^ ksw)];
       };
       get(x[0], 0);
 #pragma unroll
@@ -520,7 +519,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
       }
     }
     if (on) {
-      const uint64_t have = __ballot(pg >= 0);  // bit 2 j: group j
+      const uint64_t have = __ballot(pg >= 0);  // bit 2 j ^ of_odd: group j
       uint32_t seen = ~0u;
       if (t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != ~0ull) {  // a masked place
         asm volatile("");  // a branch: few steps have one
@@ -530,7 +529,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 #pragma unroll
           for (int q = 0; q < 16; ++q) {
             const int g16 = 2 * b + (q >> 3), tok = t + 16 * g16 + 8 * e + (q & 7);
-            const bool in = tok <= limit && tok < w.hi && ((have >> (2 * g16)) & 1);
+            const bool in = tok <= limit && tok < w.hi && ((have >> ((2 * g16) ^ of_odd)) & 1);
             seen |= in ? 1u << (16 * b + q) : 0u;
             s[b][q] = in ? s[b][q] : -__builtin_inff();
           }
@@ -569,7 +568,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
       a_u4 x[2][MB];
       auto get = [&](a_u4 (&f)[MB], int kk) {
 #pragma unroll
-        for (int b = 0; b < MB; ++b) f[b] = vb[32 * b * 8 + ((2 * kk + e) ^ sw)];
+        for (int b = 0; b < MB; ++b) f[b] = vb[32 * b * 8 + ((2 * kk + e) ^ vsw)];
       };
       get(x[0], 0);
 #pragma unroll
@@ -588,7 +587,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
           for (int q = 0; q < 16; ++q) code[q] = 0.0f;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            const bf16_t* vp = a.v + ((((int64_t)max(__builtin_amdgcn_readlane(pg, 2 * kk), 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
+            const bf16_t* vp = a.v + ((((int64_t)max(__builtin_amdgcn_readlane(pg, (2 * kk) ^ of_odd), 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
                                ((t + 16 * kk) & (ps - 1)) + 8 * e;
             code = mfma32a(attn_code(*(const a_u4*)vp), attn_ones(seen >> (8 * kk)), code);
           }
@@ -683,8 +682,8 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
   p.least = p.rows == ATTN_ROWS ? 512 : 128;
   const int64_t slots = 2 * pp_device_cus(), capacity = (int64_t)max_pages * page_size;
   const int64_t items = std::max<int64_t>(1, (rows / p.rows + n_seqs) * Hkv);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ATTN_MAX_SPLITS, (2 * slots + items - 1) / items,
-                                                          (capacity + p.least - 1) / p.least}));
+  const int64_t want = p.rows == ATTN_ROWS ? (slots + items - 1) / items : (2 * slots + items - 1) / items;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ATTN_MAX_SPLITS, want, (capacity + p.least - 1) / p.least}));
   return p;
 }
 
@@ -731,12 +730,12 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   const int64_t items = p.tiles * Hkv * p.splits;
   PP_REQUIRE(items <= 0x7ffffff0, PP_ERR_UNSUPPORTED, "%s: too many sequences and heads", what);
   hipStream_t st = (hipStream_t)stream;
-  const unsigned n = (unsigned)items, n8 = (n + 7) & ~7u;
+  const unsigned n = (unsigned)items;
 #define ATTN(D_)                                                                          \
   do {                                                                                    \
     if (p.rows == 16) attn_few_kernel<D_, 1><<<n, ATTN_THREADS, 0, st>>>(a);              \
     else if (p.rows == 32) attn_few_kernel<D_, 2><<<n, ATTN_THREADS, 0, st>>>(a);         \
-    else attn_many_kernel<D_><<<n8, ATTN_THREADS, 0, st>>>(a);                            \
+    else attn_many_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                            \
     if (p.splits > 1)                                                                     \
       attn_join_kernel<D_><<<(unsigned)(n_tokens * Hq), ATTN_THREADS, 0, st>>>(a);        \
   } while (0)
