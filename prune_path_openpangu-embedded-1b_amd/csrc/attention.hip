@@ -24,6 +24,7 @@
 // (attn_poison). So stale or foreign data in a page, and a later token's NaN, do not reach a row. A
 // row that attends nothing gives zeros.
 #include <algorithm>
+#include <cmath>
 
 #include "paged.h"
 
@@ -41,7 +42,7 @@ struct AttnArgs {
   int64_t qs[2];  // strides of token and head, in elements
   const bf16_t *k, *v;
   int Hq, Hkv, group;
-  float c;        // |scale| * log2(e): scores in powers of two
+  float c;        // |scale| * log2(e), not 0: scores in powers of two
   uint32_t flip;  // the sign of scale, on both halves of a pair of q
   bf16_t* out;
   int zero_tail;
@@ -166,7 +167,7 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 }
 
 // ------------------------------------------------------------------ few rows
-// Up to 16 NB rows of one key head; the cache bounds it. The four waves take alternate steps of 32
+// Up to 16 rows of one key head; the cache bounds it. The four waves take alternate steps of 32
 // tokens, each with its own m, l and o, and join them at the end through LDS. K and V operands come
 // straight from memory into registers. The next step's K is asked for once the present one's scores
 // are computed, its V after the second product, so a wave always has one of the two in flight with
@@ -175,9 +176,9 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // lane group g = lane / 16 with the scores of tokens 8 g .. 8 g + 7: its k of the second product.
 // P enters as a sum of two bf16 values (the rounded one and what is left, 2^-17 of it): the second
 // product costs nothing next to the loads.
-template <int D, int NB>
-__global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel(AttnArgs a) {
-  constexpr int R = 16 * NB, KS = D / 32, MB = D / 16, OS = D + 4;
+template <int D>
+__global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
+  constexpr int R = 16, KS = D / 32, MB = D / 16, OS = D + 4;
   __shared__ float o_s[4][R][OS];
   __shared__ float ml_s[4][R][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
@@ -226,41 +227,32 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
   load_k(t);
   load_v(t);
 
-  a_u4 qf[NB][KS];
-  int limit[NB];
+  a_u4 qf[KS];
+  const bool in = col < w.nr;
+  const int limit = in ? attn_limit(a, w, col) : a.seqs.capacity();
+  {
+    const int i = (w.r0 + col) / a.group;
+    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + col - i * a.group) * a.qs[1];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int r = 16 * n + col;
-    const bool in = r < w.nr;
-    limit[n] = in ? attn_limit(a, w, r) : a.seqs.capacity();
-    const int i = (w.r0 + r) / a.group;
-    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[n][s] = in ? *(const a_u4*)(src + 32 * s + 8 * g) ^ a.flip : a_mk(0, 0, 0, 0);
+    for (int s = 0; s < KS; ++s) qf[s] = in ? *(const a_u4*)(src + 32 * s + 8 * g) ^ a.flip : a_mk(0, 0, 0, 0);
   }
   const int low = attn_limit(a, w, 0);  // every row attends the tokens up to here
 
-  f32x4_t o[NB][MB];
-  float m[NB], l[NB];
+  f32x4_t o[MB];
+  float m = ATTN_LOW, l = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    m[n] = ATTN_LOW, l[n] = 0.0f;
-#pragma unroll
-    for (int b = 0; b < MB; ++b) o[n][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int b = 0; b < MB; ++b) o[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
   for (; t < w.hi; t += 128) {
     pages();
     entries(t + 256);
-    f32x4_t s[NB][2];
+    f32x4_t s[2];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        s[n][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int q = 0; q < KS; ++q) s[n][b] = mfma16(kf[b][q], qf[n][q], s[n][b]);
-      }
+      for (int q = 0; q < KS; ++q) s[b] = mfma16(kf[b][q], qf[q], s[b]);
+    }
     const bool more = t + 128 < w.hi;
     if (more) load_k(t + 128);
     // whether a place of the step is masked for any row (wave-uniform)
@@ -276,73 +268,65 @@ __global__ __launch_bounds__(ATTN_THREADS, NB == 1 ? 3 : 2) void attn_few_kernel
         for (int b = 0; b < MB; ++b) vf[b] = attn_clean(vf[b]);
       }
     }
+    float p[8];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float p[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = s[n][j >> 2][j & 3];
-      uint32_t seen = 0xffu;
-      if (part) {
-        asm volatile("");  // a branch: few steps have one
-        seen = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = pc >= 0 && t + gv + j <= limit[n] && t + gv + j < w.hi;
-          seen |= in ? 1u << j : 0u;
-          p[j] = in ? p[j] : -__builtin_inff();
-        }
-      }
-      float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-      top = fmaxf(top, pl_xor16f(top, lane));
-      top = fmaxf(top, pl_xor32f(top, lane));
-      const float mn = fmaxf(m[n], top * a.c), shrink = attn_exp2(m[n] - mn);
-      m[n] = mn;
-      float sum = 0.0f;
+    for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3];
+    uint32_t seen = 0xffu;
+    if (part) {
+      asm volatile("");  // a branch: few steps have one
+      seen = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        p[j] = attn_exp2(__fmaf_rn(p[j], a.c, -mn));
-        sum += p[j];
+        const bool in = pc >= 0 && t + gv + j <= limit && t + gv + j < w.hi;
+        seen |= in ? 1u << j : 0u;
+        p[j] = in ? p[j] : -__builtin_inff();
       }
-      l[n] = __fmaf_rn(l[n], shrink, sum);
-      uint32_t hi[4], lo[4];
+    }
+    float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    top = fmaxf(top, pl_xor16f(top, lane));
+    top = fmaxf(top, pl_xor32f(top, lane));
+    const float mn = fmaxf(m, top * a.c), shrink = attn_exp2(m - mn);
+    m = mn;
+    float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        hi[j] = f32_to_bf16x2(p[2 * j], p[2 * j + 1]);
-        lo[j] = f32_to_bf16x2(p[2 * j] - __uint_as_float(hi[j] << 16), p[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
-      }
-      const a_u4 ph = a_mk(hi[0], hi[1], hi[2], hi[3]), pl = a_mk(lo[0], lo[1], lo[2], lo[3]);
+    for (int j = 0; j < 8; ++j) {
+      p[j] = attn_exp2(__fmaf_rn(p[j], a.c, -mn));
+      sum += p[j];
+    }
+    l = __fmaf_rn(l, shrink, sum);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      hi[j] = f32_to_bf16x2(p[2 * j], p[2 * j + 1]);
+      lo[j] = f32_to_bf16x2(p[2 * j] - __uint_as_float(hi[j] << 16), p[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
+    }
+    const a_u4 ph = a_mk(hi[0], hi[1], hi[2], hi[3]), pl = a_mk(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      o[b] *= shrink;
+      o[b] = mfma16(vf[b], ph, o[b]);
+      o[b] = mfma16(vf[b], pl, o[b]);
+    }
+    if (bad) {  // what was taken out of V, read again, for the rows that attend it
+      const a_u4 one = attn_ones(seen);
+      const bf16_t* vp = at_v(pc, t);
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
-        o[n][b] *= shrink;
-        o[n][b] = mfma16(vf[b], ph, o[n][b]);
-        o[n][b] = mfma16(vf[b], pl, o[n][b]);
-      }
-      if (bad) {  // what was taken out of V, read again, for the rows that attend it
-        const a_u4 one = attn_ones(seen);
-        const bf16_t* vp = at_v(pc, t);
+        const a_u4 x = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+        const f32x4_t code = mfma16(attn_code(x), one, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-          const a_u4 x = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
-          const f32x4_t code = mfma16(attn_code(x), one, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][b][i] = attn_poison(o[n][b][i], code[i]);
-        }
+        for (int i = 0; i < 4; ++i) o[b][i] = attn_poison(o[b][i], code[i]);
       }
     }
     if (more) load_v(t + 128);
   }
 
   // the four waves' rows joined
+  l += pl_xor16f(l, lane);
+  l += pl_xor32f(l, lane);
+  if (g == 0) ml_s[wave][col][0] = m, ml_s[wave][col][1] = l;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    float sum = l[n];
-    sum += pl_xor16f(sum, lane);
-    sum += pl_xor32f(sum, lane);
-    const int r = 16 * n + col;
-    if (g == 0) ml_s[wave][r][0] = m[n], ml_s[wave][r][1] = sum;
-#pragma unroll
-    for (int b = 0; b < MB; ++b) *(f32x4_t*)&o_s[wave][r][16 * b + 4 * g] = o[n][b];
-  }
+  for (int b = 0; b < MB; ++b) *(f32x4_t*)&o_s[wave][col][16 * b + 4 * g] = o[b];
   __syncthreads();
   for (int k = tid; k < w.nr * (D / 8); k += ATTN_THREADS) {
     const int r = k / (D / 8), d = 8 * (k - r * (D / 8));
@@ -468,6 +452,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
   const int ksw = KC == 16 ? col & 15 : (col >> 1) & 7, vsw = (col >> 1) & 7;
 
   int t = w.lo, buf = 0;
+  if (tid < 2) bad_s[tid] = -1;
   entry(t);
   pn = a.seqs.page(en);
   entry(t + ATTN_KT);
@@ -481,8 +466,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
       entry(t + 2 * ATTN_KT);
       load(t + ATTN_KT, buf ^ 1);
     }
-    // a step with a masked place: only the finite part of V, and a mark where there is another (a mark
-    // by chance, before the first, costs a product of zeros)
+    // a step with a masked place: only the finite part of V, and a mark where there is another
     if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(pg < 0)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -509,6 +493,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
         for (int i = 0; i < 4; ++i) f[i] = kb[32 * (i & 1) * KC + ((2 * (q + (i >> 1)) + e) ^ ksw)];
       };
       get(x[0], 0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int q = 0; q < D / 16; q += 2) {
         if (q + 2 < D / 16) get(x[((q >> 1) + 1) & 1], q + 2);
@@ -517,6 +502,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
         for (int i = 0; i < 4; ++i) s[i & 1] = mfma32a(x[(q >> 1) & 1][i], qf[q + (i >> 1)], s[i & 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     if (on) {
       const uint64_t have = __ballot(pg >= 0);  // bit 2 j ^ of_odd: group j
@@ -551,34 +537,39 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
           for (int q = 0; q < 16; ++q) o[b][q] *= shrink;
         m = mn;
       }
-      a_u4 pf[4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t p2[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int q = 8 * (kk & 1) + 2 * j;
-          const float x = attn_exp2(__fmaf_rn(s[kk >> 1][q], a.c, -m)), y = attn_exp2(__fmaf_rn(s[kk >> 1][q + 1], a.c, -m));
-          l += x + y;
-          p2[j] = f32_to_bf16x2(x, y);
-        }
-        pf[kk] = a_mk(p2[0], p2[1], p2[2], p2[3]);
-      }
+      // the second product, 16 tokens at a time: a product's time is that of a few of the next tokens'
+      // exponentials, which stand between the products
       const a_u4* const vb = vb0 + buf * (D * 8);
-      a_u4 x[2][MB];
+      a_u4 x[2][MB], pf[2];
       auto get = [&](a_u4 (&f)[MB], int kk) {
 #pragma unroll
         for (int b = 0; b < MB; ++b) f[b] = vb[32 * b * 8 + ((2 * kk + e) ^ vsw)];
       };
+      auto weigh = [&](int kk, int j) {  // P of tokens 2 j and 2 j + 1 of 8
+        const float u = s[kk >> 1][8 * (kk & 1) + 2 * j], v = s[kk >> 1][8 * (kk & 1) + 2 * j + 1];
+        const float p0 = attn_exp2(__fmaf_rn(u, a.c, -m)), p1 = attn_exp2(__fmaf_rn(v, a.c, -m));
+        l += p0 + p1;
+        pf[kk & 1][j] = f32_to_bf16x2(p0, p1);
+      };
       get(x[0], 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) weigh(0, j);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         if (kk < 3) get(x[(kk + 1) & 1], kk + 1);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) o[b] = mfma32a(x[kk & 1][b], pf[kk], o[b]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int b = 0; b < MB; ++b) {
+          __builtin_amdgcn_sched_barrier(0);
+          o[b] = mfma32a(x[kk & 1][b], pf[kk & 1], o[b]);
+          if (kk < 3) {
+#pragma unroll
+            for (int j = b * 4 / MB; j < (b + 1) * 4 / MB; ++j) weigh(kk + 1, j);
+          }
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(0);
       if (__builtin_amdgcn_readfirstlane(bad_s[buf]) == t) {  // what was taken out of V, read again, for the rows that attend it
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
@@ -627,62 +618,88 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) 
 }
 
 // ------------------------------------------------------------------ join
-// One workgroup per row (token and query head): lane i of a wave holds the weight of range i, the
-// waves take alternate ranges and are added in wave order.
+// D / 4 threads per row (token and query head), four channels each. With few ranges a workgroup takes
+// as many rows as fit (ALONE); with many it takes one row, its groups of threads alternate ranges,
+// added in order through LDS.
 #define ATTN_MAX_SPLITS 64
+#define ATTN_JOIN_ALONE 8  // ranges up to which a row's threads add them alone
 
-template <int D>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(AttnArgs a) {
-  constexpr int W = D / 64;
-  __shared__ float acc_s[4][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
-  const int ns = min(a.pns[row], a.splits);
-  if (ns <= 1) return;  // written already
-  float m = ATTN_LOW, l = 0.0f;
-  if (lane < ns) {
-    const float2 ml = *(const float2*)(a.pml + (row * a.splits + lane) * 2);
-    m = ml.x, l = ml.y;
+template <int D, bool ALONE>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(AttnArgs a, int64_t rows) {
+  constexpr int T = D / 4, G = ATTN_THREADS / T;
+  const int g = threadIdx.x / T, d = 4 * (threadIdx.x % T);
+  const int64_t row = ALONE ? (int64_t)blockIdx.x * G + g : blockIdx.x;
+  const int ns = row < rows ? min(a.pns[row], a.splits) : 0;
+  if (ns <= 1) return;  // written already (ALONE: no barrier follows; otherwise one row, one answer)
+  const float2* const ml = (const float2*)a.pml + row * a.splits;
+  const float* const from = a.po + row * a.splits * D + d;
+  float m = ATTN_LOW;
+  for (int i = 0; i < ns; ++i) m = fmaxf(m, ml[i].x);
+  float l = 0.0f;
+  f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = ALONE ? 0 : g; i < ns; i += ALONE ? 1 : G) {
+    const float2 x = ml[i];
+    const float f = attn_exp2(x.x - m);
+    const f32x4_t p = *(const f32x4_t*)(from + (int64_t)i * D);
+    l = __fmaf_rn(x.y, f, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = __fmaf_rn(p[j], f, acc[j]);
   }
-  const float top = wave_max(m);  // every lane takes part
-  const float f = lane < ns ? attn_exp2(m - top) : 0.0f;
-  const float sum = wave_sum(f * l);
-  float acc[W] = {};
-  const float* from = a.po + row * a.splits * D + lane * W;
-#pragma unroll 2
-  for (int i = wave; i < ns; i += 4) {
-    const float x = __shfl(f, i, PP_WAVE);
-#pragma unroll
-    for (int j = 0; j < W; ++j) acc[j] = __fmaf_rn(from[(int64_t)i * D + j], x, acc[j]);
+  if (!ALONE) {
+    __shared__ f32x4_t acc_s[G][T];
+    __shared__ float l_s[G];
+    acc_s[g][d / 4] = acc;
+    if (d == 0) l_s[g] = l;
+    __syncthreads();
+    if (g) return;
+    for (int i = 1; i < G; ++i) {
+      acc += acc_s[i][d / 4];
+      l += l_s[i];
+    }
   }
-#pragma unroll
-  for (int j = 0; j < W; ++j) acc_s[wave][lane * W + j] = acc[j];
-  __syncthreads();
-  const int d = 2 * threadIdx.x;
-  if (d >= D) return;
-  float x = acc_s[0][d], y = acc_s[0][d + 1];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) x += acc_s[i][d], y += acc_s[i][d + 1];
-  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-  *(uint32_t*)(a.out + row * D + d) = f32_to_bf16x2(x * inv, y * inv);
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  *(uint2*)(a.out + row * D + d) = make_uint2(f32_to_bf16x2(acc[0] * inv, acc[1] * inv), f32_to_bf16x2(acc[2] * inv, acc[3] * inv));
 }
 
 // ------------------------------------------------------------------ host
 struct AttnPlan {
-  int rows;    // per tile: 16, 32 or ATTN_ROWS
+  int rows;    // per tile: 16 or ATTN_ROWS
   int splits, least;
   int64_t tiles;
 };
 
-static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv) {
+static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv, int D) {
   AttnPlan p;
-  const int64_t group = Hq / Hkv, rows = n_tokens * group, each = rows / std::max(n_seqs, 1);
-  p.rows = each <= 16 ? 16 : each <= 32 ? 32 : ATTN_ROWS;
+  const int64_t rows = n_tokens * (Hq / Hkv), cus = pp_device_cus(), capacity = (int64_t)max_pages * page_size;
+  auto items = [&](int tile) { return std::max<int64_t>(1, (rows / tile + n_seqs) * Hkv); };
+  // Tiles of 16 rows for single tokens and the like, and for what is short altogether: their steps
+  // cost four times as much for the same work (6 ns for 16 rows x 128 tokens of D = 128, the whole GPU
+  // at work, against 1.4), but there are eight times as many tiles. 12 heads: prompts of 128, 256, 512
+  // and 1024 tokens 6.3, 7.7, 12.0 and 26.2 us, tiles of 128 rows 10.5, 13.9, 17 to 20 and 26.1;
+  // 32 sequences of 4 x 8 rows at 8191 tokens 134 us against 108.
+  const bool few = rows <= 16 * (int64_t)n_seqs || items(16) * ((capacity + 127) / 128) <= 4096;
+  p.rows = few ? 16 : ATTN_ROWS;
   p.tiles = rows / p.rows + n_seqs + 1;
-  p.least = p.rows == ATTN_ROWS ? 512 : 128;
-  const int64_t slots = 2 * pp_device_cus(), capacity = (int64_t)max_pages * page_size;
-  const int64_t items = std::max<int64_t>(1, (rows / p.rows + n_seqs) * Hkv);
-  const int64_t want = p.rows == ATTN_ROWS ? (slots + items - 1) / items : (2 * slots + items - 1) / items;
+  p.least = few ? 128 : 512;
+  const int64_t each = items(p.rows);
+  int64_t want;
+  if (few) {
+    // As many ranges as give every CU one, and at least one per 1024 tokens of the table, so that
+    // sequences of different lengths even out; none in a table of 384, where the join costs more. 12
+    // heads, one token: 256, 512, 1024, 2048, 4096 tokens 7.0, 9.2, 13.5, 22.3, 40.6 us, in ranges of
+    // 128 8.1, 8.2, 8.8, 9.4, 12.1; 16 sequences of 1024 19.2, in 6 ranges 22.9; 64 of 1 to 8192 tokens
+    // 343 us, in 2, 8, 32 ranges 300, 271, 347.
+    want = capacity <= 384 ? 1 : std::max(cus / each, capacity / 1024);
+  } else {
+    // One round of the workgroups that the GPU holds (2 per CU at D = 128, 3 at D = 64). The tiles of a
+    // prompt differ in length, so a part of a round more does no harm while there are few ranges; with
+    // many it is a round of its own. us for 1, 2, 3, 4 ranges: prompts of 2048 tokens (204 items) 64,
+    // 48, 42, 53; of 4096 (396) 120, 89, 96, 105; of 8192 (780) 255, 267, 305, 310; for 6, 8, 12: 512
+    // new tokens at 30000 (60 items) 179, 142, 184, of D = 64 (128 items) 168, 194, 187.
+    const int64_t slots = (D == 64 ? 3 : 2) * cus;
+    want = slots / each >= 4 ? slots / each : (slots + each - 1) / each;
+  }
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ATTN_MAX_SPLITS, want, (capacity + p.least - 1) / p.least}));
   return p;
 }
@@ -695,7 +712,7 @@ static size_t attn_ws_bytes(const AttnPlan& p, int64_t rows, int D) {
 extern "C" size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size,
                                                      int Hq, int Hkv, int D) {
   if (n_tokens <= 0 || n_seqs < 0 || max_pages < 1 || page_size < 1 || Hkv < 1 || Hq < Hkv || D < 1) return 0;
-  return attn_ws_bytes(attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv), n_tokens * Hq, D);
+  return attn_ws_bytes(attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D), n_tokens * Hq, D);
 }
 
 extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs,
@@ -712,7 +729,8 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   PP_REQUIRE(q && q_strides && out_bf16, PP_ERR_INVALID, "%s: null pointer", what);
   PP_REQUIRE((((uintptr_t)q | (uintptr_t)out_bf16) & 15) == 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0,
              PP_ERR_INVALID, "%s: every head of q and out must start on a 16-byte boundary", what);
-  const AttnPlan p = attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv);
+  PP_REQUIRE(std::isfinite(scale), PP_ERR_INVALID, "%s: scale %g", what, scale);
+  const AttnPlan p = attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D);
   const size_t need = attn_ws_bytes(p, n_tokens * Hq, D);
   PP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PP_ERR_INVALID,
              "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes, need);
@@ -721,7 +739,7 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.q = (const bf16_t*)q, a.qs[0] = q_strides[0], a.qs[1] = q_strides[1];
   a.k = (const bf16_t*)k_pages, a.v = (const bf16_t*)v_pages;
   a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv;
-  a.c = fabsf(scale) * 1.4426950408889634f, a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.c = std::max(fabsf(scale) * 1.4426950408889634f, 1e-37f), a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
   a.splits = p.splits, a.least = p.least, a.tiles = (int)p.tiles;
   a.po = (float*)workspace;
@@ -731,13 +749,15 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   PP_REQUIRE(items <= 0x7ffffff0, PP_ERR_UNSUPPORTED, "%s: too many sequences and heads", what);
   hipStream_t st = (hipStream_t)stream;
   const unsigned n = (unsigned)items;
+  const int64_t rows = n_tokens * Hq;
 #define ATTN(D_)                                                                          \
   do {                                                                                    \
-    if (p.rows == 16) attn_few_kernel<D_, 1><<<n, ATTN_THREADS, 0, st>>>(a);              \
-    else if (p.rows == 32) attn_few_kernel<D_, 2><<<n, ATTN_THREADS, 0, st>>>(a);         \
+    if (p.rows == 16) attn_few_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                 \
     else attn_many_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                            \
-    if (p.splits > 1)                                                                     \
-      attn_join_kernel<D_><<<(unsigned)(n_tokens * Hq), ATTN_THREADS, 0, st>>>(a);        \
+    if (p.splits > ATTN_JOIN_ALONE)                                                       \
+      attn_join_kernel<D_, false><<<(unsigned)rows, ATTN_THREADS, 0, st>>>(a, rows);      \
+    else if (p.splits > 1)                                                                \
+      attn_join_kernel<D_, true><<<(unsigned)((rows * (D_ / 4) + ATTN_THREADS - 1) / ATTN_THREADS), ATTN_THREADS, 0, st>>>(a, rows); \
   } while (0)
   if (D == 64) ATTN(64);
   else ATTN(128);

@@ -227,8 +227,11 @@ def attend64(b, q, scale=None):
 
 
 def few(b, hq, hkv):
-    """Whether the call takes the small tiles, where P enters as two bf16 values."""
-    return b.n * (hq // hkv) // max(len(b.new), 1) <= 32
+    """Whether the call takes the small tiles, where P enters as two bf16 values: at most 16 rows a
+    sequence, or little work by what the table could hold."""
+    rows = b.n * (hq // hkv)
+    work = max(1, rows // 16 + len(b.new)) * hkv * -(-b.table.shape[1] * b.page // 128)
+    return rows <= 16 * len(b.new) or work <= 4096
 
 
 def check_attention(got, o, big, small):
@@ -248,9 +251,14 @@ ATT = [  # new, total, page, heads, kv_heads, dim
     ([33, 0, 40], [33, 50, 41], 16, 5, 1, 128), ([150], [2000], 256, 1, 1, 64), ([0, 0, 1], [5, 0, 5], 16, 2, 1, 128)]
 
 
+LONG = 1 << 20  # tokens that a table has room for beyond what is used: the large tiles where there are more than 16 rows
+
+
+@pytest.mark.parametrize("room", [0, LONG], ids=["", "long-table"])
 @pytest.mark.parametrize("new,total,page,heads,kv_heads,dim", ATT)
-def test_paged_attention(pkg, new, total, page, heads, kv_heads, dim):
-    b = Batch(new, total, page, kv_heads, dim, seed=len(new) + page)
+def test_paged_attention(pkg, new, total, page, heads, kv_heads, dim, room):
+    b = Batch(new, total, page, kv_heads, dim, seed=len(new) + page, extra=2 + room // page)
+    assert few(b, heads, kv_heads) == (room == 0 or b.n * (heads // kv_heads) <= 16 * len(new))
     q = (2 * torch.randn(b.n, heads, dim, generator=gen(dim))).to(torch.bfloat16)
     print(new, total, page, heads, kv_heads, dim, flush=True)
     got = pkg.ops.paged_attention(q.to(dev()), *b.gpu())
@@ -265,6 +273,8 @@ def test_attention_lengths_and_tables_that_hold_no_token(pkg):
     of -1 and beyond the cache in the middle: those tokens are not attended, empty rows are zero."""
     for new, total in (([3, 2, 4, 1], [1, 0, 300, 90]), ([60, 80, 50, 70], [40, 0, 400, 100])):
         b = Batch(new, total, 16, 2, 128, seed=3, extra=0)
+        if new[0] > 3:
+            b.table = torch.cat([b.table, torch.full((4, LONG // 16), -1, dtype=torch.int32)], 1)
         b.table[2, 2], b.table[2, 5], b.table[3, 0] = -1, b.pages, -7
         if new[0] == 3:
             b.table[3, :] = -1  # a row with no page at all
@@ -277,12 +287,13 @@ def test_attention_lengths_and_tables_that_hold_no_token(pkg):
         assert bool((got[:new[0] - total[0]] == 0).all()) and not bool(torch.isnan(got).any())
 
 
-@pytest.mark.parametrize("new,total", [([5, 3], [70, 3]), ([70, 60], [90, 400])])
-def test_attention_masked_places_do_not_reach_a_row(pkg, new, total):
+@pytest.mark.parametrize("new,total,room", [([5, 3], [70, 3], 0), ([70, 60], [90, 400], 0), ([70, 60], [90, 400], LONG)])
+def test_attention_masked_places_do_not_reach_a_row(pkg, new, total, room):
     """NaN and infinities in the places behind a sequence's end, in pages of other sequences and in
     later tokens' keys and values: earlier rows are as if they were not there; rows that attend them
     are not finite in the channels of V that are not."""
-    b = Batch(new, total, 32, 2, 64, seed=9)
+    b = Batch(new, total, 32, 2, 64, seed=9, extra=2 + room // 32)
+    assert few(b, 2, 2) == (room == 0)
     q = torch.randn(b.n, 2, 64, generator=gen(2)).to(torch.bfloat16)
     clean, big = attend64(b, q)
     for s, t in enumerate(total):  # behind the end
@@ -314,8 +325,8 @@ def test_attention_masked_places_do_not_reach_a_row(pkg, new, total):
 
 
 def test_attention_rows_behind_the_last_sequence(pkg):
-    for new, total in (([2, 1], [40, 33]), ([70, 66], [70, 200])):
-        b = Batch(new, total, 16, 1, 128, seed=4)
+    for new, total, room in (([2, 1], [40, 33], 0), ([70, 66], [70, 200], 0), ([70, 66], [70, 200], LONG)):
+        b = Batch(new, total, 16, 1, 128, seed=4, extra=2 + room // 16)
         q = torch.randn(b.n + 9, 2, 128, generator=gen(3)).to(torch.bfloat16).to(dev())
         got = pkg.ops.paged_attention(q, *b.gpu())
         o, big = attend64(b, q[:b.n].cpu())
@@ -340,12 +351,21 @@ def test_attention_strided_queries_scale_and_shared_pages(pkg):
     check_attention(got, *attend64(b, qkv[:, 2:6], 0.25), True)
     got = pkg.ops.paged_attention(q, *b.gpu(), scale=-0.05)
     check_attention(got, *attend64(b, qkv[:, 2:6], -0.05), True)
+    got = pkg.ops.paged_attention(q, *b.gpu(), scale=0.0)
+    check_attention(got, *attend64(b, qkv[:, 2:6], 0.0), True)
+    with pytest.raises(RuntimeError, match="scale"):
+        pkg.ops.paged_attention(q, *b.gpu(), scale=float("inf"))
+    b = Batch([70], [150], 16, 2, 128, seed=5, extra=LONG // 16)
+    qkv = torch.randn(70, 8, 128, generator=gen(6)).to(torch.bfloat16)
+    for scale in (0.25, -0.05, 0.0):
+        got = pkg.ops.paged_attention(qkv.to(dev())[:, 2:6], *b.gpu(), scale=scale)
+        check_attention(got, *attend64(b, qkv[:, 2:6], scale), False)
 
 
 def test_attention_large_scores(pkg):
     """Scores far beyond the exponential's range: one token takes all, whichever step it is in."""
-    for new, total in (([1, 1], [300, 45]), ([40, 50], [300, 50])):
-        b = Batch(new, total, 16, 1, 64, seed=6)
+    for new, total, room in (([1, 1], [300, 45], 0), ([40, 50], [300, 50], LONG)):
+        b = Batch(new, total, 16, 1, 64, seed=6, extra=2 + room // 16)
         q = torch.randn(b.n, 1, 64, generator=gen(7)).to(torch.bfloat16) * 100
         b.k *= 100
         o, big = attend64(b, q)
@@ -536,7 +556,7 @@ def test_two_graphs_and_two_streams(pkg):
     ops = pkg.ops
     cases = []
     for seed, (new, total, hq) in enumerate([([1], [3000], 2), ([1, 1], [2000, 900], 4), ([140], [2500], 2)]):
-        b = Batch(new, total, 16, 2, 128, seed=seed)
+        b = Batch(new, total, 16, 2, 128, seed=seed, extra=LONG // 16)
         q = torch.randn(b.n, hq, 128, generator=gen(seed)).to(torch.bfloat16).to(dev())
         args = b.gpu()
         cases.append((q, args, ops.paged_attention(q, *args).clone()))
