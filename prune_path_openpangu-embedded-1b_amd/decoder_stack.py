@@ -12,9 +12,15 @@ decode benchmark (src/evaluation_triton.py:403-460). ``run`` reports the prefill
 the cache -- replayed ``steps`` times, once with and once without the MoE-MLP, so the
 MoE share is device time rather than host dispatch.
 
-Attention is plain torch with contiguous right operands (the K cache is kept
+The attention of ``run`` is plain torch with contiguous right operands (the K cache is kept
 transposed, so no transposed view enters a batched bf16 product); it is harness, not
 part of the hot path.
+
+Several sequences of different lengths are served through a paged cache instead
+(``PagedKV``, ``generate``): the new tokens of all of them are packed on one axis, each
+layer appends their keys and values with the rotation on the way (``ops.kv_append``) and
+attends over the pages (``ops.paged_attention``). Prompts go in in chunks, then one greedy
+step of the whole batch is captured and replayed.
 """
 from __future__ import annotations
 
@@ -103,6 +109,31 @@ class Attention(nn.Module):
         return self.o(o.transpose(1, 2).reshape(B, L, D))
 
 
+    def forward_paged(self, x, kv: "PagedKV", layer: int, cu_q):
+        """The packed new tokens x [N, d] of ``kv``'s sequences (rows cu_q[s] .. cu_q[s + 1] of
+        sequence s, already counted in ``kv.lens``) over the paged cache."""
+        qkv = self.qkv(x).view(-1, 3, self.h, self.hd)
+        cache = (*kv.pages[layer], kv.table, kv.lens, cu_q)
+        q = ops.kv_append(qkv[:, 1], qkv[:, 2], *cache, inv_freq=kv.inv_freq, q=qkv[:, 0])
+        return self.o(ops.paged_attention(q, *cache).view(x.shape[0], -1))
+
+
+class PagedKV:
+    """The paged cache of every layer for ``seqs`` sequences of up to ``max_len`` tokens: pages of
+    ``page_size`` tokens, a block table that gives each sequence its own (scattered, as an
+    allocator would leave them), and the lengths, all on the device."""
+
+    def __init__(self, layers: int, seqs: int, max_len: int, heads: int, head_dim: int, page_size: int = 16,
+                 device="cuda:0"):
+        per = -(-max_len // page_size)
+        self.max_len = max_len
+        self.table = torch.arange(seqs * per, dtype=torch.int32, device=device).view(per, seqs).t().contiguous()
+        self.pages = [ops.paged_cache(seqs * per, page_size, heads, head_dim, device) for _ in range(layers)]
+        self.lens = torch.zeros(seqs, dtype=torch.int32, device=device)
+        self.one_each = torch.arange(seqs + 1, dtype=torch.int32, device=device)  # cu_q of a decode step
+        self.inv_freq, _ = ops.rotary_frequencies(head_dim, device=device)
+
+
 class Block(nn.Module):
     def __init__(self, cfg, args, max_len: int):
         super().__init__()
@@ -129,6 +160,10 @@ class Block(nn.Module):
         # without the MoE-MLP the step keeps the norm and the residual add, so the
         # difference of the two step times is the MoE-MLP call alone
         return x + (self.mlp(h) if moe else h)
+
+    def forward_paged(self, x, kv, layer: int, cu_q):
+        x = x + self.self_attn.forward_paged(self.input_layernorm(x), kv, layer, cu_q)
+        return x + self.mlp(self.post_attention_layernorm(x)[None])[0]
 
 
 class DecoderStack(nn.Module):
@@ -180,6 +215,62 @@ class DecoderStack(nn.Module):
             finite_t.logical_and_(torch.isfinite(logits).all().view(1))
         tok_t.copy_(logits.argmax(-1))
         pos_t.add_(1)
+
+    def forward_paged(self, ids, kv: PagedKV, cu_q):
+        """Hidden states [N, d] of the packed new tokens ids [N] (``kv.lens`` counts them)."""
+        x = self.embed_tokens(ids)
+        for i, blk in enumerate(self.layers):
+            x = blk.forward_paged(x, kv, i, cu_q)
+        return x
+
+    def step_paged(self, tok_t, kv: PagedKV):
+        """One greedy step of every sequence of ``kv`` on device state: its last token, tok_t [seqs],
+        becomes its next one."""
+        kv.lens.add_(1)
+        tok_t.copy_(self.lm_head(self.norm(self.forward_paged(tok_t, kv, kv.one_each))).argmax(-1))
+
+
+@torch.no_grad()
+def generate(model: DecoderStack, prompts: List[torch.Tensor], steps: int, chunk: int = 512, page_size: int = 16,
+             capture: bool = True) -> torch.Tensor:
+    """Greedy tokens [seqs, steps] for prompts (int64 id tensors [length >= 1]) of any lengths, served
+    together: the prompts in calls of at most ``chunk`` tokens of each, then ``steps - 1`` decode
+    steps of the batch (the step captured in a graph and replayed, or eager). ``model`` in eval mode,
+    reordered for inference, with attention heads of 64 or 128 channels."""
+    lengths = [int(p.numel()) for p in prompts]
+    if steps < 1 or not prompts or min(lengths) < 1:
+        raise ValueError("generate: at least one step and prompts of at least one token")
+    dev, attn = model.embed_tokens.weight.device, model.layers[0].self_attn
+    kv = PagedKV(len(model.layers), len(prompts), max(lengths) + steps, attn.h, attn.hd, page_size, dev)
+    tok_t = torch.zeros(len(prompts), dtype=torch.int64, device=dev)
+    for at in range(0, max(lengths), chunk):
+        new = [min(max(n - at, 0), chunk) for n in lengths]
+        cu = torch.tensor([0] + new, dtype=torch.int64).cumsum(0)
+        ids = torch.cat([p[at:at + n].to(dev) for p, n in zip(prompts, new)])
+        kv.lens.add_(torch.tensor(new, dtype=torch.int32, device=dev))
+        x = model.forward_paged(ids, kv, cu.to(device=dev, dtype=torch.int32))
+        done = [s for s, n in enumerate(new) if n and at + n == lengths[s]]
+        if done:
+            last = (cu[1:] - 1)[done].to(dev)
+            tok_t[torch.tensor(done, device=dev)] = model.lm_head(model.norm(x[last])).argmax(-1)
+    out = [tok_t.clone()]
+    graph = None
+    if capture and steps > 2:
+        lens, first = kv.lens.clone(), tok_t.clone()
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):  # warm-up outside the graph (allocator, kernels), then taken back
+            model.step_paged(tok_t, kv)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            model.step_paged(tok_t, kv)
+        kv.lens.copy_(lens)
+        tok_t.copy_(first)
+    for _ in range(steps - 1):
+        graph.replay() if graph is not None else model.step_paged(tok_t, kv)
+        out.append(tok_t.clone())
+    return torch.stack(out, 1)
 
 
 @torch.no_grad()
