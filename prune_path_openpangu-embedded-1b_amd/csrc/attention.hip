@@ -68,14 +68,14 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int 
   AttnTile w;
   const int g = a.group;
   auto first = [g](int c, int s) { return (int64_t)c * g / R + s; };
-  w.s = paged_seq_of(a.seqs, t, first);
-  w.c0 = a.seqs.start(w.s);
-  const int len = max(a.seqs.start(w.s + 1) - w.c0, 0);
+  const PagedSeq f = paged_find(a.seqs, t, first);
+  w.s = f.s, w.c0 = f.c0;
+  const int len = f.rows;
   const int64_t r0 = (t - first(w.c0, w.s)) * R;
   w.nr = r0 < 0 ? 0 : (int)max((int64_t)0, min((int64_t)R, (int64_t)len * g - r0));  // < 0: offsets out of order
   w.r0 = (int)max((int64_t)0, min(r0, (int64_t)len * g));
   const bool tail = w.s == a.seqs.n_seqs;
-  w.p0 = tail ? -(int64_t)len : (int64_t)a.seqs.kv_lens[w.s] - len;
+  w.p0 = tail ? -(int64_t)len : (int64_t)f.len - len;
   w.nt = (int)max((int64_t)0, min(w.p0 + (w.r0 + max(w.nr, 1) - 1) / g + 1, (int64_t)a.seqs.capacity()));
   // equal ranges of whole steps, none of them empty
   const int cut = max(1, min(a.splits, (w.nt + a.least - 1) / a.least));

@@ -41,20 +41,47 @@ struct PagedSeqs {
 
 // The sequence that work item t belongs to, where sequence s has the items first(start(s), s)
 // and on: the last s with first(start(s), s) <= t. `first` grows with s, by at least the items that
-// the sequence has, so the item space needs no prefix sum. One load per 64 sequences; every wave
-// finds it for itself. A result in [0, n_seqs], also for offsets out of order.
+// the sequence has, so the item space needs no prefix sum. Every wave finds it for itself, 256
+// sequences at a time: offsets and lengths come in one round of loads, and those of the sequence
+// found are taken from the lanes that have them. s is in [0, n_seqs], also for offsets out of order;
+// the rows of no sequence are number n_seqs, of length 0.
+struct PagedSeq {
+  int s, c0, rows;  // its number, its first row, how many rows
+  int len;          // its tokens in the cache
+};
 template <typename F>
-__device__ __forceinline__ int paged_seq_of(const PagedSeqs& q, int64_t t, F first) {
+__device__ __forceinline__ PagedSeq paged_find(const PagedSeqs& q, int64_t t, F first) {
   const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int s0 = 0; s0 <= q.n_seqs; s0 += 64) {
-    const int s = s0 + lane;
-    const bool in = s <= q.n_seqs && first(q.start(s), s) <= t;
-    const uint64_t b = __ballot(in);
-    n += __popcll(b);
-    if (b != ~0ull) break;
+  int n = 0, s0 = 0;
+  int c[4], k[4];
+  for (;; s0 += 256) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + 64 * i + lane;
+      c[i] = s > 0 && s <= q.n_seqs ? q.cu_q[s] : s > 0 ? q.n_rows : 0;
+      k[i] = s < q.n_seqs ? q.kv_lens[s] : 0;
+    }
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + 64 * i + lane;
+      c[i] = min(max(c[i], 0), q.n_rows);
+      m += __popcll(__ballot(s <= q.n_seqs && first(c[i], s) <= t));
+    }
+    n += m;
+    if (m < 256 || s0 + 256 > q.n_seqs) break;
   }
-  return __builtin_amdgcn_readfirstlane(max(n - 1, 0));
+  PagedSeq f;
+  f.s = __builtin_amdgcn_readfirstlane(max(n - 1, 0));
+  const int at = f.s - s0;  // < 0: the last of the 256 before
+  auto pick = [](const int (&v)[4], int j) {
+    const int x = j < 64 ? v[0] : j < 128 ? v[1] : j < 192 ? v[2] : v[3];
+    return __builtin_amdgcn_readlane(x, j & 63);
+  };
+  f.c0 = at >= 0 ? pick(c, at) : __builtin_amdgcn_readfirstlane(q.start(f.s));
+  f.len = at >= 0 ? pick(k, at) : __builtin_amdgcn_readfirstlane(q.kv_lens[f.s]);
+  f.rows = max((at >= -1 && at < 255 ? pick(c, at + 1) : __builtin_amdgcn_readfirstlane(q.start(f.s + 1))) - f.c0, 0);
+  return f;
 }
 
 static inline int paged_log2(int v) {

@@ -19,50 +19,32 @@
 #define ROT_THREADS 256
 #define ROT_TABLE 2048  // (cos, sin) entries in LDS
 
-typedef uint32_t rot_u4 __attribute__((ext_vector_type(4)));
-
-// V consecutive elements as floats (V = 8: 16-byte vectors)
+// V consecutive elements as they are in memory (V = 8: in 16-byte words)
 template <typename T, int V>
-struct RotVec;
-template <>
-struct RotVec<float, 8> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
-    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+struct RotPack {
+  T v[V];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) v[0] = *p;
+    else *this = *(const RotPack*)__builtin_assume_aligned(p, 16);
   }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
+};
+__device__ __forceinline__ float rot_f32(float x) { return x; }
+__device__ __forceinline__ float rot_f32(bf16_t x) { return bf16_to_f32(x); }
+template <int V>
+__device__ __forceinline__ void rot_store(float* p, const float (&v)[V]) {
+  if constexpr (V == 8) {
     *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
     *(float4*)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  }
-};
-template <>
-struct RotVec<bf16_t, 8> {
-  static __device__ __forceinline__ void load(const bf16_t* p, float (&v)[8]) {
-    const uint4 u = *(const uint4*)p;
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16x2(v[2 * i], v[2 * i + 1]);
-    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <>
-struct RotVec<float, 1> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[1]) { v[0] = *p; }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
-};
-template <>
-struct RotVec<bf16_t, 1> {
-  static __device__ __forceinline__ void load(const bf16_t* p, float (&v)[1]) { v[0] = bf16_to_f32(*p); }
-  static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[1]) { *p = f32_to_bf16(v[0]); }
-};
+  } else
+    *p = v[0];
+}
+template <int V>
+__device__ __forceinline__ void rot_store(bf16_t* p, const float (&v)[V]) {
+  if constexpr (V == 8)
+    *(uint4*)p = make_uint4(f32_to_bf16x2(v[0], v[1]), f32_to_bf16x2(v[2], v[3]), f32_to_bf16x2(v[4], v[5]), f32_to_bf16x2(v[6], v[7]));
+  else
+    *p = f32_to_bf16(v[0]);
+}
 
 // (m cos a, m sin a) of a = position * inv_freq
 __device__ __forceinline__ float2 rot_entry(int64_t position, double inv_freq, float m, float sign) {
@@ -73,42 +55,72 @@ __device__ __forceinline__ float2 rot_entry(int64_t position, double inv_freq, f
   return make_float2(c * m, sign * s * m);
 }
 
-// One step of a head: unit u < nr turns V pairs, the units behind them copy V channels.
-template <typename TI, typename TO, int V, bool HALF>
-__device__ __forceinline__ void rot_unit(const TI* x, TO* y, const float2* cs, int u, int nr, int rd) {
-  if (u < nr) {
-    const int a = HALF ? u * V : 2 * u * V, b = HALF ? rd / 2 + u * V : a + V;
-    float p[V], q[V], r[V], t[V];
-    RotVec<TI, V>::load(x + a, p);
-    RotVec<TI, V>::load(x + b, q);
-    if (HALF) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 w = cs[u * V + i];
-        r[i] = __fmaf_rn(p[i], w.x, -__fmul_rn(q[i], w.y));
-        t[i] = __fmaf_rn(p[i], w.y, __fmul_rn(q[i], w.x));
-      }
-    } else {
-      float in[2 * V], out[2 * V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) in[i] = p[i], in[V + i] = q[i];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 w = cs[u * V + i];
-        out[2 * i] = __fmaf_rn(in[2 * i], w.x, -__fmul_rn(in[2 * i + 1], w.y));
-        out[2 * i + 1] = __fmaf_rn(in[2 * i], w.y, __fmul_rn(in[2 * i + 1], w.x));
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) r[i] = out[i], t[i] = out[V + i];
-    }
-    RotVec<TO, V>::store(y + a, r);
-    RotVec<TO, V>::store(y + b, t);
-  } else {
-    float p[V];
-    const int a = rd + (u - nr) * V;
-    RotVec<TI, V>::load(x + a, p);
-    RotVec<TO, V>::store(y + a, p);
+// A unit of a head: u < nr turns V pairs, the units behind them copy V channels. Its loads apart from
+// the rest, so that they are on their way while cos and sin are computed.
+template <typename TI, int V, bool HALF>
+struct RotUnit {
+  RotPack<TI, V> p, q;
+  __device__ __forceinline__ void load(const TI* x, int u, int nr, int rd) {
+    if (u < nr) {
+      const int a = HALF ? u * V : 2 * u * V, b = HALF ? rd / 2 + u * V : a + V;
+      p.load(x + a);
+      q.load(x + b);
+    } else
+      p.load(x + rd + (u - nr) * V);
   }
+  template <typename TO>
+  __device__ __forceinline__ void store(TO* y, const float2* cs, int u, int nr, int rd) const {
+    float r[V], t[V];
+    if (u < nr) {
+      const int a = HALF ? u * V : 2 * u * V, b = HALF ? rd / 2 + u * V : a + V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        // the pair: one of p and one of q, or two neighbours of what p and q hold together
+        const float x1 = rot_f32(HALF ? p.v[i] : 2 * i < V ? p.v[2 * i % V] : q.v[2 * i % V]);
+        const float x2 = rot_f32(HALF ? q.v[i] : 2 * i + 1 < V ? p.v[(2 * i + 1) % V] : q.v[(2 * i + 1) % V]);
+        const float2 w = cs[u * V + i];
+        const float y1 = __fmaf_rn(x1, w.x, -__fmul_rn(x2, w.y)), y2 = __fmaf_rn(x1, w.y, __fmul_rn(x2, w.x));
+        if (HALF) {
+          r[i] = y1, t[i] = y2;
+        } else {
+          (2 * i < V ? r : t)[2 * i % V] = y1;
+          (2 * i + 1 < V ? r : t)[(2 * i + 1) % V] = y2;
+        }
+      }
+      rot_store<V>(y + a, r);
+      rot_store<V>(y + b, t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) r[i] = rot_f32(p.v[i]);
+      rot_store<V>(y + rd + (u - nr) * V, r);
+    }
+  }
+};
+
+// A workgroup's threads: 2^lgu neighbours on the units of a head, then 2^lgt tokens, then heads; all by
+// shifts (divisions cost more than the turning).
+struct RotLanes {
+  int u, i, h, hstep;
+  __device__ RotLanes(int tid, int lgu, int lgt) {
+    u = tid & ((1 << lgu) - 1);
+    i = (tid >> lgu) & ((1 << lgt) - 1);
+    h = tid >> (lgu + lgt);
+    hstep = (ROT_THREADS >> lgu) >> lgt;
+  }
+};
+static inline int rot_log2up(int64_t v) {
+  int b = 0;
+  while (((int64_t)1 << b) < v) ++b;
+  return b;
+}
+
+// cos and sin of nt tokens into LDS, position(t) theirs
+template <typename F>
+__device__ __forceinline__ void rot_table(float2* cs, const double* inv_freq, int half, int lgh, int nt, float m, float sign,
+                                          F position) {
+  for (int f = threadIdx.x & ((1 << lgh) - 1); f < half; f += ROT_THREADS)  // once, unless there are more than threads
+    for (int t = threadIdx.x >> lgh; t < nt; t += max(ROT_THREADS >> lgh, 1))
+      cs[t * half + f] = rot_entry(position(t), inv_freq[f], m, sign);
 }
 
 struct RotArgs {
@@ -119,32 +131,39 @@ struct RotArgs {
   int64_t xs[3], ys[3];  // strides of batch, token and head, in elements
   int64_t pb, pl;        // strides of the positions
   int64_t n;             // tokens
-  uint32_t L, heads;
-  int D, rd, pos64;
+  uint32_t L;
+  int heads, D, rd, pos64;
   float mscale, sign;
-  int tokens;            // per workgroup
+  int lgu, lgt, lgh;     // log2 of the threads on a head, of the tokens of a workgroup, of rd / 2 (rounded up)
 };
 
 template <typename T, int V, bool HALF>
 __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotArgs a) {
   __shared__ float2 cs_s[ROT_TABLE];
-  const int tid = threadIdx.x, half = a.rd / 2;
-  const int64_t n0 = (int64_t)blockIdx.x * a.tokens;
-  const int nt = (int)min((int64_t)a.tokens, a.n - n0);
-  for (int k = tid; k < nt * half; k += ROT_THREADS) {
-    const int t = k / half;
-    const int64_t n = n0 + t, b = n / a.L, l = n - b * a.L;
-    const int64_t at = b * a.pb + l * a.pl;
-    const int64_t p = a.pos64 ? ((const int64_t*)a.pos)[at] : (int64_t)((const int32_t*)a.pos)[at];
-    cs_s[k] = rot_entry(p, a.inv_freq[k - t * half], a.mscale, a.sign);
-  }
+  const int half = a.rd / 2, nr = half / V, per = nr + (a.D - a.rd) / V;
+  const uint32_t n0 = blockIdx.x << a.lgt;
+  const int nt = (int)min((uint32_t)1 << a.lgt, (uint32_t)a.n - n0);
+  const RotLanes w(threadIdx.x, a.lgu, a.lgt);
+  const uint32_t n = n0 + w.i, b = n / a.L, l = n - b * a.L;
+  const T* const x = (const T*)a.x + b * a.xs[0] + l * a.xs[1];
+  T* const y = (T*)a.y + b * a.ys[0] + l * a.ys[1];
+  int h = w.h + w.hstep * blockIdx.y, u = w.u;
+  bool more = w.i < nt && h < a.heads && u < per;
+  RotUnit<T, V, HALF> now, next;
+  if (more) now.load(x + h * a.xs[2], u, nr, a.rd);
+  rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, a.sign, [&](int t) {
+    const uint32_t n = n0 + t, b = n / a.L;
+    const int64_t at = b * a.pb + (n - b * a.L) * a.pl;
+    return a.pos64 ? ((const int64_t*)a.pos)[at] : (int64_t)((const int32_t*)a.pos)[at];
+  });
   __syncthreads();
-  const uint32_t nr = half / V, per = nr + (a.D - a.rd) / V, units = a.heads * per;
-  for (uint32_t k = blockIdx.y * ROT_THREADS + tid; k < nt * units; k += gridDim.y * ROT_THREADS) {
-    const uint32_t t = k / units, r = k - t * units, h = r / per, u = r - h * per;
-    const int64_t n = n0 + t, b = n / a.L, l = n - b * a.L;
-    rot_unit<T, T, V, HALF>((const T*)a.x + b * a.xs[0] + l * a.xs[1] + h * a.xs[2],
-                            (T*)a.y + b * a.ys[0] + l * a.ys[1] + h * a.ys[2], cs_s + t * half, u, nr, a.rd);
+  while (more) {
+    int h2 = h, u2 = u + (1 << a.lgu);
+    if (u2 >= per) u2 = w.u, h2 += w.hstep * gridDim.y;
+    more = h2 < a.heads;
+    if (more) next.load(x + h2 * a.xs[2], u2, nr, a.rd);
+    now.store(y + h * a.ys[2], cs_s + w.i * half, u, nr, a.rd);
+    now = next, h = h2, u = u2;
   }
 }
 
@@ -175,19 +194,21 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
   a.x = x, a.y = y, a.pos = positions, a.inv_freq = inv_freq;
   for (int i = 0; i < 3; ++i) a.xs[i] = x_strides[i], a.ys[i] = y_strides[i];
   a.pb = pos_strides[0], a.pl = pos_strides[1];
-  a.n = batch * length, a.L = (uint32_t)length, a.heads = (uint32_t)heads;
+  a.n = batch * length, a.L = (uint32_t)length, a.heads = heads;
   a.D = D, a.rd = rotary_dim, a.pos64 = pos64, a.mscale = mscale, a.sign = inverse ? -1.0f : 1.0f;
   // 16-byte vectors where every head starts on one and the parts are whole vectors
   const bool vec = rotary_dim % 16 == 0 && D % 8 == 0 && rot_aligned(x, a.xs, 3, bytes) && rot_aligned(y, a.ys, 3, bytes);
-  const int64_t units = (int64_t)heads * (vec ? rotary_dim / 16 + (D - rotary_dim) / 8 : rotary_dim / 2 + D - rotary_dim);
+  const int per = vec ? rotary_dim / 16 + (D - rotary_dim) / 8 : rotary_dim / 2 + D - rotary_dim;
+  a.lgu = std::min(8, rot_log2up(per)), a.lgh = std::min(8, rot_log2up(rotary_dim / 2));
   // Enough tokens to keep a thread on four steps, as long as that leaves two workgroups for each CU;
   // a call smaller than that spreads every token's heads over workgroups of one step.
   const int64_t cus = pp_device_cus();
-  const int64_t want = std::max<int64_t>(1, 4 * ROT_THREADS / units);
-  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>({want, a.n / (2 * cus), ROT_TABLE / (rotary_dim / 2)}));
-  const int64_t steps = (a.tokens * units + ROT_THREADS - 1) / ROT_THREADS;
-  const int64_t gx = (a.n + a.tokens - 1) / a.tokens;
-  const int64_t gy = std::max<int64_t>(1, std::min<int64_t>({steps, (2 * cus + gx - 1) / gx, 65535}));
+  a.lgt = 0;
+  while (a.lgt < 4 && a.lgu + a.lgt < 8 && ((int64_t)heads * per << a.lgt) < 4 * ROT_THREADS &&
+         (a.n >> (a.lgt + 1)) >= 2 * cus && ((rotary_dim / 2) << (a.lgt + 1)) <= ROT_TABLE)
+    ++a.lgt;
+  const int64_t gx = (a.n + (1 << a.lgt) - 1) >> a.lgt, hstep = (ROT_THREADS >> a.lgu) >> a.lgt;
+  const int64_t gy = std::max<int64_t>(1, std::min<int64_t>((heads + hstep - 1) / hstep, (2 * cus + gx - 1) / gx));
   const dim3 grid((unsigned)gx, (unsigned)gy);
   hipStream_t st = (hipStream_t)stream;
 #define ROT(T, V)                                                                            \
@@ -207,13 +228,15 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
 }
 
 // ------------------------------------------------------------------ append
-// A work item is 16 aligned positions of one sequence (so it lies in one page) and a block of heads
-// of one kind: query, key or value. Sequence s has the items (start >> 4) + 2 s and on: n new tokens
-// lie in at most (n >> 4) + 2 such groups. Query and key items turn their tokens' heads as above.
-// The value pages keep a channel's tokens next to each other, so a value item reads 16 tokens of two
-// channels per thread, a wave's lanes on consecutive channels, and writes them as two 16-byte vectors
-// a channel; a group that is not full writes its tokens' elements one by one.
-#define APP_THREADS 256
+// A work item is a group of 16 aligned positions of one sequence (so it lies in one page) and a block
+// of query or of key heads, or four such groups and a block of value heads. Sequence s has the items
+// (start >> 4) + 2 s and on: n new tokens lie in at most (n >> 4) + 2 groups (and 6 for 4 of the value
+// items). Query and key items turn their tokens' heads as above. The value pages keep a channel's
+// tokens next to each other: a thread reads 16 tokens of two channels, a wave's lanes on consecutive
+// channels, and writes them as two 16-byte vectors a channel; a group that is not full writes its
+// tokens' elements one by one. The waves of a value item take its four groups, so that in pages of 64
+// and more the 128 bytes of a channel leave the same L2 together.
+#define APP_THREADS ROT_THREADS
 #define APP_TOKENS 16
 
 struct AppArgs {
@@ -225,7 +248,10 @@ struct AppArgs {
   int Hq, Hkv, rd;
   float mscale;
   int zero_tail;
-  int per, nqb, nkb;  // heads per block, blocks of query and of key heads
+  int lgu, lgh;        // log2 of the threads on a head, and of rd / 2 (rounded up)
+  int per, nqb, nkb;   // heads per block, blocks of query and of key heads
+  int vper, nvb;       // the same of the value items
+  uint32_t values;     // value items
 };
 
 __device__ __forceinline__ uint32_t app_pair(const float* p) {
@@ -238,18 +264,30 @@ template <typename T, int D, bool HALF>
 __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
   __shared__ float2 cs_s[APP_TOKENS * D / 2];
   const int tid = threadIdx.x;
-  const int64_t t = blockIdx.x;
-  const int s = paged_seq_of(a.seqs, t, [](int c, int s) { return (int64_t)(c >> 4) + 2 * s; });
-  const int c0 = a.seqs.start(s), len = max(a.seqs.start(s + 1) - c0, 0);
+  // the grid: value items, whose way is the longest, then query and key items
+  const bool value = blockIdx.x < a.values;
+  const uint32_t id = value ? blockIdx.x : blockIdx.x - a.values, nb = value ? a.nvb : a.nqb + a.nkb;
+  const uint32_t block = id % nb, t = id / nb;
+  const int kind = value ? 2 : block < (uint32_t)a.nqb ? 0 : 1;
+  const int h0 = value ? block * a.vper : (block - (kind ? a.nqb : 0)) * a.per;
+  const int nh = min(value ? a.vper : a.per, (kind ? a.Hkv : a.Hq) - h0);
+  const int lg = value ? 6 : 4;  // log2 of the item's positions
+  const PagedSeq f = paged_find(a.seqs, t, [lg](int c, int s) { return (int64_t)(c >> lg) + 2 * s; });
+  const int s = f.s, c0 = f.c0, len = f.rows;
   const bool tail = s == a.seqs.n_seqs;  // rows of no sequence
-  const int64_t first = tail ? 0 : (int64_t)a.seqs.kv_lens[s] - len;
-  const int64_t p0 = (first & ~(int64_t)(APP_TOKENS - 1)) + APP_TOKENS * (t - ((c0 >> 4) + 2 * s));
+  const int64_t first = tail ? 0 : (int64_t)f.len - len;
+  int64_t p0 = ((first >> lg) + (t - ((c0 >> lg) + 2 * s))) << lg;
+  // value items: their four groups to the four waves, unless only one has tokens
+  bool alone = true;
+  if (value) {
+    const int64_t from = max(p0, first & ~(int64_t)(APP_TOKENS - 1));
+    alone = min(p0 + 64, first + len) - from <= APP_TOKENS;
+    p0 = alone ? from : p0 + APP_TOKENS * __builtin_amdgcn_readfirstlane(tid >> 6);
+  }
   const int lo = (int)max((int64_t)0, first - p0), hi = (int)min((int64_t)APP_TOKENS, first + len - p0);  // the group's tokens
   if (lo >= hi) return;
   const int row0 = c0 + (int)(p0 - first);  // row of the group's place 0
-  const int kind = blockIdx.y < a.nqb ? 0 : blockIdx.y < a.nqb + a.nkb ? 1 : 2;
-  const int h0 = (blockIdx.y - (kind == 0 ? 0 : kind == 1 ? a.nqb : a.nqb + a.nkb)) * a.per;
-  const int nh = min(a.per, (kind == 0 ? a.Hq : a.Hkv) - h0), nt = hi - lo;
+  const int nt = hi - lo;
   if (tail) {
     if (kind == 0 && a.zero_tail)
       for (int k = tid; k < nt * nh * (D / 8); k += APP_THREADS) {
@@ -266,15 +304,16 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
   }
   const int place = (int)(p0 & (ps - 1));
   if (kind == 2) {
+    constexpr int P = D / 2;  // pairs of channels of a head
     bf16_t* const to = a.v_pages + (((int64_t)page * a.Hkv + h0) * D << a.seqs.lp) + place;
-    for (int k = tid; k < nh * (D / 2); k += APP_THREADS) {
-      const int h = k / (D / 2), d = 2 * (k - h * (D / 2));
+    for (int k = alone ? tid : tid & 63; k < nh * P; k += alone ? APP_THREADS : 64) {
+      const int h = k / P, d = 2 * (k - h * P);
       const T* src = (const T*)a.v + (int64_t)row0 * a.vs[0] + (h0 + h) * a.vs[1] + d;
-      uint32_t w[APP_TOKENS];
-#pragma unroll
-      for (int i = 0; i < APP_TOKENS; ++i) w[i] = i >= lo && i < hi ? app_pair(src + i * a.vs[0]) : 0u;
       bf16_t* dst = to + ((int64_t)(h * D + d) << a.seqs.lp);
       if (nt == APP_TOKENS) {
+        uint32_t w[APP_TOKENS];
+#pragma unroll
+        for (int i = 0; i < APP_TOKENS; ++i) w[i] = app_pair(src + i * a.vs[0]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -289,30 +328,36 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
           }
         }
       } else {
-#pragma unroll
-        for (int i = 0; i < APP_TOKENS; ++i)
-          if (i >= lo && i < hi) {
-            dst[i] = (bf16_t)w[i];
-            dst[i + ps] = (bf16_t)(w[i] >> 16);
-          }
+#pragma unroll 4
+        for (int i = lo; i < hi; ++i) {
+          const uint32_t w = app_pair(src + i * a.vs[0]);
+          dst[i] = (bf16_t)w;
+          dst[i + ps] = (bf16_t)(w >> 16);
+        }
       }
     }
     return;
   }
-  const int half = a.rd / 2;
-  for (int k = tid; k < nt * half; k += APP_THREADS) {
-    const int i = k / half;
-    cs_s[k] = rot_entry(p0 + lo + i, a.inv_freq[k - i * half], a.mscale, 1.0f);
-  }
+  const int half = a.rd / 2, nr = half / 8, per = nr + (D - a.rd) / 8;
+  const RotLanes w(tid, a.lgu, 32 - __clz(nt - 1));  // as many tokens as there are
+  const int64_t row = row0 + lo + w.i;
+  const T* const x = (const T*)(kind == 0 ? a.q : a.k) + row * (kind == 0 ? a.qs[0] : a.ks[0]);
+  const int64_t xs = kind == 0 ? a.qs[1] : a.ks[1];
+  bf16_t* const y = kind == 0 ? a.q_out + row * a.Hq * D
+                              : a.k_pages + (((int64_t)page * a.Hkv << a.seqs.lp) + place + lo + w.i) * D;
+  const int64_t ys = kind == 0 ? D : (int64_t)D << a.seqs.lp;
+  int h = h0 + w.h;
+  bool more = w.i < nt && h < h0 + nh && w.u < per;
+  RotUnit<T, 8, HALF> now, next;
+  if (more) now.load(x + h * xs, w.u, nr, a.rd);
+  rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, 1.0f, [&](int t) { return p0 + lo + t; });
   __syncthreads();
-  const int nr = half / 8, per = nr + (D - a.rd) / 8, units = nh * per;
-  const T* const x = (const T*)(kind == 0 ? a.q : a.k);
-  const int64_t ts = kind == 0 ? a.qs[0] : a.ks[0], hs = kind == 0 ? a.qs[1] : a.ks[1];
-  for (int k = tid; k < nt * units; k += APP_THREADS) {
-    const int i = k / units, r = k - i * units, h = r / per, u = r - h * per;
-    bf16_t* y = kind == 0 ? a.q_out + ((int64_t)(row0 + lo + i) * a.Hq + h0 + h) * D
-                          : a.k_pages + ((((int64_t)page * a.Hkv + h0 + h) << a.seqs.lp) + place + lo + i) * D;
-    rot_unit<T, bf16_t, 8, HALF>(x + (int64_t)(row0 + lo + i) * ts + (h0 + h) * hs, y, cs_s + i * half, u, nr, a.rd);
+  while (more) {
+    const int h2 = h + w.hstep;
+    more = h2 < h0 + nh;
+    if (more) next.load(x + h2 * xs, w.u, nr, a.rd);
+    now.store(y + h * ys, cs_s + w.i * half, w.u, nr, a.rd);
+    now = next, h = h2;
   }
 }
 
@@ -365,9 +410,19 @@ extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void*
   for (int i = 0; i < 2; ++i) a.qs[i] = q ? q_strides[i] : 0, a.ks[i] = k_strides[i], a.vs[i] = v_strides[i];
   a.q_out = (bf16_t*)q_out, a.k_pages = (bf16_t*)k_pages, a.v_pages = (bf16_t*)v_pages;
   a.inv_freq = inv_freq, a.Hq = Hq, a.Hkv = Hkv, a.rd = rotary_dim, a.mscale = mscale, a.zero_tail = zero_tail;
-  a.per = 4;
-  a.nqb = (Hq + a.per - 1) / a.per, a.nkb = (Hkv + a.per - 1) / a.per;
-  const dim3 grid((unsigned)((n_tokens >> 4) + 2 * ((int64_t)n_seqs + 1)), (unsigned)(a.nqb + 2 * a.nkb));
+  a.lgu = rot_log2up(rotary_dim / 16 + (D - rotary_dim) / 8), a.lgh = rot_log2up(std::max(rotary_dim / 2, 1));
+  // Heads of an item. Single tokens: a group has one, so all the heads that the threads hold in one step
+  // (32, value heads 4, or 16 where there are workgroups enough); 1, 64, 256 sequences of 12 heads 3.5,
+  // 5.1, 8.8 us, in items of 4 heads 3.7, 5.7, 12.6. Chunks: 4, and one value head (64 tokens of it),
+  // 8192 tokens (151 MB, from memory) 38 us, 8 or 12 heads 42 and 41.
+  a.per = n_tokens <= 4 * (int64_t)n_seqs ? 32 : 4;
+  a.vper = n_tokens > 16 * (int64_t)n_seqs ? 1 : n_seqs >= 64 ? 16 : 4;
+  a.nqb = (Hq + a.per - 1) / a.per, a.nkb = (Hkv + a.per - 1) / a.per, a.nvb = (Hkv + a.vper - 1) / a.vper;
+  const int64_t values = ((n_tokens >> 6) + 2 * ((int64_t)n_seqs + 1)) * a.nvb;
+  const int64_t items = values + ((n_tokens >> 4) + 2 * ((int64_t)n_seqs + 1)) * (a.nqb + a.nkb);
+  PP_REQUIRE(items <= 0x7fffffff, PP_ERR_UNSUPPORTED, "%s: too many sequences and heads", what);
+  a.values = (uint32_t)values;
+  const unsigned grid = (unsigned)items;
   hipStream_t st = (hipStream_t)stream;
 #define APP(T, D_)                                                                                       \
   do {                                                                                                   \

@@ -20,7 +20,7 @@ def start(cu, s, n_rows):
 
 
 def seq_of(cu, n_rows, t, first):
-    """paged_seq_of: blocks of 64 sequences, stopping at the first block that is not all below t."""
+    """paged_find: blocks of 64 sequences, stopping at the first block that is not all below t."""
     B, n = len(cu) - 1, 0
     for s0 in range(0, B + 1, 64):
         hits = [s <= B and first(start(cu, s, n_rows), s) <= t for s in range(s0, s0 + 64)]
