@@ -148,11 +148,10 @@ __device__ __forceinline__ a_u4 attn_ones(uint32_t seen) {
 }
 
 
-// max(a, b, c) in one instruction (fmaxf first makes each operand a quiet value).
+// max(a, b, c), NaN if one is: one v_maximum3_f32 (fmaxf, which passes NaN over, first makes each operand
+// a quiet value).
 __device__ __forceinline__ float attn_max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -380,7 +379,7 @@ __device__ __forceinline__ void attn_landed() { asm volatile("s_waitcnt vmcnt(0)
 #define ATTN_SLACK 8.0f
 
 template <int D>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_many_kernel(AttnArgs a) {
+__global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kernel(AttnArgs a) {
   constexpr int KC = D / 8, NK = ATTN_KT * KC / ATTN_THREADS, NV = D * (ATTN_KT / 8) / ATTN_THREADS, MB = D / 32;
   __shared__ a_u4 k_s[2][ATTN_KT * KC];
   __shared__ a_u4 v_s[2][D * (ATTN_KT / 8)];
