@@ -83,6 +83,8 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int 
   w.ns = w.nt > 0 ? (w.nt + per - 1) / per : 0;
   w.lo = (int)min((int64_t)split * per, (int64_t)w.nt);
   w.hi = min(w.nt, w.lo + per);
+  // the same in every lane: said so, or what is computed from them takes vector registers
+  for (int* v : {&w.r0, &w.nr, &w.nt, &w.lo, &w.hi, &w.ns}) *v = __builtin_amdgcn_readfirstlane(*v);
   return w;
 }
 
@@ -370,9 +372,12 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 // asked for, before the workgroup's barrier.
 typedef __attribute__((address_space(3))) void attn_lds_t;
 __device__ __forceinline__ uint32_t attn_lds(void* p) { return (uint32_t)(uintptr_t)(attn_lds_t*)p; }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 named as clobbered: the compiler sets it anew for each use of its own
 __device__ __forceinline__ void attn_copy(const void* from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void attn_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 #define ATTN_KT 64
@@ -466,7 +471,8 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       load(t + ATTN_KT, buf ^ 1);
     }
     // a step with a masked place: only the finite part of V, and a mark where there is another
-    if (t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(pg < 0)) {
+    const bool masked = t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(pg < 0);
+    if (masked) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const a_u4 v = v_s[buf][i * ATTN_THREADS + tid];
@@ -569,7 +575,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       }
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(0);
-      if (__builtin_amdgcn_readfirstlane(bad_s[buf]) == t) {  // what was taken out of V, read again, for the rows that attend it
+      if (masked && __builtin_amdgcn_readfirstlane(bad_s[buf]) == t) {  // what was taken out of V, read again, for the rows that attend it
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
           f32x16_t code;
