@@ -407,20 +407,6 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   const int limit = in ? attn_limit(a, w, r) : 0x7fffffff;
   // tokens that every row of the wave attends, and that any does
   const int low = busy ? attn_limit(a, w, 32 * wave) : 0, top = busy ? attn_limit(a, w, min(32 * wave + 31, w.nr - 1)) : -1;
-  a_u4 qf[D / 16];
-  {
-    const int i = (w.r0 + r) / a.group;
-    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1] + 8 * e;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) qf[s] = in ? *(const a_u4*)(src + 16 * s) ^ a.flip : a_mk(0, 0, 0, 0);
-  }
-  f32x16_t o[MB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b)
-#pragma unroll
-    for (int q = 0; q < 16; ++q) o[b][q] = 0.0f;
-  float m = ATTN_LOW, l = 0.0f;
-
   const int ps = 1 << a.seqs.lp;
   // the thread's 16-byte chunk of each K copy (row krow of its 16 or 32) and of each V copy (channel
   // vrow of 32): its place in LDS is tid, so the swizzle is in what it reads
@@ -461,6 +447,19 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   pn = a.seqs.page(en);
   entry(t + ATTN_KT);
   load(t, 0);
+  a_u4 qf[D / 16];
+  {
+    const int i = (w.r0 + r) / a.group;
+    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1] + 8 * e;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = in ? *(const a_u4*)(src + 16 * s) ^ a.flip : a_mk(0, 0, 0, 0);
+  }
+  f32x16_t o[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) o[b][q] = 0.0f;
+  float m = ATTN_LOW, l = 0.0f;
   while (true) {
     attn_landed();  // the present step is in its buffer, and every wave is done with the other one
     const bool more = t + ATTN_KT < w.hi;
@@ -511,19 +510,21 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
     }
     if (on) {
       const uint64_t have = __ballot(pg >= 0);  // bit 2 j ^ of_odd: group j
-      uint32_t seen = ~0u;
+      const int last = min(limit, w.hi - 1) - t - 8 * e;  // of the lane's tokens, 16 (2 b + q / 8) + q % 8
       if (t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != ~0ull) {  // a masked place
         asm volatile("");  // a branch: few steps have one
-        seen = 0;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const int g16 = 2 * b + (q >> 3), tok = t + 16 * g16 + 8 * e + (q & 7);
-            const bool in = tok <= limit && tok < w.hi && ((have >> ((2 * g16) ^ of_odd)) & 1);
-            seen |= in ? 1u << (16 * b + q) : 0u;
-            s[b][q] = in ? s[b][q] : -__builtin_inff();
-          }
+          for (int q = 0; q < 16; ++q) s[b][q] = 16 * (2 * b + (q >> 3)) + (q & 7) <= last ? s[b][q] : -__builtin_inff();
+        if (have != ~0ull) {  // a group without a page
+          asm volatile("");
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              s[b][q] = (have >> ((2 * (2 * b + (q >> 3))) ^ of_odd)) & 1 ? s[b][q] : -__builtin_inff();
+        }
       }
       float mx = ATTN_LOW;
 #pragma unroll
@@ -585,7 +586,8 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
           for (int kk = 0; kk < 4; ++kk) {
             const bf16_t* vp = a.v + ((((int64_t)max(__builtin_amdgcn_readlane(pg, (2 * kk) ^ of_odd), 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
                                ((t + 16 * kk) & (ps - 1)) + 8 * e;
-            code = mfma32a(attn_code(*(const a_u4*)vp), attn_ones(seen >> (8 * kk)), code);
+            const int n = (have >> ((2 * kk) ^ of_odd)) & 1 ? min(max(last - 16 * kk + 1, 0), 8) : 0;  // attended of 8
+            code = mfma32a(attn_code(*(const a_u4*)vp), attn_ones((1u << n) - 1), code);
           }
 #pragma unroll
           for (int q = 0; q < 16; ++q) o[b][q] = attn_poison(o[b][q], code[q]);
