@@ -753,7 +753,7 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.pml = a.po + n_tokens * Hq * p.splits * D;
   a.pns = (int*)(a.pml + n_tokens * Hq * p.splits * 2);
   const int64_t items = p.tiles * Hkv * p.splits;
-  PP_REQUIRE(items <= 0x7ffffff0, PP_ERR_UNSUPPORTED, "%s: too many sequences and heads", what);
+  PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld tiles (at most 2^24 - 1)", what, (long long)items);
   hipStream_t st = (hipStream_t)stream;
   const unsigned n = (unsigned)items;
   const int64_t rows = n_tokens * Hq;

@@ -209,6 +209,7 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
     ++a.lgt;
   const int64_t gx = (a.n + (1 << a.lgt) - 1) >> a.lgt, hstep = (ROT_THREADS >> a.lgu) >> a.lgt;
   const int64_t gy = std::max<int64_t>(1, std::min<int64_t>((heads + hstep - 1) / hstep, (2 * cus + gx - 1) / gx));
+  PP_REQUIRE(gx <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld tokens of this head size", what, (long long)a.n);
   const dim3 grid((unsigned)gx, (unsigned)gy);
   hipStream_t st = (hipStream_t)stream;
 #define ROT(T, V)                                                                            \
@@ -420,7 +421,7 @@ extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void*
   a.nqb = (Hq + a.per - 1) / a.per, a.nkb = (Hkv + a.per - 1) / a.per, a.nvb = (Hkv + a.vper - 1) / a.vper;
   const int64_t values = ((n_tokens >> 6) + 2 * ((int64_t)n_seqs + 1)) * a.nvb;
   const int64_t items = values + ((n_tokens >> 4) + 2 * ((int64_t)n_seqs + 1)) * (a.nqb + a.nkb);
-  PP_REQUIRE(items <= 0x7fffffff, PP_ERR_UNSUPPORTED, "%s: too many sequences and heads", what);
+  PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld work items (at most 2^24 - 1)", what, (long long)items);
   a.values = (uint32_t)values;
   const unsigned grid = (unsigned)items;
   hipStream_t st = (hipStream_t)stream;

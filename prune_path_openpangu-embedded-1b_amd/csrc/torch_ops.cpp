@@ -481,8 +481,8 @@ void same_device(const char* name, const Tensor& ref, std::initializer_list<cons
   }
 }
 
-// x [..., heads, D] with positions [...] as (batch, length): the leading axes merged where their
-// strides allow it, at most two left.
+// x [N, heads, D] or [B, L, heads, D] with positions of the leading shape. Strides go to the kernel;
+// only channels that are not next to each other are copied first.
 Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
                   double mscale, bool inverse) {
   const int lay = rotary_layout(layout, "rotary");
@@ -590,6 +590,10 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   const int lay = rotary_layout(layout, name);
   TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
               "prunepath.kv_append: k and v must be [N, kv_heads, D] of one dtype");
+  if (q)
+    TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(2) == k.size(2) &&
+                    q->scalar_type() == k.scalar_type() && q->stride(2) == 1,
+                "prunepath.kv_append: q must be [N, heads, D] of k's dtype, channels contiguous");
   const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, k.size(0), q ? q->size(1) : 0, k.size(2));
   TORCH_CHECK(k.size(1) == p.Hkv, "prunepath.kv_append: ", k.size(1), " heads for a cache of ", p.Hkv);
   TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, "prunepath.kv_append: channels must be contiguous");
@@ -600,9 +604,6 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
                 "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
   int64_t qs[2] = {0, 0};
   if (q) {
-    TORCH_CHECK(q->dim() == 3 && q->size(0) == p.n && q->size(2) == p.D && q->scalar_type() == k.scalar_type() &&
-                    q->stride(2) == 1,
-                "prunepath.kv_append: q must be [N, heads, D] of k's dtype, channels contiguous");
     TORCH_CHECK(q_out->scalar_type() == at::kBFloat16 && q_out->sizes() == q->sizes() && q_out->is_contiguous(),
                 "prunepath.kv_append: q_out must be contiguous bfloat16 of q's shape");
     same_device(name, k, {&*q, &*q_out});

@@ -443,6 +443,52 @@ def test_kv_append_without_rotation_and_without_a_place(pkg):
     assert torch.equal(kp.cpu(), want_k) and torch.equal(vp.cpu(), want_v)
 
 
+@pytest.mark.parametrize("seqs", [255, 256, 257, 300, 520])
+def test_many_sequences(pkg, seqs):
+    """Offsets are looked through 256 sequences at a time: single tokens, empty sequences and chunks
+    around the borders of such blocks, appended and attended."""
+    new = [1] * seqs
+    for s in (0, 63, 64, 200, 255, 256, 257, 511):
+        if s < seqs:
+            new[s] = 0 if s % 2 == 0 else 3
+    total = [n + s % 23 for s, n in enumerate(new)]
+    b = Batch(new, total, 16, 1, 64, seed=seqs)
+    kv = torch.randn(2, b.n + 2, 1, 64, generator=gen(seqs)).to(torch.bfloat16)
+    q = torch.randn(b.n + 2, 2, 64, generator=gen(seqs + 1)).to(torch.bfloat16)
+    kp, vp, table, lens, cu = b.gpu()
+    pkg.ops.kv_append(kv[0].to(dev()), kv[1].to(dev()), kp, vp, table, lens, cu)
+    for row, s, p in b.rows():
+        at = b.place(s, p)
+        b.k[at[0], :, at[1]], b.v[at[0], :, :, at[1]] = kv[0, row], kv[1, row]
+    assert torch.equal(kp.cpu(), b.k) and torch.equal(vp.cpu(), b.v)
+    got = pkg.ops.paged_attention(q.to(dev()), kp, vp, table, lens, cu)
+    o, big = attend64(b, q[:b.n])
+    check_attention(got[:b.n], o, big, few(b, 2, 1))
+    assert bool((got[b.n:] == 0).all())
+
+
+def test_rotary_entry_point_in_place(pkg):
+    """The C entry point writes a tensor onto itself, with strides of its own."""
+    import ctypes
+    lib = pkg._lib.lib()
+    f = pkg.ops.rotary_frequencies(32)[0].to(dev())
+    for D, first in ((64, 0), (36, 1)):  # whole vectors, and elements one by one
+        rows = torch.randn(2, 7, 9, D, generator=gen(D)).to(dev())
+        x = rows[:, :, first:first + 4]
+        want = pkg.ops.rotary(x, torch.arange(7, device=dev()).expand(2, 7), f)
+        pos = torch.arange(7, device=dev())
+        st = (ctypes.c_int64 * 3)(*x.stride()[:3])
+        ps = (ctypes.c_int64 * 2)(0, 1)
+        p = ctypes.c_void_p
+        keep = rows.clone()
+        rc = lib.pp_rotary(p(x.data_ptr()), 0, st, p(pos.data_ptr()), 1, ps, 2, 7, 4, D, p(f.data_ptr()), 32, 0, 1.0, 0,
+                           p(x.data_ptr()), st, p(torch.cuda.current_stream().cuda_stream))
+        pkg._lib.check(rc, "pp_rotary")
+        assert torch.equal(x, want)
+        keep[:, :, first:first + 4] = want
+        assert torch.equal(rows, keep)  # nothing beside it
+
+
 def test_paged_refusals(pkg):
     ops = pkg.ops
     b = Batch([2], [20], 16, 2, 64)

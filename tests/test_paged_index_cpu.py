@@ -20,10 +20,10 @@ def start(cu, s, n_rows):
 
 
 def seq_of(cu, n_rows, t, first):
-    """paged_find: blocks of 64 sequences, stopping at the first block that is not all below t."""
+    """paged_find: blocks of 256 sequences, stopping at the first block that is not all below t."""
     B, n = len(cu) - 1, 0
-    for s0 in range(0, B + 1, 64):
-        hits = [s <= B and first(start(cu, s, n_rows), s) <= t for s in range(s0, s0 + 64)]
+    for s0 in range(0, B + 1, 256):
+        hits = [s <= B and first(start(cu, s, n_rows), s) <= t for s in range(s0, s0 + 256)]
         n += sum(hits)
         if not all(hits):
             break
@@ -32,7 +32,7 @@ def seq_of(cu, n_rows, t, first):
 
 def batches():
     rng = random.Random(7)
-    for B in (0, 1, 2, 3, 63, 64, 65, 130):
+    for B in (0, 1, 2, 3, 64, 130, 255, 256, 300):
         for kind in ("one", "ragged", "empty"):
             new = [1 if kind == "one" else rng.choice([0, 1, 2, 17, 40]) if kind == "ragged" else 0 for _ in range(B)]
             for pad in (0, 1, 37):
@@ -213,3 +213,24 @@ def test_wrappers_refuse_cpu_tensors():
         ops.kv_append(x, x, *args)
     with pytest.raises(RuntimeError, match="GPU"):
         ops.paged_attention(x, *args)
+
+
+def test_shapes_without_a_gpu():
+    """Fake tensors: the ops' results have their shapes and types, the in-place ones return nothing."""
+    import torch
+    t = import_pkg()._lib.torch_ops()
+    m = dict(device="meta")
+    f = torch.empty(32, dtype=torch.float64, **m)
+    x = torch.empty(3, 5, 4, 64, dtype=torch.bfloat16, **m).transpose(1, 2)
+    y = t.rotary(x.transpose(1, 2), torch.empty(3, 5, dtype=torch.int64, **m), f)
+    assert y.shape == (3, 5, 4, 64) and y.dtype == torch.bfloat16
+    cache = (torch.empty(9, 2, 16, 64, dtype=torch.bfloat16, **m), torch.empty(9, 2, 64, 16, dtype=torch.bfloat16, **m),
+             torch.empty(2, 3, dtype=torch.int32, **m), torch.empty(2, dtype=torch.int32, **m),
+             torch.empty(3, dtype=torch.int32, **m))
+    kv, q = torch.empty(5, 2, 64, **m), torch.empty(5, 4, 64, **m)
+    assert t.kv_append(kv, kv, *cache, f) is None
+    r = t.kv_append_q(q, kv, kv, *cache, f)
+    assert r.shape == q.shape and r.dtype == torch.bfloat16
+    assert t.kv_append_q_into(q, r, kv, kv, *cache, f) is None
+    assert t.paged_attention(r, *cache, 0.1).shape == r.shape
+    assert t.paged_attention_into(r, *cache, 0.1, r) is None
