@@ -22,7 +22,7 @@
 // Masked places: their scores are replaced, not added to, and a step that has any multiplies the
 // finite part of V only; what is not finite in V goes to the rows that attend it by a second product
 // (attn_poison). So stale or foreign data in a page, and a later token's NaN, do not reach a row. A
-// row that attends nothing gives zeros.
+// row that attends nothing gives zeros, and so does one whose scores are all -inf.
 #include <algorithm>
 #include <cmath>
 
@@ -177,6 +177,9 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // lane group g = lane / 16 with the scores of tokens 8 g .. 8 g + 7: its k of the second product.
 // P enters as a sum of two bf16 values (the rounded one and what is left, 2^-17 of it): the second
 // product costs nothing next to the loads.
+// Measured, 12 heads of 128: one token on each of 64 sequences of 8192 555 us (3.2 GB, 5.8 TB/s, where a
+// large copy reaches 5.05), of 1 to 8192 tokens 271 us (5.6 TB/s); one sequence of 1152 tokens 6.5 us
+// with the join's 3.1, chains of offsets, table, K and join rather than bytes.
 template <int D>
 __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   constexpr int R = 16, KS = D / 32, MB = D / 16, OS = D + 4;
@@ -358,9 +361,15 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------ many rows
-// 128 rows of one key head, 32 to each of four waves; the matrix cores bound it. Steps of 64 tokens:
-// K [64][D] and V^T [D][64] go through registers into one of two LDS buffers, the next step's while
-// the present one is computed (one barrier a step). Row m of the K tile is the token whose number
+// 128 rows of one key head, 32 to each of four waves. Steps of 64 tokens: K [64][D] and V^T [D][64]
+// are copied into one of two LDS buffers without passing through registers, the next step's while
+// the present one is computed (one barrier a step).
+// The matrix cores bound it, and what stands beside them in a step: at D = 128, two waves on a SIMD, a wave's
+// step takes 4300 clocks, of which its products would take 1024; the issue of its 8 copies 1400, the
+// first product 770, the maximum 360, the second product with the exponentials 1000, the barrier 300.
+// Measured: 12 heads of 128, a prompt of 8192 tokens 248 us (832 TFLOP/s), of 4096 90 us (568), of 2048
+// 36 us and 7 of the join; 512 new tokens at 30000 140 us. Eight waves on 256 rows, which halve the
+// copies, take 264 us for the 8192. Row m of the K tile is the token whose number
 // within its 16 has bits 2 and 3 of m swapped, which leaves lane half e = lane / 32 with the scores of
 // tokens 16 b + 8 e .. + 7: its k of the second product. The 16-byte chunks of an LDS row are
 // permuted, so that the 16 lanes that read at a time, on 16 different rows, meet all 64 banks: in rows
@@ -625,7 +634,9 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
 }
 
 // ------------------------------------------------------------------ join
-// D / 4 threads per row (token and query head), four channels each. With few ranges a workgroup takes
+// D / 4 threads per row (token and query head), four channels each. Bound by the read of the ranges'
+// results, which the caches still hold (7 us for 2048 tokens of 12 heads in two ranges, 50 MB), and by its
+// chain of loads when they are few (3.1 us for 12 rows of nine). With few ranges a workgroup takes
 // as many rows as fit (ALONE); with many it takes one row, its groups of threads alternate ranges,
 // added in order through LDS.
 #define ATTN_MAX_SPLITS 64
@@ -736,7 +747,8 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   PP_REQUIRE(q && q_strides && out_bf16, PP_ERR_INVALID, "%s: null pointer", what);
   PP_REQUIRE((((uintptr_t)q | (uintptr_t)out_bf16) & 15) == 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0,
              PP_ERR_INVALID, "%s: every head of q and out must start on a 16-byte boundary", what);
-  PP_REQUIRE(std::isfinite(scale), PP_ERR_INVALID, "%s: scale %g", what, scale);
+  const float c = fabsf(scale) * 1.4426950408889634f;
+  PP_REQUIRE(std::isfinite(c), PP_ERR_INVALID, "%s: scale %g", what, scale);
   const AttnPlan p = attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D);
   const size_t need = attn_ws_bytes(p, n_tokens * Hq, D);
   PP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PP_ERR_INVALID,
@@ -746,25 +758,28 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.q = (const bf16_t*)q, a.qs[0] = q_strides[0], a.qs[1] = q_strides[1];
   a.k = (const bf16_t*)k_pages, a.v = (const bf16_t*)v_pages;
   a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv;
-  a.c = std::max(fabsf(scale) * 1.4426950408889634f, 1e-37f), a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.c = std::max(c, 1e-37f), a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
   a.splits = p.splits, a.least = p.least, a.tiles = (int)p.tiles;
   a.po = (float*)workspace;
   a.pml = a.po + n_tokens * Hq * p.splits * D;
   a.pns = (int*)(a.pml + n_tokens * Hq * p.splits * 2);
-  const int64_t items = p.tiles * Hkv * p.splits;
-  PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld tiles (at most 2^24 - 1)", what, (long long)items);
+  const int64_t items = p.tiles * Hkv * p.splits, rows = n_tokens * Hq;
+  const bool alone = p.splits <= ATTN_JOIN_ALONE;
+  // (the join's are never more: calls of 16-row tiles have at most 8 rows to a tile, and one of more than 8
+  // ranges has as many workgroups; 128-row tiles are cut into ranges only where they are fewer than the GPU holds)
+  PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld workgroups (at most 2^24 - 1)", what, (long long)items);
+  const int64_t joins = alone ? (rows * (D / 4) + ATTN_THREADS - 1) / ATTN_THREADS : rows;
   hipStream_t st = (hipStream_t)stream;
-  const unsigned n = (unsigned)items;
-  const int64_t rows = n_tokens * Hq;
+  const unsigned n = (unsigned)items, nj = (unsigned)joins;
 #define ATTN(D_)                                                                          \
   do {                                                                                    \
     if (p.rows == 16) attn_few_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                 \
     else attn_many_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                            \
-    if (p.splits > ATTN_JOIN_ALONE)                                                       \
-      attn_join_kernel<D_, false><<<(unsigned)rows, ATTN_THREADS, 0, st>>>(a, rows);      \
-    else if (p.splits > 1)                                                                \
-      attn_join_kernel<D_, true><<<(unsigned)((rows * (D_ / 4) + ATTN_THREADS - 1) / ATTN_THREADS), ATTN_THREADS, 0, st>>>(a, rows); \
+    if (p.splits > 1) {                                                                   \
+      if (alone) attn_join_kernel<D_, true><<<nj, ATTN_THREADS, 0, st>>>(a, rows);        \
+      else attn_join_kernel<D_, false><<<nj, ATTN_THREADS, 0, st>>>(a, rows);             \
+    }                                                                                     \
   } while (0)
   if (D == 64) ATTN(64);
   else ATTN(128);

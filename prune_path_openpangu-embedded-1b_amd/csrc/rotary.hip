@@ -11,7 +11,10 @@
 // 2^-24 of the angle: 0.06 rad at a million radians.
 //
 // Memory bound: one read, one write. cos and sin of a workgroup's tokens are computed once into
-// LDS, then its threads stream the tokens' heads in 16-byte vectors, 8 pairs a step.
+// LDS, then its threads stream the tokens' heads in 16-byte vectors, 8 pairs a step, the next step's
+// loads ahead of the present one's stores. bf16, 8192 tokens of 36 heads of 128 (151 MB): 28.5 us,
+// 5.3 TB/s, where a large copy reaches 5.05; float32, 16384 tokens of 12 heads (201 MB): 49.6 us,
+// 4.1 TB/s; one token 2.2 us, a launch.
 #include <algorithm>
 
 #include "paged.h"
@@ -237,6 +240,9 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
 // channels, and writes them as two 16-byte vectors a channel; a group that is not full writes its
 // tokens' elements one by one. The waves of a value item take its four groups, so that in pages of 64
 // and more the 128 bytes of a channel leave the same L2 together.
+// Bound by memory for chunks (8192 tokens of 36 heads, 151 MB: 37 us, 4.1 TB/s; the rotation alone of as
+// many bytes 28.5), by the chain offsets, table, rows for single tokens (3.9 us for one, 5.4 for 64, 9.1
+// for 256 of them).
 #define APP_THREADS ROT_THREADS
 #define APP_TOKENS 16
 

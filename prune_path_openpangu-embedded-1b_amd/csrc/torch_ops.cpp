@@ -481,6 +481,50 @@ void same_device(const char* name, const Tensor& ref, std::initializer_list<cons
   }
 }
 
+// The stride of a dimension as the kernels take it: that of one of a single element says nothing, and must
+// not fail the checks of alignment.
+int64_t step(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// The bytes from a tensor's first element to its last.
+struct Span {
+  uintptr_t first, end;
+  explicit Span(const Tensor& t) : first((uintptr_t)t.data_ptr()), end(first) {
+    int64_t n = 1;
+    const auto sizes = t.sizes(), strides = t.strides();
+    for (size_t i = 0; i < sizes.size(); ++i) {
+      if (sizes[i] == 0) return;
+      n += (sizes[i] - 1) * strides[i];
+    }
+    end += (uintptr_t)(n * (int64_t)t.element_size());
+  }
+};
+
+// What a call writes lies apart from what it reads, but for an output that is the input itself.
+void apart(const char* name, const Span& out, const Span& in) {
+  TORCH_CHECK(out.end <= in.first || in.end <= out.first, "prunepath.", name, ": an output overlaps another argument");
+}
+bool same_rows(const Tensor& out, const Tensor& in) {
+  return out.data_ptr() == in.data_ptr() && out.scalar_type() == in.scalar_type() && in.is_contiguous();
+}
+
+// No gradient goes through these ops; a call that would need one is refused.
+void inference_only(const char* name, std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(t == nullptr || !t->requires_grad(), "prunepath.", name,
+                ": inference only, but an argument requires a gradient (call it under torch.no_grad())");
+}
+
+// x with channels next to each other, and an empty result of its shape that has them so: the strides are the
+// same for real and for fake tensors.
+Tensor rotary_input(const Tensor& x) {
+  return x.sym_size(-1) > 1 && x.sym_stride(-1) != 1 ? x.contiguous() : x;
+}
+Tensor rotary_output(const Tensor& in) {
+  Tensor out = at::empty_like(in);
+  return out.sym_size(-1) > 1 && out.sym_stride(-1) != 1 ? at::empty_symint(in.sym_sizes(), in.options()) : out;
+}
+
 // x [N, heads, D] or [B, L, heads, D] with positions of the leading shape. Strides go to the kernel;
 // only channels that are not next to each other are copied first.
 Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
@@ -495,14 +539,13 @@ Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_fr
               "prunepath.rotary: inv_freq must be contiguous float64 [rotary_dim / 2]");
   same_device("rotary", x, {&x, &positions, &inv_freq});
   const c10::DeviceGuard g(x.device());
-  const Tensor in = x.size(-1) > 1 && x.stride(-1) != 1 ? x.contiguous() : x;
-  Tensor out = at::empty_like(in);
-  if (out.size(-1) > 1 && out.stride(-1) != 1) out = at::empty(in.sizes(), in.options());
+  const Tensor in = rotary_input(x);
+  Tensor out = rotary_output(in);
   const int64_t d = in.dim();
   const bool four = d == 4;
-  const int64_t xs[3] = {four ? in.stride(0) : 0, in.stride(d - 3), in.stride(d - 2)};
-  const int64_t ys[3] = {four ? out.stride(0) : 0, out.stride(d - 3), out.stride(d - 2)};
-  const int64_t ps[2] = {four ? positions.stride(0) : 0, positions.stride(d - 3)};
+  const int64_t xs[3] = {four ? step(in, 0) : 0, step(in, d - 3), step(in, d - 2)};
+  const int64_t ys[3] = {four ? step(out, 0) : 0, step(out, d - 3), step(out, d - 2)};
+  const int64_t ps[2] = {four ? step(positions, 0) : 0, step(positions, d - 3)};
   check_rc(pp_rotary(in.data_ptr(), x_code(in, "rotary"), xs, positions.data_ptr(),
                      positions.scalar_type() == at::kLong, ps, four ? in.size(0) : 1, in.size(d - 3),
                      (int)in.size(d - 2), (int)in.size(d - 1), inv_freq.data_ptr<double>(), (int)(2 * inv_freq.numel()),
@@ -512,7 +555,7 @@ Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_fr
 }
 
 Tensor rotary_meta(const Tensor& x, const Tensor&, const Tensor&, c10::string_view, double, bool) {
-  return at::empty_like(x);
+  return rotary_output(rotary_input(x));
 }
 
 // The op's gradient in x is the op with the opposite angles, which has a gradient in its turn.
@@ -547,6 +590,8 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
                        double mscale, bool inverse) {
+  TORCH_CHECK(!c10::GradMode::is_enabled() || !inv_freq.requires_grad(),
+              "prunepath.rotary: no gradient in inv_freq");
   if (c10::GradMode::is_enabled() && x.requires_grad())
     return RotaryFunction::apply(x, positions, inv_freq, layout, mscale, inverse);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -602,15 +647,30 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   if (inv_freq)
     TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
                 "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
+  inference_only(name, {q ? &*q : nullptr, q ? &*q_out : nullptr, &k, &v, &k_pages, &v_pages, inv_freq ? &*inv_freq : nullptr});
+  const Span sk(k), sv(v), kp(k_pages), vp(v_pages);
+  for (const Span* in : {&sk, &sv}) {
+    apart(name, kp, *in);
+    apart(name, vp, *in);
+  }
+  apart(name, kp, vp);
   int64_t qs[2] = {0, 0};
   if (q) {
     TORCH_CHECK(q_out->scalar_type() == at::kBFloat16 && q_out->sizes() == q->sizes() && q_out->is_contiguous(),
                 "prunepath.kv_append: q_out must be contiguous bfloat16 of q's shape");
     same_device(name, k, {&*q, &*q_out});
-    qs[0] = q->stride(0), qs[1] = q->stride(1);
+    const Span sq(*q);
+    apart(name, kp, sq);
+    apart(name, vp, sq);
+    if (!zero_tail) {  // a given q_out
+      const Span so(*q_out);
+      for (const Span* in : {&sk, &sv, &kp, &vp}) apart(name, so, *in);
+      if (!same_rows(*q_out, *q)) apart(name, so, sq);
+    }
+    qs[0] = step(*q, 0), qs[1] = step(*q, 1);
   }
   const c10::DeviceGuard g(k.device());
-  const int64_t ks[2] = {k.stride(0), k.stride(1)}, vs[2] = {v.stride(0), v.stride(1)};
+  const int64_t ks[2] = {step(k, 0), step(k, 1)}, vs[2] = {step(v, 0), step(v, 1)};
   check_rc(pp_kv_append(q ? q->data_ptr() : nullptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, x_code(k, name), p.n,
                         (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
                         block_table.data_ptr<int32_t>(), (int)p.max_pages, (int)p.pages, (int)p.page, (int)p.Hq,
@@ -661,12 +721,19 @@ void attention_into(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, q.size(0), q.size(1), q.size(2));
   need_gpu(name, q, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &out});
   same_device(name, q, {&q});
+  inference_only(name, {&q, &k_pages, &v_pages, &out});
+  if (!zero_tail) {  // a given out
+    const Span so(out);
+    apart(name, so, Span(k_pages));
+    apart(name, so, Span(v_pages));
+    if (!same_rows(out, q)) apart(name, so, Span(q));
+  }
   const c10::DeviceGuard g(q.device());
   const size_t need = pp_paged_attention_workspace_bytes(p.n, (int)p.seqs, (int)p.max_pages, (int)p.page, (int)p.Hq,
                                                          (int)p.Hkv, (int)p.D);
   Tensor ws;
   if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
-  const int64_t qs[2] = {q.stride(0), q.stride(1)};
+  const int64_t qs[2] = {step(q, 0), step(q, 1)};
   check_rc(pp_paged_attention(q.data_ptr(), qs, p.n, (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
                               block_table.data_ptr<int32_t>(), (int)p.max_pages, k_pages.data_ptr(), v_pages.data_ptr(),
                               (int)p.pages, (int)p.page, (int)p.Hq, (int)p.Hkv, (int)p.D, (float)scale, out.data_ptr(),
@@ -787,7 +854,7 @@ TORCH_LIBRARY_IMPL(prunepath, Meta, m) {
 
 TORCH_LIBRARY_IMPL(prunepath, Autograd, m) {
   m.impl("rotary", &rotary_autograd);
-  // inference: no gradient is recorded
+  // inference: the kernels refuse arguments that require a gradient (inference_only)
   for (const char* name : {"kv_append", "kv_append_q", "kv_append_q_into", "paged_attention", "paged_attention_into"})
     m.impl(name, torch::CppFunction::makeFallthrough());
 }

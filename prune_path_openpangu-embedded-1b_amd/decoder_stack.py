@@ -238,9 +238,16 @@ def generate(model: DecoderStack, prompts: List[torch.Tensor], steps: int, chunk
     steps of the batch (the step captured in a graph and replayed, or eager). ``model`` in eval mode,
     reordered for inference, with attention heads of 64 or 128 channels."""
     lengths = [int(p.numel()) for p in prompts]
-    if steps < 1 or not prompts or min(lengths) < 1:
-        raise ValueError("generate: at least one step and prompts of at least one token")
-    dev, attn = model.embed_tokens.weight.device, model.layers[0].self_attn
+    if steps < 1 or chunk < 1 or not prompts or min(lengths) < 1 or any(p.dim() != 1 for p in prompts):
+        raise ValueError("generate: at least one step, chunks and 1-D prompts of at least one token")
+    dev = model.embed_tokens.weight.device
+    with torch.cuda.device(dev):  # streams and the graph are the current device's
+        return _generate(model, prompts, lengths, steps, chunk, page_size, capture, dev)
+
+
+@torch.no_grad()
+def _generate(model, prompts, lengths, steps, chunk, page_size, capture, dev):
+    attn = model.layers[0].self_attn
     kv = PagedKV(len(model.layers), len(prompts), max(lengths) + steps, attn.h, attn.hd, page_size, dev)
     tok_t = torch.zeros(len(prompts), dtype=torch.int64, device=dev)
     for at in range(0, max(lengths), chunk):

@@ -406,8 +406,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     no token: what falls there is dropped. No two tokens of a call may have the same place.
 
     q [N, heads, D]: turned as k is, returned as bf16 [N, heads, D] (in ``q_out``, which may be q
-    itself, if given). Rows behind cu_q[seqs] append nothing; in a new result they are zeros, in
-    q_out they stay. inference only: no gradient."""
+    itself, if given; other overlaps of what is written are refused). Rows behind cu_q[seqs] append
+    nothing; in a new result they are zeros, in q_out they stay. Inference only: arguments that require
+    a gradient are refused outside torch.no_grad()."""
     ops = L.torch_ops()
     if q is None:
         if q_out is not None:
@@ -427,10 +428,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     paged cache: the token at position p attends the positions 0 .. p of its sequence, query head h
     the key head h // (heads / kv_heads). q bf16 [N, heads, D] -> bf16 [N, heads, D]
     (``torch.ops.prunepath.paged_attention``, or ``paged_attention_into`` writing ``out``); scale
-    defaults to D^-0.5. Scores and softmax in fp32. A row that attends nothing is zero. Rows behind
-    cu_q[seqs] are zero in a new result and stay in ``out``. Single tokens, chunks and whole prompts,
-    in one call; lengths are read on the device, so a captured call serves lengths that grow.
-    Inference only: no gradient."""
+    defaults to D^-0.5. Scores and softmax in fp32. A row that attends nothing, or whose scores are all
+    -inf, is zero. Rows behind cu_q[seqs] are zero in a new result and stay in ``out`` (which may be q
+    itself; other overlaps are refused). Single tokens, chunks and whole prompts, in one call; lengths
+    are read on the device, so a captured call serves lengths that grow. Inference only: arguments that
+    require a gradient are refused outside torch.no_grad()."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     ops = L.torch_ops()

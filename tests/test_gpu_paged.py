@@ -515,6 +515,59 @@ def test_paged_refusals(pkg):
             bad()
 
 
+def test_gradients_and_overlaps_are_refused(pkg):
+    ops = pkg.ops
+    kp, vp, table, lens, cu = Batch([2], [20], 16, 2, 64).gpu()
+    cache = (kp, vp, table, lens, cu)
+    x = torch.ones(2, 2, 64, dtype=torch.bfloat16, device=dev())
+    f = ops.rotary_frequencies(64)[0].to(dev())
+    want = x.clone().requires_grad_()
+    pos = torch.arange(2, device=dev())
+    rows = torch.zeros(5, 2, 64, dtype=torch.bfloat16, device=dev())
+    for bad in (lambda: ops.paged_attention(want, *cache), lambda: ops.paged_attention(x, *cache, out=want),
+                lambda: ops.kv_append(want, x, *cache), lambda: ops.kv_append(x, want, *cache),
+                lambda: ops.kv_append(x, x, *cache, q=want), lambda: ops.rotary(x, pos, f.clone().requires_grad_()),
+                lambda: ops.paged_attention(rows[:2], *cache, out=rows[1:3]),
+                lambda: ops.paged_attention(x, *cache, out=kp[0, 0, :4].view(2, 2, 64)),
+                lambda: ops.kv_append(x, x, *cache, q=rows[:2], q_out=rows[1:3]),
+                lambda: ops.kv_append(x, x, *cache, q=x, q_out=x),  # q itself, but k and v too
+                lambda: ops.kv_append(x, x, kp, kp.view(vp.shape), table, lens, cu),
+                lambda: ops.kv_append(kp[0, 0, :4].view(2, 2, 64), x, *cache)):
+        with pytest.raises(RuntimeError, match="prunepath.*(gradient|overlaps)"):
+            bad()
+    with torch.no_grad():
+        a = ops.paged_attention(want, *cache)
+    b = x.clone()
+    assert ops.paged_attention(b, *cache, out=b) is b and torch.equal(a, b)  # q itself
+
+
+def test_strides_of_single_rows_and_heads_say_nothing(pkg):
+    """One token or one head at a stride that is no multiple of 8 elements."""
+    ops = pkg.ops
+    f = ops.rotary_frequencies(64)[0]
+    kp, vp, table, lens, cu = Batch([1], [20], 16, 1, 64).gpu()
+    x = torch.randn(64, generator=gen(3)).to(torch.bfloat16).to(dev())
+    odd, even = x.as_strided((1, 1, 64), (77, 33, 1)), x.clone().view(1, 1, 64)
+    assert torch.equal(ops.kv_append(odd, odd, kp, vp, table, lens, cu, f.to(dev()), q=odd),
+                       ops.kv_append(even, even, kp, vp, table, lens, cu, f.to(dev()), q=even))
+    assert torch.equal(ops.paged_attention(odd, kp, vp, table, lens, cu),
+                       ops.paged_attention(even, kp, vp, table, lens, cu))
+    check_turn(ops.rotary(odd, torch.full((1,), 7, device=dev()), f.to(dev())), odd, torch.full((1,), 7), f, "half")
+
+
+def test_rows_of_nothing_but_minus_infinity(pkg):
+    """Scores of -inf for every attended token give zeros, a single finite one that token's value."""
+    for new in (2, 40):
+        b = Batch([new], [60], 16, 1, 64, seed=9)
+        kp, vp, table, lens, cu = b.gpu()
+        q = torch.ones(new, 1, 64, dtype=torch.bfloat16, device=dev())
+        kp.fill_(float("-inf"))
+        assert not pkg.ops.paged_attention(q, kp, vp, table, lens, cu).any()
+        page, place = int(b.table[0, 5 // 16]), 5
+        kp[page, 0, place] = 0
+        assert torch.equal(pkg.ops.paged_attention(q, kp, vp, table, lens, cu)[:, 0], vp[page, 0, :, place].expand(new, 64))
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(12, 12, 128, 16), (6, 2, 64, 32)])
 def test_chunks_then_tokens_as_a_server_runs_them(pkg, heads, kv_heads, dim, page):

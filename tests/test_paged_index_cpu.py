@@ -80,6 +80,28 @@ def test_append_groups_cover_every_token_once():
         assert len(seen) == N
 
 
+def test_append_value_items_cover_every_token_once():
+    """Items of 64 positions: their four groups to the four waves, or the one group that has tokens to all."""
+    for cu, N, kv in batches():
+        B = len(cu) - 1
+        seen = {}
+        for t in range((N >> 6) + 2 * (B + 1)):
+            first = lambda c, s: (c >> 6) + 2 * s  # noqa: E731
+            s = seq_of(cu, N, t, first)
+            c0 = start(cu, s, N)
+            length = max(start(cu, s + 1, N) - c0, 0)
+            p = 0 if s == B else kv[s] - length
+            at = ((p >> 6) + t - first(c0, s)) << 6
+            begin = max(at, p & ~15)
+            alone = min(at + 64, p + length) - begin <= 16
+            for p0 in [begin] if alone else range(at, at + 64, 16):
+                for i in range(max(0, p - p0), min(16, p + length - p0)):
+                    row = c0 + (p0 - p) + i
+                    assert c0 <= row < c0 + length and row not in seen
+                    seen[row] = p0 & 15
+        assert len(seen) == N and not any(seen.values())  # groups start at multiples of 16: in one page
+
+
 def test_offsets_out_of_order_stay_inside():
     rng = random.Random(3)
     for _ in range(200):
@@ -234,3 +256,36 @@ def test_shapes_without_a_gpu():
     assert t.kv_append_q_into(q, r, kv, kv, *cache, f) is None
     assert t.paged_attention(r, *cache, 0.1).shape == r.shape
     assert t.paged_attention_into(r, *cache, 0.1, r) is None
+
+
+def test_rotary_strides_without_a_gpu():
+    """A fake result has the strides of the real one: the input's where its channels are next to each other,
+    contiguous otherwise."""
+    import torch
+    t = import_pkg()._lib.torch_ops()
+    f, pos = torch.empty(32, dtype=torch.float64, device="meta"), torch.empty(3, 5, dtype=torch.int64, device="meta")
+    for make, want in ((lambda z: z(3, 4, 5, 64).transpose(1, 2), (1280, 64, 320, 1)),
+                       (lambda z: z(3, 5, 64, 4).transpose(2, 3), (1280, 256, 64, 1)),
+                       (lambda z: z(3, 5, 9, 64)[:, :, :4], (1280, 256, 64, 1))):
+        assert t.rotary(make(lambda *n: torch.empty(*n, device="meta")), pos, f).stride() == want
+
+
+def test_generate_refusals():
+    import torch
+    ds = import_pkg().decoder_stack
+    one = torch.ones(3, dtype=torch.int64)
+    for kw in (dict(prompts=[one], steps=0), dict(prompts=[], steps=2), dict(prompts=[one[:0]], steps=2),
+               dict(prompts=[one], steps=2, chunk=0), dict(prompts=[one], steps=2, chunk=-4),
+               dict(prompts=[one.view(1, 3)], steps=2)):
+        with pytest.raises(ValueError, match="generate"):
+            ds.generate(None, **kw)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 3.0e38])
+def test_scales_beyond_float32_are_refused(scale):
+    assert _lib().pp_paged_attention(P, S2, 4, 2, P, P, P, 64, P, P, 9, 16, 4, 2, 128, scale, P, 0, P, 1 << 30, None) == 1
+
+
+def test_launches_beyond_the_grid_are_refused():
+    rc = _lib().pp_paged_attention(P, S2, 1 << 20, 1 << 20, P, P, P, 600, P, P, 9, 16, 32, 2, 64, 0.1, P, 0, P, 1 << 62, None)
+    assert rc == 3 and "workgroups" in _lib().pp_last_error().decode()
