@@ -93,6 +93,12 @@ __device__ __forceinline__ int64_t attn_row(const AttnArgs& a, const AttnTile& w
   return (int64_t)(w.c0 + i) * a.Hq + h * a.group + (w.r0 + r - i * a.group);
 }
 
+// The queries of row r.
+__device__ __forceinline__ const bf16_t* attn_query(const AttnArgs& a, const AttnTile& w, int h, int r) {
+  const int i = (w.r0 + r) / a.group;
+  return a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1];
+}
+
 // Last position that row r attends.
 __device__ __forceinline__ int attn_limit(const AttnArgs& a, const AttnTile& w, int r) {
   return (int)min(w.p0 + (w.r0 + r) / a.group, (int64_t)a.seqs.capacity() - 1);
@@ -202,11 +208,18 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   int pk, pv;                                 // their pages, -1: none
   int pc;                                     // the present V's
   a_u4 kf[2][KS], vf[MB];
+  // Loads are asked for without a branch, of the last row or entry where there is none: with one, the
+  // wait for each stands where the two sides meet.
+  const int32_t* const table = a.seqs.table + (int64_t)w.s * a.seqs.max_pages;
+  const int last_entry = (w.hi - 1) >> a.seqs.lp;
   auto entries = [&](int t) {
-    ek = t + gk < w.hi ? a.seqs.entry(w.s, (t + gk) >> a.seqs.lp) : -1;
-    ev = t + gv < w.hi ? a.seqs.entry(w.s, (t + gv) >> a.seqs.lp) : -1;
+    ek = table[min((t + gk) >> a.seqs.lp, last_entry)];
+    ev = table[min((t + gv) >> a.seqs.lp, last_entry)];
   };
-  auto pages = [&] { pk = a.seqs.page(ek), pv = a.seqs.page(ev); };
+  auto pages = [&](int t) {
+    pk = t + gk < w.hi ? a.seqs.page(ek) : -1;
+    pv = t + gv < w.hi ? a.seqs.page(ev) : -1;
+  };
   // places without a page read page 0, and are masked
   auto load_k = [&](int t) {
     const bf16_t* kp = a.k + ((((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((t + gk) & (ps - 1)) + (col & 3)) * D + 8 * g;
@@ -226,20 +239,19 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   };
   int t = w.lo + 32 * wave;
   entries(t);
-  pages();
-  entries(t + 128);
-  load_k(t);
-  load_v(t);
-
   a_u4 qf[KS];
   const bool in = col < w.nr;
   const int limit = in ? attn_limit(a, w, col) : a.seqs.capacity();
-  {
-    const int i = (w.r0 + col) / a.group;
-    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + col - i * a.group) * a.qs[1];
+  const bf16_t* const src = attn_query(a, w, h, min(col, w.nr - 1)) + 8 * g;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = in ? *(const a_u4*)(src + 32 * s + 8 * g) ^ a.flip : a_mk(0, 0, 0, 0);
-  }
+  for (int s = 0; s < KS; ++s) qf[s] = *(const a_u4*)(src + 32 * s);
+  paged_asked();
+  pages(t);
+  entries(t + 128);
+  load_k(t);
+  load_v(t);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = in ? qf[s] ^ a.flip : a_mk(0, 0, 0, 0);
   const int low = attn_limit(a, w, 0);  // every row attends the tokens up to here
 
   f32x4_t o[MB];
@@ -248,7 +260,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   for (int b = 0; b < MB; ++b) o[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
   for (; t < w.hi; t += 128) {
-    pages();
+    pages(t + 128);
     entries(t + 256);
     f32x4_t s[2];
 #pragma unroll
@@ -427,10 +439,12 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   // next. Lanes 0 .. 7 have vc = lane ^ of_odd: lane 2 j ^ of_odd has group j's.
   const int of_odd = 4 * (wave & 1);
   int pg, pn, en;  // en: the table entry of the step after the next
-  auto entry = [&](int t) {
-    const int at = t + 16 * (vc >> 1);
-    en = at < w.hi ? a.seqs.entry(w.s, at >> a.seqs.lp) : -1;
-  };
+  const int32_t* const table = a.seqs.table + (int64_t)w.s * a.seqs.max_pages;
+  const int last_entry = (w.hi - 1) >> a.seqs.lp;
+  // The entry is asked for without a branch, beyond the range for its last one's: with one, the wait for it
+  // stood where the two sides meet, behind the copies, and so for all of them (8192 tokens 248 us).
+  auto entry = [&](int t) { en = table[min((t + 16 * (vc >> 1)) >> a.seqs.lp, last_entry)]; };
+  auto page = [&](int t) { return t + 16 * (vc >> 1) < w.hi ? a.seqs.page(en) : -1; };
   const uint32_t k_lds = attn_lds(&k_s[0][64 * wave]), v_lds = attn_lds(&v_s[0][64 * wave]);
   auto load = [&](int t, int buf) {  // places without a page read page 0, and are masked
 #pragma unroll
@@ -453,16 +467,16 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   int t = w.lo, buf = 0;
   if (tid < 2) bad_s[tid] = -1;
   entry(t);
-  pn = a.seqs.page(en);
+  a_u4 qf[D / 16];
+  const bf16_t* const src = attn_query(a, w, h, min(r, w.nr - 1)) + 8 * e;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) qf[s] = *(const a_u4*)(src + 16 * s);
+  paged_asked();
+  pn = page(t);
   entry(t + ATTN_KT);
   load(t, 0);
-  a_u4 qf[D / 16];
-  {
-    const int i = (w.r0 + r) / a.group;
-    const bf16_t* src = a.q + (int64_t)(w.c0 + i) * a.qs[0] + (int64_t)(h * a.group + w.r0 + r - i * a.group) * a.qs[1] + 8 * e;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) qf[s] = in ? *(const a_u4*)(src + 16 * s) ^ a.flip : a_mk(0, 0, 0, 0);
-  }
+  for (int s = 0; s < D / 16; ++s) qf[s] = in ? qf[s] ^ a.flip : a_mk(0, 0, 0, 0);
   f32x16_t o[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b)
@@ -473,11 +487,9 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
     attn_landed();  // the present step is in its buffer, and every wave is done with the other one
     const bool more = t + ATTN_KT < w.hi;
     pg = pn;
-    if (more) {
-      pn = a.seqs.page(en);
-      entry(t + 2 * ATTN_KT);
-      load(t + ATTN_KT, buf ^ 1);
-    }
+    pn = page(t + ATTN_KT);
+    entry(t + 2 * ATTN_KT);
+    if (more) load(t + ATTN_KT, buf ^ 1);
     // a step with a masked place: only the finite part of V, and a mark where there is another
     const bool masked = t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(pg < 0);
     if (masked) {

@@ -39,6 +39,9 @@ struct PagedSeqs {
   __device__ int capacity() const { return max_pages << lp; }  // at most 2^30 (checked by the host)
 };
 
+// The loads above are not moved below this line, to where their values are used.
+__device__ __forceinline__ void paged_asked() { asm volatile("" ::: "memory"); }
+
 // The sequence that work item t belongs to, where sequence s has the items first(start(s), s)
 // and on: the last s with first(start(s), s) <= t. `first` grows with s, by at least the items that
 // the sequence has, so the item space needs no prefix sum. Every wave finds it for itself, 256
@@ -54,18 +57,21 @@ __device__ __forceinline__ PagedSeq paged_find(const PagedSeqs& q, int64_t t, F 
   const int lane = threadIdx.x & 63;
   int n = 0, s0 = 0;
   int c[4], k[4];
+  const int32_t* const lens = q.n_seqs ? q.kv_lens : q.cu_q;  // (of no sequence: an address that can be read)
   for (;; s0 += 256) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {  // no branches: all eight loads are on their way together
       const int s = s0 + 64 * i + lane;
-      c[i] = s > 0 && s <= q.n_seqs ? q.cu_q[s] : s > 0 ? q.n_rows : 0;
-      k[i] = s < q.n_seqs ? q.kv_lens[s] : 0;
+      c[i] = q.cu_q[min(s, q.n_seqs)];
+      k[i] = lens[max(min(s, q.n_seqs - 1), 0)];
     }
+    paged_asked();
     int m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int s = s0 + 64 * i + lane;
-      c[i] = min(max(c[i], 0), q.n_rows);
+      c[i] = s == 0 ? 0 : s > q.n_seqs ? q.n_rows : min(max(c[i], 0), q.n_rows);
+      k[i] = s < q.n_seqs ? k[i] : 0;
       m += __popcll(__ballot(s <= q.n_seqs && first(c[i], s) <= t));
     }
     n += m;
