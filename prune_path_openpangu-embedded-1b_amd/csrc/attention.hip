@@ -486,6 +486,16 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   while (true) {
     attn_landed();  // the present step is in its buffer, and every wave is done with the other one
     const bool more = t + ATTN_KT < w.hi;
+    // operands of the first product, two k steps at a time: the first two's are on their way before the
+    // copies, the next two's before the present two's products
+    const a_u4* const kb = kb0 + buf * (ATTN_KT * KC);
+    a_u4 xk[2][4];
+    auto get_k = [&](a_u4 (&f)[4], int q) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = kb[32 * (i & 1) * KC + ((2 * (q + (i >> 1)) + e) ^ ksw)];
+    };
+    get_k(xk[0], 0);
+    __builtin_amdgcn_sched_barrier(0);
     pg = pn;
     pn = page(t + ATTN_KT);
     entry(t + 2 * ATTN_KT);
@@ -510,26 +520,27 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int q = 0; q < 16; ++q) s[b][q] = 0.0f;
-      const a_u4* const kb = kb0 + buf * (ATTN_KT * KC);
-      // operands of two k steps at a time, the next two's on their way
-      a_u4 x[2][4];
-      auto get = [&](a_u4 (&f)[4], int q) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = kb[32 * (i & 1) * KC + ((2 * (q + (i >> 1)) + e) ^ ksw)];
-      };
-      get(x[0], 0);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int q = 0; q < D / 16; q += 2) {
-        if (q + 2 < D / 16) get(x[((q >> 1) + 1) & 1], q + 2);
+        if (q + 2 < D / 16) get_k(xk[((q >> 1) + 1) & 1], q + 2);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i & 1] = mfma32a(x[(q >> 1) & 1][i], qf[q + (i >> 1)], s[i & 1]);
+        for (int i = 0; i < 4; ++i) s[i & 1] = mfma32a(xk[(q >> 1) & 1][i], qf[q + (i >> 1)], s[i & 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
     }
     if (on) {
+      // the second product's first operands
+      const a_u4* const vb = vb0 + buf * (D * 8);
+      a_u4 x[2][MB], pf[2];
+      auto get = [&](a_u4 (&f)[MB], int kk) {
+#pragma unroll
+        for (int b = 0; b < MB; ++b) f[b] = vb[32 * b * 8 + ((2 * kk + e) ^ vsw)];
+      };
+      get(x[0], 0);
+      __builtin_amdgcn_sched_barrier(0);
       const uint64_t have = __ballot(pg >= 0);  // bit 2 j ^ of_odd: group j
       const int last = min(limit, w.hi - 1) - t - 8 * e;  // of the lane's tokens, 16 (2 b + q / 8) + q % 8
       if (t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != ~0ull) {  // a masked place
@@ -566,19 +577,12 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       }
       // the second product, 16 tokens at a time: a product's time is that of a few of the next tokens'
       // exponentials, which stand between the products
-      const a_u4* const vb = vb0 + buf * (D * 8);
-      a_u4 x[2][MB], pf[2];
-      auto get = [&](a_u4 (&f)[MB], int kk) {
-#pragma unroll
-        for (int b = 0; b < MB; ++b) f[b] = vb[32 * b * 8 + ((2 * kk + e) ^ vsw)];
-      };
       auto weigh = [&](int kk, int j) {  // P of tokens 2 j and 2 j + 1 of 8
         const float u = s[kk >> 1][8 * (kk & 1) + 2 * j], v = s[kk >> 1][8 * (kk & 1) + 2 * j + 1];
         const float p0 = attn_exp2(__fmaf_rn(u, a.c, -m)), p1 = attn_exp2(__fmaf_rn(v, a.c, -m));
         l += p0 + p1;
         pf[kk & 1][j] = f32_to_bf16x2(p0, p1);
       };
-      get(x[0], 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) weigh(0, j);
       __builtin_amdgcn_s_setprio(1);
