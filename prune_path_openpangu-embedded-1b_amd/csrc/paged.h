@@ -29,11 +29,7 @@ struct PagedSeqs {
     if (s > n_seqs) return n_rows;
     return min(max(cu_q[s], 0), n_rows);
   }
-  // entry e of sequence s's table (-1 beyond it), and the page that it names, -1 for none: apart, so
-  // that a kernel can ask for entries well before it looks at them
-  __device__ int entry(int s, int64_t e) const {
-    return e < 0 || e >= max_pages ? -1 : table[(int64_t)s * max_pages + e];
-  }
+  // the page that an entry of the table names, -1 for none
   __device__ int page(int entry) const { return (unsigned)entry < (unsigned)num_pages ? entry : -1; }
   // positions that the table has room for
   __device__ int capacity() const { return max_pages << lp; }  // at most 2^30 (checked by the host)

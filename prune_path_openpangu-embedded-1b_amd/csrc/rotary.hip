@@ -96,6 +96,7 @@ struct RotUnit {
 #pragma unroll
       for (int i = 0; i < V; ++i) r[i] = rot_f32(p.v[i]);
       rot_store<V>(y + rd + (u - nr) * V, r);
+      asm volatile("");  // the two sides' last stores, merged, went out as 4 and 12 bytes
     }
   }
 };
@@ -279,6 +280,10 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
   const int h0 = value ? block * a.vper : (block - (kind ? a.nqb : 0)) * a.per;
   const int nh = min(value ? a.vper : a.per, (kind ? a.Hkv : a.Hq) - h0);
   const int lg = value ? 6 : 4;  // log2 of the item's positions
+  // what does not depend on the sequence is asked for before it is found, and further down the table's entry
+  // before the rows: the chain of loads is what a call of single tokens takes
+  const int half = a.rd / 2, pair = tid & ((1 << a.lgh) - 1);
+  const double freq = half ? a.inv_freq[min(pair, half - 1)] : 0.0;
   const PagedSeq f = paged_find(a.seqs, t, [lg](int c, int s) { return (int64_t)(c >> lg) + 2 * s; });
   const int s = f.s, c0 = f.c0, len = f.rows;
   const bool tail = s == a.seqs.n_seqs;  // rows of no sequence
@@ -304,15 +309,15 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
     return;
   }
   const int ps = 1 << a.seqs.lp;
-  int page = -1;
-  if (kind != 0) {
-    page = p0 < 0 ? -1 : a.seqs.page(a.seqs.entry(s, p0 >> a.seqs.lp));
-    if (page < 0) return;
-  }
+  const int64_t at = p0 >> a.seqs.lp;
+  const int entry = kind ? a.seqs.table[(int64_t)s * a.seqs.max_pages + min(max(at, (int64_t)0), (int64_t)a.seqs.max_pages - 1)] : 0;
+  paged_asked();
+  const bool place_ok = at >= 0 && at < a.seqs.max_pages;
+  auto no_page = [&] { return !place_ok || a.seqs.page(entry) < 0; };
   const int place = (int)(p0 & (ps - 1));
   if (kind == 2) {
     constexpr int P = D / 2;  // pairs of channels of a head
-    bf16_t* const to = a.v_pages + (((int64_t)page * a.Hkv + h0) * D << a.seqs.lp) + place;
+    bf16_t* const to = a.v_pages + (((int64_t)entry * a.Hkv + h0) * D << a.seqs.lp) + place;
     for (int k = alone ? tid : tid & 63; k < nh * P; k += alone ? APP_THREADS : 64) {
       const int h = k / P, d = 2 * (k - h * P);
       const T* src = (const T*)a.v + (int64_t)row0 * a.vs[0] + (h0 + h) * a.vs[1] + d;
@@ -321,6 +326,8 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
         uint32_t w[APP_TOKENS];
 #pragma unroll
         for (int i = 0; i < APP_TOKENS; ++i) w[i] = app_pair(src + i * a.vs[0]);
+        paged_asked();
+        if (no_page()) return;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -335,9 +342,14 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
           }
         }
       } else {
+        uint32_t w = app_pair(src + lo * a.vs[0]);
+        paged_asked();
+        if (no_page()) return;
+        dst[lo] = (bf16_t)w;
+        dst[lo + ps] = (bf16_t)(w >> 16);
 #pragma unroll 4
-        for (int i = lo; i < hi; ++i) {
-          const uint32_t w = app_pair(src + i * a.vs[0]);
+        for (int i = lo + 1; i < hi; ++i) {
+          w = app_pair(src + i * a.vs[0]);
           dst[i] = (bf16_t)w;
           dst[i + ps] = (bf16_t)(w >> 16);
         }
@@ -345,19 +357,22 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
     }
     return;
   }
-  const int half = a.rd / 2, nr = half / 8, per = nr + (D - a.rd) / 8;
+  const int nr = half / 8, per = nr + (D - a.rd) / 8;
   const RotLanes w(tid, a.lgu, 32 - __clz(nt - 1));  // as many tokens as there are
   const int64_t row = row0 + lo + w.i;
   const T* const x = (const T*)(kind == 0 ? a.q : a.k) + row * (kind == 0 ? a.qs[0] : a.ks[0]);
   const int64_t xs = kind == 0 ? a.qs[1] : a.ks[1];
   bf16_t* const y = kind == 0 ? a.q_out + row * a.Hq * D
-                              : a.k_pages + (((int64_t)page * a.Hkv << a.seqs.lp) + place + lo + w.i) * D;
+                              : a.k_pages + (((int64_t)entry * a.Hkv << a.seqs.lp) + place + lo + w.i) * D;
   const int64_t ys = kind == 0 ? D : (int64_t)D << a.seqs.lp;
   int h = h0 + w.h;
   bool more = w.i < nt && h < h0 + nh && w.u < per;
   RotUnit<T, 8, HALF> now, next;
   if (more) now.load(x + h * xs, w.u, nr, a.rd);
-  rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, 1.0f, [&](int t) { return p0 + lo + t; });
+  paged_asked();
+  if (pair < half)
+    for (int t = tid >> a.lgh; t < nt; t += APP_THREADS >> a.lgh) cs_s[t * half + pair] = rot_entry(p0 + lo + t, freq, a.mscale, 1.0f);
+  if (kind && no_page()) return;
   __syncthreads();
   while (more) {
     const int h2 = h + w.hstep;
