@@ -11,10 +11,10 @@
 // 2^-24 of the angle: 0.06 rad at a million radians.
 //
 // Memory bound: one read, one write. cos and sin of a workgroup's tokens are computed once into
-// LDS, then its threads stream the tokens' heads in 16-byte vectors, 8 pairs a step, the next step's
-// loads ahead of the present one's stores. bf16, 8192 tokens of 36 heads of 128 (151 MB): 28.5 us,
-// 5.3 TB/s, where a large copy reaches 5.05; float32, 16384 tokens of 12 heads (201 MB): 49.6 us,
-// 4.1 TB/s; one token 2.2 us, a launch.
+// LDS, then its threads stream the tokens' heads in 16-byte vectors, the next step's loads ahead of the
+// present one's stores. bf16, 8192 tokens of 36 heads of 128 (151 MB): 27.3 us, 5.5 TB/s, where a large
+// copy reaches 5.05; float32, 16384 tokens of 12 heads (201 MB): 38.0 us, 5.3 TB/s; one token 2.2 us, a
+// launch.
 #include <algorithm>
 
 #include "paged.h"
@@ -22,7 +22,7 @@
 #define ROT_THREADS 256
 #define ROT_TABLE 2048  // (cos, sin) entries in LDS
 
-// V consecutive elements as they are in memory (V = 8: in 16-byte words)
+// V consecutive elements as they are in memory (more than one: in 16-byte words)
 template <typename T, int V>
 struct RotPack {
   T v[V];
@@ -35,11 +35,10 @@ __device__ __forceinline__ float rot_f32(float x) { return x; }
 __device__ __forceinline__ float rot_f32(bf16_t x) { return bf16_to_f32(x); }
 template <int V>
 __device__ __forceinline__ void rot_store(float* p, const float (&v)[V]) {
-  if constexpr (V == 8) {
-    *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
-    *(float4*)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  } else
-    *p = v[0];
+  if constexpr (V == 1) *p = v[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *(float4*)(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
 }
 template <int V>
 __device__ __forceinline__ void rot_store(bf16_t* p, const float (&v)[V]) {
@@ -200,9 +199,11 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
   a.pb = pos_strides[0], a.pl = pos_strides[1];
   a.n = batch * length, a.L = (uint32_t)length, a.heads = heads;
   a.D = D, a.rd = rotary_dim, a.pos64 = pos64, a.mscale = mscale, a.sign = inverse ? -1.0f : 1.0f;
-  // 16-byte vectors where every head starts on one and the parts are whole vectors
-  const bool vec = rotary_dim % 16 == 0 && D % 8 == 0 && rot_aligned(x, a.xs, 3, bytes) && rot_aligned(y, a.ys, 3, bytes);
-  const int per = vec ? rotary_dim / 16 + (D - rotary_dim) / 8 : rotary_dim / 2 + D - rotary_dim;
+  // 16-byte vectors where every head starts on one and the parts are whole vectors. (float32 in steps of 8
+  // pairs, whose two loads of a vector each meet every other 16 bytes: 16384 tokens of 12 heads 50 us.)
+  const int V = 16 / bytes;
+  const bool vec = rotary_dim % (2 * V) == 0 && D % V == 0 && rot_aligned(x, a.xs, 3, bytes) && rot_aligned(y, a.ys, 3, bytes);
+  const int per = vec ? (rotary_dim / 2 + D - rotary_dim) / V : rotary_dim / 2 + D - rotary_dim;
   a.lgu = std::min(8, rot_log2up(per)), a.lgh = std::min(8, rot_log2up(rotary_dim / 2));
   // Enough tokens to keep a thread on four steps, as long as that leaves two workgroups for each CU;
   // a call smaller than that spreads every token's heads over workgroups of one step.
@@ -222,7 +223,7 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
     else rotary_kernel<T, V, false><<<grid, ROT_THREADS, 0, st>>>(a);                        \
   } while (0)
   if (dtype == PP_DTYPE_F32) {
-    if (vec) ROT(float, 8);
+    if (vec) ROT(float, 4);
     else ROT(float, 1);
   } else {
     if (vec) ROT(bf16_t, 8);
@@ -242,7 +243,7 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
 // tokens' elements one by one. The waves of a value item take its four groups, so that in pages of 64
 // and more the 128 bytes of a channel leave the same L2 together.
 // Bound by memory for chunks (8192 tokens of 36 heads, 151 MB: 37 us, 4.1 TB/s; the rotation alone of as
-// many bytes 28.5), by the chain offsets, table, rows for single tokens (3.9 us for one, 5.4 for 64, 9.1
+// many bytes 27.3), by the chain offsets, table, rows for single tokens (3.9 us for one, 5.4 for 64, 9.1
 // for 256 of them).
 #define APP_THREADS ROT_THREADS
 #define APP_TOKENS 16
