@@ -375,17 +375,19 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 // ------------------------------------------------------------------ many rows
 // 128 rows of one key head, 32 to each of four waves. Steps of 64 tokens: K [64][D] and V^T [D][64]
 // are copied into one of two LDS buffers without passing through registers, the next step's while
-// the present one is computed (one barrier a step).
-// The matrix cores bound it, and what stands beside them in a step: at D = 128, two waves on a SIMD, a wave's
-// step takes 4300 clocks, of which its products would take 1024; the issue of its 8 copies 1400, the
-// first product 770, the maximum 360, the second product with the exponentials 1000, the barrier 300.
-// Measured: 12 heads of 128, a prompt of 8192 tokens 248 us (832 TFLOP/s), of 4096 90 us (568), of 2048
-// 36 us and 7 of the join; 512 new tokens at 30000 140 us. Eight waves on 256 rows, which halve the
-// copies, take 264 us for the 8192. Row m of the K tile is the token whose number
+// the present one is computed (one barrier a step). Row m of the K tile is the token whose number
 // within its 16 has bits 2 and 3 of m swapped, which leaves lane half e = lane / 32 with the scores of
 // tokens 16 b + 8 e .. + 7: its k of the second product. The 16-byte chunks of an LDS row are
 // permuted, so that the 16 lanes that read at a time, on 16 different rows, meet all 64 banks: in rows
 // of 256 bytes chunk c sits at place c ^ (row % 16), in rows of 128 at c ^ (row / 2 % 8).
+// Bound by the SIMDs: at D = 128 a wave's step (two waves on a SIMD, prompts of 16384 tokens) takes 2300
+// clocks, of which its products take 1024 and the vector instructions issue for 1200, more than half
+// of it exponentials and their arguments; the counters agree (47 % and 50 %). Neither priorities, nor the
+// order of the compiler, nor 256 rows on eight waves, with the second product of one half beside the first
+// of the other, change it by more than 3 %; LDS is busy for a quarter of the time, without conflicts,
+// and 86 % of its copies come from L2.
+// Measured: 12 heads of 128, a prompt of 8192 tokens 230 us (890 TFLOP/s; 223 in pages of 64), of 4096 87 us
+// (590), of 2048 37 us with the join; 512 new tokens at 30000 132 us (720).
 #define ATTN_ROWS 128
 
 // 16 bytes per lane from memory into LDS at lds + 16 lane, by the copy path that does not pass through
@@ -709,9 +711,9 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
   auto items = [&](int tile) { return std::max<int64_t>(1, (rows / tile + n_seqs) * Hkv); };
   // Tiles of 16 rows for single tokens and the like, and for what is short altogether: their steps
   // cost four times as much for the same work (6 ns for 16 rows x 128 tokens of D = 128, the whole GPU
-  // at work, against 1.4), but there are eight times as many tiles. 12 heads: prompts of 128, 256, 512
-  // and 1024 tokens 6.3, 7.7, 12.0 and 26.2 us, tiles of 128 rows 10.5, 13.9, 17 to 20 and 26.1;
-  // 32 sequences of 4 x 8 rows at 8191 tokens 134 us against 108.
+  // at work, against 1.4), but there are eight times as many tiles. 12 heads: prompts of 200, 512, 700
+  // and 1024 tokens 6.9, 12.3, 16.7 and 25.0 us, tiles of 128 rows 10.8, 17.5, 21.2 and 23.3; 128 new
+  // tokens at 8000 51 against 32; 32 sequences of 4 x 8 rows at 8191 tokens 147 against 103.
   const bool few = rows <= 16 * (int64_t)n_seqs || items(16) * ((capacity + 127) / 128) <= 4096;
   p.rows = few ? 16 : ATTN_ROWS;
   p.tiles = rows / p.rows + n_seqs + 1;
@@ -726,13 +728,18 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
     // 343 us, in 2, 8, 32 ranges 300, 271, 347.
     want = capacity <= 384 ? 1 : std::max(cus / each, capacity / 1024);
   } else {
-    // One round of the workgroups that the GPU holds (2 per CU at D = 128, 3 at D = 64). The tiles of a
-    // prompt differ in length, so a part of a round more does no harm while there are few ranges; with
-    // many it is a round of its own. us for 1, 2, 3, 4 ranges: prompts of 2048 tokens (204 items) 64,
-    // 48, 42, 53; of 4096 (396) 120, 89, 96, 105; of 8192 (780) 255, 267, 305, 310; for 6, 8, 12: 512
-    // new tokens at 30000 (60 items) 179, 142, 184, of D = 64 (128 items) 168, 194, 187.
+    // One round of the workgroups that the GPU holds (2 per CU at D = 128, 3 at D = 64): a part of a round more
+    // is a round of its own where all tiles are about as long, in a chunk of one sequence far behind the
+    // cache's start (a table of twice its tokens and more). Those of a prompt and of several sequences
+    // differ, and there a part of a round does no harm while there are few ranges.
+    // us for 1, 2, 3, 4 ranges: prompts of 2048 tokens (204 items) 49, 42, 37, 45; of 4096 (396) 97, 86, 93,
+    // 103; of 8192 (780) 231, and 265 with even one tile cut; new tokens at 8000: 1500 (144) 196, 135, 113,
+    // 133, 2048 208, 154, 174, 150, 4096 306, 318, 331, 319; for 6, 8, 10: 512 new at 30000 (60) 157, 137,
+    // 126, of D = 64 (500 at 29511, 128 items) 165, 184, 194;
+    // for 1, 2: nine sequences of 700 new tokens at 4000 and single ones 116, 86.
     const int64_t slots = (D == 64 ? 3 : 2) * cus;
-    want = slots / each >= 4 ? slots / each : (slots + each - 1) / each;
+    const bool even = n_seqs == 1 && capacity >= 2 * n_tokens;
+    want = even || slots / each >= 4 ? slots / each : (slots + each - 1) / each;
   }
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ATTN_MAX_SPLITS, want, (capacity + p.least - 1) / p.least}));
   return p;

@@ -289,3 +289,11 @@ def test_scales_beyond_float32_are_refused(scale):
 def test_launches_beyond_the_grid_are_refused():
     rc = _lib().pp_paged_attention(P, S2, 1 << 20, 1 << 20, P, P, P, 600, P, P, 9, 16, 32, 2, 64, 0.1, P, 0, P, 1 << 62, None)
     assert rc == 3 and "workgroups" in _lib().pp_last_error().decode()
+
+
+@pytest.mark.parametrize("seqs", [0, 1, 5])
+@pytest.mark.parametrize("n,maxp", [(1, 1), (4096, 8), (1 << 20, 1 << 16)])
+def test_workspace_of_any_batch(n, seqs, maxp):
+    """No sequence at all among them; room for at most 64 ranges of a row."""
+    b = _lib().pp_paged_attention_workspace_bytes(n, seqs, maxp, 16, 12, 4, 128)
+    assert 0 <= b <= n * 12 * (64 * 130 * 4 + 4)
