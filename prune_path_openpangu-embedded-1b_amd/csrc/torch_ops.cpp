@@ -28,7 +28,9 @@
 #include <c10/hip/HIPStream.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/stack.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include "../../include/prunepath_moe.h"
@@ -567,35 +569,43 @@ Tensor rotary_call(const Tensor& x, const Tensor& positions, const Tensor& inv_f
   return op.call(x, positions, inv_freq, layout, mscale, inverse);
 }
 
-struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& positions,
-                        const Tensor& inv_freq, c10::string_view layout, double mscale, bool inverse) {
-    ctx->save_for_backward({positions, inv_freq});
-    ctx->saved_data["layout"] = std::string(layout);
-    ctx->saved_data["mscale"] = mscale;
-    ctx->saved_data["inverse"] = inverse;
-    at::AutoDispatchBelowADInplaceOrView below;
-    return rotary_call(x, positions, inv_freq, layout, mscale, inverse);
+// A node of its own rather than an autograd::Function, whose context and outputs cost 3 us more a step.
+struct RotaryBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable positions, inv_freq;
+  std::string layout;
+  double mscale = 1.0;
+  bool inverse = false;
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    if (!grads[0].defined()) return {Tensor()};
+    return {rotary_call(grads[0], positions.unpack(), inv_freq.unpack(), layout, mscale, !inverse)};
   }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
-                                                 torch::autograd::variable_list grads) {
-    const auto saved = ctx->get_saved_variables();
-    Tensor g;
-    if (grads[0].defined())
-      g = rotary_call(grads[0], saved[0], saved[1], ctx->saved_data["layout"].toStringRef(),
-                      ctx->saved_data["mscale"].toDouble(), !ctx->saved_data["inverse"].toBool());
-    return {g, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  void release_variables() override {
+    positions.reset_data();
+    inv_freq.reset_data();
   }
+  std::string name() const override { return "RotaryBackward"; }
 };
 
 Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
                        double mscale, bool inverse) {
   TORCH_CHECK(!c10::GradMode::is_enabled() || !inv_freq.requires_grad(),
               "prunepath.rotary: no gradient in inv_freq");
-  if (c10::GradMode::is_enabled() && x.requires_grad())
-    return RotaryFunction::apply(x, positions, inv_freq, layout, mscale, inverse);
-  at::AutoDispatchBelowADInplaceOrView below;
-  return rotary_call(x, positions, inv_freq, layout, mscale, inverse);
+  TORCH_CHECK(!x._fw_grad(0).defined(), "prunepath.rotary: no forward-mode gradient");
+  std::shared_ptr<RotaryBackward> node;
+  if (c10::GradMode::is_enabled() && x.requires_grad()) {
+    node = std::shared_ptr<RotaryBackward>(new RotaryBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->positions = torch::autograd::SavedVariable(positions, false);
+    node->inv_freq = torch::autograd::SavedVariable(inv_freq, false);
+    node->layout = std::string(layout), node->mscale = mscale, node->inverse = inverse;
+  }
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    y = rotary_call(x, positions, inv_freq, layout, mscale, inverse);
+  }
+  if (node) torch::autograd::set_history(y, node);
+  return y;
 }
 
 // ------------------------------------------------------------------ paged cache

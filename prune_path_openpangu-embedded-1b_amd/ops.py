@@ -379,7 +379,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
     pairs (i, i + rotary_dim / 2) for layout "half", (2 i, 2 i + 1) for "interleaved"; cos and sin
     times mscale; the other channels unchanged. positions int32 or int64 of x's leading shape,
     inv_freq float64 (``rotary_frequencies``). A new tensor of x's dtype; differentiable in x (the
-    gradient is the turn by the opposite angles, exact at any order)."""
+    gradient is the turn by the opposite angles, exact at any order; capture it, as any backward, with no
+    eager graph of the same leaves alive)."""
     return L.torch_ops().rotary(x, positions, inv_freq, layout, mscale, False)
 
 

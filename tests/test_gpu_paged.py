@@ -150,6 +150,26 @@ def test_rotary_second_gradient(pkg):
     check_turn(g.grad, v, pos, f, "half", what="second gradient")
 
 
+def test_rotary_backward_twice_and_forward_mode(pkg):
+    """The graph of a call serves one backward, or more where it is kept; forward mode is refused."""
+    ops = pkg.ops
+    f, pos = ops.rotary_frequencies(32)[0].to(dev()), torch.arange(3, device=dev())
+    x = torch.randn(3, 2, 32, device=dev()).requires_grad_()
+    y = ops.rotary(x, pos, f).sum()
+    a, = torch.autograd.grad(y, x, retain_graph=True)
+    b, = torch.autograd.grad(y, x)
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x)
+    y = ops.rotary(x, pos, f)
+    pos.add_(1)  # what the backward needs is no longer there
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y.sum(), x)
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        ops.rotary(fw.make_dual(x.detach(), torch.ones_like(x)), pos, f)
+
+
 def test_rotary_refusals(pkg):
     ops = pkg.ops
     f = ops.rotary_frequencies(32)[0].to(dev())
