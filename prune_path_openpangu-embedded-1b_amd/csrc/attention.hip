@@ -380,12 +380,15 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 // tokens 16 b + 8 e .. + 7: its k of the second product. The 16-byte chunks of an LDS row are
 // permuted, so that the 16 lanes that read at a time, on 16 different rows, meet all 64 banks: in rows
 // of 256 bytes chunk c sits at place c ^ (row % 16), in rows of 128 at c ^ (row / 2 % 8).
-// Bound by the SIMDs: at D = 128 a wave's step (two waves on a SIMD, prompts of 16384 tokens) takes 2300
-// clocks, of which its products take 1024 and the vector instructions issue for 1200, more than half
-// of it exponentials and their arguments; the counters agree (47 % and 50 %). Neither priorities, nor the
-// order of the compiler, nor 256 rows on eight waves, with the second product of one half beside the first
-// of the other, change it by more than 3 %; LDS is busy for a quarter of the time, without conflicts,
-// and 86 % of its copies come from L2.
+// Two workgroups share a CU at D = 128, and a wave's step takes 4300 clocks, where its products take 1024 and
+// its vector instructions issue for 1200: 390 at the barrier, 1080 until the 8 copies are issued (30
+// bytes a clock and CU, with the other workgroup's), 910 in the first product, 460 for the maximum, 1160 in the
+// second product, 340 for the sums. The counters have the matrix cores busy for 47 %, the vector units for
+// 50, LDS for 24 without conflicts, and 86 % of the copies' lines in L2. A part that was shortened
+// came back as waiting elsewhere: copies between the products (8192 tokens 245 us instead of 233), V's
+// behind the first product (242; 512 tokens at 30000 129 instead of 137), sums beside the last products,
+// 256 rows on eight waves with the second product of one half beside the first of the other (236), no
+// priorities (232).
 // Measured: 12 heads of 128, a prompt of 8192 tokens 230 us (890 TFLOP/s; 223 in pages of 64), of 4096 87 us
 // (590), of 2048 37 us with the join; 512 new tokens at 30000 132 us (720).
 #define ATTN_ROWS 128
