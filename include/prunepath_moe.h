@@ -340,7 +340,7 @@ int pp_masked_gate_bwd(const void* d_out, const void* inter, int dtype, const fl
 /* x [batch][length][heads][D] (dtype) -> y of the same dtype. x_strides, y_strides: host arrays of
  * 3, the strides of batch, token and head in elements; channels are contiguous. positions
  * [batch][length] int32 or int64 (pos64), pos_strides: host array of 2. Any alignment (16-byte
- * vectors where every head starts on a 16-byte boundary, rotary_dim % 16 == 0 and D % 8 == 0).
+ * vectors where every head starts on a 16-byte boundary and rotary_dim / 2 and D are whole ones).
  * inverse: turn by the opposite angles (the transposed map: the gradient of x from that of y).
  * y may be x itself with the same strides. */
 int pp_rotary(const void* x, int dtype, const int64_t* x_strides, const void* positions, int pos64,
@@ -373,9 +373,9 @@ int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const i
 
 /* Attention of the new tokens over the cache that holds them: the token at position p attends the
  * positions 0 .. p, query head h the key head h / (Hq / Hkv). q [n_tokens][Hq][D] bfloat16 (strides
- * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous. Scores, softmax and sums in float32. A
- * row that attends nothing gives zeros; what a masked place holds, NaN and infinities too, does not
- * reach a row. Rows behind cu_q[n_seqs] are zeroed if zero_tail, else left as they are. workspace:
+ * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous (q itself, if q is). Scores, softmax and sums
+ * in float32. A row that attends nothing, or whose scores are all -inf, gives zeros; what a masked
+ * place holds, NaN and infinities too, does not reach a row. Rows behind cu_q[n_seqs] are zeroed if zero_tail, else left as they are. workspace:
  * pp_paged_attention_workspace_bytes of the same sizes (0: none), no initialisation, 16-byte
  * aligned; calls that may overlap need one each. The same bits on every call. */
 size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq,

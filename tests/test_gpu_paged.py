@@ -561,6 +561,18 @@ def test_gradients_and_overlaps_are_refused(pkg):
     assert ops.paged_attention(b, *cache, out=b) is b and torch.equal(a, b)  # q itself
 
 
+@pytest.mark.parametrize("new,total,page,heads,kv_heads,room", [
+    ([1, 3], [700, 40], 16, 8, 2, 0), ([200, 1], [1500, 9], 64, 4, 1, 0), ([200, 1], [1500, 9], 64, 4, 1, LONG),
+    ([70, 60], [90, 400], 16, 4, 4, LONG)])
+def test_attention_into_the_queries(pkg, new, total, page, heads, kv_heads, room):
+    """out = q, in one range and in several, by both tiles: the bits of a result of its own."""
+    b = Batch(new, total, page, kv_heads, 128, extra=2 + room // page)
+    cache = b.gpu()
+    q = torch.randn(b.n, heads, 128, generator=gen(5)).to(torch.bfloat16).to(dev())
+    want = pkg.ops.paged_attention(q, *cache)
+    assert pkg.ops.paged_attention(q, *cache, out=q) is q and torch.equal(q, want)
+
+
 def test_strides_of_single_rows_and_heads_say_nothing(pkg):
     """One token or one head at a stride that is no multiple of 8 elements."""
     ops = pkg.ops
