@@ -387,8 +387,8 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 // 50, LDS for 24 without conflicts, and 86 % of the copies' lines in L2. A part that was shortened
 // came back as waiting elsewhere: copies between the products (8192 tokens 245 us instead of 233), V's
 // behind the first product (242; 512 tokens at 30000 129 instead of 137), sums beside the last products,
-// 256 rows on eight waves with the second product of one half beside the first of the other (236), no
-// priorities (232).
+// 256 rows on eight waves with the second product of one half beside the first of the other (236) or on
+// four, one a SIMD (319), no priorities (232).
 // Measured: 12 heads of 128, a prompt of 8192 tokens 230 us (890 TFLOP/s; 223 in pages of 64), of 4096 87 us
 // (590), of 2048 37 us with the join; 512 new tokens at 30000 132 us (720).
 #define ATTN_ROWS 128
