@@ -1,0 +1,34 @@
+"""Values at the ends of their range in the attention over the paged cache. The restatement in float64 and the
+tolerances are those of test_gpu_paged."""
+import pytest
+import torch
+
+from helpers import dev
+from test_gpu_paged import LONG, Batch, attend64, check_attention, few, gen
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [([1, 1], [300, 200], 0), ([3], [700], 0), ([40, 50], [300, 90], LONG)]  # 16-row tiles, 128-row tiles
+
+
+# ------------------------------------------------------------------ infinities in attended values
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,total,room", FORMS)
+def test_attended_infinities(pkg, new, total, room, dim):
+    """Of tokens that every row attends, in steps without a masked place: a channel with one infinity is
+    that infinity, one with both or with NaN is NaN, the others are as they were."""
+    b = Batch(new, total, 16, 2, dim, seed=dim, extra=2 + room // 16)
+    assert few(b, 2, 2) == (room == 0)
+    q = torch.randn(b.n, 2, dim, generator=gen(1)).to(torch.bfloat16)
+    o, big = attend64(b, q)
+    inf = float("inf")
+    want = o.clone()
+    for p, h, d, x in ((7, 0, 5, inf), (40, 0, 20, -inf), (9, 1, 33, inf), (41, 1, 33, -inf), (12, 1, 50, float("nan"))):
+        id, off = b.place(0, p)
+        b.v[id, h, d, off] = x
+        want[:new[0], h, d] += x
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu()).cpu()
+    odd = ~torch.isfinite(want)
+    assert int(odd.sum()) == 4 * new[0]
+    assert torch.allclose(got[odd].double(), want[odd], equal_nan=True)
+    check_attention(torch.where(odd, o.to(got.dtype), got), o, big, few(b, 2, 2))
