@@ -32,3 +32,19 @@ def test_attended_infinities(pkg, new, total, room, dim):
     assert int(odd.sum()) == 4 * new[0]
     assert torch.allclose(got[odd].double(), want[odd], equal_nan=True)
     check_attention(torch.where(odd, o.to(got.dtype), got), o, big, few(b, 2, 2))
+
+
+# ------------------------------------------------------------------ scores of any size
+@pytest.mark.parametrize("power", [8, 14, 20, 40, 54])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("new,total,room", FORMS)
+def test_scores_beyond_the_exponential(pkg, new, total, room, sign, power):
+    """Scores of 2^(2 power) and more, exact in float32 and apart by 2^-7 of themselves: each row takes the
+    largest alone (equal ones in equal parts)."""
+    b = Batch(new, total, 16, 1, 64, seed=power, extra=2 + room // 16)
+    assert few(b, 1, 1) == (room == 0)
+    q = torch.full((b.n, 1, 64), sign * 2.0 ** power, dtype=torch.bfloat16)
+    j = torch.randint(0, 128, (b.pages, 1, 16, 1), generator=gen(power))
+    b.k = ((1 + j / 128) * 2.0 ** power).expand(b.pages, 1, 16, 64).to(torch.bfloat16).contiguous()
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu(), scale=0.1)
+    check_attention(got, *attend64(b, q, 0.1), few(b, 1, 1))
