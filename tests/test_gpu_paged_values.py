@@ -48,3 +48,15 @@ def test_scores_beyond_the_exponential(pkg, new, total, room, sign, power):
     b.k = ((1 + j / 128) * 2.0 ** power).expand(b.pages, 1, 16, 64).to(torch.bfloat16).contiguous()
     got = pkg.ops.paged_attention(q.to(dev()), *b.gpu(), scale=0.1)
     check_attention(got, *attend64(b, q, 0.1), few(b, 1, 1))
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -126, 2.0 ** -130])
+@pytest.mark.parametrize("new,total,room", FORMS)
+def test_scales_next_to_zero(pkg, new, total, room, scale):
+    """Scores up to 2^126 under scales that leave next to nothing of them: 0 takes the mean."""
+    b = Batch(new, total, 16, 1, 64, seed=3, extra=2 + room // 16)
+    q = torch.full((b.n, 1, 64), 2.0 ** 60, dtype=torch.bfloat16)
+    j = torch.randint(0, 64, (b.pages, 1, 16, 1), generator=gen(4))
+    b.k = ((j - 32) / 32 * 2.0 ** 60).expand(b.pages, 1, 16, 64).to(torch.bfloat16).contiguous()
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu(), scale=scale)
+    check_attention(got, *attend64(b, q, scale), few(b, 1, 1))
