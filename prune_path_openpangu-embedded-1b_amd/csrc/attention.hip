@@ -34,7 +34,7 @@ typedef uint32_t a_u4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ a_u4 a_mk(uint32_t x, uint32_t y, uint32_t z, uint32_t w) { return a_u4{x, y, z, w}; }
 
 #define ATTN_THREADS 256
-#define ATTN_LOW -3.0e38f  // running maximum before the first score
+#define ATTN_LOW -0x1.fffffep127f  // running maximum before the first score: no finite one is less
 // Running maxima from which on the exponent s c - m is taken of the rounded product. One fma leaves what the
 // rounding took off m's own product, up to 2^-24 of m: from 2^31 on the row's largest score itself would come
 // out infinite or as nothing. (The test costs tiles of 128 rows 0.8 %: 8192 tokens 234.0 us without, 235.7.)

@@ -60,3 +60,14 @@ def test_scales_next_to_zero(pkg, new, total, room, scale):
     b.k = ((j - 32) / 32 * 2.0 ** 60).expand(b.pages, 1, 16, 64).to(torch.bfloat16).contiguous()
     got = pkg.ops.paged_attention(q.to(dev()), *b.gpu(), scale=scale)
     check_attention(got, *attend64(b, q, scale), few(b, 1, 1))
+
+
+@pytest.mark.parametrize("scale", [0.25, 0.5, 0.68])
+@pytest.mark.parametrize("new,total,room", FORMS)
+def test_scores_next_to_the_lowest_float(pkg, new, total, room, scale):
+    """Every score is 64 * -2^60 * 1.875 * 2^61 = -3.19e38, finite: the mean, not a row of nothing."""
+    b = Batch(new, total, 16, 1, 64, seed=5, extra=2 + room // 16)
+    q = torch.full((b.n, 1, 64), -(2.0 ** 60), dtype=torch.bfloat16)
+    b.k.fill_(1.875 * 2.0 ** 61)
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu(), scale=scale)
+    check_attention(got, *attend64(b, q, scale), few(b, 1, 1))
