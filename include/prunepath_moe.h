@@ -331,8 +331,9 @@ int pp_masked_gate_bwd(const void* d_out, const void* inter, int dtype, const fl
  * Pair i of a head (of its first rotary_dim channels) turns by position * inv_freq[i]
  * (float64 on the device, rotary_dim / 2 of them): y1 = mscale (x1 cos - x2 sin),
  * y2 = mscale (x1 sin + x2 cos); the other channels are copied. layout: the pair is
- * channels (i, rotary_dim / 2 + i) or (2 i, 2 i + 1). The angle is good to 2^-51 of
- * itself, whatever the position.
+ * channels (i, rotary_dim / 2 + i) or (2 i, 2 i + 1). cos and sin are float32
+ * (good to 2^-21 of themselves) of an angle that is good to 2^-51 of itself, whatever the
+ * position.
  * ------------------------------------------------------------------------- */
 #define PP_ROTARY_HALF 0
 #define PP_ROTARY_INTERLEAVED 1

@@ -1,5 +1,7 @@
-"""Values at the ends of their range in the attention over the paged cache. The restatement in float64 and the
-tolerances are those of test_gpu_paged."""
+"""Values at the ends of their range in the rotary positions and the attention over the paged cache. The
+restatement in float64 and the tolerances are those of test_gpu_paged."""
+import math
+
 import pytest
 import torch
 
@@ -71,3 +73,22 @@ def test_scores_next_to_the_lowest_float(pkg, new, total, room, scale):
     b.k.fill_(1.875 * 2.0 ** 61)
     got = pkg.ops.paged_attention(q.to(dev()), *b.gpu(), scale=scale)
     check_attention(got, *attend64(b, q, scale), few(b, 1, 1))
+
+
+# ------------------------------------------------------------------ angles next to the zeros of cos and sin
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_angles_next_to_a_quarter_turn(pkg, layout):
+    """(1, 0) turned by angles within 2^-24 of multiples of a quarter turn is (cos, sin), good to 2^-21 of
+    itself however small: the angle beyond a float32 must not be lost. (sincospif is good to 4 units of
+    2^-23; what a float32 half turn leaves of the angle is added to first order, 2^-50 off; the float64 product
+    is good to 2^-51 of angles up to 7, and the rest is room for the float64 restatement's own 2 pi.)"""
+    k = torch.arange(1, 5, dtype=torch.float64)[:, None]
+    part = torch.tensor([-0.45, -0.2, -0.01, 0.03, 0.3, 0.48], dtype=torch.float64)[None]
+    f = (math.pi * (0.5 * k + part * 2.0 ** -24)).flatten()
+    x = torch.zeros(1, 1, 2 * f.numel(), dtype=torch.float32)
+    i = torch.arange(f.numel())
+    first, second = (i, i + f.numel()) if layout == "half" else (2 * i, 2 * i + 1)
+    x[..., first] = 1.0
+    y = pkg.ops.rotary(x.to(dev()), torch.ones(1, dtype=torch.int64, device=dev()), f.to(dev()), layout).cpu().double()
+    for got, want in ((y[0, 0, first], f.cos()), (y[0, 0, second], f.sin())):
+        assert bool(((got - want).abs() <= 2.0 ** -21 * want.abs() + 2.0 ** -48).all()), (got - want).abs().max()
