@@ -774,7 +774,8 @@ static size_t attn_ws_bytes(const AttnPlan& p, int64_t rows, int D) {
 
 extern "C" size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size,
                                                      int Hq, int Hkv, int D) {
-  if (n_tokens <= 0 || n_seqs < 0 || max_pages < 1 || page_size < 1 || Hkv < 1 || Hq < Hkv || D < 1) return 0;
+  if (pp_paged_sizes("pp_paged_attention", n_tokens, n_seqs, max_pages, 1, page_size, Hq, Hkv, D)) return 0;
+  if (n_tokens == 0 || Hq == 0) return 0;
   return attn_ws_bytes(attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D), n_tokens * Hq, D);
 }
 

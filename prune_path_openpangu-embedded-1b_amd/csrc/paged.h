@@ -92,7 +92,9 @@ static inline int paged_log2(int v) {
   return -1;
 }
 
-// Checks of the arguments that the append and the attention have in common.
+// Checks of the sizes, and of all the arguments, that the append and the attention have in common.
+int pp_paged_sizes(const char* what, int64_t n_tokens, int n_seqs, int max_pages, int num_pages, int page_size, int Hq,
+                   int Hkv, int D);
 int pp_paged_check(const char* what, int64_t n_tokens, int n_seqs, const void* cu_q, const void* kv_lens,
                    const void* block_table, int max_pages, const void* k_pages, const void* v_pages, int num_pages,
                    int page_size, int Hq, int Hkv, int D);

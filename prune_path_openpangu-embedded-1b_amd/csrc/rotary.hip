@@ -387,9 +387,8 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
   }
 }
 
-int pp_paged_check(const char* what, int64_t n_tokens, int n_seqs, const void* cu_q, const void* kv_lens,
-                   const void* block_table, int max_pages, const void* k_pages, const void* v_pages, int num_pages,
-                   int page_size, int Hq, int Hkv, int D) {
+int pp_paged_sizes(const char* what, int64_t n_tokens, int n_seqs, int max_pages, int num_pages, int page_size, int Hq,
+                   int Hkv, int D) {
   PP_REQUIRE(D == 64 || D == 128, PP_ERR_UNSUPPORTED, "%s: head size %d unsupported (64 or 128)", what, D);
   PP_REQUIRE(page_size >= 16 && page_size <= 4096 && paged_log2(page_size) >= 0, PP_ERR_UNSUPPORTED,
              "%s: page size %d unsupported (a power of two, 16 to 4096)", what, page_size);
@@ -397,11 +396,18 @@ int pp_paged_check(const char* what, int64_t n_tokens, int n_seqs, const void* c
              "%s: %d query heads on %d key heads (need a multiple)", what, Hq, Hkv);
   PP_REQUIRE(n_seqs >= 0 && n_seqs <= (1 << 20) && max_pages >= 1 && num_pages >= 1, PP_ERR_INVALID,
              "%s: %d sequences, a table of %d pages, a cache of %d", what, n_seqs, max_pages, num_pages);
-  PP_REQUIRE(n_tokens >= 0 && n_tokens * (int64_t)std::max(Hq, Hkv) <= 0x7fffffff, PP_ERR_UNSUPPORTED,
+  PP_REQUIRE(n_tokens >= 0 && n_tokens <= 0x7fffffff / std::max(Hq, Hkv), PP_ERR_UNSUPPORTED,
              "%s: %lld tokens of %d heads", what, (long long)n_tokens, std::max(Hq, Hkv));
   PP_REQUIRE((int64_t)max_pages * page_size <= (1 << 30), PP_ERR_UNSUPPORTED,
              "%s: a table of %d pages of %d tokens (at most 2^30 tokens)", what, max_pages, page_size);
-  if (n_tokens == 0) return PP_OK;
+  return PP_OK;
+}
+
+int pp_paged_check(const char* what, int64_t n_tokens, int n_seqs, const void* cu_q, const void* kv_lens,
+                   const void* block_table, int max_pages, const void* k_pages, const void* v_pages, int num_pages,
+                   int page_size, int Hq, int Hkv, int D) {
+  const int rc = pp_paged_sizes(what, n_tokens, n_seqs, max_pages, num_pages, page_size, Hq, Hkv, D);
+  if (rc || n_tokens == 0) return rc;
   PP_REQUIRE(cu_q && k_pages && v_pages && (n_seqs == 0 || (kv_lens && block_table)), PP_ERR_INVALID,
              "%s: null pointer", what);
   PP_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, PP_ERR_INVALID, "%s: pages not 16-byte aligned", what);
