@@ -658,8 +658,9 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
     TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
                 "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
   inference_only(name, {q ? &*q : nullptr, q ? &*q_out : nullptr, &k, &v, &k_pages, &v_pages, inv_freq ? &*inv_freq : nullptr});
-  const Span sk(k), sv(v), kp(k_pages), vp(v_pages);
-  for (const Span* in : {&sk, &sv}) {
+  const Span sk(k), sv(v), kp(k_pages), vp(v_pages), st(block_table), sl(kv_lens), sc(cu_q);
+  const Span sf = inv_freq ? Span(*inv_freq) : st;
+  for (const Span* in : {&sk, &sv, &st, &sl, &sc, &sf}) {
     apart(name, kp, *in);
     apart(name, vp, *in);
   }
@@ -674,7 +675,7 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
     apart(name, vp, sq);
     if (!zero_tail) {  // a given q_out
       const Span so(*q_out);
-      for (const Span* in : {&sk, &sv, &kp, &vp}) apart(name, so, *in);
+      for (const Span* in : {&sk, &sv, &kp, &vp, &st, &sl, &sc, &sf}) apart(name, so, *in);
       if (!same_rows(*q_out, *q)) apart(name, so, sq);
     }
     qs[0] = step(*q, 0), qs[1] = step(*q, 1);
@@ -734,8 +735,7 @@ void attention_into(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   inference_only(name, {&q, &k_pages, &v_pages, &out});
   if (!zero_tail) {  // a given out
     const Span so(out);
-    apart(name, so, Span(k_pages));
-    apart(name, so, Span(v_pages));
+    for (const Tensor* in : {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q}) apart(name, so, Span(*in));
     if (!same_rows(out, q)) apart(name, so, Span(q));
   }
   const c10::DeviceGuard g(q.device());

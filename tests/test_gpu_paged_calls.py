@@ -1,0 +1,37 @@
+"""Calls of the rotary positions and the paged cache that the other files do not make: outputs on top of the
+tables that a call reads, gradients and versions around calls in place, schemas and fake results of the ops."""
+import pytest
+import torch
+
+from helpers import dev
+from test_gpu_paged import Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_outputs_on_top_of_the_tables_are_refused(pkg):
+    """block_table, kv_lens, cu_q and inv_freq are read while pages and outputs are written."""
+    ops = pkg.ops
+    kp, vp, table, lens, cu = Batch([2], [20], 16, 2, 64).gpu()
+    cache = (kp, vp, table, lens, cu)
+    x = torch.ones(2, 2, 64, dtype=torch.bfloat16, device=dev())
+    f = ops.rotary_frequencies(64)[0].to(dev())
+
+    def inside(t, like):  # like's size and type, in t's memory
+        return t.view(-1).view(like.dtype)[:like.numel()].view(like.shape).copy_(like)
+
+    for given in (kp, vp):
+        for i in (2, 3, 4):
+            with pytest.raises(RuntimeError, match="prunepath.*overlaps"):
+                ops.kv_append(x, x.clone(), *cache[:i], inside(given, cache[i]), *cache[i + 1:])
+        with pytest.raises(RuntimeError, match="prunepath.*overlaps"):
+            ops.kv_append(x, x.clone(), *cache, inside(given, f))
+    out = torch.zeros_like(x)
+    for i in (2, 3, 4):
+        on = (*cache[:i], inside(out, cache[i]), *cache[i + 1:])
+        with pytest.raises(RuntimeError, match="prunepath.*overlaps"):
+            ops.paged_attention(x, *on, out=out)
+        with pytest.raises(RuntimeError, match="prunepath.*overlaps"):
+            ops.kv_append(x, x.clone(), *on, q=x.clone(), q_out=out)
+    with pytest.raises(RuntimeError, match="prunepath.*overlaps"):
+        ops.kv_append(x, x.clone(), *cache, inside(out, f), q=x.clone(), q_out=out)
