@@ -509,14 +509,6 @@ bool same_rows(const Tensor& out, const Tensor& in) {
   return out.data_ptr() == in.data_ptr() && out.scalar_type() == in.scalar_type() && in.is_contiguous();
 }
 
-// No gradient goes through these ops; a call that would need one is refused.
-void inference_only(const char* name, std::initializer_list<const Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const Tensor* t : ts)
-    TORCH_CHECK(t == nullptr || !t->requires_grad(), "prunepath.", name,
-                ": inference only, but an argument requires a gradient (call it under torch.no_grad())");
-}
-
 // x with channels next to each other, and an empty result of its shape that has them so: the strides are the
 // same for real and for fake tensors.
 Tensor rotary_input(const Tensor& x) {
@@ -657,7 +649,6 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   if (inv_freq)
     TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
                 "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
-  inference_only(name, {q ? &*q : nullptr, q ? &*q_out : nullptr, &k, &v, &k_pages, &v_pages, inv_freq ? &*inv_freq : nullptr});
   const Span sk(k), sv(v), kp(k_pages), vp(v_pages), st(block_table), sl(kv_lens), sc(cu_q);
   const Span sf = inv_freq ? Span(*inv_freq) : st;
   for (const Span* in : {&sk, &sv, &st, &sl, &sc, &sf}) {
@@ -732,7 +723,6 @@ void attention_into(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, q.size(0), q.size(1), q.size(2));
   need_gpu(name, q, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &out});
   same_device(name, q, {&q});
-  inference_only(name, {&q, &k_pages, &v_pages, &out});
   if (!zero_tail) {  // a given out
     const Span so(out);
     for (const Tensor* in : {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q}) apart(name, so, Span(*in));
@@ -769,6 +759,42 @@ Tensor paged_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const
 }
 void paged_attention_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                double, const Tensor&) {}
+
+// ------------------------------------------------------------------ ops for inference
+void refuse_gradient(const char* op, const Tensor& t) {
+  TORCH_CHECK(!t.requires_grad(), "prunepath.", op,
+              ": inference only, but an argument requires a gradient (call it under torch.no_grad())");
+}
+void refuse_gradient(const char* op, const optional<Tensor>& t) {
+  if (t && t->defined()) refuse_gradient(op, *t);
+}
+template <typename T>
+void refuse_gradient(const char*, const T&) {}
+
+// The kernel of an op's Autograd key: a call that would need a gradient is refused, any other goes on to the
+// key below. It stands there, not in the GPU's kernel, so that traced calls meet it too: under the tracer the
+// GPU's kernel only ever runs with gradients off.
+template <typename Op, typename R, typename... A>
+struct Inference {
+  static R call(c10::DispatchKeySet keys, A... args) {
+    if (c10::GradMode::is_enabled()) (refuse_gradient(Op::name(), args), ...);
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow((std::string("prunepath::") + Op::name()).c_str(), "")
+                         .template typed<R(A...)>();
+    return op.redispatch(keys & c10::after_autograd_keyset, args...);
+  }
+};
+template <typename Op, typename R, typename... A>
+constexpr auto inference(R (*)(A...)) {
+  return &Inference<Op, R, A...>::call;
+}
+#define INFERENCE(m, op)                                        \
+  do {                                                          \
+    struct Op {                                                 \
+      static const char* name() { return #op; }                 \
+    };                                                          \
+    m.impl(#op, inference<Op>(&op##_gpu));                      \
+  } while (0)
 
 void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
   TORCH_CHECK(false, op.schema().name(), ": tensors must be on the GPU (got cpu); there is no CPU implementation");
@@ -864,9 +890,11 @@ TORCH_LIBRARY_IMPL(prunepath, Meta, m) {
 
 TORCH_LIBRARY_IMPL(prunepath, Autograd, m) {
   m.impl("rotary", &rotary_autograd);
-  // inference: the kernels refuse arguments that require a gradient (inference_only)
-  for (const char* name : {"kv_append", "kv_append_q", "kv_append_q_into", "paged_attention", "paged_attention_into"})
-    m.impl(name, torch::CppFunction::makeFallthrough());
+  INFERENCE(m, kv_append);
+  INFERENCE(m, kv_append_q);
+  INFERENCE(m, kv_append_q_into);
+  INFERENCE(m, paged_attention);
+  INFERENCE(m, paged_attention_into);
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CPU, m) {

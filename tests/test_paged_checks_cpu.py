@@ -19,3 +19,58 @@ def test_sizes_that_wrap_are_refused(kw):
 def test_workspace_of_sizes_that_are_refused(n, seqs, maxp, page, hq, hkv, d):
     """None: the call itself says what is wrong with them."""
     assert _lib().pp_paged_attention_workspace_bytes(n, seqs, maxp, page, hq, hkv, d) == 0
+
+
+# ------------------------------------------------------------------ gradients and tangents
+def _fake(device="meta", seqs=2, n=5, heads=4, kv=2, dim=64, page=16):
+    """(ops, q, k, v, cache, inv_freq) of a call, on a device without values."""
+    import torch
+    m = dict(device=device)
+    bf = dict(dtype=torch.bfloat16, **m)
+    cache = (torch.empty(9, kv, page, dim, **bf), torch.empty(9, kv, dim, page, **bf),
+             torch.empty(seqs, 3, dtype=torch.int32, **m), torch.empty(seqs, dtype=torch.int32, **m),
+             torch.empty(seqs + 1, dtype=torch.int32, **m))
+    return (import_pkg()._lib.torch_ops(), torch.empty(n, heads, dim, **bf), torch.empty(n, kv, dim, **bf),
+            torch.empty(n, kv, dim, **bf), cache, torch.empty(dim // 2, dtype=torch.float64, **m))
+
+
+def _calls():
+    """(name, call(ops, q, k, v, cache, inv_freq)) of every op for inference."""
+    import torch
+    return {"kv_append": lambda t, q, k, v, c, f: t.kv_append(k, v, *c, f),
+            "kv_append_q": lambda t, q, k, v, c, f: t.kv_append_q(q, k, v, *c, f),
+            "kv_append_q_into": lambda t, q, k, v, c, f: t.kv_append_q_into(q, torch.empty_like(q), k, v, *c, f),
+            "paged_attention": lambda t, q, k, v, c, f: t.paged_attention(q, *c, 0.1),
+            "paged_attention_into": lambda t, q, k, v, c, f: t.paged_attention_into(q, *c, 0.1, torch.empty_like(q))}
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("name", list(_calls()))
+def test_gradients_are_refused_without_a_gpu(name, which):
+    """Whichever argument (q, k, v, k_pages, inv_freq) requires one, if the call takes it; not under no_grad."""
+    import torch
+    t, q, k, v, cache, f = _fake()
+    (q, k, v, cache[0], f)[which].requires_grad_()
+    takes = {"kv_append": (1, 2, 3, 4), "paged_attention": (0, 3), "paged_attention_into": (0, 3)}.get(name, range(5))
+    if which in takes:
+        with pytest.raises(RuntimeError, match=f"prunepath.{name}: inference only"):
+            _calls()[name](t, q, k, v, cache, f)
+    with torch.no_grad():
+        _calls()[name](t, q, k, v, cache, f)
+
+
+def test_gradients_are_refused_in_compiled_code():
+    """A traced call meets the refusal as an eager one does: no result without its gradient."""
+    import torch
+    t, q, k, v, cache, f = _fake()
+    p = torch.empty(64, 64, dtype=torch.bfloat16, device="meta", requires_grad=True)
+    w = torch.empty(64, 3, dtype=torch.bfloat16, device="meta", requires_grad=True)
+    attend = lambda q, p, w: (t.paged_attention(q @ p, *cache, 0.1) @ w).sum()  # noqa: E731
+    append = lambda q, p, w: (t.kv_append_q(q @ p, k, v, *cache, f) @ w).sum()  # noqa: E731
+    for fn in (attend, append):
+        torch._dynamo.reset()
+        with pytest.raises(Exception, match="inference only"):
+            torch.compile(fn, backend="aot_eager")(q, p, w)
+    with torch.no_grad():
+        torch._dynamo.reset()
+        assert torch.compile(attend, backend="aot_eager")(q, p, w).shape == ()
