@@ -582,7 +582,7 @@ Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& i
                        double mscale, bool inverse) {
   TORCH_CHECK(!c10::GradMode::is_enabled() || !inv_freq.requires_grad(),
               "prunepath.rotary: no gradient in inv_freq");
-  TORCH_CHECK(!x._fw_grad(0).defined(), "prunepath.rotary: no forward-mode gradient");
+  TORCH_CHECK(!x._fw_grad(0).defined() && !inv_freq._fw_grad(0).defined(), "prunepath.rotary: no forward-mode gradient");
   std::shared_ptr<RotaryBackward> node;
   if (c10::GradMode::is_enabled() && x.requires_grad()) {
     node = std::shared_ptr<RotaryBackward>(new RotaryBackward(), torch::autograd::deleteNode);
@@ -762,7 +762,8 @@ void paged_attention_into_meta(const Tensor&, const Tensor&, const Tensor&, cons
 
 // ------------------------------------------------------------------ ops for inference
 void refuse_gradient(const char* op, const Tensor& t) {
-  TORCH_CHECK(!t.requires_grad(), "prunepath.", op,
+  TORCH_CHECK(!t._fw_grad(0).defined(), "prunepath.", op, ": no forward-mode gradient");
+  TORCH_CHECK(!c10::GradMode::is_enabled() || !t.requires_grad(), "prunepath.", op,
               ": inference only, but an argument requires a gradient (call it under torch.no_grad())");
 }
 void refuse_gradient(const char* op, const optional<Tensor>& t) {
@@ -771,13 +772,13 @@ void refuse_gradient(const char* op, const optional<Tensor>& t) {
 template <typename T>
 void refuse_gradient(const char*, const T&) {}
 
-// The kernel of an op's Autograd key: a call that would need a gradient is refused, any other goes on to the
-// key below. It stands there, not in the GPU's kernel, so that traced calls meet it too: under the tracer the
-// GPU's kernel only ever runs with gradients off.
+// The kernel of an op's Autograd key: a call that would need a gradient, or has a tangent, is refused, any
+// other goes on to the key below. It stands there, not in the GPU's kernel, so that traced calls meet it too:
+// under the tracer the GPU's kernel only ever runs with gradients off.
 template <typename Op, typename R, typename... A>
 struct Inference {
   static R call(c10::DispatchKeySet keys, A... args) {
-    if (c10::GradMode::is_enabled()) (refuse_gradient(Op::name(), args), ...);
+    (refuse_gradient(Op::name(), args), ...);
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow((std::string("prunepath::") + Op::name()).c_str(), "")
                          .template typed<R(A...)>();

@@ -59,6 +59,33 @@ def test_gradients_are_refused_without_a_gpu(name, which):
         _calls()[name](t, q, k, v, cache, f)
 
 
+@pytest.mark.parametrize("name", list(_calls()))
+def test_tangents_are_refused(name):
+    import torch
+    import torch.autograd.forward_ad as fw
+    t, q, k, v, cache, f = _fake()
+    with fw.dual_level():
+        dual = lambda x: fw.make_dual(x, torch.empty_like(x))  # noqa: E731
+        for args in ((dual(q), k, v, cache, f), (q, dual(k), v, cache, f), (q, k, v, (cache[0], dual(cache[1]), *cache[2:]), f)):
+            if name.startswith("paged") and args[1] is not k or name == "kv_append" and args[0] is not q:
+                continue
+            with torch.no_grad(), pytest.raises(RuntimeError, match=f"prunepath.{name}: .*forward-mode"):
+                _calls()[name](t, *args)
+
+
+def test_tangents_of_the_rotation_are_refused():
+    """Of x and of the frequencies alike."""
+    import torch
+    import torch.autograd.forward_ad as fw
+    t, q, _, _, _, f = _fake()
+    pos = torch.empty(5, dtype=torch.int64, device="meta")
+    with fw.dual_level():
+        for x, g in ((fw.make_dual(q, torch.empty_like(q)), f), (q, fw.make_dual(f, torch.empty_like(f)))):
+            with pytest.raises(RuntimeError, match="prunepath.rotary: no forward-mode"):
+                t.rotary(x, pos, g)
+    assert t.rotary(q, pos, f).shape == q.shape
+
+
 def test_gradients_are_refused_in_compiled_code():
     """A traced call meets the refusal as an eager one does: no result without its gradient."""
     import torch
