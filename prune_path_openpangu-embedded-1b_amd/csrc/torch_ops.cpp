@@ -31,6 +31,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include "../../include/prunepath_moe.h"
@@ -789,12 +790,55 @@ template <typename Op, typename R, typename... A>
 constexpr auto inference(R (*)(A...)) {
   return &Inference<Op, R, A...>::call;
 }
-#define INFERENCE(m, op)                                        \
-  do {                                                          \
-    struct Op {                                                 \
-      static const char* name() { return #op; }                 \
-    };                                                          \
-    m.impl(#op, inference<Op>(&op##_gpu));                      \
+// The kernel of an op's ADInplaceOrView key: what the op has written (its arguments of the given numbers)
+// counts as changed, so that a backward that saved it before raises, as after torch's own operations in place.
+void changed(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+void changed(const optional<Tensor>& t) {
+  if (t) changed(*t);
+}
+template <typename T>
+void changed(const T&) {}
+
+template <typename Op, unsigned numbers, typename R, typename... A>
+struct Written {
+  static R call(c10::DispatchKeySet keys, A... args) {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow((std::string("prunepath::") + Op::name()).c_str(), "")
+                         .template typed<R(A...)>();
+    const auto count = [&] {
+      unsigned i = 0;
+      ((numbers >> i++ & 1 ? changed(args) : void()), ...);
+    };
+    if constexpr (std::is_void_v<R>) {
+      op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
+      count();
+    } else {
+      R out = op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
+      count();
+      return out;
+    }
+  }
+};
+template <typename Op, unsigned numbers, typename R, typename... A>
+constexpr auto written(R (*)(A...)) {
+  return &Written<Op, numbers, R, A...>::call;
+}
+
+#define INFERENCE(m, op)                        \
+  do {                                          \
+    struct Op {                                 \
+      static const char* name() { return #op; } \
+    };                                          \
+    m.impl(#op, inference<Op>(&op##_gpu));      \
+  } while (0)
+#define WRITES(m, op, fn, numbers)              \
+  do {                                          \
+    struct Op {                                 \
+      static const char* name() { return #op; } \
+    };                                          \
+    m.impl(#op, written<Op, numbers>(&fn));     \
   } while (0)
 
 void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
@@ -896,6 +940,13 @@ TORCH_LIBRARY_IMPL(prunepath, Autograd, m) {
   INFERENCE(m, kv_append_q_into);
   INFERENCE(m, paged_attention);
   INFERENCE(m, paged_attention_into);
+}
+
+TORCH_LIBRARY_IMPL(prunepath, ADInplaceOrView, m) {
+  WRITES(m, kv_append, kv_append_gpu, 1 << 2 | 1 << 3);
+  WRITES(m, kv_append_q, kv_append_q_gpu, 1 << 3 | 1 << 4);
+  WRITES(m, kv_append_q_into, kv_append_q_into_gpu, 1 << 1 | 1 << 4 | 1 << 5);
+  WRITES(m, paged_attention_into, paged_attention_into_gpu, 1 << 7);
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CPU, m) {

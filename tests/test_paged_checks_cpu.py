@@ -101,3 +101,48 @@ def test_gradients_are_refused_in_compiled_code():
     with torch.no_grad():
         torch._dynamo.reset()
         assert torch.compile(attend, backend="aot_eager")(q, p, w).shape == ()
+
+
+# ------------------------------------------------------------------ versions
+def test_written_arguments_count_as_changed():
+    """Each op bumps the version of what its schema says it writes, and of nothing else."""
+    import torch
+    t, q, k, v, cache, f = _fake()
+    out = torch.empty_like(q)
+    every = [q, k, v, *cache, f, out]
+    for op, args in ((t.kv_append, (k, v, *cache, f)), (t.kv_append_q, (q, k, v, *cache, f)),
+                     (t.kv_append_q_into, (q, out, k, v, *cache, f)), (t.paged_attention, (q, *cache, 0.1)),
+                     (t.paged_attention_into, (q, *cache, 0.1, out))):
+        schema = op.default._schema.arguments
+        writes = [a for a, s in zip(args, schema) if s.alias_info is not None and s.alias_info.is_write]
+        before = [x._version for x in every]
+        op(*args)
+        for x, old in zip(every, before):
+            assert x._version == old + any(x is w for w in writes), op
+
+
+def test_a_backward_that_saved_what_a_call_overwrote_raises():
+    import torch
+    t, q, k, v, cache, f = _fake()
+    w = torch.empty_like(q, requires_grad=True)
+    for call in (lambda b: t.paged_attention_into(q, *cache, 0.1, b), lambda b: t.kv_append_q_into(q, b, k, v, *cache, f)):
+        buf = torch.empty_like(q)
+        y = (buf * w).sum()
+        call(buf)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+    y = (cache[0] * torch.empty_like(cache[0], requires_grad=True)).sum()
+    t.kv_append(k, v, *cache, f)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+
+
+def test_inference_tensors_are_written_as_before():
+    """Tensors made in inference mode have no version: a call outside of it writes them all the same."""
+    import torch
+    with torch.inference_mode():
+        t, q, k, v, cache, f = _fake()
+        t.kv_append(k, v, *cache, f)
+    with torch.no_grad():
+        t.kv_append(k, v, *cache, f)
+        t.paged_attention_into(q, *cache, 0.1, torch.empty_like(q))
