@@ -35,3 +35,23 @@ def test_outputs_on_top_of_the_tables_are_refused(pkg):
             ops.kv_append(x, x.clone(), *on, q=x.clone(), q_out=out)
     with pytest.raises(RuntimeError, match="prunepath.*overlaps"):
         ops.kv_append(x, x.clone(), *cache, inside(out, f), q=x.clone(), q_out=out)
+
+
+def test_opcheck(pkg):
+    """Schemas, registrations and fake results of the six ops, with and without gradients where there are any."""
+    from torch.library import opcheck
+    t = pkg._lib.torch_ops()
+    kp, vp, table, lens, cu = Batch([3, 2], [20, 5], 16, 2, 64).gpu()
+    cache = (kp, vp, table, lens, cu)
+    f = pkg.ops.rotary_frequencies(64)[0].to(dev())
+    q, k, v = (torch.randn(5, h, 64, device=dev(), dtype=torch.bfloat16) for h in (4, 2, 2))
+    pos = torch.arange(5, device=dev())
+    x = torch.randn(5, 3, 64, device=dev())
+    for op, args in ((t.rotary, (x, pos, f)), (t.rotary, (x.clone().requires_grad_(), pos, f, "interleaved", 1.5, True)),
+                     (t.rotary, (x.bfloat16().transpose(1, 2).contiguous().transpose(1, 2), pos.int(), f)),
+                     (t.kv_append, (k, v, *cache, f)), (t.kv_append, (k.float(), v.float(), *cache)),
+                     (t.kv_append_q, (q, k, v, *cache, f, "interleaved", 1.5)),
+                     (t.kv_append_q_into, (q, torch.zeros_like(q), k, v, *cache, f)),
+                     (t.paged_attention, (q, *cache, 0.1)), (t.paged_attention_into, (q, *cache, 0.1, torch.zeros_like(q)))):
+        print(f"opcheck {op}", flush=True)
+        opcheck(op, args)
