@@ -943,6 +943,12 @@ TORCH_LIBRARY_IMPL(prunepath, Autograd, m) {
 }
 
 TORCH_LIBRARY_IMPL(prunepath, ADInplaceOrView, m) {
+  WRITES(m, decode_workspace_init, decode_workspace_init_gpu, 1 << 0);
+  WRITES(m, moe_decode, moe_decode_gpu, 1 << 7);
+  WRITES(m, moe_decode_into, decode_into, 1 << 7 | 1 << 8);
+  WRITES(m, moe_decode_batch, moe_decode_batch_gpu, 1 << 7 | 1 << 8);
+  WRITES(m, moe_decode_batch_into, decode_batch_into, 1 << 7 | 1 << 8 | 1 << 9 | 1 << 10 | 1 << 11);
+  WRITES(m, moe_prefill_into, prefill_into, 1 << 7 | 1 << 8 | 1 << 9 | 1 << 10);
   WRITES(m, kv_append, kv_append_gpu, 1 << 2 | 1 << 3);
   WRITES(m, kv_append_q, kv_append_q_gpu, 1 << 3 | 1 << 4);
   WRITES(m, kv_append_q_into, kv_append_q_into_gpu, 1 << 1 | 1 << 4 | 1 << 5);

@@ -146,3 +146,25 @@ def test_inference_tensors_are_written_as_before():
     with torch.no_grad():
         t.kv_append(k, v, *cache, f)
         t.paged_attention_into(q, *cache, 0.1, torch.empty_like(q))
+
+
+def test_what_the_expert_ops_write_counts_as_changed():
+    """The in-place ops of the experts: workspaces, outputs and routing outputs, as their schemas say."""
+    import torch
+    t = import_pkg()._lib.torch_ops()
+    m = dict(device="meta")
+    E, G, H, N = 16, 32, 256, 5
+    u8 = lambda: torch.empty(4096, dtype=torch.uint8, **m)  # noqa: E731
+    x, rp, packed = torch.empty(N, H, **m), torch.empty(E, H, **m), u8()
+    out, logits, mask = torch.empty(N, H, dtype=torch.bfloat16, **m), torch.empty(N, E, **m), torch.empty(N, E, dtype=torch.uint8, **m)
+    common = (rp, None, E, G, 0.7, packed)
+    for op, args in ((t.decode_workspace_init, (u8(), H, E)), (t.moe_decode, (x[0], *common, u8())),
+                     (t.moe_decode_into, (x[0], *common, u8(), out[:1])), (t.moe_decode_batch, (x, *common, u8(), u8())),
+                     (t.moe_decode_batch_into, (x, *common, u8(), u8(), out, logits, mask)),
+                     (t.moe_decode_batch_into, (x, *common, u8(), u8(), out)),
+                     (t.moe_prefill_into, (x, *common, u8(), out, logits, mask)), (t.moe_prefill_into, (x, *common, u8(), out))):
+        schema = op.default._schema.arguments
+        tensors = [(a, s.alias_info is not None and s.alias_info.is_write) for a, s in zip(args, schema) if torch.is_tensor(a)]
+        before = [a._version for a, _ in tensors]
+        op(*args)
+        assert [a._version - b for (a, _), b in zip(tensors, before)] == [int(w) for _, w in tensors], op
