@@ -570,9 +570,15 @@ struct RotaryBackward : public torch::autograd::Node {
   bool inverse = false;
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     if (!grads[0].defined()) return {Tensor()};
-    return {rotary_call(grads[0], positions.unpack(), inv_freq.unpack(), layout, mscale, !inverse)};
+    Tensor p, f;
+    {
+      std::lock_guard<std::mutex> lock(mutex_);  // another thread's backward of the same graph may release them
+      p = positions.unpack(), f = inv_freq.unpack();
+    }
+    return {rotary_call(grads[0], p, f, layout, mscale, !inverse)};
   }
   void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
     positions.reset_data();
     inv_freq.reset_data();
   }

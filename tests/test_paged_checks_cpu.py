@@ -168,3 +168,36 @@ def test_what_the_expert_ops_write_counts_as_changed():
         before = [a._version for a, _ in tensors]
         op(*args)
         assert [a._version - b for (a, _), b in zip(tensors, before)] == [int(w) for _, w in tensors], op
+
+
+# ------------------------------------------------------------------ threads
+def test_backwards_of_one_graph_in_several_threads():
+    """Threads that run the backward of one graph, which its first one releases: each has its gradient or is told
+    that the graph is used up, and none meets what another is releasing."""
+    import threading
+    import torch
+    t, q, _, _, _, f = _fake()
+    pos = torch.empty(5, dtype=torch.int64, device="meta")
+    x = q.detach().requires_grad_()
+    g = torch.empty_like(q)
+    for keep in (True, False):
+        for _ in range(30):
+            y, odd, got = t.rotary(x, pos, f), [], []
+            ready = threading.Barrier(4)
+
+            def run():
+                ready.wait()
+                try:
+                    for _ in range(3):
+                        got.append(torch.autograd.grad(y, x, g, retain_graph=keep)[0].shape)
+                except RuntimeError as e:
+                    if "second time" not in str(e):
+                        odd.append(e)
+
+            threads = [threading.Thread(target=run) for _ in range(4)]
+            for th in threads:
+                th.start()
+            for th in threads:
+                th.join()
+            assert not odd and got and all(s == x.shape for s in got)
+            assert not keep or len(got) == 12
