@@ -520,18 +520,33 @@ Tensor rotary_output(const Tensor& in) {
   return out.sym_size(-1) > 1 && out.sym_stride(-1) != 1 ? at::empty_symint(in.sym_sizes(), in.options()) : out;
 }
 
-// x [N, heads, D] or [B, L, heads, D] with positions of the leading shape. Strides go to the kernel;
-// only channels that are not next to each other are copied first.
-Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
-                  double mscale, bool inverse) {
-  const int lay = rotary_layout(layout, "rotary");
+// The checks of shapes and types are the same for real and for fake tensors: sizes may be symbolic.
+bool same_sizes(const Tensor& a, const Tensor& b, int64_t dims) {
+  for (int64_t i = 0; i < dims; ++i)
+    if (!a.sym_size(i).sym_eq(b.sym_size(i)).expect_true(__FILE__, __LINE__)) return false;
+  return true;
+}
+
+void rotary_check(const Tensor& x, const Tensor& positions, const Tensor& inv_freq) {
   TORCH_CHECK(x.dim() == 3 || x.dim() == 4, "prunepath.rotary: x must be [N, heads, D] or [B, L, heads, D]");
-  TORCH_CHECK(positions.dim() == x.dim() - 2 && positions.sizes() == x.sizes().slice(0, x.dim() - 2),
+  x_code(x, "rotary");
+  TORCH_CHECK(positions.dim() == x.dim() - 2 && same_sizes(x, positions, x.dim() - 2),
               "prunepath.rotary: positions must have x's leading shape");
   TORCH_CHECK(positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt,
               "prunepath.rotary: positions must be int32 or int64");
   TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && inv_freq.is_contiguous(),
               "prunepath.rotary: inv_freq must be contiguous float64 [rotary_dim / 2]");
+  const c10::SymInt pairs = inv_freq.sym_size(0);
+  TORCH_SYM_CHECK(pairs.sym_ge(1).sym_and((pairs * 2).sym_le(x.sym_size(-1))), "prunepath.rotary: ", pairs,
+                  " pairs for heads of ", x.sym_size(-1), " channels");
+}
+
+// x [N, heads, D] or [B, L, heads, D] with positions of the leading shape. Strides go to the kernel;
+// only channels that are not next to each other are copied first.
+Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                  double mscale, bool inverse) {
+  const int lay = rotary_layout(layout, "rotary");
+  rotary_check(x, positions, inv_freq);
   same_device("rotary", x, {&x, &positions, &inv_freq});
   const c10::DeviceGuard g(x.device());
   const Tensor in = rotary_input(x);
@@ -549,7 +564,9 @@ Tensor rotary_gpu(const Tensor& x, const Tensor& positions, const Tensor& inv_fr
   return out;
 }
 
-Tensor rotary_meta(const Tensor& x, const Tensor&, const Tensor&, c10::string_view, double, bool) {
+Tensor rotary_meta(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, c10::string_view layout, double, bool) {
+  rotary_layout(layout, "rotary");
+  rotary_check(x, positions, inv_freq);
   return rotary_output(rotary_input(x));
 }
 
@@ -608,32 +625,75 @@ Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& i
 }
 
 // ------------------------------------------------------------------ paged cache
+// Heads, D and the cache of a call: shapes, types and what the kernels take of them.
+void paged_check(const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                 const Tensor& kv_lens, const Tensor& cu_q, const c10::SymInt& Hq, const c10::SymInt& D) {
+  TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
+                  v_pages.scalar_type() == at::kBFloat16,
+              "prunepath.", name, ": k_pages [pages, kv_heads, page, D] and v_pages [pages, kv_heads, D, page] bfloat16 required");
+  TORCH_SYM_CHECK(k_pages.sym_size(3).sym_eq(D).sym_and(v_pages.sym_size(2).sym_eq(D))
+                      .sym_and(v_pages.sym_size(0).sym_eq(k_pages.sym_size(0)))
+                      .sym_and(v_pages.sym_size(1).sym_eq(k_pages.sym_size(1)))
+                      .sym_and(v_pages.sym_size(3).sym_eq(k_pages.sym_size(2))),
+                  "prunepath.", name, ": shapes of k_pages ", k_pages.sym_sizes(), ", v_pages ", v_pages.sym_sizes(),
+                  " and head size ", D, " disagree");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && kv_lens.dim() == 1 &&
+                  kv_lens.scalar_type() == at::kInt && cu_q.dim() == 1 && cu_q.scalar_type() == at::kInt,
+              "prunepath.", name, ": block_table [seqs, max_pages], kv_lens [seqs] and cu_q [seqs + 1] must be int32");
+  const c10::SymInt seqs = kv_lens.sym_size(0), Hkv = k_pages.sym_size(1);
+  TORCH_SYM_CHECK(block_table.sym_size(0).sym_eq(seqs).sym_and(cu_q.sym_size(0).sym_eq(seqs + 1)), "prunepath.", name,
+                  ": block_table ", block_table.sym_sizes(), ", kv_lens ", kv_lens.sym_sizes(), " and cu_q ",
+                  cu_q.sym_sizes(), " disagree");
+  TORCH_SYM_CHECK(Hkv.sym_ge(1), "prunepath.", name, ": a cache of no heads");
+  TORCH_SYM_CHECK((Hq % Hkv).sym_eq(0), "prunepath.", name, ": ", Hq, " query heads on ", Hkv,
+                  " key heads (need a multiple)");
+  TORCH_SYM_CHECK(D.sym_eq(64).sym_or(D.sym_eq(128)), "prunepath.", name, ": head size ", D, " unsupported (64 or 128)");
+}
+
 struct Paged {
   int64_t n, seqs, Hq, Hkv, D, pages, max_pages, page;
 };
 
-Paged paged_check(const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                  const Tensor& kv_lens, const Tensor& cu_q, int64_t n, int64_t Hq, int64_t D) {
-  TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
-                  v_pages.scalar_type() == at::kBFloat16,
-              "prunepath.", name, ": k_pages [pages, kv_heads, page, D] and v_pages [pages, kv_heads, D, page] bfloat16 required");
+Paged paged_sizes(const char* name, const Tensor& k_pages, const Tensor& block_table, int64_t n, int64_t Hq) {
   Paged p;
-  p.n = n, p.Hq = Hq, p.D = D;
+  p.n = n, p.Hq = Hq, p.D = k_pages.size(3);
   p.pages = k_pages.size(0), p.Hkv = k_pages.size(1), p.page = k_pages.size(2);
-  TORCH_CHECK(k_pages.size(3) == D && v_pages.size(0) == p.pages && v_pages.size(1) == p.Hkv && v_pages.size(2) == D &&
-                  v_pages.size(3) == p.page,
-              "prunepath.", name, ": shapes of k_pages ", k_pages.sizes(), ", v_pages ", v_pages.sizes(),
-              " and head size ", D, " disagree");
-  TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && kv_lens.dim() == 1 &&
-                  kv_lens.scalar_type() == at::kInt && cu_q.dim() == 1 && cu_q.scalar_type() == at::kInt,
-              "prunepath.", name, ": block_table [seqs, max_pages], kv_lens [seqs] and cu_q [seqs + 1] must be int32");
-  p.seqs = kv_lens.size(0), p.max_pages = block_table.size(1);
-  TORCH_CHECK(block_table.size(0) == p.seqs && cu_q.size(0) == p.seqs + 1, "prunepath.", name, ": block_table ",
-              block_table.sizes(), ", kv_lens ", kv_lens.sizes(), " and cu_q ", cu_q.sizes(), " disagree");
+  p.seqs = block_table.size(0), p.max_pages = block_table.size(1);
   TORCH_CHECK(p.pages <= 0x7fffffff && p.max_pages <= 0x7fffffff && p.page <= 0x7fffffff && p.Hkv <= 0x7fffffff &&
                   p.seqs <= 0x7fffffff && Hq <= 0x7fffffff,
               "prunepath.", name, ": a size beyond 2^31");
   return p;
+}
+
+// q and q_out: a tensor or nullptr
+void kv_append_check(const Tensor* q, const Tensor* q_out, const Tensor& k, const Tensor& v, const Tensor& k_pages,
+                     const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                     const optional<Tensor>& inv_freq) {
+  const char* const name = "kv_append";
+  x_code(k, name);
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.scalar_type() == v.scalar_type() && same_sizes(k, v, 3),
+              "prunepath.kv_append: k and v must be [N, kv_heads, D] of one dtype");
+  if (q)
+    TORCH_CHECK(q->dim() == 3 && q->scalar_type() == k.scalar_type() &&
+                    q->sym_size(0).sym_eq(k.sym_size(0)).sym_and(q->sym_size(2).sym_eq(k.sym_size(2)))
+                        .sym_and(q->sym_stride(2).sym_eq(1)).expect_true(__FILE__, __LINE__),
+                "prunepath.kv_append: q must be [N, heads, D] of k's dtype, channels contiguous");
+  paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, q ? q->sym_size(1) : c10::SymInt(0), k.sym_size(2));
+  TORCH_SYM_CHECK(k.sym_size(1).sym_eq(k_pages.sym_size(1)), "prunepath.kv_append: ", k.sym_size(1),
+                  " heads for a cache of ", k_pages.sym_size(1));
+  TORCH_SYM_CHECK(k.sym_stride(2).sym_eq(1).sym_and(v.sym_stride(2).sym_eq(1)),
+                  "prunepath.kv_append: channels must be contiguous");
+  if (inv_freq) {
+    TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
+                "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
+    const c10::SymInt rd = inv_freq->sym_size(0) * 2;
+    TORCH_SYM_CHECK(rd.sym_le(k.sym_size(2)).sym_and((rd % 16).sym_eq(0)), "prunepath.kv_append: rotary_dim ", rd,
+                    " unsupported (a multiple of 16 up to the head size ", k.sym_size(2), ")");
+  }
+  if (q_out)
+    TORCH_CHECK(q_out->scalar_type() == at::kBFloat16 && q_out->dim() == 3 && same_sizes(*q_out, *q, 3) &&
+                    q_out->is_contiguous(),
+                "prunepath.kv_append: q_out must be contiguous bfloat16 of q's shape");
 }
 
 void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bool zero_tail, const Tensor& k,
@@ -642,20 +702,10 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
                     c10::string_view layout, double mscale) {
   const char* const name = "kv_append";
   const int lay = rotary_layout(layout, name);
-  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
-              "prunepath.kv_append: k and v must be [N, kv_heads, D] of one dtype");
-  if (q)
-    TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(2) == k.size(2) &&
-                    q->scalar_type() == k.scalar_type() && q->stride(2) == 1,
-                "prunepath.kv_append: q must be [N, heads, D] of k's dtype, channels contiguous");
-  const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, k.size(0), q ? q->size(1) : 0, k.size(2));
-  TORCH_CHECK(k.size(1) == p.Hkv, "prunepath.kv_append: ", k.size(1), " heads for a cache of ", p.Hkv);
-  TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, "prunepath.kv_append: channels must be contiguous");
+  kv_append_check(q ? &*q : nullptr, q ? &*q_out : nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+  const Paged p = paged_sizes(name, k_pages, block_table, k.size(0), q ? q->size(1) : 0);
   need_gpu(name, k, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, inv_freq ? &*inv_freq : nullptr});
   same_device(name, k, {&k, &v});
-  if (inv_freq)
-    TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
-                "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
   const Span sk(k), sv(v), kp(k_pages), vp(v_pages), st(block_table), sl(kv_lens), sc(cu_q);
   const Span sf = inv_freq ? Span(*inv_freq) : st;
   for (const Span* in : {&sk, &sv, &st, &sl, &sc, &sf}) {
@@ -665,8 +715,6 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   apart(name, kp, vp);
   int64_t qs[2] = {0, 0};
   if (q) {
-    TORCH_CHECK(q_out->scalar_type() == at::kBFloat16 && q_out->sizes() == q->sizes() && q_out->is_contiguous(),
-                "prunepath.kv_append: q_out must be contiguous bfloat16 of q's shape");
     same_device(name, k, {&*q, &*q_out});
     const Span sq(*q);
     apart(name, kp, sq);
@@ -710,24 +758,42 @@ void kv_append_q_into_gpu(const Tensor& q, const Tensor& q_out, const Tensor& k,
   kv_append_into(q, q_out, false, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale);
 }
 
-void kv_append_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                    const Tensor&, const optional<Tensor>&, c10::string_view, double) {}
-Tensor kv_append_q_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                        const Tensor&, const Tensor&, const optional<Tensor>&, c10::string_view, double) {
+void kv_append_meta(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                    const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                    const optional<Tensor>& inv_freq, c10::string_view layout, double) {
+  rotary_layout(layout, "kv_append");
+  kv_append_check(nullptr, nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+}
+Tensor kv_append_q_meta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                        const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                        const optional<Tensor>& inv_freq, c10::string_view layout, double) {
+  rotary_layout(layout, "kv_append");
+  kv_append_check(&q, nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
   return at::empty_symint(q.sym_sizes(), q.options().dtype(at::kBFloat16));
 }
-void kv_append_q_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                           const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, c10::string_view,
-                           double) {}
+void kv_append_q_into_meta(const Tensor& q, const Tensor& q_out, const Tensor& k, const Tensor& v, const Tensor& k_pages,
+                           const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                           const optional<Tensor>& inv_freq, c10::string_view layout, double) {
+  rotary_layout(layout, "kv_append");
+  kv_append_check(&q, &q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+}
+
+// out: a tensor or nullptr
+void attention_check(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                     const Tensor& kv_lens, const Tensor& cu_q, const Tensor* out) {
+  TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.sym_stride(2).sym_eq(1).expect_true(__FILE__, __LINE__),
+              "prunepath.paged_attention: q must be bfloat16 [N, heads, D], channels contiguous");
+  if (out)
+    TORCH_CHECK(out->scalar_type() == at::kBFloat16 && out->dim() == 3 && same_sizes(*out, q, 3) && out->is_contiguous(),
+                "prunepath.paged_attention: out must be contiguous bfloat16 of q's shape");
+  paged_check("paged_attention", k_pages, v_pages, block_table, kv_lens, cu_q, q.sym_size(1), q.sym_size(2));
+}
 
 void attention_into(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
                     const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out, bool zero_tail) {
   const char* const name = "paged_attention";
-  TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.stride(2) == 1,
-              "prunepath.paged_attention: q must be bfloat16 [N, heads, D], channels contiguous");
-  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.is_contiguous(),
-              "prunepath.paged_attention: out must be contiguous bfloat16 of q's shape");
-  const Paged p = paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, q.size(0), q.size(1), q.size(2));
+  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, &out);
+  const Paged p = paged_sizes(name, k_pages, block_table, q.size(0), q.size(1));
   need_gpu(name, q, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &out});
   same_device(name, q, {&q});
   if (!zero_tail) {  // a given out
@@ -760,12 +826,15 @@ Tensor paged_attention_gpu(const Tensor& q, const Tensor& k_pages, const Tensor&
   return out;
 }
 
-Tensor paged_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                            double) {
+Tensor paged_attention_meta(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                            const Tensor& kv_lens, const Tensor& cu_q, double) {
+  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, nullptr);
   return at::empty_symint(q.sym_sizes(), q.options());
 }
-void paged_attention_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                               double, const Tensor&) {}
+void paged_attention_into_meta(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                               const Tensor& kv_lens, const Tensor& cu_q, double, const Tensor& out) {
+  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, &out);
+}
 
 // ------------------------------------------------------------------ ops for inference
 void refuse_gradient(const char* op, const Tensor& t) {

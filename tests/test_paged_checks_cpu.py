@@ -201,3 +201,51 @@ def test_backwards_of_one_graph_in_several_threads():
                 th.join()
             assert not odd and got and all(s == x.shape for s in got)
             assert not keep or len(got) == 12
+
+
+# ------------------------------------------------------------------ shapes of fake tensors
+def test_fake_calls_check_what_real_ones_do():
+    import torch
+    t, q, k, v, cache, f = _fake()
+    kp, vp, table, lens, cu = cache
+    pos, i32 = torch.empty(5, dtype=torch.int64, device="meta"), dict(dtype=torch.int32, device="meta")
+    e = torch.empty_like
+    bad = {"positions of another length": lambda: t.rotary(q, pos[:4], f), "float positions": lambda: t.rotary(q, pos.float(), f),
+           "more pairs than channels": lambda: t.rotary(q[..., :32], pos, f), "float frequencies": lambda: t.rotary(q, pos, f.float()),
+           "no pairs": lambda: t.rotary(q, pos, f[:0]), "a layout": lambda: t.rotary(q, pos, f, "other"),
+           "half precision": lambda: t.rotary(q.half(), pos, f), "two dimensions": lambda: t.rotary(q[0], pos, f),
+           "heads on no multiple": lambda: t.paged_attention(q[:, :3].contiguous(), *cache, 0.1),
+           "channels": lambda: t.paged_attention(torch.empty(5, 3, 96, dtype=q.dtype, device="meta"), *cache, 0.1),
+           "head size": lambda: t.paged_attention(torch.empty(5, 2, 96, dtype=q.dtype, device="meta"), kp.new_empty(9, 2, 16, 96),
+                                                  vp.new_empty(9, 2, 96, 16), table, lens, cu, 0.1),
+           "float queries": lambda: t.paged_attention(q.float(), *cache, 0.1),
+           "pages as they are": lambda: t.paged_attention(q, kp, kp, table, lens, cu, 0.1),
+           "offsets": lambda: t.paged_attention(q, kp, vp, table, lens, cu[:2], 0.1),
+           "a long table": lambda: t.paged_attention(q, kp, vp, table.long(), lens, cu, 0.1),
+           "an output": lambda: t.paged_attention_into(q, *cache, 0.1, e(q)[:, :2]),
+           "a float output": lambda: t.paged_attention_into(q, *cache, 0.1, q.float()),
+           "sequences": lambda: t.kv_append(k, v, kp, vp, table, torch.empty(3, **i32), torch.empty(4, **i32), f),
+           "values": lambda: t.kv_append(k, v[:4], *cache, f), "types": lambda: t.kv_append(k, v.float(), *cache, f),
+           "heads of the cache": lambda: t.kv_append(k[:, :1], v[:, :1], *cache, f),
+           "pairs": lambda: t.kv_append(k, v, *cache, f[:4]), "a layout of the append": lambda: t.kv_append(k, v, *cache, f, "other"),
+           "query rows": lambda: t.kv_append_q(q[:4], k, v, *cache, f), "query type": lambda: t.kv_append_q(q.float(), k, v, *cache, f),
+           "query output": lambda: t.kv_append_q_into(q, e(q).transpose(0, 1), k, v, *cache, f)}
+    for what, call in bad.items():
+        with pytest.raises(RuntimeError, match="prunepath"):
+            call()
+            print("not refused:", what)
+
+
+def test_fake_calls_with_symbolic_sizes():
+    """Tokens, sequences and the table's width may be symbols; the result follows them."""
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    t, q, k, v, cache, f = _fake()
+
+    def step(q, k, v, kp, vp, table, lens, cu, f):
+        return t.paged_attention(t.kv_append_q(q, k, v, kp, vp, table, lens, cu, f), kp, vp, table, lens, cu, 0.1)
+
+    with torch.no_grad():
+        gm = make_fx(step, tracing_mode="symbolic")(q, k, v, *cache, f)
+    out = [n.meta["val"] for n in gm.graph.nodes if n.op == "call_function" and "paged_attention" in str(n.target)]
+    assert len(out) == 1 and not isinstance(out[0].shape[0], int) and out[0].dtype == torch.bfloat16
