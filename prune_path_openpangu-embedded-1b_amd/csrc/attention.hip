@@ -50,7 +50,8 @@ struct AttnArgs {
   uint32_t keep, flip;  // bits of a pair of q: all, or none where scale is 0; the sign of scale
   bf16_t* out;
   int zero_tail;
-  int splits, least;  // most ranges of a tile; fewest tokens of a range
+  int splits;         // most ranges of a tile
+  int base, behind;   // ranges of a tile, see attn_cut
   float *po, *pml;    // workspace: [row][split][D], [row][split][2]
   int* pns;           // workspace: splits of a row
   int tiles;          // tiles of rows, of every sequence together
@@ -67,6 +68,18 @@ struct AttnTile {
   int ns;        // ranges of the tile (0: nothing is attended)
 };
 
+// Ranges of a tile that attends nt tokens, of a sequence of len. It goes by the tokens that are there, not
+// by the table's width, which may be any number of times theirs.
+template <int R>
+__device__ __forceinline__ int attn_cut(const AttnArgs& a, int nt, int len) {
+  int cut;
+  if (R == 16)  // `base` ranges of 128 tokens and more, and at least one per 1024; up to 384 tokens the join costs more
+    cut = nt <= 384 ? 1 : max(min(a.base, (nt + 127) / 128), nt >> 10);
+  else  // of 512 tokens and more, `behind` ranges in a chunk of one sequence far behind the cache's start
+    cut = min(a.seqs.n_seqs == 1 && (int64_t)len >= 2 * (int64_t)a.seqs.n_rows ? a.behind : a.base, (nt + 511) / 512);
+  return max(1, min(cut, a.splits));
+}
+
 template <int R>
 __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int split) {
   AttnTile w;
@@ -82,7 +95,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int 
   w.p0 = tail ? -(int64_t)len : (int64_t)f.len - len;
   w.nt = (int)max((int64_t)0, min(w.p0 + (w.r0 + max(w.nr, 1) - 1) / g + 1, (int64_t)a.seqs.capacity()));
   // equal ranges of whole steps, none of them empty
-  const int cut = max(1, min(a.splits, (w.nt + a.least - 1) / a.least));
+  const int cut = attn_cut<R>(a, w.nt, f.len);
   const int per = ((w.nt + cut - 1) / cut + 127) / 128 * 128;
   w.ns = w.nt > 0 ? (w.nt + per - 1) / per : 0;
   w.lo = (int)min((int64_t)split * per, (int64_t)w.nt);
@@ -198,8 +211,16 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   __shared__ float o_s[4][R][OS];
   __shared__ float ml_s[4][R][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.splits;
-  const int item = blockIdx.x / a.splits, h = item % a.Hkv;
+  // Items are (split, tile, head), the heads fastest: a tile's later ranges, which many do not have, behind every
+  // tile's first. (Next to them, ranges of one number met on few of the XCDs: 64 sequences of 2000 tokens in a
+  // table of eight ranges 607 us instead of 142.) The last tile, as a rule of no sequence, behind everything: the
+  // workgroups that have work are the first ones, one to a CU if they are few (one token at 8191 15 us, 19
+  // without). Workgroup b runs on XCD b % 8: ranges of one number begin half way round from those before, for
+  // where every other tile is empty and half of the XCDs would have all the work (32 sequences of two rows, 4
+  // heads, 119 us instead of 140).
+  const int items = (a.tiles - 1) * a.Hkv, most = items * a.splits, b = blockIdx.x;
+  const int split = b < most ? b / items : (b - most) / a.Hkv, turn = split * (items - 4) & 7;
+  const int item = b < most ? (b - split * items + turn) % items : items + (b - most) % a.Hkv, h = item % a.Hkv;
   const AttnTile w = attn_tile<R>(a, item / a.Hkv, split);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
@@ -680,6 +701,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
 // as many rows as fit (ALONE); with many it takes one row, its groups of threads alternate ranges,
 // added in order through LDS.
 #define ATTN_MAX_SPLITS 64
+#define ATTN_SPREAD 16  // workgroups of 16-row tiles per CU beyond which more ranges even nothing out
 #define ATTN_JOIN_ALONE 8  // ranges up to which a row's threads add them alone
 
 template <int D, bool ALONE>
@@ -723,12 +745,12 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(AttnArgs a, int
 // ------------------------------------------------------------------ host
 struct AttnPlan {
   int rows;    // per tile: 16 or ATTN_ROWS
-  int splits, least;
+  int splits, base, behind;
   int64_t tiles;
 };
 
 static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv, int D) {
-  AttnPlan p;
+  AttnPlan p = {};
   const int64_t rows = n_tokens * (Hq / Hkv), cus = pp_device_cus(), capacity = (int64_t)max_pages * page_size;
   auto items = [&](int tile) { return std::max<int64_t>(1, (rows / tile + n_seqs) * Hkv); };
   // Tiles of 16 rows for single tokens and the like, and for what is short altogether: their steps
@@ -739,20 +761,23 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
   const bool few = rows <= 16 * (int64_t)n_seqs || items(16) * ((capacity + 127) / 128) <= 4096;
   p.rows = few ? 16 : ATTN_ROWS;
   p.tiles = rows / p.rows + n_seqs + 1;
-  p.least = few ? 128 : 512;
   const int64_t each = items(p.rows);
-  int64_t want;
+  int64_t most;
   if (few) {
-    // As many ranges as give every CU one, and at least one per 1024 tokens of the table, so that
-    // sequences of different lengths even out; none in a table of 384, where the join costs more. 12
-    // heads, one token: 256, 512, 1024, 2048, 4096 tokens 7.0, 9.2, 13.5, 22.3, 40.6 us, in ranges of
-    // 128 8.1, 8.2, 8.8, 9.4, 12.1; 16 sequences of 1024 19.2, in 6 ranges 22.9; 64 of 1 to 8192 tokens
-    // 343 us, in 2, 8, 32 ranges 300, 271, 347.
-    want = capacity <= 384 ? 1 : std::max(cus / each, capacity / 1024);
+    // As many ranges as give every CU one, and at least one per 1024 tokens, so that sequences of different
+    // lengths even out. 12 heads, one token: 256, 512, 1024, 2048, 4096 tokens 7.0, 9.2, 13.5, 22.3, 40.6 us, in
+    // ranges of 128 8.1, 8.2, 8.8, 9.4, 12.1; 16 sequences of 1024 19.2, in 6 ranges 22.9; 64 of 1 to 8192 tokens
+    // in 1, 2, 8 ranges 343, 300, 271. The width of the table and ATTN_SPREAD workgroups a CU bound them, and so
+    // the grid and the workspace: for 8, 16, 32 a CU 64 sequences of 1 to 8192 tokens 292, 283, 280 us, 64 of 500
+    // in a table of 32000 tokens 36, 42, 51 (33 in one of 512; by the width alone 192); the workspace stays below
+    // that many workgroups' 16 rows of D + 2 floats, 35 MB, and one more range of every row.
+    p.base = (int)std::max<int64_t>(1, cus / each);
+    most = capacity <= 384 ? 1 : std::max<int64_t>(p.base, std::min(capacity / 1024, (ATTN_SPREAD * cus + each - 1) / each));
+    most = std::min(most, (capacity + 127) / 128);
   } else {
     // One round of the workgroups that the GPU holds (2 per CU at D = 128, 3 at D = 64): a part of a round more
     // is a round of its own where all tiles are about as long, in a chunk of one sequence far behind the
-    // cache's start (a table of twice its tokens and more). Those of a prompt and of several sequences
+    // cache's start (`behind`: as long again and more before it). Those of a prompt and of several sequences
     // differ, and there a part of a round does no harm while there are few ranges.
     // us for 1, 2, 3, 4 ranges: prompts of 2048 tokens (204 items) 49, 42, 37, 45; of 4096 (396) 97, 86, 93,
     // 103; of 8192 (780) 231, and 265 with even one tile cut; new tokens at 8000: 1500 (144) 196, 135, 113,
@@ -760,10 +785,11 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
     // 126, of D = 64 (500 at 29511, 128 items) 165, 184, 194;
     // for 1, 2: nine sequences of 700 new tokens at 4000 and single ones 116, 86.
     const int64_t slots = (D == 64 ? 3 : 2) * cus;
-    const bool even = n_seqs == 1 && capacity >= 2 * n_tokens;
-    want = even || slots / each >= 4 ? slots / each : (slots + each - 1) / each;
+    p.behind = (int)std::max<int64_t>(1, slots / each);
+    p.base = p.behind >= 4 ? p.behind : (int)((slots + each - 1) / each);
+    most = std::min<int64_t>(p.base, (capacity + 511) / 512);
   }
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ATTN_MAX_SPLITS, want, (capacity + p.least - 1) / p.least}));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ATTN_MAX_SPLITS, most));
   return p;
 }
 
@@ -806,7 +832,7 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv;
   a.c = c != 0.0f ? c : 1.0f, a.keep = c != 0.0f ? ~0u : 0u, a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
-  a.splits = p.splits, a.least = p.least, a.tiles = (int)p.tiles;
+  a.splits = p.splits, a.base = p.base, a.behind = p.behind, a.tiles = (int)p.tiles;
   a.po = (float*)workspace;
   a.pml = a.po + n_tokens * Hq * p.splits * D;
   a.pns = (int*)(a.pml + n_tokens * Hq * p.splits * 2);
@@ -814,7 +840,11 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   const bool alone = p.splits <= ATTN_JOIN_ALONE;
   // (the join's are never more: calls of 16-row tiles have at most 8 rows to a tile, and one of more than 8
   // ranges has as many workgroups; 128-row tiles are cut into ranges only where they are fewer than the GPU holds)
-  PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld workgroups (at most 2^24 - 1)", what, (long long)items);
+  // The limit counts a range per 1024 tokens of the table (64 at most), though a launch of that size has fewer:
+  // so it goes by the shapes alone, not by the GPU's size.
+  const int64_t widest = p.rows == 16 ? std::min<int64_t>(ATTN_MAX_SPLITS, (int64_t)max_pages * page_size / 1024) : 1;
+  const int64_t counted = std::max(items, p.tiles * Hkv * widest);
+  PP_REQUIRE(counted <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld workgroups (at most 2^24 - 1)", what, (long long)counted);
   const int64_t joins = alone ? (rows * (D / 4) + ATTN_THREADS - 1) / ATTN_THREADS : rows;
   hipStream_t st = (hipStream_t)stream;
   const unsigned n = (unsigned)items, nj = (unsigned)joins;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from helpers import dev
-from test_gpu_paged import Batch
+from test_gpu_paged import Batch, attend64, check_attention, few, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,20 @@ def test_opcheck(pkg):
                      (t.paged_attention, (q, *cache, 0.1)), (t.paged_attention_into, (q, *cache, 0.1, torch.zeros_like(q)))):
         print(f"opcheck {op}", flush=True)
         opcheck(op, args)
+
+
+@pytest.mark.parametrize("new,total,heads,kv_heads,dim", [
+    ([1] * 20, [3000, 1, 17, 384, 385, 1023, 1025, 2047, 2600, 40, 700, 129, 2049, 5, 64, 1500, 1, 900, 3001, 333], 4, 2, 128),
+    ([2] * 7, [2, 5000, 100, 2048, 4097, 33, 1024], 8, 1, 64), ([1], [5000], 12, 12, 128), ([150], [3000], 2, 2, 128),
+    ([1500], [1500], 2, 1, 128), ([40, 30, 90], [2500, 30, 700], 6, 3, 64)])
+def test_tables_wider_than_their_sequences(pkg, new, total, heads, kv_heads, dim):
+    """A table of 65536 tokens and one as long as the longest sequence: several ranges and the join in both."""
+    for extra in (0, 65536 // 32 - -(-max(total) // 32)):
+        b = Batch(new, total, 32, kv_heads, dim, seed=dim, extra=extra)
+        q = (1.5 * torch.randn(b.n, heads, dim, generator=gen(3))).to(torch.bfloat16)
+        rows = slice(0, b.n) if b.n < 200 else slice(b.n - 40, b.n)
+        got = pkg.ops.paged_attention(q.to(dev()), *b.gpu())
+        if b.n >= 200:  # (the last rows of a long prompt stand for all)
+            b.rows = lambda b=b: ((r, s, p) for r, s, p in Batch.rows(b) if r >= rows.start)
+        o, big = attend64(b, q)
+        check_attention(got[rows], o[rows], big[rows], few(b, heads, kv_heads))

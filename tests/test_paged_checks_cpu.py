@@ -249,3 +249,45 @@ def test_fake_calls_with_symbolic_sizes():
         gm = make_fx(step, tracing_mode="symbolic")(q, k, v, *cache, f)
     out = [n.meta["val"] for n in gm.graph.nodes if n.op == "call_function" and "paged_attention" in str(n.target)]
     assert len(out) == 1 and not isinstance(out[0].shape[0], int) and out[0].dtype == torch.bfloat16
+
+
+# ------------------------------------------------------------------ ranges of the attention's tiles
+@pytest.mark.parametrize("n,seqs,hq,hkv,d", [(1, 1, 12, 12, 128), (64, 64, 12, 12, 128), (256, 256, 32, 8, 128),
+                                             (4096, 256, 12, 12, 128), (4096, 256, 32, 32, 128), (2048, 1, 12, 12, 64),
+                                             (1736, 9, 24, 4, 128), (65536, 4096, 64, 8, 128)])
+def test_workspace_does_not_follow_the_tables_width(n, seqs, hq, hkv, d):
+    """A range of every row, and of all together at most 16 tiles of 16 rows (or two of 128) for each of 256 CUs: no
+    table of any width asks for more."""
+    rows = n * hq
+    most = rows * (4 * (d + 2) * 2 + 4) + 256 * 16 * 16 * 4 * (d + 2)
+    for pages in (8, 64, 512, 4096, 65536):
+        assert 0 <= _lib().pp_paged_attention_workspace_bytes(n, seqs, pages, 16, hq, hkv, d) <= most
+
+
+def test_ranges_by_length_cover_the_tokens():
+    """The cut of csrc/attention.hip restated: any bounds, any lengths; never more ranges than the workspace has."""
+    up = lambda x, y: -(-x // y)  # noqa: E731
+    for splits in (1, 2, 7, 21, 64):
+        for base, behind in ((1, 1), (2, 2), (5, 4), (21, 21), (64, 64), (256, 0)):
+            for nt in (1, 31, 128, 384, 385, 511, 513, 1024, 2049, 8191, 30011, 65537, 1 << 20):
+                for few, far in ((True, False), (False, False), (False, True)):
+                    cut = (1 if nt <= 384 else max(min(base, up(nt, 128)), nt >> 10)) if few else min(behind if far else base, up(nt, 512))
+                    cut = max(1, min(cut, splits))
+                    per = up(up(nt, cut), 128) * 128
+                    ns = up(nt, per)
+                    assert 1 <= ns <= splits and (ns - 1) * per < nt <= ns * per
+
+
+def test_items_of_16_row_tiles_are_each_taken_once():
+    """Workgroups -> (split, tile, head) of csrc/attention.hip restated."""
+    for tiles, heads, splits in ((1, 1, 1), (1, 3, 4), (2, 12, 21), (18, 12, 8), (65, 4, 8), (70, 1, 11), (9, 5, 64)):
+        items, seen = (tiles - 1) * heads, set()
+        for b in range(tiles * heads * splits):
+            if b < items * splits:
+                split = b // items
+                item = (b - split * items + (split * (items - 4) & 7)) % items
+            else:
+                split, item = (b - items * splits) // heads, items + (b - items * splits) % heads
+            seen.add((split, item // heads, item % heads))
+        assert len(seen) == tiles * heads * splits and max(s for s, _, _ in seen) == splits - 1
+        assert max(t for _, t, _ in seen) == tiles - 1
