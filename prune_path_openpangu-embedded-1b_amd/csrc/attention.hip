@@ -753,12 +753,17 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
   AttnPlan p = {};
   const int64_t rows = n_tokens * (Hq / Hkv), cus = pp_device_cus(), capacity = (int64_t)max_pages * page_size;
   auto items = [&](int tile) { return std::max<int64_t>(1, (rows / tile + n_seqs) * Hkv); };
-  // Tiles of 16 rows for single tokens and the like, and for what is short altogether: their steps
-  // cost four times as much for the same work (6 ns for 16 rows x 128 tokens of D = 128, the whole GPU
-  // at work, against 1.4), but there are eight times as many tiles. 12 heads: prompts of 200, 512, 700
-  // and 1024 tokens 6.9, 12.3, 16.7 and 25.0 us, tiles of 128 rows 10.8, 17.5, 21.2 and 23.3; 128 new
-  // tokens at 8000 51 against 32; 32 sequences of 4 x 8 rows at 8191 tokens 147 against 103.
-  const bool few = rows <= 16 * (int64_t)n_seqs || items(16) * ((capacity + 127) / 128) <= 4096;
+  // Tiles of 16 rows for single tokens and the like, for what does not fill the GPU, and for what is short
+  // altogether: their steps cost four times as much for the same work (6 ns for 16 rows x 128 tokens of D = 128,
+  // the whole GPU at work, against 1.4), but there are eight times as many tiles. 12 heads: prompts of 200, 512,
+  // 700 and 1024 tokens 6.9, 12.3, 16.7 and 25.0 us, tiles of 128 rows 10.8, 17.5, 21.2 and 23.3; 128 new tokens
+  // at 8000 51 against 32. Sequences of one length, 64 of up to 8000 tokens: 1, 4, 8, 16 rows each 423, 422, 439,
+  // 470 us, tiles of 128 rows 468, 452, 462, 455; 32 heads on 8, 4, 8, 16 rows 298, 305, 406 against 292, 295,
+  // 298; one of 8000, 8 rows, 11.5 against 19.0. Up to 4 rows a sequence, as a mean, so that a chunk among
+  // single tokens does not come to tiles of 16 rows, which is what the step of a server has: 63 single tokens and
+  // 900 at 8000 362 us, in tiles of 128 rows 229; 255 and 3800 at 4000 953 and 449 (32 heads on 8 1756 and 577).
+  const bool few = rows <= 4 * (int64_t)n_seqs || (rows <= 16 * (int64_t)n_seqs && items(16) <= cus) ||
+                   items(16) * ((capacity + 127) / 128) <= 4096;
   p.rows = few ? 16 : ATTN_ROWS;
   p.tiles = rows / p.rows + n_seqs + 1;
   const int64_t each = items(p.rows);

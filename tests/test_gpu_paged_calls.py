@@ -72,3 +72,13 @@ def test_tables_wider_than_their_sequences(pkg, new, total, heads, kv_heads, dim
             b.rows = lambda b=b: ((r, s, p) for r, s, p in Batch.rows(b) if r >= rows.start)
         o, big = attend64(b, q)
         check_attention(got[rows], o[rows], big[rows], few(b, heads, kv_heads))
+
+
+@pytest.mark.parametrize("singles,chunk,heads,kv_heads,dim", [(40, 200, 2, 2, 128), (64, 130, 8, 2, 64), (100, 33, 12, 12, 128)])
+def test_a_chunk_among_single_tokens(pkg, singles, chunk, heads, kv_heads, dim):
+    """The step of a server: single tokens of many sequences and one sequence's chunk."""
+    new = [1] * (singles // 2) + [chunk] + [1] * (singles - singles // 2)
+    total = [n + (37 * i) % 301 for i, n in enumerate(new)]
+    b = Batch(new, total, 16, kv_heads, dim, seed=chunk, extra=4096)
+    q = (1.5 * torch.randn(b.n, heads, dim, generator=gen(chunk))).to(torch.bfloat16)
+    check_attention(pkg.ops.paged_attention(q.to(dev()), *b.gpu()), *attend64(b, q), False)
