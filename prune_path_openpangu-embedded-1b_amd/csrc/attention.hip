@@ -843,8 +843,9 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.pns = (int*)(a.pml + n_tokens * Hq * p.splits * 2);
   const int64_t items = p.tiles * Hkv * p.splits, rows = n_tokens * Hq;
   const bool alone = p.splits <= ATTN_JOIN_ALONE;
-  // (the join's are never more: calls of 16-row tiles have at most 8 rows to a tile, and one of more than 8
-  // ranges has as many workgroups; 128-row tiles are cut into ranges only where they are fewer than the GPU holds)
+  // (the join's are never more: eight rows each and more where there are few ranges, which is two workgroups to a
+  // tile of 16 rows; calls of more than 8 ranges, and cut tiles of 128 rows, are no more than the GPU holds some
+  // times over)
   // The limit counts a range per 1024 tokens of the table (64 at most), though a launch of that size has fewer:
   // so it goes by the shapes alone, not by the GPU's size.
   const int64_t widest = p.rows == 16 ? std::min<int64_t>(ATTN_MAX_SPLITS, (int64_t)max_pages * page_size / 1024) : 1;

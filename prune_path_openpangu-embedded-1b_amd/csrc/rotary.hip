@@ -446,9 +446,11 @@ extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void*
   // Heads of an item. Single tokens: a group has one, so all the heads that the threads hold in one step
   // (32, value heads 4, or 16 where there are workgroups enough); 1, 64, 256 sequences of 12 heads 3.5,
   // 5.1, 8.8 us, in items of 4 heads 3.7, 5.7, 12.6. Chunks: 4, and one value head (64 tokens of it),
-  // 8192 tokens (151 MB, from memory) 38 us, 8 or 12 heads 42 and 41.
+  // 8192 tokens (151 MB, from memory) 38 us, 8 or 12 heads 42 and 41. Between them, and where a chunk is among
+  // single tokens, 4 value heads: 64 sequences of 4 and 16 tokens 8.7 and 16.6 us, with 16 13.4 and 27.5; 64
+  // single tokens and 512 8.9 against 13.2, 255 and 3800 24 against 34 (with one 31).
   a.per = n_tokens <= 4 * (int64_t)n_seqs ? 32 : 4;
-  a.vper = n_tokens > 16 * (int64_t)n_seqs ? 1 : n_seqs >= 64 ? 16 : 4;
+  a.vper = n_tokens > 16 * (int64_t)n_seqs ? 1 : n_seqs >= 64 && n_tokens <= 2 * (int64_t)n_seqs ? 16 : 4;
   a.nqb = (Hq + a.per - 1) / a.per, a.nkb = (Hkv + a.per - 1) / a.per, a.nvb = (Hkv + a.vper - 1) / a.vper;
   const int64_t values = ((n_tokens >> 6) + 2 * ((int64_t)n_seqs + 1)) * a.nvb;
   const int64_t items = values + ((n_tokens >> 4) + 2 * ((int64_t)n_seqs + 1)) * (a.nqb + a.nkb);

@@ -82,3 +82,18 @@ def test_a_chunk_among_single_tokens(pkg, singles, chunk, heads, kv_heads, dim):
     b = Batch(new, total, 16, kv_heads, dim, seed=chunk, extra=4096)
     q = (1.5 * torch.randn(b.n, heads, dim, generator=gen(chunk))).to(torch.bfloat16)
     check_attention(pkg.ops.paged_attention(q.to(dev()), *b.gpu()), *attend64(b, q), False)
+
+
+@pytest.mark.parametrize("new", [[1] * 30 + [100] + [1] * 40, [4] * 66, [2] * 70, [1] * 64 + [1100]], ids=len)
+def test_append_of_uneven_batches(pkg, new):
+    """Many sequences with few tokens each, and a chunk among single tokens: keys and values as they are, without a
+    rotation, in their places and nowhere else."""
+    total = [n + (29 * i) % 90 for i, n in enumerate(new)]
+    b = Batch(new, total, 16, 5, 64, seed=len(new))
+    kv = torch.randn(2, b.n + 3, 5, 64, generator=gen(7)).to(torch.bfloat16)
+    kp, vp, table, lens, cu = b.gpu()
+    pkg.ops.kv_append(kv[0].to(dev()), kv[1].to(dev()), kp, vp, table, lens, cu)
+    for row, s, p in b.rows():
+        at = b.place(s, p)
+        b.k[at[0], :, at[1]], b.v[at[0], :, :, at[1]] = kv[0, row], kv[1, row]
+    assert torch.equal(kp.cpu(), b.k) and torch.equal(vp.cpu(), b.v)
