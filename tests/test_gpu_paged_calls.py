@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from helpers import dev
-from test_gpu_paged import Batch, attend64, check_attention, few, gen
+from test_gpu_paged import LONG, Batch, attend64, check_attention, few, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,40 @@ def test_append_of_uneven_batches(pkg, new):
         at = b.place(s, p)
         b.k[at[0], :, at[1]], b.v[at[0], :, :, at[1]] = kv[0, row], kv[1, row]
     assert torch.equal(kp.cpu(), b.k) and torch.equal(vp.cpu(), b.v)
+
+
+@pytest.mark.parametrize("seqs", [255, 256, 257, 300])
+def test_many_sequences_in_large_tiles(pkg, seqs):
+    """Around the borders of 256 sequences with tiles of 128 rows: chunks, single tokens, empty sequences and rows
+    of no sequence."""
+    new = [(i * 7) % 4 for i in range(seqs)]
+    for s in (0, 63, 64, 254, 255, 256, 257, 299):
+        if s < seqs:
+            new[s] = 9 + s % 30
+    total = [n + i % 40 for i, n in enumerate(new)]
+    b = Batch(new, total, 16, 1, 64, seed=seqs, extra=LONG // 16 // 64)
+    assert not few(b, 16, 1)
+    q = torch.randn(b.n + 5, 16, 64, generator=gen(seqs)).to(torch.bfloat16)
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu())
+    check_attention(got[:b.n], *attend64(b, q[:b.n]), False)
+    assert bool((got[b.n:] == 0).all())
+
+
+@pytest.mark.parametrize("new,total,heads,kv_heads,dim,ranges", [
+    ([300] * 4, [1900, 300, 1100, 650], 24, 12, 128, 2), ([700, 1, 600], [1300, 900, 2100], 12, 12, 128, 4),
+    ([900] * 3, [1000, 2500, 900], 8, 8, 64, 4), ([1000], [2600], 12, 12, 128, 5)])
+def test_large_tiles_in_a_few_ranges(pkg, new, total, heads, kv_heads, dim, ranges):
+    """2 to 8 ranges of a tile, joined by the rows' own threads. The last rows of every sequence, which attend most,
+    stand for all."""
+    page = 64
+    b = Batch(new, total, page, kv_heads, dim, seed=ranges, extra=2 + LONG // page)
+    each = (b.n * (heads // kv_heads) // 128 + len(new)) * kv_heads
+    slots = (3 if dim == 64 else 2) * 256
+    assert not few(b, heads, kv_heads) and ranges == (slots // each if slots // each >= 4 else -(-slots // each))
+    q = (1.5 * torch.randn(b.n, heads, dim, generator=gen(5))).to(torch.bfloat16)
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu()).cpu()
+    rows = [(r, s, p) for r, s, p in b.rows() if p >= b.total[s] - 6 or p == b.total[s] - b.new[s]]
+    b.rows = lambda: rows
+    o, big = attend64(b, q)
+    at = [r for r, _, _ in rows]
+    check_attention(got[at], o[at], big[at], False)

@@ -92,3 +92,58 @@ def test_angles_next_to_a_quarter_turn(pkg, layout):
     y = pkg.ops.rotary(x.to(dev()), torch.ones(1, dtype=torch.int64, device=dev()), f.to(dev()), layout).cpu().double()
     for got, want in ((y[0, 0, first], f.cos()), (y[0, 0, second], f.sin())):
         assert bool(((got - want).abs() <= 2.0 ** -21 * want.abs() + 2.0 ** -48).all()), (got - want).abs().max()
+
+
+# ------------------------------------------------------------------ masked places and rows of nothing, both tiles
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,total,room", [([5, 3], [70, 3], 0), ([70, 60], [90, 400], LONG), ([130, 33], [900, 40], LONG)])
+def test_what_is_masked_does_not_reach_a_row(pkg, new, total, room, dim):
+    """NaN and infinities behind the sequences' ends and in pages that no table names; then in the last new token's
+    value (three channels) and key: that row alone has them."""
+    b = Batch(new, total, 16, 2, dim, seed=dim, extra=2 + room // 16)
+    assert few(b, 2, 2) == (room == 0)
+    q = torch.randn(b.n, 2, dim, generator=gen(2)).to(torch.bfloat16)
+    clean, big = attend64(b, q)
+    for s, t in enumerate(total):
+        id, off = b.place(s, t - 1)
+        b.k[id, :, off + 1:] = float("nan")
+        b.v[id, 0, :, off + 1:], b.v[id, 1, :, off + 1:] = float("inf"), float("nan")
+    unused = sorted(set(range(b.pages)) - set(b.table.flatten().tolist()))
+    b.k[unused], b.v[unused] = float("nan"), -float("inf")
+    check_attention(pkg.ops.paged_attention(q.to(dev()), *b.gpu()), clean, big, few(b, 2, 2))
+    last = new[0] - 1
+    id, off = b.place(0, total[0] - 1)
+    for h, d, x in ((0, 5, float("nan")), (0, dim - 1, float("inf")), (1, 33, -float("inf"))):
+        b.v[id, h, d, off] = x
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu()).cpu()
+    assert math.isnan(got[last, 0, 5]) and got[last, 0, dim - 1] == float("inf") and got[last, 1, 33] == -float("inf")
+    keep = torch.ones(got.shape, dtype=torch.bool)
+    keep[last, 0, 5] = keep[last, 0, dim - 1] = keep[last, 1, 33] = False
+    check_attention(torch.where(keep, got, clean.to(got.dtype)), clean, big, few(b, 2, 2))
+    b.v[id, 0, 5, off] = b.v[id, 0, dim - 1, off] = b.v[id, 1, 33, off] = 0.0
+    b.k[id, 0, off, 3] = float("nan")
+    got = pkg.ops.paged_attention(q.to(dev()), *b.gpu()).cpu()
+    assert bool(torch.isnan(got[last, 0]).all())
+    got[last], clean[last] = 0, 0
+    check_attention(got, clean, big, few(b, 2, 2))
+
+
+@pytest.mark.parametrize("scale", [0.125, 1.0, 4.0, -0.5])
+@pytest.mark.parametrize("new,total,room", [([2], [60], 0), ([40], [60], LONG), ([40], [1500], LONG), ([1], [2000], 0)])
+def test_rows_of_minus_infinity_in_both_tiles(pkg, new, total, room, scale):
+    """Scores of -inf for every attended token give zeros; one finite score among them, in whichever range, that
+    token's value; a NaN among them NaN."""
+    b = Batch(new, total, 16, 1, 64, seed=9, extra=2 + room // 16)
+    assert few(b, 1, 1) == (room == 0)
+    kp, vp, table, lens, cu = b.gpu()
+    q = torch.full((b.n, 1, 64), 1.0 if scale > 0 else -1.0, dtype=torch.bfloat16, device=dev())
+    kp.fill_(float("-inf"))
+    assert not pkg.ops.paged_attention(q, kp, vp, table, lens, cu, scale=scale).any()
+    for p in (5, total[0] - new[0]):  # the first row's own place among them
+        id, off = b.place(0, p)
+        kp[id, 0, off] = -3.0
+        got = pkg.ops.paged_attention(q, kp, vp, table, lens, cu, scale=scale)[:, 0]
+        assert torch.equal(got, vp[id, 0, :, off].expand(b.n, 64))
+        kp[id, 0, off] = float("nan")
+        assert bool(pkg.ops.paged_attention(q, kp, vp, table, lens, cu, scale=scale).isnan().all())
+        kp[id, 0, off] = float("-inf")
