@@ -33,6 +33,7 @@ typedef uint32_t a_u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ a_u4 a_mk(uint32_t x, uint32_t y, uint32_t z, uint32_t w) { return a_u4{x, y, z, w}; }
 
+typedef short attn_bf16x2 __attribute__((ext_vector_type(2)));
 #define ATTN_THREADS 256
 #define ATTN_LOW -0x1.fffffep127f  // running maximum before the first score: no finite one is less
 // Running maxima from which on the exponent s c - m is taken of the rounded product. One fma leaves what the
@@ -177,6 +178,10 @@ __device__ __forceinline__ a_u4 attn_ones(uint32_t seen) {
 // a quiet value).
 __device__ __forceinline__ float attn_max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+// l plus both halves of a pair of bf16 values: one v_dot2_f32_bf16
+__device__ __forceinline__ float attn_sum2(uint32_t pair, float l) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(attn_bf16x2, pair), __builtin_bit_cast(attn_bf16x2, 0x3f803f80u), l, false);
 }
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -409,6 +414,10 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 // tokens 16 b + 8 e .. + 7: its k of the second product. The 16-byte chunks of an LDS row are
 // permuted, so that the 16 lanes that read at a time, on 16 different rows, meet all 64 banks: in rows
 // of 256 bytes chunk c sits at place c ^ (row % 16), in rows of 128 at c ^ (row / 2 % 8).
+// P enters the second product as one bf16 value, and l sums the values as they are rounded, so that weights
+// still add up to 1: 2^-8 of a weight at most, 3e-4 of a result in the 2-norm (5e-4 with the sum of the values
+// before) beside the 1.7e-3 of its own rounding to bf16. Two parts, as above, would take 512 clocks more of the
+// matrix cores a step.
 // Two workgroups share a CU at D = 128, and a wave's step takes 4300 clocks, where its products take 1024 and
 // its vector instructions issue for 1200: 390 at the barrier, 1080 until the 8 copies are issued (30
 // bytes a clock and CU, with the other workgroup's), 910 in the first product, 460 for the maximum, 1160 in the
@@ -625,8 +634,8 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       auto weigh = [&](int kk, int j) {  // P of tokens 2 j and 2 j + 1 of 8
         const float u = s[kk >> 1][8 * (kk & 1) + 2 * j], v = s[kk >> 1][8 * (kk & 1) + 2 * j + 1];
         const float p0 = attn_exp2(__fmaf_rn(u, cw, -mw)), p1 = attn_exp2(__fmaf_rn(v, cw, -mw));
-        l += p0 + p1;
         pf[kk & 1][j] = f32_to_bf16x2(p0, p1);
+        l = attn_sum2(pf[kk & 1][j], l);
       };
 #pragma unroll
       for (int j = 0; j < 4; ++j) weigh(0, j);
