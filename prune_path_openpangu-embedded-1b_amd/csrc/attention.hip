@@ -855,10 +855,10 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   // (the join's are never more: eight rows each and more where there are few ranges, which is two workgroups to a
   // tile of 16 rows; calls of more than 8 ranges, and cut tiles of 128 rows, are no more than the GPU holds some
   // times over)
-  // The limit counts a range per 1024 tokens of the table (64 at most), though a launch of that size has fewer:
-  // so it goes by the shapes alone, not by the GPU's size.
-  const int64_t widest = p.rows == 16 ? std::min<int64_t>(ATTN_MAX_SPLITS, (int64_t)max_pages * page_size / 1024) : 1;
-  const int64_t counted = std::max(items, p.tiles * Hkv * widest);
+  // The limit goes by the shapes alone, not by the GPU's size or the tile: up to 16 rows a sequence it counts tiles
+  // of 16 rows with a range per 1024 tokens of the table (64 at most), which a launch never has.
+  const int64_t per_head = n_tokens * a.group, ranges = std::min<int64_t>(ATTN_MAX_SPLITS, (int64_t)max_pages * page_size / 1024);
+  const int64_t counted = std::max(items, per_head <= 16 * (int64_t)n_seqs ? (per_head / 16 + n_seqs + 1) * Hkv * ranges : 0);
   PP_REQUIRE(counted <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld workgroups (at most 2^24 - 1)", what, (long long)counted);
   const int64_t joins = alone ? (rows * (D / 4) + ATTN_THREADS - 1) / ATTN_THREADS : rows;
   hipStream_t st = (hipStream_t)stream;
