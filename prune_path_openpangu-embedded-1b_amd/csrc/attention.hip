@@ -48,7 +48,7 @@ struct AttnArgs {
   const bf16_t *k, *v;
   int Hq, Hkv, group;
   float c;        // |scale| * log2(e), not 0 (masked scores are -inf): scores in powers of two
-  uint32_t keep, flip;  // bits of a pair of q: all, or none where scale is 0; the sign of scale
+  uint32_t flip;  // the sign of scale, on both halves of a pair of q
   bf16_t* out;
   int zero_tail;
   int splits;         // most ranges of a tile
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   load_k(t);
   load_v(t);
 #pragma unroll
-  for (int s = 0; s < KS; ++s) qf[s] = in ? (qf[s] & a.keep) ^ a.flip : a_mk(0, 0, 0, 0);
+  for (int s = 0; s < KS; ++s) qf[s] = in ? qf[s] ^ a.flip : a_mk(0, 0, 0, 0);
   const int low = attn_limit(a, w, 0);  // every row attends the tokens up to here
 
   f32x4_t o[MB];
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   entry(t + ATTN_KT);
   load(t, 0);
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) qf[s] = in ? (qf[s] & a.keep) ^ a.flip : a_mk(0, 0, 0, 0);
+  for (int s = 0; s < D / 16; ++s) qf[s] = in ? qf[s] ^ a.flip : a_mk(0, 0, 0, 0);
   f32x16_t o[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b)
@@ -855,7 +855,7 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.q = (const bf16_t*)q, a.qs[0] = q_strides[0], a.qs[1] = q_strides[1];
   a.k = (const bf16_t*)k_pages, a.v = (const bf16_t*)v_pages;
   a.Hq = Hq, a.Hkv = Hkv, a.group = Hq / Hkv;
-  a.c = c != 0.0f ? c : 1.0f, a.keep = c != 0.0f ? ~0u : 0u, a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.c = std::max(c, 0x1p-149f), a.flip = scale < 0.0f ? 0x80008000u : 0u;  // (for 0: 2^-21 of any float32)
   a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
   a.splits = p.splits, a.base = p.base, a.behind = p.behind, a.tiles = (int)p.tiles;
   a.po = (float*)workspace;
