@@ -181,6 +181,11 @@ __device__ __forceinline__ a_u4 attn_ones(uint32_t seen) {
 }
 
 
+// The bf16 value below p (0 for 0), as a float's bits.
+__device__ __forceinline__ uint32_t attn_upper(float p) {
+  return __builtin_elementwise_sub_sat(__float_as_uint(p), 1u) & 0xffff0000u;
+}
+
 // max(a, b, c), NaN if one is: one v_maximum3_f32 (fmaxf, which passes NaN over, first makes each operand
 // a quiet value).
 __device__ __forceinline__ float attn_max3(float a, float b, float c) {
@@ -211,8 +216,8 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // K operand row m of block b (16 tokens) is token 8 (m / 4) + 4 b + m % 4 of the step, which leaves
 // lane group g = lane / 16 with the scores of tokens 8 g .. 8 g + 7: its k of the second product.
 // P enters as a sum of two bf16 values, its upper bits and what is left, rounded (2^-15 of P at most): the
-// second product costs nothing next to the loads. The second part is at least 2^-17 of P, so that an infinity
-// of V in an attended place gives that infinity: 0, and what is left of an upper part rounded up, would make it
+// second product costs nothing next to the loads. The upper part is below P, so that an infinity of V in an
+// attended place gives that infinity: nothing left, or what is left of an upper part rounded up, would make it
 // NaN.
 // Measured, 12 heads of 128: one token on each of 64 sequences of 8192 555 us (3.2 GB, 5.8 TB/s, where a
 // large copy reaches 5.05), of 1 to 8192 tokens 271 us (5.6 TB/s); one sequence of 1152 tokens 6.5 us
@@ -352,10 +357,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t u = __float_as_uint(p[2 * j]), v = __float_as_uint(p[2 * j + 1]) & 0xffff0000u;
+      const uint32_t u = attn_upper(p[2 * j]), v = attn_upper(p[2 * j + 1]);
       hi[j] = (u >> 16) | v;
-      lo[j] = f32_to_bf16x2(fmaxf(p[2 * j] - __uint_as_float(u & 0xffff0000u), 0x1p-17f * p[2 * j]),
-                            fmaxf(p[2 * j + 1] - __uint_as_float(v), 0x1p-17f * p[2 * j + 1]));
+      lo[j] = f32_to_bf16x2(p[2 * j] - __uint_as_float(u), p[2 * j + 1] - __uint_as_float(v));
     }
     const a_u4 ph = a_mk(hi[0], hi[1], hi[2], hi[3]), pl = a_mk(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
