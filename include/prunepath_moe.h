@@ -376,7 +376,8 @@ int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const i
  * positions 0 .. p, query head h the key head h / (Hq / Hkv). q [n_tokens][Hq][D] bfloat16 (strides
  * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous (q itself, if q is). Scores, softmax and sums
  * in float32. A row that attends nothing, or whose scores are all -inf, gives zeros; what a masked
- * place holds, NaN and infinities too, does not reach a row. Rows behind cu_q[n_seqs] are zeroed
+ * place holds, NaN and infinities too, does not reach a row, and an infinity in a value that a row
+ * attends gives that infinity (NaN beside its opposite, or where its token's weight underflows). Rows behind cu_q[n_seqs] are zeroed
  * if zero_tail, else left as they are. workspace: pp_paged_attention_workspace_bytes of the same
  * sizes (0: none, also for sizes that the call refuses), no initialisation, 16-byte aligned; calls
  * that may overlap need one each. The same bits on every call. */

@@ -22,7 +22,9 @@
 // Masked places: their scores are replaced, not added to, and a step that has any multiplies the
 // finite part of V only; what is not finite in V goes to the rows that attend it by a second product
 // (attn_poison). So stale or foreign data in a page, and a later token's NaN, do not reach a row. A
-// row that attends nothing gives zeros, and so does one whose scores are all -inf.
+// row that attends nothing gives zeros, and so does one whose scores are all -inf. An infinity of V
+// gives the rows that attend it that infinity; NaN beside its opposite, or where the weight of its
+// token underflows in a step without a masked place or in the join of the ranges.
 #include <algorithm>
 #include <cmath>
 
@@ -219,9 +221,9 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // second product costs nothing next to the loads. The upper part is below P, so that an infinity of V in an
 // attended place gives that infinity: nothing left, or what is left of an upper part rounded up, would make it
 // NaN.
-// Measured, 12 heads of 128: one token on each of 64 sequences of 8192 555 us (3.2 GB, 5.8 TB/s, where a
-// large copy reaches 5.05), of 1 to 8192 tokens 271 us (5.6 TB/s); one sequence of 1152 tokens 6.5 us
-// with the join's 3.1, chains of offsets, table, K and join rather than bytes.
+// Measured, 12 heads of 128: one token on each of 64 sequences of 8192 557 us (3.2 GB, 5.8 TB/s, where a
+// large copy reaches 4.9), of 1 to 8192 tokens 270 us (5.6 TB/s); one sequence of 1152 tokens 8.9 us with
+// the join's 3.5, chains of offsets, table, K and join rather than bytes.
 template <int D>
 __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   constexpr int R = 16, KS = D / 32, MB = D / 16, OS = D + 4;
@@ -438,8 +440,8 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
 // behind the first product (242; 512 tokens at 30000 129 instead of 137), sums beside the last products,
 // 256 rows on eight waves with the second product of one half beside the first of the other (236) or on
 // four, one a SIMD (319), no priorities (232).
-// Measured: 12 heads of 128, a prompt of 8192 tokens 230 us (890 TFLOP/s; 223 in pages of 64), of 4096 87 us
-// (590), of 2048 37 us with the join; 512 new tokens at 30000 132 us (720).
+// Measured: 12 heads of 128, a prompt of 8192 tokens 238 us (870 TFLOP/s; as much in pages of 64), of 4096 85 us
+// (605), of 2048 37 us, 7 of them the join's; 512 new tokens at 30000 131 us (730).
 #define ATTN_ROWS 128
 
 // 16 bytes per lane from memory into LDS at lds + 16 lane, by the copy path that does not pass through

@@ -348,8 +348,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
     * "ntk": base grows by factor^(dim / (dim - 2)), so that the slowest pair turns factor times
       slower and the fastest as before;
     * "yarn": pairs that make fewer than ``turns[0]`` turns over the original length are divided by
-      factor, those with more than ``turns[1]`` stay, a linear ramp between; mscale is
-      0.1 ln(factor) + 1."""
+      factor, those with more than ``turns[1]`` stay, between them a ramp that is linear in the number
+      of turns (not in the pair's index, as some checkpoints have it: for those compute inv_freq and pass
+      it); mscale is 0.1 ln(factor) + 1."""
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary_frequencies: dim must be an even number from 2 on (got {dim})")
     if not (base > 0 and factor > 0):
@@ -409,7 +410,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     q [N, heads, D]: turned as k is, returned as bf16 [N, heads, D] (in ``q_out``, which may be q
     itself, if given; other overlaps of what is written are refused). Rows behind cu_q[seqs] append
     nothing; in a new result they are zeros, in q_out they stay. Inference only: arguments that require
-    a gradient are refused outside torch.no_grad()."""
+    a gradient are refused outside torch.no_grad(), tangents always."""
     ops = L.torch_ops()
     if q is None:
         if q_out is not None:
@@ -430,10 +431,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     the key head h // (heads / kv_heads). q bf16 [N, heads, D] -> bf16 [N, heads, D]
     (``torch.ops.prunepath.paged_attention``, or ``paged_attention_into`` writing ``out``); scale
     defaults to D^-0.5. Scores and softmax in fp32. A row that attends nothing, or whose scores are all
-    -inf, is zero. Rows behind cu_q[seqs] are zero in a new result and stay in ``out`` (which may be q
-    itself; other overlaps are refused). Single tokens, chunks and whole prompts, in one call; lengths
-    are read on the device, so a captured call serves lengths that grow. Inference only: arguments that
-    require a gradient are refused outside torch.no_grad()."""
+    -inf, is zero; an infinity in a value that a row attends gives that infinity. Rows behind cu_q[seqs]
+    are zero in a new result and stay in ``out`` (which may be q itself; other overlaps are refused). Single
+    tokens, chunks and whole prompts, in one call; lengths are read on the device, so a captured call serves
+    lengths that grow, in a table of any width. Inference only: arguments that require a gradient are
+    refused outside torch.no_grad(), tangents always."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     ops = L.torch_ops()
