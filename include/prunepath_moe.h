@@ -349,6 +349,30 @@ int pp_rotary(const void* x, int dtype, const int64_t* x_strides, const void* po
               const double* inv_freq, int rotary_dim, int layout, float mscale, int inverse, void* y,
               const int64_t* y_strides, void* stream);
 
+/* Norms of queries and keys for each head, with the rotation in the same pass: y = R (w x r), r = 1 / sqrt(mean(x^2) + eps)
+ * over the D channels of a head, R the rotation above, w [D] one weight a channel for all query heads and one for all key
+ * heads (of float32, or like x: w_dtype). q [batch][length][Hq][D], k [batch][length][Hk][D] (dtype, strides as above, any
+ * alignment) -> q_out, k_out of the same dtype, contiguous. Hq or Hk may be 0 (its pointers are not read then). 2 <= D <= 256.
+ * Sums and everything between load and store in float32; heads whose squares leave its range included.
+ *
+ * pp_qk_norm_rotary_bwd: with dq and dk of q_out's and k_out's shapes (any strides), the gradients q_grad and k_grad
+ * (contiguous, dtype) and, unless NULL, q_weight_grad and k_weight_grad [D] (w_dtype; zeros where there is nothing to sum).
+ * workspace (where a weight's gradient is asked for): pp_qk_norm_rotary_workspace_bytes, no initialisation, 16-byte
+ * aligned; calls that may overlap need one each. The same bits on every call. */
+int pp_qk_norm_rotary(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                      const void* q_weight, const void* k_weight, int w_dtype, const void* positions, int pos64,
+                      const int64_t* pos_strides, int64_t batch, int64_t length, int Hq, int Hk, int D,
+                      const double* inv_freq, int rotary_dim, int layout, float mscale, float eps, void* q_out,
+                      void* k_out, void* stream);
+size_t pp_qk_norm_rotary_workspace_bytes(int dtype, int64_t batch, int64_t length, int Hq, int Hk, int D, int rotary_dim);
+int pp_qk_norm_rotary_bwd(const void* dq, const int64_t* dq_strides, const void* dk, const int64_t* dk_strides,
+                          const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                          const void* q_weight, const void* k_weight, int w_dtype, const void* positions, int pos64,
+                          const int64_t* pos_strides, int64_t batch, int64_t length, int Hq, int Hk, int D,
+                          const double* inv_freq, int rotary_dim, int layout, float mscale, float eps, void* q_grad,
+                          void* k_grad, void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
 /* A ragged batch over a paged cache, as pp_kv_append and pp_paged_attention take it. n_tokens
  * packed rows; sequence s has the new tokens cu_q[s] .. cu_q[s + 1] (n_seqs + 1 nondecreasing
  * offsets, the first taken as 0, clamped to n_tokens) and kv_lens[s] tokens in the cache once they
@@ -372,6 +396,34 @@ int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const i
                  int page_size, int Hq, int Hkv, int D, const double* inv_freq, int rotary_dim, int layout,
                  float mscale, void* k_pages, void* v_pages, void* q_out, int zero_tail, void* stream);
 
+/* pp_kv_append with the norms of queries and keys on the way, into a cache of 16 or of 8 bits.
+ *
+ * q_weight, k_weight [D] (w_dtype: float32, or dtype; both NULL: no norms; q_weight NULL without q): every head is
+ * normed as above before it is turned.
+ *
+ * k_scales, v_scales (both NULL: the bfloat16 cache): a cache of 8 bits. k_pages [num_pages][Hkv][page_size][D] and
+ * v_pages [num_pages][Hkv][page_size / 16][D][16] hold e4m3 values, k_scales and v_scales
+ * [num_pages][Hkv][page_size / 16] a power of two for each block of 16 places as its biased exponent (2^(byte - 127),
+ * bytes 10 to 246). A block's scale is the least whose 448-fold holds the call's values in it; where the sequence has tokens
+ * in the block in front of the call's (appended before), at least the scale that they have, and they are brought to
+ * the new one. Each value is rounded once, from float32, to nearest even; what is not finite is held as NaN and
+ * does not count in the scale. No two sequences may share a block that the call writes. */
+int pp_kv_append_with(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                      const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs, const int32_t* cu_q,
+                      const int32_t* kv_lens, const int32_t* block_table, int max_pages, int num_pages,
+                      int page_size, int Hq, int Hkv, int D, const double* inv_freq, int rotary_dim, int layout,
+                      float mscale, const void* q_weight, const void* k_weight, int w_dtype, float eps, void* k_pages,
+                      void* v_pages, void* k_scales, void* v_scales, void* q_out, int zero_tail, void* stream);
+
+/* The cache (of 16 bits, or of 8 with its scales) read back: row i of sequence s, of cu_q as above with n_rows rows, is
+ * position kv_lens[s] - (its rows) + i, so that the offsets of an append read what it wrote, and those of the whole
+ * lengths everything. k_out and v_out [n_rows][Hkv][D] bfloat16 (a value of 8 bits times its scale is one, exactly),
+ * contiguous, 16-byte aligned. Rows whose place no page holds are zeros; rows behind cu_q[n_seqs] are zeroed if
+ * zero_tail, else left as they are. */
+int pp_kv_read(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, int64_t n_rows,
+               int n_seqs, const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
+               int num_pages, int page_size, int Hkv, int D, void* k_out, void* v_out, int zero_tail, void* stream);
+
 /* Attention of the new tokens over the cache that holds them: the token at position p attends the
  * positions 0 .. p, query head h the key head h / (Hq / Hkv). q [n_tokens][Hq][D] bfloat16 (strides
  * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous (q itself, if q is). Scores, softmax and sums
@@ -388,6 +440,19 @@ int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens
                        const void* k_pages, const void* v_pages, int num_pages, int page_size, int Hq, int Hkv,
                        int D, float scale, void* out_bf16, int zero_tail, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* pp_paged_attention over a cache of 16 or of 8 bits (k_scales, v_scales as above, both NULL: bfloat16), of a window and the
+ * first tokens: with window > 0 the token at position p attends the positions t <= p with t > p - window or t < sinks
+ * (window 0: all up to p, sinks without meaning). Pages that no row attends are not read. Over 8 bits: as over the
+ * bfloat16 numbers that the cache stands for, NaN as there. workspace:
+ * pp_paged_attention_with_workspace_bytes of the same sizes. */
+size_t pp_paged_attention_with_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv,
+                                               int D, int eight_bits, int64_t window, int64_t sinks);
+int pp_paged_attention_with(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs, const int32_t* cu_q,
+                            const int32_t* kv_lens, const int32_t* block_table, int max_pages, const void* k_pages,
+                            const void* v_pages, const void* k_scales, const void* v_scales, int num_pages,
+                            int page_size, int Hq, int Hkv, int D, float scale, int64_t window, int64_t sinks,
+                            void* out_bf16, int zero_tail, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

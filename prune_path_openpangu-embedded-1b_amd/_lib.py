@@ -84,6 +84,25 @@ SIGNATURES = {
     "pp_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                    c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p,
                                    c_size_t, c_void_p]),
+    "pp_qk_norm_rotary": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                  c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_int, c_int,
+                                  c_float, c_float, c_void_p, c_void_p, c_void_p]),
+    "pp_qk_norm_rotary_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int]),
+    "pp_qk_norm_rotary_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64,
+                                      c_int, c_int, c_int, c_void_p, c_int, c_int, c_float, c_float, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "pp_kv_append_with": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int,
+                                  c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                                  c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "pp_kv_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                           c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "pp_paged_attention_with_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                           c_int64, c_int64]),
+    "pp_paged_attention_with": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                        c_float, c_int64, c_int64, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
 }
 
 

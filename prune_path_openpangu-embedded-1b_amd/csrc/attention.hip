@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "fp8.h"
 #include "paged.h"
 
 // 16 bytes in registers (a plain vector type: arrays of the struct type were kept in LDS)
@@ -58,6 +59,8 @@ struct AttnArgs {
   float *po, *pml;    // workspace: [row][split][D], [row][split][2]
   int* pns;           // workspace: splits of a row
   int tiles;          // tiles of rows, of every sequence together
+  const uint8_t *ks, *vs;  // scales of an 8-bit cache: [page][head][16 tokens]
+  int window, sinks;  // tokens that a row attends, itself among them, and first tokens that every row does (window 0: all)
 };
 
 // What a workgroup works on.
@@ -69,6 +72,11 @@ struct AttnTile {
   int nt;        // tokens that the tile's last row attends
   int lo, hi;    // tokens of this range
   int ns;        // ranges of the tile (0: nothing is attended)
+  // With a window, nt, lo and hi leave out the gap between the first tokens that stay visible and the first that a window
+  // reaches: token t of them is token t of the sequence below `keep`, t + gap from there on.
+  int keep, gap;
+  template <bool WIN>
+  __device__ __forceinline__ int at(int t) const { return !WIN || t < keep ? t : t + gap; }
 };
 
 // Most ranges of a tile in this call: `behind` in a chunk of one sequence far behind the cache's start. (Asked
@@ -90,7 +98,8 @@ __device__ __forceinline__ int attn_cut(const AttnArgs& a, int nt, int ranges) {
   return max(1, min(cut, a.splits));
 }
 
-template <int R>
+// STEP: tokens of a step, which lie on one side of the gap.
+template <int R, bool WIN, int STEP>
 __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int split, int ranges) {
   AttnTile w;
   const int g = a.group;
@@ -104,6 +113,14 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int 
   const bool tail = w.s == a.seqs.n_seqs;
   w.p0 = tail ? -(int64_t)len : (int64_t)f.len - len;
   w.nt = (int)max((int64_t)0, min(w.p0 + (w.r0 + max(w.nr, 1) - 1) / g + 1, (int64_t)a.seqs.capacity()));
+  w.keep = w.gap = 0;
+  if constexpr (WIN) {
+    // the first token that the first row's window reaches
+    const int start = (int)max((int64_t)0, min(w.p0 + w.r0 / g - a.window + 1, (int64_t)w.nt));
+    w.keep = (min(a.sinks, start) + STEP - 1) / STEP * STEP;
+    w.gap = max(0, (start & ~15) - w.keep);
+    w.nt -= w.gap;
+  }
   // equal ranges of whole steps, none of them empty
   const int cut = attn_cut<R>(a, w.nt, ranges);
   const int per = ((w.nt + cut - 1) / cut + 127) / 128 * 128;
@@ -112,6 +129,8 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int 
   w.hi = min(w.nt, w.lo + per);
   // the same in every lane: said so, or what is computed from them takes vector registers
   for (int* v : {&w.r0, &w.nr, &w.nt, &w.lo, &w.hi, &w.ns}) *v = __builtin_amdgcn_readfirstlane(*v);
+  if constexpr (WIN)
+    for (int* v : {&w.keep, &w.gap}) *v = __builtin_amdgcn_readfirstlane(*v);
   return w;
 }
 
@@ -129,6 +148,11 @@ __device__ __forceinline__ const bf16_t* attn_query(const AttnArgs& a, const Att
 // Last position that row r attends.
 __device__ __forceinline__ int attn_limit(const AttnArgs& a, const AttnTile& w, int r) {
   return (int)min(w.p0 + (w.r0 + r) / a.group, (int64_t)a.seqs.capacity() - 1);
+}
+
+// First position of row r's window (of its place, wherever the table ends).
+__device__ __forceinline__ int attn_from(const AttnArgs& a, const AttnTile& w, int r) {
+  return (int)max(w.p0 + (w.r0 + r) / a.group - a.window + 1, (int64_t)0);
 }
 
 // Rows that attend nothing: zeros (rows of no sequence: only if the call owns the output).
@@ -183,6 +207,12 @@ __device__ __forceinline__ a_u4 attn_ones(uint32_t seen) {
 }
 
 
+// 16 values of 8 bits times their scale, as two operands.
+__device__ __forceinline__ void attn_wide(const a_u4 v, float scale, a_u4& lo, a_u4& hi) {
+  lo = a_mk(fp8_bf16<false>(v[0], scale), fp8_bf16<true>(v[0], scale), fp8_bf16<false>(v[1], scale), fp8_bf16<true>(v[1], scale));
+  hi = a_mk(fp8_bf16<false>(v[2], scale), fp8_bf16<true>(v[2], scale), fp8_bf16<false>(v[3], scale), fp8_bf16<true>(v[3], scale));
+}
+
 // The bf16 value below p (0 for 0), as a float's bits.
 __device__ __forceinline__ uint32_t attn_upper(float p) {
   return __builtin_elementwise_sub_sat(__float_as_uint(p), 1u) & 0xffff0000u;
@@ -224,9 +254,11 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // Measured, 12 heads of 128: one token on each of 64 sequences of 8192 557 us (3.2 GB, 5.8 TB/s, where a
 // large copy reaches 4.9), of 1 to 8192 tokens 270 us (5.6 TB/s); one sequence of 1152 tokens 8.9 us with
 // the join's 3.5, chains of offsets, table, K and join rather than bytes.
-template <int D>
-__global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
+template <int D, bool EIGHT, bool WIN>
+__global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(AttnArgs a) {
   constexpr int R = 16, KS = D / 32, MB = D / 16, OS = D + 4;
+  constexpr int TOK = EIGHT ? 16 : 8, ST = 4 * TOK, KB = TOK / 4;  // tokens of a lane, of a step, blocks of a step's K
+  constexpr int KL = EIGHT ? D / 64 : KS;                          // 16-byte pieces of a K row to a lane
   __shared__ float o_s[4][R][OS];
   __shared__ float ml_s[4][R][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
@@ -240,7 +272,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   const int items = (a.tiles - 1) * a.Hkv, most = items * a.splits, b = blockIdx.x;
   const int split = b < most ? b / items : (b - most) / a.Hkv, turn = split * (items - 4) & 7;
   const int item = b < most ? (b - split * items + turn) % items : items + (b - most) % a.Hkv, h = item % a.Hkv;
-  const AttnTile w = attn_tile<R>(a, item / a.Hkv, split, a.base);
+  const AttnTile w = attn_tile<R, WIN, ST>(a, item / a.Hkv, split, a.base);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
     if (split == 0) attn_zero(a, w, h, D);
@@ -249,18 +281,20 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   if (split >= w.ns) return;
 
   const int ps = 1 << a.seqs.lp;
-  const int gk = 8 * (col >> 2), gv = 8 * g;  // the lane's tokens of K and of V, within a step
+  const int gk = TOK * (col >> 2), gv = TOK * g;  // the lane's tokens of K and of V, within a step
   int ek, ev;                                 // their table entries
   int pk, pv;                                 // their pages, -1: none
   int pc;                                     // the present V's
-  a_u4 kf[2][KS], vf[MB];
+  a_u4 kf[KB][KL], vf[MB];
+  uint32_t sk = 0, sv = 0;                    // 8 bits: the scales of what kf and vf hold
   // Loads are asked for without a branch, of the last row or entry where there is none: with one, the
   // wait for each stands where the two sides meet.
   const int32_t* const table = a.seqs.table + (int64_t)w.s * a.seqs.max_pages;
-  const int last_entry = (w.hi - 1) >> a.seqs.lp;
+  const int last_entry = w.at<WIN>(w.hi - 1) >> a.seqs.lp;
   auto entries = [&](int t) {
-    ek = table[min((t + gk) >> a.seqs.lp, last_entry)];
-    ev = table[min((t + gv) >> a.seqs.lp, last_entry)];
+    const int at = w.at<WIN>(t);
+    ek = table[min((at + gk) >> a.seqs.lp, last_entry)];
+    ev = table[min((at + gv) >> a.seqs.lp, last_entry)];
   };
   auto pages = [&](int t) {
     pk = t + gk < w.hi ? a.seqs.page(ek) : -1;
@@ -268,120 +302,185 @@ __global__ __launch_bounds__(ATTN_THREADS, 3) void attn_few_kernel(AttnArgs a) {
   };
   // places without a page read page 0, and are masked
   auto load_k = [&](int t) {
-    const bf16_t* kp = a.k + ((((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((t + gk) & (ps - 1)) + (col & 3)) * D + 8 * g;
+    const int64_t row = (((int64_t)max(pk, 0) * a.Hkv + h) << a.seqs.lp) + ((w.at<WIN>(t) + gk) & (ps - 1));
+    if constexpr (EIGHT) {
+      const uint8_t* kp = (const uint8_t*)a.k + (row + (col & 3)) * D + 16 * g;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kf[b][s] = *(const a_u4*)(kp + 4 * b * D + 32 * s);
+        for (int s = 0; s < KL; ++s) kf[b][s] = *(const a_u4*)(kp + 4 * b * D + 64 * s);
+      sk = a.ks[row >> 4];
+    } else {
+      const bf16_t* kp = a.k + (row + (col & 3)) * D + 8 * g;
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int s = 0; s < KL; ++s) kf[b][s] = *(const a_u4*)(kp + 4 * b * D + 32 * s);
+    }
   };
   auto at_v = [&](int page, int t) {
-    return a.v + ((((int64_t)max(page, 0) * a.Hkv + h) * D + col) << a.seqs.lp) + ((t + gv) & (ps - 1));
+    return a.v + ((((int64_t)max(page, 0) * a.Hkv + h) * D + col) << a.seqs.lp) + ((w.at<WIN>(t) + gv) & (ps - 1));
   };
   auto load_v = [&](int t) {
     pc = pv;
-    const bf16_t* vp = at_v(pv, t);
+    if constexpr (EIGHT) {
+      const int64_t block = ((((int64_t)max(pv, 0) * a.Hkv + h) << a.seqs.lp) + ((w.at<WIN>(t) + gv) & (ps - 1))) >> 4;
+      const a_u4* vp = (const a_u4*)((const uint8_t*)a.v + block * (16 * D)) + col;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) vf[b] = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+      for (int b = 0; b < MB; ++b) vf[b] = vp[16 * b];
+      sv = a.vs[block];
+    } else {
+      const bf16_t* vp = at_v(pv, t);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) vf[b] = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+    }
   };
-  int t = w.lo + 32 * wave;
+  int t = w.lo + ST * wave;
   entries(t);
   a_u4 qf[KS];
   const bool in = col < w.nr;
   const int limit = in ? attn_limit(a, w, col) : a.seqs.capacity();
-  const bf16_t* const src = attn_query(a, w, h, min(col, w.nr - 1)) + 8 * g;
+  // (8 bits: a lane's 16 channels of K are two operands, so the queries' go the same way)
+  const bf16_t* const src = attn_query(a, w, h, min(col, w.nr - 1)) + TOK * g;
 #pragma unroll
-  for (int s = 0; s < KS; ++s) qf[s] = *(const a_u4*)(src + 32 * s);
+  for (int s = 0; s < KS; ++s) qf[s] = *(const a_u4*)(src + (EIGHT ? 64 * (s >> 1) + 8 * (s & 1) : 32 * s));
   paged_asked();
   pages(t);
-  entries(t + 128);
+  entries(t + 4 * ST);
   load_k(t);
   load_v(t);
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = in ? qf[s] ^ a.flip : a_mk(0, 0, 0, 0);
   const int low = attn_limit(a, w, 0);  // every row attends the tokens up to here
+  // windows: the row's first token, and the first that every row's holds
+  const int from = WIN ? attn_from(a, w, min(col, w.nr - 1)) : 0, high = WIN ? attn_from(a, w, w.nr - 1) : 0;
 
   f32x4_t o[MB];
   float m = ATTN_LOW, l = 0.0f;
 #pragma unroll
   for (int b = 0; b < MB; ++b) o[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (; t < w.hi; t += 128) {
-    pages(t + 128);
-    entries(t + 256);
-    f32x4_t s[2];
+  for (; t < w.hi; t += 4 * ST) {
+    const int rt = w.at<WIN>(t);  // the step's first position
+    pages(t + 4 * ST);
+    entries(t + 8 * ST);
+    f32x4_t s[KB];
+    const float fk = fp8_factor(sk), fv = fp8_factor(sv);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < KB; ++b) {
       s[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int q = 0; q < KS; ++q) s[b] = mfma16(kf[b][q], qf[q], s[b]);
+      for (int q = 0; q < KL; ++q) {
+        if constexpr (EIGHT) {
+          a_u4 k0, k1;
+          attn_wide(kf[b][q], fk, k0, k1);
+          s[b] = mfma16(k0, qf[2 * q], s[b]);
+          s[b] = mfma16(k1, qf[2 * q + 1], s[b]);
+        } else {
+          s[b] = mfma16(kf[b][q], qf[q], s[b]);
+        }
+      }
     }
-    const bool more = t + 128 < w.hi;
-    if (more) load_k(t + 128);
+    const bool more = t + 4 * ST < w.hi;
+    if (more) load_k(t + 4 * ST);
     // whether a place of the step is masked for any row (wave-uniform)
-    const bool part = t + 31 > low || t + 32 > w.hi || __ballot(pc < 0) != 0;
+    const bool part = rt + ST - 1 > low || t + ST > w.hi || (WIN && rt < high) || __ballot(pc < 0) != 0;
     bool bad = false;
     if (part) {
       uint32_t any = 0;
 #pragma unroll
-      for (int b = 0; b < MB; ++b) any |= attn_bad(vf[b]);
-      bad = __ballot((any & 0x80008000u) != 0) != 0;
-      if (bad) {
+      for (int b = 0; b < MB; ++b) {
+        if constexpr (EIGHT) any |= fp8_bad(vf[b][0]) | fp8_bad(vf[b][1]) | fp8_bad(vf[b][2]) | fp8_bad(vf[b][3]);
+        else any |= attn_bad(vf[b]);
+      }
+      bad = __ballot((any & (EIGHT ? 0x80808080u : 0x80008000u)) != 0 || (EIGHT && sv > FP8_HIGH)) != 0;
+      if (!EIGHT && bad) {
 #pragma unroll
         for (int b = 0; b < MB; ++b) vf[b] = attn_clean(vf[b]);
       }
     }
-    float p[8];
+    float p[TOK];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3];
-    uint32_t seen = 0xffu;
+    for (int j = 0; j < TOK; ++j) p[j] = s[j >> 2][j & 3];
+    uint32_t seen = (1u << TOK) - 1;
     if (part) {
       asm volatile("");  // a branch: few steps have one
       seen = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = pc >= 0 && t + gv + j <= limit && t + gv + j < w.hi;
+      for (int j = 0; j < TOK; ++j) {
+        const int at = rt + gv + j;
+        const bool in = pc >= 0 && at <= limit && t + gv + j < w.hi && (!WIN || at >= from || at < a.sinks);
         seen |= in ? 1u << j : 0u;
         p[j] = in ? p[j] : -__builtin_inff();
       }
     }
     float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+    if constexpr (EIGHT)
+      top = fmaxf(top, fmaxf(fmaxf(fmaxf(p[8], p[9]), fmaxf(p[10], p[11])), fmaxf(fmaxf(p[12], p[13]), fmaxf(p[14], p[15]))));
     top = fmaxf(top, pl_xor16f(top, lane));
     top = fmaxf(top, pl_xor32f(top, lane));
     const float mn = fmaxf(m, top * a.c), shrink = attn_exp2(m - mn);
     m = mn;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < TOK; ++j) {
       p[j] = attn_exp2(__fmul_rn(p[j], a.c) - mn);  // (in two steps, see ATTN_FAR: the loads hide the second)
       sum += p[j];
     }
     l = __fmaf_rn(l, shrink, sum);
-    uint32_t hi[4], lo[4];
+    uint32_t hi[TOK / 2], lo[TOK / 2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < TOK / 2; ++j) {
       const uint32_t u = attn_upper(p[2 * j]), v = attn_upper(p[2 * j + 1]);
       hi[j] = (u >> 16) | v;
       lo[j] = f32_to_bf16x2(p[2 * j] - __uint_as_float(u), p[2 * j + 1] - __uint_as_float(v));
     }
     const a_u4 ph = a_mk(hi[0], hi[1], hi[2], hi[3]), pl = a_mk(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      o[b] *= shrink;
-      o[b] = mfma16(vf[b], ph, o[b]);
-      o[b] = mfma16(vf[b], pl, o[b]);
-    }
-    if (bad) {  // what was taken out of V, read again, for the rows that attend it
-      const a_u4 one = attn_ones(seen);
-      const bf16_t* vp = at_v(pc, t);
+    if constexpr (EIGHT) {
+      const a_u4 ph2 = a_mk(hi[4], hi[5], hi[6], hi[7]), pl2 = a_mk(lo[4], lo[5], lo[6], lo[7]);
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
-        const a_u4 x = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
-        const f32x4_t code = mfma16(attn_code(x), one, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+        a_u4 v0, v1, all0, all1;
+        attn_wide(vf[b], fv, v0, v1);
+        if (bad) {  // only the finite part of V, and what is not finite for the rows that attend it
+          asm volatile("");
+          all0 = v0, all1 = v1;
+          v0 = attn_clean(v0), v1 = attn_clean(v1);
+        }
+        o[b] *= shrink;
+        o[b] = mfma16(v0, ph, o[b]);
+        o[b] = mfma16(v1, ph2, o[b]);
+        o[b] = mfma16(v0, pl, o[b]);
+        o[b] = mfma16(v1, pl2, o[b]);
+        if (bad) {
+          asm volatile("");
+          f32x4_t code = mfma16(attn_code(all0), attn_ones(seen), f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+          code = mfma16(attn_code(all1), attn_ones(seen >> 8), code);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[b][i] = attn_poison(o[b][i], code[i]);
+          for (int i = 0; i < 4; ++i) o[b][i] = attn_poison(o[b][i], code[i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        o[b] *= shrink;
+        o[b] = mfma16(vf[b], ph, o[b]);
+        o[b] = mfma16(vf[b], pl, o[b]);
+      }
+      if (bad) {  // what was taken out of V, read again, for the rows that attend it
+        const a_u4 one = attn_ones(seen);
+        const bf16_t* vp = at_v(pc, t);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          const a_u4 x = *(const a_u4*)(vp + ((int64_t)(16 * b) << a.seqs.lp));
+          const f32x4_t code = mfma16(attn_code(x), one, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[b][i] = attn_poison(o[b][i], code[i]);
+        }
       }
     }
-    if (more) load_v(t + 128);
+    if (more) load_v(t + 4 * ST);
   }
 
   // the four waves' rows joined
@@ -460,7 +559,7 @@ __device__ __forceinline__ void attn_landed() { asm volatile("s_waitcnt vmcnt(0)
 #define ATTN_KT 64
 #define ATTN_SLACK 8.0f
 
-template <int D>
+template <int D, bool EIGHT, bool WIN>
 __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kernel(AttnArgs a) {
   constexpr int KC = D / 8, NK = ATTN_KT * KC / ATTN_THREADS, NV = D * (ATTN_KT / 8) / ATTN_THREADS, MB = D / 32;
   __shared__ a_u4 k_s[2][ATTN_KT * KC];
@@ -475,7 +574,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   const int ranges = max(1, min(attn_ranges(a), a.splits));
   const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % ranges, tile = a.tiles - 1 - rest / ranges;
   if (tile < 0) return;
-  const AttnTile w = attn_tile<ATTN_ROWS>(a, tile, split, ranges);
+  const AttnTile w = attn_tile<ATTN_ROWS, WIN, ATTN_KT>(a, tile, split, ranges);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
     if (split == 0) attn_zero(a, w, h, D);
@@ -488,6 +587,9 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   const int limit = in ? attn_limit(a, w, r) : 0x7fffffff;
   // tokens that every row of the wave attends, and that any does
   const int low = busy ? attn_limit(a, w, 32 * wave) : 0, top = busy ? attn_limit(a, w, min(32 * wave + 31, w.nr - 1)) : -1;
+  // windows: the row's first token, the first that any of the wave's rows attends, that all of the wave's do, all of the tile's
+  const int from = WIN ? attn_from(a, w, min(r, w.nr - 1)) : 0, bottom = WIN && busy ? attn_from(a, w, 32 * wave) : 0;
+  const int high = WIN && busy ? attn_from(a, w, min(32 * wave + 31, w.nr - 1)) : 0, high0 = WIN ? attn_from(a, w, w.nr - 1) : 0;
   const int ps = 1 << a.seqs.lp;
   // the thread's 16-byte chunk of each K copy (row krow of its 16 or 32) and of each V copy (channel
   // vrow of 32): its place in LDS is tid, so the swizzle is in what it reads
@@ -497,16 +599,52 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   const uint32_t koff = (((krow & 3) | ((krow & 4) << 1) | ((krow & 8) >> 1)) * D + 8 * kc) * 2;  // its row's token
   // The page of the lane's group of 16 tokens, vc / 2, of a step, -1: none: of the present step and the
   // next. Lanes 0 .. 7 have vc = lane ^ of_odd: lane 2 j ^ of_odd has group j's.
-  const int of_odd = 4 * (wave & 1);
+  const int of_odd = EIGHT ? 0 : 4 * (wave & 1), group = EIGHT ? (lane >> 1) & 3 : vc >> 1;
   int pg, pn, en;  // en: the table entry of the step after the next
   const int32_t* const table = a.seqs.table + (int64_t)w.s * a.seqs.max_pages;
-  const int last_entry = (w.hi - 1) >> a.seqs.lp;
+  const int last_entry = w.at<WIN>(w.hi - 1) >> a.seqs.lp;
   // The entry is asked for without a branch, beyond the range for its last one's: with one, the wait for it
   // stood where the two sides meet, behind the copies, and so for all of them (8192 tokens 248 us).
-  auto entry = [&](int t) { en = table[min((t + 16 * (vc >> 1)) >> a.seqs.lp, last_entry)]; };
-  auto page = [&](int t) { return t + 16 * (vc >> 1) < w.hi ? a.seqs.page(en) : -1; };
+  auto entry = [&](int t) { en = table[min((w.at<WIN>(t) + 16 * group) >> a.seqs.lp, last_entry)]; };
+  auto page = [&](int t) { return t + 16 * group < w.hi ? a.seqs.page(en) : -1; };
   const uint32_t k_lds = attn_lds(&k_s[0][64 * wave]), v_lds = attn_lds(&v_s[0][64 * wave]);
+  // 8 bits: what a thread copies goes through its registers, asked for a step ahead and widened to the same places: 16
+  // channels of K row 32 i + tid / 8 (at D = 64 row tid / 4), and 16 tokens, of group 2 i + tid / 128 (tid / 64), of V channel
+  // tid % D.
+  constexpr int N8 = D / 64, C8 = D / 16;
+  a_u4 k8[N8], v8[N8];
+  uint32_t sk8[N8], sv8[N8];
+  const int m8 = tid / C8;  // its first K row
+  auto group_k = [&](int i) { return D == 128 ? 2 * i + (wave >> 1) : wave; };
+  auto ask = [&](int t) {
+    const int at = w.at<WIN>(t);
+#pragma unroll
+    for (int i = 0; i < N8; ++i) {
+      const int j = group_k(i), p = __builtin_amdgcn_readlane(pn, 2 * j);
+      const int64_t first = (((int64_t)max(p, 0) * a.Hkv + h) << a.seqs.lp) + ((at + 16 * j) & (ps - 1));
+      const int row = (m8 & 3) | ((m8 & 4) << 1) | ((m8 & 8) >> 1);
+      k8[i] = *(const a_u4*)((const uint8_t*)a.k + (first + row) * D + 16 * (tid % C8));
+      v8[i] = ((const a_u4*)((const uint8_t*)a.v + first * D))[tid % D];
+      sk8[i] = a.ks[first >> 4], sv8[i] = a.vs[first >> 4];
+    }
+  };
+  auto widen = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < N8; ++i) {
+      const int m = m8 + 32 * i, sw = KC == 16 ? m & 15 : (m >> 1) & 7, c = 2 * (tid % C8), ch = tid % D, vs = (ch >> 1) & 7, j = group_k(i);
+      a_u4 x, y;
+      attn_wide(k8[i], fp8_factor(sk8[i]), x, y);
+      k_s[buf][m * KC + (c ^ sw)] = x, k_s[buf][m * KC + ((c + 1) ^ sw)] = y;
+      attn_wide(v8[i], fp8_factor(sv8[i]), x, y);
+      v_s[buf][ch * 8 + ((2 * j) ^ vs)] = x, v_s[buf][ch * 8 + ((2 * j + 1) ^ vs)] = y;
+    }
+  };
   auto load = [&](int t, int buf) {  // places without a page read page 0, and are masked
+    if constexpr (EIGHT) {
+      ask(t);
+      return;
+    }
+    t = w.at<WIN>(t);
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int j = KC == 16 ? i : 2 * i + k16;  // its group of 16 tokens
@@ -535,6 +673,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   pn = page(t);
   entry(t + ATTN_KT);
   load(t, 0);
+  if constexpr (EIGHT) widen(0);
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) qf[s] = in ? qf[s] ^ a.flip : a_mk(0, 0, 0, 0);
   f32x16_t o[MB];
@@ -562,7 +701,8 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
     entry(t + 2 * ATTN_KT);
     if (more) load(t + ATTN_KT, buf ^ 1);
     // a step with a masked place: only the finite part of V, and a mark where there is another
-    const bool masked = t + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || __ballot(pg < 0);
+    const int rt = w.at<WIN>(t);  // the step's first position
+    const bool masked = rt + ATTN_KT - 1 > low0 || t + ATTN_KT > w.hi || (WIN && rt < high0) || __ballot(pg < 0);
     if (masked) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -574,7 +714,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       }
       wg_lds_barrier();
     }
-    const bool on = t <= top;  // some row of the wave attends the step
+    const bool on = rt <= top && (!WIN || rt + ATTN_KT > bottom || rt < a.sinks);  // some row of the wave attends the step
     f32x16_t s[2];
     if (on) {
 #pragma unroll
@@ -603,13 +743,17 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
       get(x[0], 0);
       __builtin_amdgcn_sched_barrier(0);
       const uint64_t have = __ballot(pg >= 0);  // bit 2 j ^ of_odd: group j
-      const int last = min(limit, w.hi - 1) - t - 8 * e;  // of the lane's tokens, 16 (2 b + q / 8) + q % 8
-      if (t + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || have != ~0ull) {  // a masked place
+      const int last = min(limit - rt, w.hi - 1 - t) - 8 * e;  // of the lane's tokens, 16 (2 b + q / 8) + q % 8
+      const int first = from - rt - 8 * e, kept = a.sinks - rt - 8 * e;
+      if (rt + ATTN_KT - 1 > low || t + ATTN_KT > w.hi || (WIN && rt < high) || have != ~0ull) {  // a masked place
         asm volatile("");  // a branch: few steps have one
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) s[b][q] = 16 * (2 * b + (q >> 3)) + (q & 7) <= last ? s[b][q] : -__builtin_inff();
+          for (int q = 0; q < 16; ++q) {
+            const int i = 16 * (2 * b + (q >> 3)) + (q & 7);
+            s[b][q] = i <= last && (!WIN || i >= first || i < kept) ? s[b][q] : -__builtin_inff();
+          }
         if (have != ~0ull) {  // a group without a page
           asm volatile("");
 #pragma unroll
@@ -680,10 +824,24 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
           for (int q = 0; q < 16; ++q) code[q] = 0.0f;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            const bf16_t* vp = a.v + ((((int64_t)max(__builtin_amdgcn_readlane(pg, (2 * kk) ^ of_odd), 0) * a.Hkv + h) * D + 32 * b + col) << a.seqs.lp) +
-                               ((t + 16 * kk) & (ps - 1)) + 8 * e;
+            const int64_t head = (int64_t)max(__builtin_amdgcn_readlane(pg, (2 * kk) ^ of_odd), 0) * a.Hkv + h;
+            const int place = (rt + 16 * kk) & (ps - 1);
             const int n = (have >> ((2 * kk) ^ of_odd)) & 1 ? min(max(last - 16 * kk + 1, 0), 8) : 0;  // attended of 8
-            code = mfma32a(attn_code(*(const a_u4*)vp), attn_ones((1u << n) - 1), code);
+            uint32_t seen = (1u << n) - 1;
+            if constexpr (WIN) {
+              const uint32_t before = (1u << min(max(first - 16 * kk, 0), 8)) - 1, stay = (1u << min(max(kept - 16 * kk, 0), 8)) - 1;
+              seen &= ~before | stay;
+            }
+            a_u4 x;
+            if constexpr (EIGHT) {
+              const int64_t block = ((head << a.seqs.lp) + place) >> 4;
+              const uint2 y = *(const uint2*)((const uint8_t*)a.v + (block * D + 32 * b + col) * 16 + 8 * e);
+              const float f = fp8_factor(a.vs[block]);
+              x = a_mk(fp8_bf16<false>(y.x, f), fp8_bf16<true>(y.x, f), fp8_bf16<false>(y.y, f), fp8_bf16<true>(y.y, f));
+            } else {
+              x = *(const a_u4*)(a.v + ((head * D + 32 * b + col) << a.seqs.lp) + place + 8 * e);
+            }
+            code = mfma32a(attn_code(x), attn_ones(seen), code);
           }
 #pragma unroll
           for (int q = 0; q < 16; ++q) o[b][q] = attn_poison(o[b][q], code[q]);
@@ -694,6 +852,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
     if (!more) break;
     buf ^= 1;
     t += ATTN_KT;
+    if constexpr (EIGHT) widen(buf);
   }
 
   l += pl_xor32f(l, lane);
@@ -775,9 +934,12 @@ struct AttnPlan {
   int64_t tiles;
 };
 
-static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv, int D) {
+// (window and sinks: what a tile's steps hold of them at most, as though the table were no longer)
+static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv, int D, int64_t window,
+                          int64_t sinks) {
   AttnPlan p = {};
-  const int64_t rows = n_tokens * (Hq / Hkv), cus = pp_device_cus(), capacity = (int64_t)max_pages * page_size;
+  const int64_t rows = n_tokens * (Hq / Hkv), cus = pp_device_cus(), room = (int64_t)max_pages * page_size;
+  const int64_t capacity = window > 0 ? std::min(room, window + std::min(sinks, room) + 2 * ATTN_ROWS) : room;
   auto items = [&](int tile) { return std::max<int64_t>(1, (rows / tile + n_seqs) * Hkv); };
   // Tiles of 16 rows for single tokens and the like, for what does not fill the GPU, and for what is short
   // altogether: their steps cost four times as much for the same work (6 ns for 16 rows x 128 tokens of D = 128,
@@ -829,30 +991,43 @@ static size_t attn_ws_bytes(const AttnPlan& p, int64_t rows, int D) {
   return (size_t)rows * p.splits * (D + 2) * 4 + (size_t)rows * 4;
 }
 
-extern "C" size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size,
-                                                     int Hq, int Hkv, int D) {
-  if (pp_paged_sizes("pp_paged_attention", n_tokens, n_seqs, max_pages, 1, page_size, Hq, Hkv, D)) return 0;
-  if (n_tokens == 0 || Hq == 0) return 0;
-  return attn_ws_bytes(attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D), n_tokens * Hq, D);
+static int attn_window(const char* what, int64_t window, int64_t sinks) {
+  PP_REQUIRE(window >= 0 && sinks >= 0, PP_ERR_INVALID, "%s: window %lld, %lld first tokens", what, (long long)window, (long long)sinks);
+  return PP_OK;
 }
 
-extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs,
-                                  const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
-                                  int max_pages, const void* k_pages, const void* v_pages, int num_pages,
-                                  int page_size, int Hq, int Hkv, int D, float scale, void* out_bf16, int zero_tail,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" size_t pp_paged_attention_with_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv,
+                                                          int D, int eight_bits, int64_t window, int64_t sinks) {
   const char* const what = "pp_paged_attention";
+  if (pp_paged_sizes(what, n_tokens, n_seqs, max_pages, 1, page_size, Hq, Hkv, D) || attn_window(what, window, sinks)) return 0;
+  if (n_tokens == 0 || Hq == 0) return 0;
+  return attn_ws_bytes(attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D, window, sinks), n_tokens * Hq, D);
+}
+
+extern "C" size_t pp_paged_attention_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size,
+                                                     int Hq, int Hkv, int D) {
+  return pp_paged_attention_with_workspace_bytes(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D, 0, 0, 0);
+}
+
+static int attend(const char* what, const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs, const int32_t* cu_q,
+                  const int32_t* kv_lens, const int32_t* block_table, int max_pages, const void* k_pages, const void* v_pages,
+                  const void* k_scales, const void* v_scales, int num_pages, int page_size, int Hq, int Hkv, int D, float scale,
+                  int64_t window, int64_t sinks, void* out_bf16, int zero_tail, void* workspace, size_t workspace_bytes,
+                  void* stream) {
   int rc = pp_paged_check(what, n_tokens, n_seqs, cu_q, kv_lens, block_table, max_pages, k_pages, v_pages, num_pages,
                           page_size, Hq, Hkv, D);
   if (rc) return rc;
   PP_REQUIRE(Hq >= 1, PP_ERR_INVALID, "%s: no query heads", what);
+  PP_REQUIRE(!k_scales == !v_scales, PP_ERR_INVALID, "%s: scales of keys and of values belong together", what);
+  rc = attn_window(what, window, sinks);
+  if (rc) return rc;
   if (n_tokens == 0) return PP_OK;
   PP_REQUIRE(q && q_strides && out_bf16, PP_ERR_INVALID, "%s: null pointer", what);
   PP_REQUIRE((((uintptr_t)q | (uintptr_t)out_bf16) & 15) == 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0,
              PP_ERR_INVALID, "%s: every head of q and out must start on a 16-byte boundary", what);
   const float c = fabsf(scale) * 1.4426950408889634f;
   PP_REQUIRE(std::isfinite(c), PP_ERR_INVALID, "%s: scale %g", what, scale);
-  const AttnPlan p = attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D);
+  const AttnPlan p = attn_plan(n_tokens, n_seqs, max_pages, page_size, Hq, Hkv, D, window, sinks);
   const size_t need = attn_ws_bytes(p, n_tokens * Hq, D);
   PP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PP_ERR_INVALID,
              "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes, need);
@@ -864,6 +1039,9 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   a.c = std::max(c, 0x1p-149f), a.flip = scale < 0.0f ? 0x80008000u : 0u;  // (for 0: 2^-21 of any float32)
   a.out = (bf16_t*)out_bf16, a.zero_tail = zero_tail;
   a.splits = p.splits, a.base = p.base, a.behind = p.behind, a.tiles = (int)p.tiles;
+  a.ks = (const uint8_t*)k_scales, a.vs = (const uint8_t*)v_scales;
+  // (no position is beyond 2^31, none in the table beyond 2^30)
+  a.window = (int)std::min<int64_t>(window, 0x7fffffff), a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
   a.po = (float*)workspace;
   a.pml = a.po + n_tokens * Hq * p.splits * D;
   a.pns = (int*)(a.pml + n_tokens * Hq * p.splits * 2);
@@ -880,10 +1058,17 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   const int64_t joins = alone ? (rows * (D / 4) + ATTN_THREADS - 1) / ATTN_THREADS : rows;
   hipStream_t st = (hipStream_t)stream;
   const unsigned n = (unsigned)items, nj = (unsigned)joins;
+#define ATTN_KIND(D_, EIGHT_, WIN_)                                                       \
+  do {                                                                                    \
+    if (p.rows == 16) attn_few_kernel<D_, EIGHT_, WIN_><<<n, ATTN_THREADS, 0, st>>>(a);   \
+    else attn_many_kernel<D_, EIGHT_, WIN_><<<n, ATTN_THREADS, 0, st>>>(a);               \
+  } while (0)
 #define ATTN(D_)                                                                          \
   do {                                                                                    \
-    if (p.rows == 16) attn_few_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                 \
-    else attn_many_kernel<D_><<<n, ATTN_THREADS, 0, st>>>(a);                            \
+    if (k_scales && window > 0) ATTN_KIND(D_, true, true);                                \
+    else if (k_scales) ATTN_KIND(D_, true, false);                                        \
+    else if (window > 0) ATTN_KIND(D_, false, true);                                      \
+    else ATTN_KIND(D_, false, false);                                                     \
     if (p.splits > 1) {                                                                   \
       if (alone) attn_join_kernel<D_, true><<<nj, ATTN_THREADS, 0, st>>>(a, rows);        \
       else attn_join_kernel<D_, false><<<nj, ATTN_THREADS, 0, st>>>(a, rows);             \
@@ -892,5 +1077,26 @@ extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64
   if (D == 64) ATTN(64);
   else ATTN(128);
 #undef ATTN
+#undef ATTN_KIND
   return pp_check_launch(what);
+}
+
+extern "C" int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs,
+                                  const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                                  int max_pages, const void* k_pages, const void* v_pages, int num_pages,
+                                  int page_size, int Hq, int Hkv, int D, float scale, void* out_bf16, int zero_tail,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  return attend("pp_paged_attention", q, q_strides, n_tokens, n_seqs, cu_q, kv_lens, block_table, max_pages, k_pages, v_pages,
+                nullptr, nullptr, num_pages, page_size, Hq, Hkv, D, scale, 0, 0, out_bf16, zero_tail, workspace,
+                workspace_bytes, stream);
+}
+
+extern "C" int pp_paged_attention_with(const void* q, const int64_t* q_strides, int64_t n_tokens, int n_seqs, const int32_t* cu_q,
+                                       const int32_t* kv_lens, const int32_t* block_table, int max_pages, const void* k_pages,
+                                       const void* v_pages, const void* k_scales, const void* v_scales, int num_pages,
+                                       int page_size, int Hq, int Hkv, int D, float scale, int64_t window, int64_t sinks,
+                                       void* out_bf16, int zero_tail, void* workspace, size_t workspace_bytes, void* stream) {
+  return attend("pp_paged_attention_with", q, q_strides, n_tokens, n_seqs, cu_q, kv_lens, block_table, max_pages, k_pages,
+                v_pages, k_scales, v_scales, num_pages, page_size, Hq, Hkv, D, scale, window, sinks, out_bf16, zero_tail,
+                workspace, workspace_bytes, stream);
 }

@@ -18,116 +18,9 @@
 // copy reaches 5.05; float32, 16384 tokens of 12 heads (201 MB): 38.0 us, 5.3 TB/s; one token 2.2 us, a
 // launch.
 #include <algorithm>
+#include <cmath>
 
-#include "paged.h"
-
-#define ROT_THREADS 256
-#define ROT_TABLE 2048  // (cos, sin) entries in LDS
-
-// V consecutive elements as they are in memory (more than one: in 16-byte words)
-template <typename T, int V>
-struct RotPack {
-  T v[V];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (V == 1) v[0] = *p;
-    else *this = *(const RotPack*)__builtin_assume_aligned(p, 16);
-  }
-};
-__device__ __forceinline__ float rot_f32(float x) { return x; }
-__device__ __forceinline__ float rot_f32(bf16_t x) { return bf16_to_f32(x); }
-template <int V>
-__device__ __forceinline__ void rot_store(float* p, const float (&v)[V]) {
-  if constexpr (V == 1) *p = v[0];
-  else
-#pragma unroll
-    for (int i = 0; i < V; i += 4) *(float4*)(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-}
-template <int V>
-__device__ __forceinline__ void rot_store(bf16_t* p, const float (&v)[V]) {
-  if constexpr (V == 8)
-    *(uint4*)p = make_uint4(f32_to_bf16x2(v[0], v[1]), f32_to_bf16x2(v[2], v[3]), f32_to_bf16x2(v[4], v[5]), f32_to_bf16x2(v[6], v[7]));
-  else
-    *p = f32_to_bf16(v[0]);
-}
-
-// (m cos a, m sin a) of a = position * inv_freq
-__device__ __forceinline__ float2 rot_entry(int64_t position, double inv_freq, float m, float sign) {
-  const double turns = (double)position * (inv_freq * 0.15915494309189533577);
-  const double exact = 2.0 * (turns - rint(turns));
-  const float half_turns = (float)exact, left = (float)((exact - half_turns) * 3.14159265358979323846);
-  float s, c;
-  sincospif(half_turns, &s, &c);
-  return make_float2(__fmaf_rn(-s, left, c) * m, sign * __fmaf_rn(c, left, s) * m);
-}
-
-// A unit of a head: u < nr turns V pairs, the units behind them copy V channels. Its loads apart from
-// the rest, so that they are on their way while cos and sin are computed.
-template <typename TI, int V, bool HALF>
-struct RotUnit {
-  RotPack<TI, V> p, q;
-  __device__ __forceinline__ void load(const TI* x, int u, int nr, int rd) {
-    if (u < nr) {
-      const int a = HALF ? u * V : 2 * u * V, b = HALF ? rd / 2 + u * V : a + V;
-      p.load(x + a);
-      q.load(x + b);
-    } else
-      p.load(x + rd + (u - nr) * V);
-  }
-  template <typename TO>
-  __device__ __forceinline__ void store(TO* y, const float2* cs, int u, int nr, int rd) const {
-    float r[V], t[V];
-    if (u < nr) {
-      const int a = HALF ? u * V : 2 * u * V, b = HALF ? rd / 2 + u * V : a + V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        // the pair: one of p and one of q, or two neighbours of what p and q hold together
-        const float x1 = rot_f32(HALF ? p.v[i] : 2 * i < V ? p.v[2 * i % V] : q.v[2 * i % V]);
-        const float x2 = rot_f32(HALF ? q.v[i] : 2 * i + 1 < V ? p.v[(2 * i + 1) % V] : q.v[(2 * i + 1) % V]);
-        const float2 w = cs[u * V + i];
-        const float y1 = __fmaf_rn(x1, w.x, -__fmul_rn(x2, w.y)), y2 = __fmaf_rn(x1, w.y, __fmul_rn(x2, w.x));
-        if (HALF) {
-          r[i] = y1, t[i] = y2;
-        } else {
-          (2 * i < V ? r : t)[2 * i % V] = y1;
-          (2 * i + 1 < V ? r : t)[(2 * i + 1) % V] = y2;
-        }
-      }
-      rot_store<V>(y + a, r);
-      rot_store<V>(y + b, t);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) r[i] = rot_f32(p.v[i]);
-      rot_store<V>(y + rd + (u - nr) * V, r);
-      asm volatile("");  // the two sides' last stores, merged, went out as 4 and 12 bytes
-    }
-  }
-};
-
-// A workgroup's threads: 2^lgu neighbours on the units of a head, then 2^lgt tokens, then heads; all by
-// shifts (divisions cost more than the turning).
-struct RotLanes {
-  int u, i, h, hstep;
-  __device__ RotLanes(int tid, int lgu, int lgt) {
-    u = tid & ((1 << lgu) - 1);
-    i = (tid >> lgu) & ((1 << lgt) - 1);
-    h = tid >> (lgu + lgt);
-    hstep = (ROT_THREADS >> lgu) >> lgt;
-  }
-};
-static inline int rot_log2up(int64_t v) {
-  int b = 0;
-  while (((int64_t)1 << b) < v) ++b;
-  return b;
-}
-
-// cos and sin of nt tokens into LDS, position(t) theirs
-template <typename F>
-__device__ __forceinline__ void rot_table(float2* cs, const double* inv_freq, int half, int lgh, int nt, float m, float sign,
-                                          F position) {
-  for (int f = threadIdx.x & ((1 << lgh) - 1); f < half; f += ROT_THREADS)  // once, unless there are more than threads
-    for (int t = threadIdx.x >> lgh; t < nt; t += max(ROT_THREADS >> lgh, 1))
-      cs[t * half + f] = rot_entry(position(t), inv_freq[f], m, sign);
-}
+#include "append.h"
 
 struct RotArgs {
   const void* x;
@@ -171,12 +64,6 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotArgs a) {
     now.store(y + h * a.ys[2], cs_s + w.i * half, u, nr, a.rd);
     now = next, h = h2, u = u2;
   }
-}
-
-static bool rot_aligned(const void* p, const int64_t* s, int n, int bytes) {
-  bool ok = ((uintptr_t)p & 15) == 0;
-  for (int i = 0; i < n; ++i) ok = ok && (s[i] * bytes) % 16 == 0;
-  return ok;
 }
 
 extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, const void* positions, int pos64,
@@ -248,31 +135,13 @@ extern "C" int pp_rotary(const void* x, int dtype, const int64_t* x_strides, con
 // Bound by memory for chunks (8192 tokens of 36 heads, 151 MB: 37 us, 4.1 TB/s; the rotation alone of as
 // many bytes 27.3), by the chain offsets, table, rows for single tokens (3.9 us for one, 5.4 for 64, 9.1
 // for 256 of them).
-#define APP_THREADS ROT_THREADS
-#define APP_TOKENS 16
-
-struct AppArgs {
-  PagedSeqs seqs;
-  const void *q, *k, *v;
-  int64_t qs[2], ks[2], vs[2];  // strides of token and head, in elements
-  bf16_t *q_out, *k_pages, *v_pages;
-  const double* inv_freq;
-  int Hq, Hkv, rd;
-  float mscale;
-  int zero_tail;
-  int lgu, lgh;        // log2 of the threads on a head, and of rd / 2 (rounded up)
-  int per, nqb, nkb;   // heads per block, blocks of query and of key heads
-  int vper, nvb;       // the same of the value items
-  uint32_t values;     // value items
-};
-
 __device__ __forceinline__ uint32_t app_pair(const float* p) {
   const float2 f = *(const float2*)p;
   return f32_to_bf16x2(f.x, f.y);
 }
 __device__ __forceinline__ uint32_t app_pair(const bf16_t* p) { return *(const uint32_t*)p; }
 
-template <typename T, int D, bool HALF>
+template <typename T, int D, bool HALF, bool NORM>
 __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
   __shared__ float2 cs_s[APP_TOKENS * D / 2];
   const int tid = threadIdx.x;
@@ -361,30 +230,10 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
     }
     return;
   }
-  const int nr = half / 8, per = nr + (D - a.rd) / 8;
-  const RotLanes w(tid, a.lgu, 32 - __clz(nt - 1));  // as many tokens as there are
-  const int64_t row = row0 + lo + w.i;
-  const T* const x = (const T*)(kind == 0 ? a.q : a.k) + row * (kind == 0 ? a.qs[0] : a.ks[0]);
-  const int64_t xs = kind == 0 ? a.qs[1] : a.ks[1];
-  bf16_t* const y = kind == 0 ? a.q_out + row * a.Hq * D
-                              : a.k_pages + (((int64_t)entry * a.Hkv << a.seqs.lp) + place + lo + w.i) * D;
-  const int64_t ys = kind == 0 ? D : (int64_t)D << a.seqs.lp;
-  int h = h0 + w.h;
-  bool more = w.i < nt && h < h0 + nh && w.u < per;
-  RotUnit<T, 8, HALF> now, next;
-  if (more) now.load(x + h * xs, w.u, nr, a.rd);
-  paged_asked();
-  if (pair < half)
-    for (int t = tid >> a.lgh; t < nt; t += APP_THREADS >> a.lgh) cs_s[t * half + pair] = rot_entry(p0 + lo + t, freq, a.mscale, 1.0f);
-  if (kind && no_page()) return;
-  __syncthreads();
-  while (more) {
-    const int h2 = h + w.hstep;
-    more = h2 < h0 + nh;
-    if (more) next.load(x + h2 * xs, w.u, nr, a.rd);
-    now.store(y + h * ys, cs_s + w.i * half, w.u, nr, a.rd);
-    now = next, h = h2;
-  }
+  bf16_t* const to = kind == 0 ? a.q_out + (int64_t)(row0 + lo) * a.Hq * D
+                               : a.k_pages + (((int64_t)entry * a.Hkv << a.seqs.lp) + place + lo) * D;
+  app_turn<T, D, HALF, NORM>(a, kind, cs_s, freq, pair, half, row0 + lo, nt, h0, nh, p0 + lo, to,
+                             kind == 0 ? (int64_t)a.Hq * D : D, kind == 0 ? D : (int64_t)D << a.seqs.lp, [&] { return kind && no_page(); });
 }
 
 int pp_paged_sizes(const char* what, int64_t n_tokens, int n_seqs, int max_pages, int num_pages, int page_size, int Hq,
@@ -414,13 +263,12 @@ int pp_paged_check(const char* what, int64_t n_tokens, int n_seqs, const void* c
   return PP_OK;
 }
 
-extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                            const void* v, const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs,
-                            const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
-                            int num_pages, int page_size, int Hq, int Hkv, int D, const double* inv_freq,
-                            int rotary_dim, int layout, float mscale, void* k_pages, void* v_pages, void* q_out,
-                            int zero_tail, void* stream) {
-  const char* const what = "pp_kv_append";
+static int append(const char* what, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                  const void* v, const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs, const int32_t* cu_q,
+                  const int32_t* kv_lens, const int32_t* block_table, int max_pages, int num_pages, int page_size, int Hq,
+                  int Hkv, int D, const double* inv_freq, int rotary_dim, int layout, float mscale, const void* q_weight,
+                  const void* k_weight, int w_dtype, float eps, void* k_pages, void* v_pages, void* k_scales, void* v_scales,
+                  void* q_out, int zero_tail, void* stream) {
   if (!q) Hq = 0;
   int rc = pp_paged_check(what, n_tokens, n_seqs, cu_q, kv_lens, block_table, max_pages, k_pages, v_pages, num_pages,
                           page_size, Hq, Hkv, D);
@@ -430,19 +278,30 @@ extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void*
   if (!inv_freq) rotary_dim = 0;
   PP_REQUIRE(rotary_dim >= 0 && rotary_dim <= D && rotary_dim % 16 == 0, PP_ERR_UNSUPPORTED,
              "%s: rotary_dim %d unsupported (a multiple of 16 up to the head size %d)", what, rotary_dim, D);
+  PP_REQUIRE(!k_scales == !v_scales, PP_ERR_INVALID, "%s: scales of keys and of values belong together", what);
+  PP_REQUIRE(!k_weight ? !q_weight : !q || q_weight, PP_ERR_INVALID, "%s: norms of queries and of keys belong together", what);
+  if (k_weight) {
+    PP_REQUIRE(w_dtype == PP_DTYPE_F32 || w_dtype == dtype, PP_ERR_INVALID, "%s: weights of dtype %d for heads of %d", what, w_dtype, dtype);
+    PP_REQUIRE(eps >= 0.0f && std::isfinite(eps), PP_ERR_INVALID, "%s: eps %g", what, eps);
+  }
   if (n_tokens == 0) return PP_OK;
   PP_REQUIRE(k && v && k_strides && v_strides && (!q || (q_strides && q_out)), PP_ERR_INVALID, "%s: null pointer", what);
   const int bytes = dtype == PP_DTYPE_F32 ? 4 : 2;
   PP_REQUIRE(rot_aligned(k, k_strides, 2, bytes) && rot_aligned(v, v_strides, 2, bytes) &&
                  (!q || (rot_aligned(q, q_strides, 2, bytes) && ((uintptr_t)q_out & 15) == 0)),
              PP_ERR_INVALID, "%s: every head of q, k, v and q_out must start on a 16-byte boundary", what);
-  AppArgs a;
+  AppArgs a = {};
   a.seqs = {cu_q, kv_lens, block_table, (int)n_tokens, n_seqs, max_pages, num_pages, paged_log2(page_size)};
   a.q = q, a.k = k, a.v = v;
   for (int i = 0; i < 2; ++i) a.qs[i] = q ? q_strides[i] : 0, a.ks[i] = k_strides[i], a.vs[i] = v_strides[i];
   a.q_out = (bf16_t*)q_out, a.k_pages = (bf16_t*)k_pages, a.v_pages = (bf16_t*)v_pages;
   a.inv_freq = inv_freq, a.Hq = Hq, a.Hkv = Hkv, a.rd = rotary_dim, a.mscale = mscale, a.zero_tail = zero_tail;
+  a.qw = q_weight, a.kw = k_weight, a.w32 = w_dtype == PP_DTYPE_F32, a.eps = eps;
   a.lgu = rot_log2up(rotary_dim / 16 + (D - rotary_dim) / 8), a.lgh = rot_log2up(std::max(rotary_dim / 2, 1));
+  if (k_scales) {
+    a.k8 = (uint8_t*)k_pages, a.v8 = (uint8_t*)v_pages, a.k_scales = (uint8_t*)k_scales, a.v_scales = (uint8_t*)v_scales;
+    return app8_launch(what, a, dtype, D, layout, n_tokens, (hipStream_t)stream);
+  }
   // Heads of an item. Single tokens: a group has one, so all the heads that the threads hold in one step
   // (32, value heads 4, or 16 where there are workgroups enough); 1, 64, 256 sequences of 12 heads 3.5,
   // 5.1, 8.8 us, in items of 4 heads 3.7, 5.7, 12.6. Chunks: 4, and one value head (64 tokens of it),
@@ -458,10 +317,15 @@ extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void*
   a.values = (uint32_t)values;
   const unsigned grid = (unsigned)items;
   hipStream_t st = (hipStream_t)stream;
+#define APP_NORM(T, D_, HALF_)                                                                           \
+  do {                                                                                                   \
+    if (k_weight) kv_append_kernel<T, D_, HALF_, true><<<grid, APP_THREADS, 0, st>>>(a);                 \
+    else kv_append_kernel<T, D_, HALF_, false><<<grid, APP_THREADS, 0, st>>>(a);                         \
+  } while (0)
 #define APP(T, D_)                                                                                       \
   do {                                                                                                   \
-    if (layout == PP_ROTARY_HALF) kv_append_kernel<T, D_, true><<<grid, APP_THREADS, 0, st>>>(a);        \
-    else kv_append_kernel<T, D_, false><<<grid, APP_THREADS, 0, st>>>(a);                                \
+    if (layout == PP_ROTARY_HALF) APP_NORM(T, D_, true);                                                 \
+    else APP_NORM(T, D_, false);                                                                         \
   } while (0)
   if (dtype == PP_DTYPE_F32) {
     if (D == 64) APP(float, 64);
@@ -471,5 +335,29 @@ extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void*
     else APP(bf16_t, 128);
   }
 #undef APP
+#undef APP_NORM
   return pp_check_launch(what);
+}
+
+extern "C" int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                            const void* v, const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs,
+                            const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
+                            int num_pages, int page_size, int Hq, int Hkv, int D, const double* inv_freq,
+                            int rotary_dim, int layout, float mscale, void* k_pages, void* v_pages, void* q_out,
+                            int zero_tail, void* stream) {
+  return append("pp_kv_append", q, q_strides, k, k_strides, v, v_strides, dtype, n_tokens, n_seqs, cu_q, kv_lens, block_table,
+                max_pages, num_pages, page_size, Hq, Hkv, D, inv_freq, rotary_dim, layout, mscale, nullptr, nullptr, 0, 0.0f,
+                k_pages, v_pages, nullptr, nullptr, q_out, zero_tail, stream);
+}
+
+extern "C" int pp_kv_append_with(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                 const void* v, const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs,
+                                 const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
+                                 int num_pages, int page_size, int Hq, int Hkv, int D, const double* inv_freq,
+                                 int rotary_dim, int layout, float mscale, const void* q_weight, const void* k_weight,
+                                 int w_dtype, float eps, void* k_pages, void* v_pages, void* k_scales, void* v_scales,
+                                 void* q_out, int zero_tail, void* stream) {
+  return append("pp_kv_append_with", q, q_strides, k, k_strides, v, v_strides, dtype, n_tokens, n_seqs, cu_q, kv_lens,
+                block_table, max_pages, num_pages, page_size, Hq, Hkv, D, inv_freq, rotary_dim, layout, mscale, q_weight,
+                k_weight, w_dtype, eps, k_pages, v_pages, k_scales, v_scales, q_out, zero_tail, stream);
 }

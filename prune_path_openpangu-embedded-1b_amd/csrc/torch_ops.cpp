@@ -19,7 +19,7 @@
 //   moe_prefill(_into)    TauSparseMoE.forward_prefill (:532-604)
 //   masked_gate(_bwd)     MoELayer.forward's expert gating and its backward
 //                         (src/MoEBlock_origin.py:205-212)
-//   rotary, kv_append(_q), paged_attention(_into)
+//   rotary, qk_norm_rotary(_bwd), kv_append(_q), kv_read(_into), paged_attention(_into)
 //                         no counterpart in the reference's own code: the attention side of a
 //                         decoder that serves several sequences
 #include <ATen/ATen.h>
@@ -624,14 +624,230 @@ Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& i
   return y;
 }
 
+// ------------------------------------------------------------------ norms of queries and keys
+// Query and key heads of the same tokens, [N, heads, D] or [B, L, heads, D].
+void norm_check(const char* name, const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                const Tensor& positions, const Tensor& inv_freq) {
+  TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && q.dim() == k.dim() && q.scalar_type() == k.scalar_type(), "prunepath.", name,
+              ": q and k must be [N, heads, D] or [B, L, heads, D] of one dtype");
+  x_code(q, name);
+  TORCH_CHECK(same_sizes(q, k, q.dim() - 2), "prunepath.", name, ": q and k of different tokens");
+  const c10::SymInt D = q.sym_size(-1);
+  TORCH_SYM_CHECK(k.sym_size(-1).sym_eq(D), "prunepath.", name, ": query heads of ", D, " channels and key heads of ", k.sym_size(-1));
+  TORCH_SYM_CHECK(D.sym_ge(2).sym_and(D.sym_le(256)), "prunepath.", name, ": head size ", D, " unsupported (2 to 256)");
+  for (const Tensor* w : {&q_weight, &k_weight}) {
+    TORCH_CHECK(w->dim() == 1 && (w->scalar_type() == at::kFloat || w->scalar_type() == q.scalar_type()) &&
+                    w->scalar_type() == q_weight.scalar_type() && w->is_contiguous(),
+                "prunepath.", name, ": weights must be contiguous [D], both float32 or both like q");
+    TORCH_SYM_CHECK(w->sym_size(0).sym_eq(D), "prunepath.", name, ": ", w->sym_size(0), " weights for heads of ", D, " channels");
+  }
+  TORCH_CHECK(positions.dim() == q.dim() - 2 && same_sizes(q, positions, q.dim() - 2), "prunepath.", name,
+              ": positions must have q's leading shape");
+  TORCH_CHECK(positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt, "prunepath.", name,
+              ": positions must be int32 or int64");
+  TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && inv_freq.is_contiguous(), "prunepath.", name,
+              ": inv_freq must be contiguous float64 [rotary_dim / 2]");
+  const c10::SymInt pairs = inv_freq.sym_size(0);
+  TORCH_SYM_CHECK(pairs.sym_ge(1).sym_and((pairs * 2).sym_le(D)), "prunepath.", name, ": ", pairs, " pairs for heads of ", D, " channels");
+}
+
+// Strides of batch, token and head.
+struct NormStrides {
+  int64_t s[3];
+  explicit NormStrides(const Tensor& t) : s{t.dim() == 4 ? step(t, 0) : 0, step(t, t.dim() - 3), step(t, t.dim() - 2)} {}
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rotary_gpu(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                              const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                                              double mscale, double eps) {
+  const char* const name = "qk_norm_rotary";
+  const int lay = rotary_layout(layout, name);
+  norm_check(name, q, k, q_weight, k_weight, positions, inv_freq);
+  same_device(name, q, {&q, &k, &q_weight, &k_weight, &positions, &inv_freq});
+  const c10::DeviceGuard g(q.device());
+  const Tensor qi = rotary_input(q), ki = rotary_input(k);
+  Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  const int64_t d = q.dim();
+  const NormStrides qs(qi), ks(ki);
+  const int64_t ps[2] = {d == 4 ? step(positions, 0) : 0, step(positions, d - 3)};
+  check_rc(pp_qk_norm_rotary(qi.data_ptr(), qs.s, ki.data_ptr(), ks.s, x_code(q, name), q_weight.data_ptr(), k_weight.data_ptr(),
+                             w_code(q_weight, name), positions.data_ptr(), positions.scalar_type() == at::kLong, ps,
+                             d == 4 ? q.size(0) : 1, q.size(d - 3), (int)q.size(d - 2), (int)k.size(d - 2), (int)q.size(d - 1),
+                             inv_freq.data_ptr<double>(), (int)(2 * inv_freq.numel()), lay, (float)mscale, (float)eps,
+                             qo.data_ptr(), ko.data_ptr(), stream_of(q)),
+           name);
+  return {qo, ko};
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rotary_meta(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                               const Tensor& positions, const Tensor& inv_freq, c10::string_view layout, double,
+                                               double) {
+  rotary_layout(layout, "qk_norm_rotary");
+  norm_check("qk_norm_rotary", q, k, q_weight, k_weight, positions, inv_freq);
+  return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options())};
+}
+
+void norm_bwd_check(const Tensor& dq, const Tensor& dk, const Tensor& q, const Tensor& k, const Tensor& q_weight,
+                    const Tensor& k_weight, const Tensor& positions, const Tensor& inv_freq) {
+  const char* const name = "qk_norm_rotary_bwd";
+  norm_check(name, q, k, q_weight, k_weight, positions, inv_freq);
+  TORCH_CHECK(dq.dim() == q.dim() && dk.dim() == k.dim() && dq.scalar_type() == q.scalar_type() && dk.scalar_type() == k.scalar_type() &&
+                  same_sizes(dq, q, q.dim()) && same_sizes(dk, k, k.dim()),
+              "prunepath.qk_norm_rotary_bwd: dq and dk must be like q and k");
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd_gpu(const Tensor& dq, const Tensor& dk, const Tensor& q,
+                                                                  const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                                                  const Tensor& positions, const Tensor& inv_freq,
+                                                                  c10::string_view layout, double mscale, double eps,
+                                                                  bool weights) {
+  const char* const name = "qk_norm_rotary_bwd";
+  const int lay = rotary_layout(layout, name);
+  norm_bwd_check(dq, dk, q, k, q_weight, k_weight, positions, inv_freq);
+  same_device(name, q, {&dq, &dk, &q, &k, &q_weight, &k_weight, &positions, &inv_freq});
+  const c10::DeviceGuard g(q.device());
+  const Tensor qi = rotary_input(q), ki = rotary_input(k), dqi = rotary_input(dq), dki = rotary_input(dk);
+  Tensor qg = at::empty(q.sizes(), q.options()), kg = at::empty(k.sizes(), k.options());
+  Tensor wq = at::empty({weights ? q.size(-1) : 0}, q_weight.options()), wk = at::empty({weights ? q.size(-1) : 0}, k_weight.options());
+  const int64_t d = q.dim(), B = d == 4 ? q.size(0) : 1, L = q.size(d - 3);
+  const NormStrides qs(qi), ks(ki), dqs(dqi), dks(dki);
+  const int64_t ps[2] = {d == 4 ? step(positions, 0) : 0, step(positions, d - 3)};
+  const int rd = (int)(2 * inv_freq.numel());
+  const size_t need = weights ? pp_qk_norm_rotary_workspace_bytes(x_code(q, name), B, L, (int)q.size(d - 2), (int)k.size(d - 2),
+                                                                  (int)q.size(d - 1), rd)
+                              : 0;
+  Tensor ws;
+  if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+  check_rc(pp_qk_norm_rotary_bwd(dqi.data_ptr(), dqs.s, dki.data_ptr(), dks.s, qi.data_ptr(), qs.s, ki.data_ptr(), ks.s,
+                                 x_code(q, name), q_weight.data_ptr(), k_weight.data_ptr(), w_code(q_weight, name),
+                                 positions.data_ptr(), positions.scalar_type() == at::kLong, ps, B, L, (int)q.size(d - 2),
+                                 (int)k.size(d - 2), (int)q.size(d - 1), inv_freq.data_ptr<double>(), rd, lay, (float)mscale,
+                                 (float)eps, qg.data_ptr(), kg.data_ptr(), weights ? wq.data_ptr() : nullptr,
+                                 weights ? wk.data_ptr() : nullptr, need ? ws.data_ptr() : nullptr, need, stream_of(q)),
+           name);
+  return {qg, kg, wq, wk};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd_meta(const Tensor& dq, const Tensor& dk, const Tensor& q,
+                                                                   const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                                                   const Tensor& positions, const Tensor& inv_freq,
+                                                                   c10::string_view layout, double, double, bool weights) {
+  rotary_layout(layout, "qk_norm_rotary_bwd");
+  norm_bwd_check(dq, dk, q, k, q_weight, k_weight, positions, inv_freq);
+  const c10::SymInt n = weights ? q.sym_size(-1) : c10::SymInt(0);
+  return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options()),
+          at::empty_symint({n}, q_weight.options()), at::empty_symint({n}, k_weight.options())};
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rotary_call(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                               const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                                               double mscale, double eps) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("prunepath::qk_norm_rotary", "")
+                       .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                         const Tensor&, c10::string_view, double, double)>();
+  return op.call(q, k, q_weight, k_weight, positions, inv_freq, layout, mscale, eps);
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd_call(const Tensor& dq, const Tensor& dk, const Tensor& q,
+                                                                   const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                                                   const Tensor& positions, const Tensor& inv_freq,
+                                                                   c10::string_view layout, double mscale, double eps,
+                                                                   bool weights) {
+  static auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("prunepath::qk_norm_rotary_bwd", "")
+          .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                            const Tensor&, const Tensor&, const Tensor&, c10::string_view, double,
+                                                            double, bool)>();
+  return op.call(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, layout, mscale, eps, weights);
+}
+
+struct QkNormBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable saved[6];  // q, k, their weights, positions, inv_freq
+  std::string layout;
+  double mscale = 1.0, eps = 0.0;
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const bool has_q = grads[0].defined(), has_k = grads[1].defined();
+    if (!has_q && !has_k) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    Tensor t[6];
+    {
+      std::lock_guard<std::mutex> lock(mutex_);  // another thread's backward of the same graph may release them
+      for (int i = 0; i < 6; ++i) t[i] = saved[i].unpack();
+    }
+    // what has no gradient takes part with no heads
+    for (int i = 0; i < 2; ++i)
+      if (!grads[i].defined()) {
+        t[i] = t[i].narrow(-2, 0, 0);
+        grads[i] = at::empty_symint(t[i].sym_sizes(), t[i].options());
+      }
+    const bool weights = task_should_compute_output(2) || task_should_compute_output(3);
+    auto [dq, dk, wq, wk] = qk_norm_rotary_bwd_call(grads[0], grads[1], t[0], t[1], t[2], t[3], t[4], t[5], layout, mscale, eps, weights);
+    auto asked = [&](int i, bool has, const Tensor& x) { return has && task_should_compute_output(i) ? x : Tensor(); };
+    return {asked(0, has_q, dq), asked(1, has_k, dk), asked(2, has_q, wq), asked(3, has_k, wk)};
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& s : saved) s.reset_data();
+  }
+  std::string name() const override { return "QkNormRotaryBackward"; }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
+                                                   const Tensor& positions, const Tensor& inv_freq, c10::string_view layout,
+                                                   double mscale, double eps) {
+  const Tensor* const in[6] = {&q, &k, &q_weight, &k_weight, &positions, &inv_freq};
+  const bool grad = c10::GradMode::is_enabled();
+  TORCH_CHECK(!grad || !inv_freq.requires_grad(), "prunepath.qk_norm_rotary: no gradient in inv_freq");
+  for (const Tensor* t : in) TORCH_CHECK(!t->_fw_grad(0).defined(), "prunepath.qk_norm_rotary: no forward-mode gradient");
+  std::shared_ptr<QkNormBackward> node;
+  if (grad && (q.requires_grad() || k.requires_grad() || q_weight.requires_grad() || k_weight.requires_grad())) {
+    node = std::shared_ptr<QkNormBackward>(new QkNormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(q, k, q_weight, k_weight));
+    for (int i = 0; i < 6; ++i) node->saved[i] = torch::autograd::SavedVariable(*in[i], false);
+    node->layout = std::string(layout), node->mscale = mscale, node->eps = eps;
+  }
+  std::tuple<Tensor, Tensor> y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    y = qk_norm_rotary_call(q, k, q_weight, k_weight, positions, inv_freq, layout, mscale, eps);
+  }
+  if (node) {
+    torch::autograd::set_history(std::get<0>(y), node);
+    torch::autograd::set_history(std::get<1>(y), node);
+  }
+  return y;
+}
+
 // ------------------------------------------------------------------ paged cache
 // Heads, D and the cache of a call: shapes, types and what the kernels take of them.
-void paged_check(const char* name, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                 const Tensor& kv_lens, const Tensor& cu_q, const c10::SymInt& Hq, const c10::SymInt& D) {
-  TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
-                  v_pages.scalar_type() == at::kBFloat16,
-              "prunepath.", name, ": k_pages [pages, kv_heads, page, D] and v_pages [pages, kv_heads, D, page] bfloat16 required");
-  TORCH_SYM_CHECK(k_pages.sym_size(3).sym_eq(D).sym_and(v_pages.sym_size(2).sym_eq(D))
+void paged_check(const char* name, const Tensor& k_pages, const Tensor& v_pages, const optional<Tensor>& k_scales,
+                 const optional<Tensor>& v_scales, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                 const c10::SymInt& Hq, const c10::SymInt& D) {
+  TORCH_CHECK(k_scales.has_value() == v_scales.has_value(), "prunepath.", name, ": scales of keys and of values belong together");
+  if (k_scales) {
+    TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 5 && k_pages.scalar_type() == at::kFloat8_e4m3fn &&
+                    v_pages.scalar_type() == at::kFloat8_e4m3fn,
+                "prunepath.", name, ": with scales k_pages [pages, kv_heads, page, D] and v_pages [pages, kv_heads, page / 16, D, 16] "
+                "float8_e4m3fn required");
+    TORCH_CHECK(k_scales->dim() == 3 && v_scales->dim() == 3 && k_scales->scalar_type() == at::kFloat8_e8m0fnu &&
+                    v_scales->scalar_type() == at::kFloat8_e8m0fnu,
+                "prunepath.", name, ": scales must be float8_e8m0fnu [pages, kv_heads, page / 16]");
+    const c10::SymInt blocks = v_pages.sym_size(2);
+    TORCH_SYM_CHECK(k_pages.sym_size(3).sym_eq(D).sym_and(v_pages.sym_size(3).sym_eq(D)).sym_and(v_pages.sym_size(4).sym_eq(16))
+                        .sym_and(k_pages.sym_size(2).sym_eq(blocks * 16)).sym_and(v_pages.sym_size(0).sym_eq(k_pages.sym_size(0)))
+                        .sym_and(v_pages.sym_size(1).sym_eq(k_pages.sym_size(1))),
+                    "prunepath.", name, ": shapes of k_pages ", k_pages.sym_sizes(), ", v_pages ", v_pages.sym_sizes(),
+                    " and head size ", D, " disagree");
+    for (const Tensor* s : {&*k_scales, &*v_scales})
+      TORCH_SYM_CHECK(s->sym_size(0).sym_eq(k_pages.sym_size(0)).sym_and(s->sym_size(1).sym_eq(k_pages.sym_size(1)))
+                          .sym_and(s->sym_size(2).sym_eq(blocks)),
+                      "prunepath.", name, ": scales ", s->sym_sizes(), " for pages ", k_pages.sym_sizes());
+  } else {
+    TORCH_CHECK(k_pages.dim() == 4 && v_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
+                    v_pages.scalar_type() == at::kBFloat16,
+                "prunepath.", name, ": k_pages [pages, kv_heads, page, D] and v_pages [pages, kv_heads, D, page] bfloat16 required");
+  }
+  if (!k_scales) TORCH_SYM_CHECK(k_pages.sym_size(3).sym_eq(D).sym_and(v_pages.sym_size(2).sym_eq(D))
                       .sym_and(v_pages.sym_size(0).sym_eq(k_pages.sym_size(0)))
                       .sym_and(v_pages.sym_size(1).sym_eq(k_pages.sym_size(1)))
                       .sym_and(v_pages.sym_size(3).sym_eq(k_pages.sym_size(2))),
@@ -668,7 +884,8 @@ Paged paged_sizes(const char* name, const Tensor& k_pages, const Tensor& block_t
 // q and q_out: a tensor or nullptr
 void kv_append_check(const Tensor* q, const Tensor* q_out, const Tensor& k, const Tensor& v, const Tensor& k_pages,
                      const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                     const optional<Tensor>& inv_freq) {
+                     const optional<Tensor>& inv_freq, const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
+                     const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
   const char* const name = "kv_append";
   x_code(k, name);
   TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.scalar_type() == v.scalar_type() && same_sizes(k, v, 3),
@@ -678,7 +895,17 @@ void kv_append_check(const Tensor* q, const Tensor* q_out, const Tensor& k, cons
                     q->sym_size(0).sym_eq(k.sym_size(0)).sym_and(q->sym_size(2).sym_eq(k.sym_size(2)))
                         .sym_and(q->sym_stride(2).sym_eq(1)).expect_true(__FILE__, __LINE__),
                 "prunepath.kv_append: q must be [N, heads, D] of k's dtype, channels contiguous");
-  paged_check(name, k_pages, v_pages, block_table, kv_lens, cu_q, q ? q->sym_size(1) : c10::SymInt(0), k.sym_size(2));
+  paged_check(name, k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, cu_q, q ? q->sym_size(1) : c10::SymInt(0), k.sym_size(2));
+  TORCH_CHECK(q ? q_weight.has_value() == k_weight.has_value() : !q_weight.has_value(),
+              "prunepath.kv_append: norms of queries and of keys belong together");
+  for (const optional<Tensor>* w : {&q_weight, &k_weight})
+    if (*w) {
+      TORCH_CHECK((*w)->dim() == 1 && ((*w)->scalar_type() == at::kFloat || (*w)->scalar_type() == k.scalar_type()) &&
+                      (*w)->scalar_type() == (*k_weight).scalar_type(),
+                  "prunepath.kv_append: weights must be [D], both float32 or both like k");
+      TORCH_SYM_CHECK((*w)->sym_size(0).sym_eq(k.sym_size(2)), "prunepath.kv_append: ", (*w)->sym_size(0), " weights for heads of ",
+                      k.sym_size(2), " channels");
+    }
   TORCH_SYM_CHECK(k.sym_size(1).sym_eq(k_pages.sym_size(1)), "prunepath.kv_append: ", k.sym_size(1),
                   " heads for a cache of ", k_pages.sym_size(1));
   TORCH_SYM_CHECK(k.sym_stride(2).sym_eq(1).sym_and(v.sym_stride(2).sym_eq(1)),
@@ -699,141 +926,255 @@ void kv_append_check(const Tensor* q, const Tensor* q_out, const Tensor& k, cons
 void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bool zero_tail, const Tensor& k,
                     const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
                     const Tensor& kv_lens, const Tensor& cu_q, const optional<Tensor>& inv_freq,
-                    c10::string_view layout, double mscale) {
+                    c10::string_view layout, double mscale, const optional<Tensor>& q_weight,
+                    const optional<Tensor>& k_weight, double eps, const optional<Tensor>& k_scales,
+                    const optional<Tensor>& v_scales) {
   const char* const name = "kv_append";
   const int lay = rotary_layout(layout, name);
-  kv_append_check(q ? &*q : nullptr, q ? &*q_out : nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+  kv_append_check(q ? &*q : nullptr, q ? &*q_out : nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, q_weight,
+                  k_weight, k_scales, v_scales);
+  auto given = [](const optional<Tensor>& t) { return t ? &*t : nullptr; };
   const Paged p = paged_sizes(name, k_pages, block_table, k.size(0), q ? q->size(1) : 0);
-  need_gpu(name, k, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, inv_freq ? &*inv_freq : nullptr});
+  need_gpu(name, k, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, given(inv_freq), given(q_weight), given(k_weight),
+                     given(k_scales), given(v_scales)});
   same_device(name, k, {&k, &v});
   const Span sk(k), sv(v), kp(k_pages), vp(v_pages), st(block_table), sl(kv_lens), sc(cu_q);
-  const Span sf = inv_freq ? Span(*inv_freq) : st;
-  for (const Span* in : {&sk, &sv, &st, &sl, &sc, &sf}) {
+  auto span = [&](const optional<Tensor>& t) { return t ? Span(*t) : st; };
+  const Span sf = span(inv_freq), sqw = span(q_weight), skw = span(k_weight);
+  std::vector<const Span*> reads = {&sk, &sv, &st, &sl, &sc, &sf, &sqw, &skw};
+  for (const Span* in : reads) {
     apart(name, kp, *in);
     apart(name, vp, *in);
   }
   apart(name, kp, vp);
+  const Span ks8 = k_scales ? Span(*k_scales) : kp, vs8 = v_scales ? Span(*v_scales) : vp;
+  if (k_scales) {
+    for (const Span* in : reads) {
+      apart(name, ks8, *in);
+      apart(name, vs8, *in);
+    }
+    for (const Span* pages : {&kp, &vp}) {
+      apart(name, ks8, *pages);
+      apart(name, vs8, *pages);
+    }
+    apart(name, ks8, vs8);
+  }
   int64_t qs[2] = {0, 0};
   if (q) {
     same_device(name, k, {&*q, &*q_out});
     const Span sq(*q);
-    apart(name, kp, sq);
-    apart(name, vp, sq);
+    for (const Span* out : {&kp, &vp, &ks8, &vs8}) apart(name, *out, sq);
     if (!zero_tail) {  // a given q_out
       const Span so(*q_out);
-      for (const Span* in : {&sk, &sv, &kp, &vp, &st, &sl, &sc, &sf}) apart(name, so, *in);
+      for (const Span* out : {&kp, &vp, &ks8, &vs8}) apart(name, so, *out);
+      for (const Span* in : reads) apart(name, so, *in);
       if (!same_rows(*q_out, *q)) apart(name, so, sq);
     }
     qs[0] = step(*q, 0), qs[1] = step(*q, 1);
   }
   const c10::DeviceGuard g(k.device());
   const int64_t ks[2] = {step(k, 0), step(k, 1)}, vs[2] = {step(v, 0), step(v, 1)};
-  check_rc(pp_kv_append(q ? q->data_ptr() : nullptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, x_code(k, name), p.n,
-                        (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
-                        block_table.data_ptr<int32_t>(), (int)p.max_pages, (int)p.pages, (int)p.page, (int)p.Hq,
-                        (int)p.Hkv, (int)p.D, (const double*)ptr(inv_freq), inv_freq ? (int)(2 * inv_freq->numel()) : 0,
-                        lay, (float)mscale, k_pages.data_ptr(), v_pages.data_ptr(), q ? q_out->data_ptr() : nullptr,
-                        zero_tail, stream_of(k)),
+  check_rc(pp_kv_append_with(q ? q->data_ptr() : nullptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, x_code(k, name), p.n,
+                             (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
+                             block_table.data_ptr<int32_t>(), (int)p.max_pages, (int)p.pages, (int)p.page, (int)p.Hq,
+                             (int)p.Hkv, (int)p.D, (const double*)ptr(inv_freq), inv_freq ? (int)(2 * inv_freq->numel()) : 0,
+                             lay, (float)mscale, ptr(q_weight), ptr(k_weight), k_weight ? w_code(*k_weight, name) : 0, (float)eps,
+                             k_pages.data_ptr(), v_pages.data_ptr(), (void*)ptr(k_scales), (void*)ptr(v_scales),
+                             q ? q_out->data_ptr() : nullptr, zero_tail, stream_of(k)),
            name);
 }
 
 void kv_append_gpu(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                    const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                   const optional<Tensor>& inv_freq, c10::string_view layout, double mscale) {
+                   const optional<Tensor>& inv_freq, c10::string_view layout, double mscale, const optional<Tensor>& k_weight, double eps,
+                   const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
   kv_append_into(c10::nullopt, c10::nullopt, false, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq,
-                 layout, mscale);
+                 layout, mscale, c10::nullopt, k_weight, eps, k_scales, v_scales);
 }
 
 Tensor kv_append_q_gpu(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                        const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                       const optional<Tensor>& inv_freq, c10::string_view layout, double mscale) {
+                       const optional<Tensor>& inv_freq, c10::string_view layout, double mscale, const optional<Tensor>& q_weight,
+                       const optional<Tensor>& k_weight, double eps, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
   Tensor out = at::empty(q.sizes(), q.options().dtype(at::kBFloat16));
-  kv_append_into(q, out, true, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale);
+  kv_append_into(q, out, true, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale, q_weight, k_weight, eps,
+                 k_scales, v_scales);
   return out;
 }
 
 void kv_append_q_into_gpu(const Tensor& q, const Tensor& q_out, const Tensor& k, const Tensor& v, const Tensor& k_pages,
                           const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                          const optional<Tensor>& inv_freq, c10::string_view layout, double mscale) {
-  kv_append_into(q, q_out, false, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale);
+                          const optional<Tensor>& inv_freq, c10::string_view layout, double mscale, const optional<Tensor>& q_weight,
+                          const optional<Tensor>& k_weight, double eps, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
+  kv_append_into(q, q_out, false, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale, q_weight, k_weight,
+                 eps, k_scales, v_scales);
 }
 
 void kv_append_meta(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                     const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                    const optional<Tensor>& inv_freq, c10::string_view layout, double) {
+                    const optional<Tensor>& inv_freq, c10::string_view layout, double, const optional<Tensor>& k_weight, double,
+                    const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
   rotary_layout(layout, "kv_append");
-  kv_append_check(nullptr, nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+  kv_append_check(nullptr, nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, c10::nullopt, k_weight, k_scales,
+                  v_scales);
 }
 Tensor kv_append_q_meta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                         const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                        const optional<Tensor>& inv_freq, c10::string_view layout, double) {
+                        const optional<Tensor>& inv_freq, c10::string_view layout, double, const optional<Tensor>& q_weight,
+                        const optional<Tensor>& k_weight, double, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
   rotary_layout(layout, "kv_append");
-  kv_append_check(&q, nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+  kv_append_check(&q, nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, q_weight, k_weight, k_scales, v_scales);
   return at::empty_symint(q.sym_sizes(), q.options().dtype(at::kBFloat16));
 }
 void kv_append_q_into_meta(const Tensor& q, const Tensor& q_out, const Tensor& k, const Tensor& v, const Tensor& k_pages,
                            const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
-                           const optional<Tensor>& inv_freq, c10::string_view layout, double) {
+                           const optional<Tensor>& inv_freq, c10::string_view layout, double, const optional<Tensor>& q_weight,
+                           const optional<Tensor>& k_weight, double, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
   rotary_layout(layout, "kv_append");
-  kv_append_check(&q, &q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq);
+  kv_append_check(&q, &q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, q_weight, k_weight, k_scales, v_scales);
+}
+
+// ------------------------------------------------------------------ read
+void read_check(const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+                const c10::SymInt& rows, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
+  TORCH_CHECK(k_pages.dim() == 4, "prunepath.kv_read: k_pages must be [pages, kv_heads, page, D]");
+  paged_check("kv_read", k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, cu_q, c10::SymInt(0), k_pages.sym_size(3));
+  TORCH_SYM_CHECK(rows.sym_ge(0), "prunepath.kv_read: ", rows, " rows");
+}
+void read_check_out(const Tensor& k_pages, const Tensor& k_out, const Tensor& v_out) {
+  for (const Tensor* t : {&k_out, &v_out}) {
+    TORCH_CHECK(t->dim() == 3 && t->scalar_type() == at::kBFloat16 && t->is_contiguous(),
+                "prunepath.kv_read: results must be contiguous bfloat16 [rows, kv_heads, D]");
+    TORCH_SYM_CHECK(t->sym_size(0).sym_eq(k_out.sym_size(0)).sym_and(t->sym_size(1).sym_eq(k_pages.sym_size(1)))
+                        .sym_and(t->sym_size(2).sym_eq(k_pages.sym_size(3))),
+                    "prunepath.kv_read: results ", t->sym_sizes(), " for pages ", k_pages.sym_sizes());
+  }
+}
+
+void read_into(const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens, const Tensor& cu_q,
+               const Tensor& k_out, const Tensor& v_out, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales,
+               bool zero_tail) {
+  const char* const name = "kv_read";
+  const Paged p = paged_sizes(name, k_pages, block_table, k_out.size(0), 0);
+  need_gpu(name, k_pages, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &k_out, &v_out, k_scales ? &*k_scales : nullptr,
+                           v_scales ? &*v_scales : nullptr});
+  if (!zero_tail) {  // given results
+    const Span ko(k_out), vo(v_out);
+    apart(name, ko, vo);
+    for (const Tensor* in : {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, k_scales ? &*k_scales : &k_pages,
+                             v_scales ? &*v_scales : &v_pages}) {
+      apart(name, ko, Span(*in));
+      apart(name, vo, Span(*in));
+    }
+  }
+  const c10::DeviceGuard g(k_pages.device());
+  check_rc(pp_kv_read(k_pages.data_ptr(), v_pages.data_ptr(), ptr(k_scales), ptr(v_scales), p.n, (int)p.seqs,
+                      cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(), (int)p.max_pages,
+                      (int)p.pages, (int)p.page, (int)p.Hkv, (int)p.D, k_out.data_ptr(), v_out.data_ptr(), zero_tail,
+                      stream_of(k_pages)),
+           name);
+}
+
+std::tuple<Tensor, Tensor> kv_read_gpu(const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                                       const Tensor& kv_lens, const Tensor& cu_q, c10::SymInt rows,
+                                       const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
+  read_check(k_pages, v_pages, block_table, kv_lens, cu_q, rows, k_scales, v_scales);
+  const int64_t n = rows.guard_int(__FILE__, __LINE__);
+  auto bf = k_pages.options().dtype(at::kBFloat16);
+  Tensor k = at::empty({n, k_pages.size(1), k_pages.size(3)}, bf), v = at::empty_like(k);
+  read_into(k_pages, v_pages, block_table, kv_lens, cu_q, k, v, k_scales, v_scales, true);
+  return {k, v};
+}
+void kv_read_into_gpu(const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens,
+                      const Tensor& cu_q, const Tensor& k_out, const Tensor& v_out, const optional<Tensor>& k_scales,
+                      const optional<Tensor>& v_scales) {
+  read_check(k_pages, v_pages, block_table, kv_lens, cu_q, 0, k_scales, v_scales);
+  read_check_out(k_pages, k_out, v_out);
+  read_into(k_pages, v_pages, block_table, kv_lens, cu_q, k_out, v_out, k_scales, v_scales, false);
+}
+std::tuple<Tensor, Tensor> kv_read_meta(const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                                        const Tensor& kv_lens, const Tensor& cu_q, c10::SymInt rows,
+                                        const optional<Tensor>& k_scales, const optional<Tensor>& v_scales) {
+  read_check(k_pages, v_pages, block_table, kv_lens, cu_q, rows, k_scales, v_scales);
+  auto bf = k_pages.options().dtype(at::kBFloat16);
+  const std::vector<c10::SymInt> shape = {rows, k_pages.sym_size(1), k_pages.sym_size(3)};
+  return {at::empty_symint(shape, bf), at::empty_symint(shape, bf)};
+}
+void kv_read_into_meta(const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table, const Tensor& kv_lens,
+                       const Tensor& cu_q, const Tensor& k_out, const Tensor& v_out, const optional<Tensor>& k_scales,
+                       const optional<Tensor>& v_scales) {
+  read_check(k_pages, v_pages, block_table, kv_lens, cu_q, 0, k_scales, v_scales);
+  read_check_out(k_pages, k_out, v_out);
 }
 
 // out: a tensor or nullptr
 void attention_check(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                     const Tensor& kv_lens, const Tensor& cu_q, const Tensor* out) {
+                     const Tensor& kv_lens, const Tensor& cu_q, const optional<Tensor>& k_scales, const optional<Tensor>& v_scales,
+                     int64_t window, int64_t sinks, const Tensor* out) {
   TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.sym_stride(2).sym_eq(1).expect_true(__FILE__, __LINE__),
               "prunepath.paged_attention: q must be bfloat16 [N, heads, D], channels contiguous");
   if (out)
     TORCH_CHECK(out->scalar_type() == at::kBFloat16 && out->dim() == 3 && same_sizes(*out, q, 3) && out->is_contiguous(),
                 "prunepath.paged_attention: out must be contiguous bfloat16 of q's shape");
-  paged_check("paged_attention", k_pages, v_pages, block_table, kv_lens, cu_q, q.sym_size(1), q.sym_size(2));
+  TORCH_CHECK(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "prunepath.paged_attention: a window of ", window, " tokens and ",
+              sinks, " first ones (a window of at least 1, and first tokens only beside one; 0 and 0: none)");
+  paged_check("paged_attention", k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, cu_q, q.sym_size(1), q.sym_size(2));
 }
 
 void attention_into(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                    const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out, bool zero_tail) {
+                    const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out, bool zero_tail,
+                    const optional<Tensor>& k_scales, const optional<Tensor>& v_scales, int64_t window, int64_t sinks) {
   const char* const name = "paged_attention";
-  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, &out);
+  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, k_scales, v_scales, window, sinks, &out);
   const Paged p = paged_sizes(name, k_pages, block_table, q.size(0), q.size(1));
-  need_gpu(name, q, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &out});
+  need_gpu(name, q, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, &out, k_scales ? &*k_scales : nullptr,
+                     v_scales ? &*v_scales : nullptr});
   same_device(name, q, {&q});
   if (!zero_tail) {  // a given out
     const Span so(out);
-    for (const Tensor* in : {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q}) apart(name, so, Span(*in));
+    for (const Tensor* in : {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, k_scales ? &*k_scales : &k_pages,
+                             v_scales ? &*v_scales : &v_pages})
+      apart(name, so, Span(*in));
     if (!same_rows(out, q)) apart(name, so, Span(q));
   }
   const c10::DeviceGuard g(q.device());
-  const size_t need = pp_paged_attention_workspace_bytes(p.n, (int)p.seqs, (int)p.max_pages, (int)p.page, (int)p.Hq,
-                                                         (int)p.Hkv, (int)p.D);
+  const size_t need = pp_paged_attention_with_workspace_bytes(p.n, (int)p.seqs, (int)p.max_pages, (int)p.page, (int)p.Hq,
+                                                              (int)p.Hkv, (int)p.D, k_scales.has_value(), window, sinks);
   Tensor ws;
   if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
   const int64_t qs[2] = {step(q, 0), step(q, 1)};
-  check_rc(pp_paged_attention(q.data_ptr(), qs, p.n, (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
-                              block_table.data_ptr<int32_t>(), (int)p.max_pages, k_pages.data_ptr(), v_pages.data_ptr(),
-                              (int)p.pages, (int)p.page, (int)p.Hq, (int)p.Hkv, (int)p.D, (float)scale, out.data_ptr(),
-                              zero_tail, need ? ws.data_ptr() : nullptr, need, stream_of(q)),
+  check_rc(pp_paged_attention_with(q.data_ptr(), qs, p.n, (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
+                                   block_table.data_ptr<int32_t>(), (int)p.max_pages, k_pages.data_ptr(), v_pages.data_ptr(),
+                                   ptr(k_scales), ptr(v_scales), (int)p.pages, (int)p.page, (int)p.Hq, (int)p.Hkv, (int)p.D,
+                                   (float)scale, window, sinks, out.data_ptr(), zero_tail, need ? ws.data_ptr() : nullptr, need,
+                                   stream_of(q)),
            name);
 }
 
 void paged_attention_into_gpu(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                              const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out) {
-  attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale, out, false);
+                              const Tensor& kv_lens, const Tensor& cu_q, double scale, const Tensor& out, const optional<Tensor>& k_scales,
+                              const optional<Tensor>& v_scales, int64_t window, int64_t sinks) {
+  attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale, out, false, k_scales, v_scales, window, sinks);
 }
 
 Tensor paged_attention_gpu(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                           const Tensor& kv_lens, const Tensor& cu_q, double scale) {
+                           const Tensor& kv_lens, const Tensor& cu_q, double scale, const optional<Tensor>& k_scales,
+                           const optional<Tensor>& v_scales, int64_t window, int64_t sinks) {
   Tensor out = at::empty(q.sizes(), q.options());
-  attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale, out, true);
+  attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale, out, true, k_scales, v_scales, window, sinks);
   return out;
 }
 
 Tensor paged_attention_meta(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                            const Tensor& kv_lens, const Tensor& cu_q, double) {
-  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, nullptr);
+                            const Tensor& kv_lens, const Tensor& cu_q, double, const optional<Tensor>& k_scales,
+                            const optional<Tensor>& v_scales, int64_t window, int64_t sinks) {
+  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, k_scales, v_scales, window, sinks, nullptr);
   return at::empty_symint(q.sym_sizes(), q.options());
 }
 void paged_attention_into_meta(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
-                               const Tensor& kv_lens, const Tensor& cu_q, double, const Tensor& out) {
-  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, &out);
+                               const Tensor& kv_lens, const Tensor& cu_q, double, const Tensor& out, const optional<Tensor>& k_scales,
+                               const optional<Tensor>& v_scales, int64_t window, int64_t sinks) {
+  attention_check(q, k_pages, v_pages, block_table, kv_lens, cu_q, k_scales, v_scales, window, sinks, &out);
 }
 
 // ------------------------------------------------------------------ ops for inference
@@ -901,6 +1242,20 @@ constexpr auto written(R (*)(A...)) {
   return &Written<Op, numbers, R, A...>::call;
 }
 
+// The gradient of qk_norm_rotary has none of its own.
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd_autograd(const Tensor& dq, const Tensor& dk,
+                                                                       const Tensor& q, const Tensor& k, const Tensor& q_weight,
+                                                                       const Tensor& k_weight, const Tensor& positions,
+                                                                       const Tensor& inv_freq, c10::string_view layout,
+                                                                       double mscale, double eps, bool weights) {
+  for (const Tensor* t : {&dq, &dk, &q, &k, &q_weight, &k_weight, &inv_freq}) {
+    TORCH_CHECK(!t->_fw_grad(0).defined(), "prunepath.qk_norm_rotary_bwd: no forward-mode gradient");
+    TORCH_CHECK(!c10::GradMode::is_enabled() || !t->requires_grad(), "prunepath.qk_norm_rotary: no second derivative");
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return qk_norm_rotary_bwd_call(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, layout, mscale, eps, weights);
+}
+
 #define INFERENCE(m, op)                        \
   do {                                          \
     struct Op {                                 \
@@ -949,17 +1304,30 @@ TORCH_LIBRARY(prunepath, m) {
         "bool need_d_inter=True) -> (Tensor d_inter, Tensor d_gates)");
   m.def("rotary(Tensor x, Tensor positions, Tensor inv_freq, str layout='half', float mscale=1.0, bool inverse=False) "
         "-> Tensor");
+  m.def("qk_norm_rotary(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
+        "str layout='half', float mscale=1.0, float eps=1e-06) -> (Tensor q, Tensor k)");
+  m.def("qk_norm_rotary_bwd(Tensor dq, Tensor dk, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor positions, "
+        "Tensor inv_freq, str layout='half', float mscale=1.0, float eps=1e-06, bool weights=True) -> "
+        "(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight)");
   m.def("kv_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor block_table, Tensor kv_lens, "
-        "Tensor cu_q, Tensor? inv_freq=None, str layout='half', float mscale=1.0) -> ()");
+        "Tensor cu_q, Tensor? inv_freq=None, str layout='half', float mscale=1.0, Tensor? k_weight=None, float eps=1e-06, "
+        "Tensor(d!)? k_scales=None, Tensor(e!)? v_scales=None) -> ()");
   m.def("kv_append_q(Tensor q, Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor block_table, "
-        "Tensor kv_lens, Tensor cu_q, Tensor? inv_freq=None, str layout='half', float mscale=1.0) -> Tensor");
+        "Tensor kv_lens, Tensor cu_q, Tensor? inv_freq=None, str layout='half', float mscale=1.0, Tensor? q_weight=None, "
+        "Tensor? k_weight=None, float eps=1e-06, Tensor(d!)? k_scales=None, Tensor(e!)? v_scales=None) -> Tensor");
   m.def("kv_append_q_into(Tensor q, Tensor(c!) q_out, Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, "
         "Tensor block_table, Tensor kv_lens, Tensor cu_q, Tensor? inv_freq=None, str layout='half', "
-        "float mscale=1.0) -> ()");
+        "float mscale=1.0, Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-06, Tensor(d!)? k_scales=None, "
+        "Tensor(e!)? v_scales=None) -> ()");
+  m.def("kv_read(Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor kv_lens, Tensor cu_q, SymInt rows, "
+        "Tensor? k_scales=None, Tensor? v_scales=None) -> (Tensor k, Tensor v)");
+  m.def("kv_read_into(Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor kv_lens, Tensor cu_q, Tensor(a!) k_out, "
+        "Tensor(b!) v_out, Tensor? k_scales=None, Tensor? v_scales=None) -> ()");
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor kv_lens, Tensor cu_q, "
-        "float scale) -> Tensor");
+        "float scale, Tensor? k_scales=None, Tensor? v_scales=None, int window=0, int sinks=0) -> Tensor");
   m.def("paged_attention_into(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor kv_lens, "
-        "Tensor cu_q, float scale, Tensor(a!) out) -> ()");
+        "Tensor cu_q, float scale, Tensor(a!) out, Tensor? k_scales=None, Tensor? v_scales=None, int window=0, "
+        "int sinks=0) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CUDA, m) {
@@ -978,9 +1346,13 @@ TORCH_LIBRARY_IMPL(prunepath, CUDA, m) {
   m.impl("masked_gate", &masked_gate_gpu);
   m.impl("masked_gate_bwd", &masked_gate_bwd_gpu);
   m.impl("rotary", &rotary_gpu);
+  m.impl("qk_norm_rotary", &qk_norm_rotary_gpu);
+  m.impl("qk_norm_rotary_bwd", &qk_norm_rotary_bwd_gpu);
   m.impl("kv_append", &kv_append_gpu);
   m.impl("kv_append_q", &kv_append_q_gpu);
   m.impl("kv_append_q_into", &kv_append_q_into_gpu);
+  m.impl("kv_read", &kv_read_gpu);
+  m.impl("kv_read_into", &kv_read_into_gpu);
   m.impl("paged_attention", &paged_attention_gpu);
   m.impl("paged_attention_into", &paged_attention_into_gpu);
 }
@@ -1001,18 +1373,26 @@ TORCH_LIBRARY_IMPL(prunepath, Meta, m) {
   m.impl("masked_gate", &masked_gate_meta);
   m.impl("masked_gate_bwd", &masked_gate_bwd_meta);
   m.impl("rotary", &rotary_meta);
+  m.impl("qk_norm_rotary", &qk_norm_rotary_meta);
+  m.impl("qk_norm_rotary_bwd", &qk_norm_rotary_bwd_meta);
   m.impl("kv_append", &kv_append_meta);
   m.impl("kv_append_q", &kv_append_q_meta);
   m.impl("kv_append_q_into", &kv_append_q_into_meta);
+  m.impl("kv_read", &kv_read_meta);
+  m.impl("kv_read_into", &kv_read_into_meta);
   m.impl("paged_attention", &paged_attention_meta);
   m.impl("paged_attention_into", &paged_attention_into_meta);
 }
 
 TORCH_LIBRARY_IMPL(prunepath, Autograd, m) {
   m.impl("rotary", &rotary_autograd);
+  m.impl("qk_norm_rotary", &qk_norm_rotary_autograd);
+  m.impl("qk_norm_rotary_bwd", &qk_norm_rotary_bwd_autograd);
   INFERENCE(m, kv_append);
   INFERENCE(m, kv_append_q);
   INFERENCE(m, kv_append_q_into);
+  INFERENCE(m, kv_read);
+  INFERENCE(m, kv_read_into);
   INFERENCE(m, paged_attention);
   INFERENCE(m, paged_attention_into);
 }
@@ -1024,16 +1404,18 @@ TORCH_LIBRARY_IMPL(prunepath, ADInplaceOrView, m) {
   WRITES(m, moe_decode_batch, moe_decode_batch_gpu, 1 << 7 | 1 << 8);
   WRITES(m, moe_decode_batch_into, decode_batch_into, 1 << 7 | 1 << 8 | 1 << 9 | 1 << 10 | 1 << 11);
   WRITES(m, moe_prefill_into, prefill_into, 1 << 7 | 1 << 8 | 1 << 9 | 1 << 10);
-  WRITES(m, kv_append, kv_append_gpu, 1 << 2 | 1 << 3);
-  WRITES(m, kv_append_q, kv_append_q_gpu, 1 << 3 | 1 << 4);
-  WRITES(m, kv_append_q_into, kv_append_q_into_gpu, 1 << 1 | 1 << 4 | 1 << 5);
+  WRITES(m, kv_append, kv_append_gpu, 1 << 2 | 1 << 3 | 1 << 12 | 1 << 13);
+  WRITES(m, kv_append_q, kv_append_q_gpu, 1 << 3 | 1 << 4 | 1 << 14 | 1 << 15);
+  WRITES(m, kv_append_q_into, kv_append_q_into_gpu, 1 << 1 | 1 << 4 | 1 << 5 | 1 << 15 | 1 << 16);
+  WRITES(m, kv_read_into, kv_read_into_gpu, 1 << 5 | 1 << 6);
   WRITES(m, paged_attention_into, paged_attention_into_gpu, 1 << 7);
 }
 
 TORCH_LIBRARY_IMPL(prunepath, CPU, m) {
   for (const char* name : {"route", "route_logits", "bucket", "pack_experts", "pack_router", "decode_workspace_init",
                            "moe_decode", "moe_decode_into", "moe_decode_batch", "moe_decode_batch_into",
-                           "moe_prefill", "moe_prefill_into", "masked_gate", "masked_gate_bwd", "rotary", "kv_append",
-                           "kv_append_q", "kv_append_q_into", "paged_attention", "paged_attention_into"})
+                           "moe_prefill", "moe_prefill_into", "masked_gate", "masked_gate_bwd", "rotary",
+                           "qk_norm_rotary", "qk_norm_rotary_bwd", "kv_append", "kv_append_q", "kv_append_q_into", "kv_read",
+                           "kv_read_into", "paged_attention", "paged_attention_into"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&refuse_cpu>());
 }

@@ -385,6 +385,18 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
     return L.torch_ops().rotary(x, positions, inv_freq, layout, mscale, False)
 
 
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                   positions: torch.Tensor, inv_freq: torch.Tensor, layout: str = "half", mscale: float = 1.0,
+                   eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, k) with every head normed, x / sqrt(mean(x^2) + eps) times a weight for each channel, and turned as by
+    ``rotary``, in one launch (``torch.ops.prunepath.qk_norm_rotary``). q [N, heads, D] and k [N, kv_heads, D], or
+    [B, L, heads, D] and [B, L, kv_heads, D], fp32 or bf16, any strides (parts of a joint projection's rows); the weights
+    [D], both fp32 or both of q's dtype; D from 2 to 256; positions and inv_freq as ``rotary`` takes them. Computed in fp32,
+    rounded once. New contiguous tensors of q's dtype; differentiable once, in q, k and the weights, whose gradients are
+    sums in a fixed order (capture a backward, as any, with no eager graph of the same leaves alive)."""
+    return L.torch_ops().qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, layout, mscale, eps)
+
+
 # ----------------------------------------------------------------------------- paged cache
 def paged_cache(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device=None):
     """(k_pages [num_pages, kv_heads, page_size, head_dim], v_pages [num_pages, kv_heads, head_dim,
@@ -394,10 +406,28 @@ def paged_cache(num_pages: int, page_size: int, kv_heads: int, head_dim: int, de
     return k, torch.empty(num_pages, kv_heads, head_dim, page_size, dtype=torch.bfloat16, device=device)
 
 
+def paged_cache8(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device=None):
+    """((k_pages, v_pages), scales): a cache of 8 bits, float8_e4m3fn, for ``kv_append``, ``kv_read`` and ``paged_attention``
+    with ``scales=scales``. k_pages [num_pages, kv_heads, page_size, head_dim], v_pages [num_pages, kv_heads, page_size / 16,
+    head_dim, 16] (a channel's 16 tokens next to each other), scales = (k_scales, v_scales), each [num_pages, kv_heads,
+    page_size / 16] float8_e8m0fnu: a power of two for each block of 16 tokens and head. Uninitialised, sizes as of
+    ``paged_cache``."""
+    blocks = page_size // 16
+    k = torch.empty(num_pages, kv_heads, page_size, head_dim, dtype=torch.float8_e4m3fn, device=device)
+    v = torch.empty(num_pages, kv_heads, blocks, head_dim, 16, dtype=torch.float8_e4m3fn, device=device)
+    ks, vs = (torch.empty(num_pages, kv_heads, blocks, dtype=torch.float8_e8m0fnu, device=device) for _ in range(2))
+    return (k, v), (ks, vs)
+
+
+Scales = Optional[Tuple[torch.Tensor, torch.Tensor]]
+
+
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
               block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor,
               inv_freq: Optional[torch.Tensor] = None, layout: str = "half", mscale: float = 1.0,
-              q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+              q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+              q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              scales: Scales = None) -> Optional[torch.Tensor]:
     """Appends the new tokens' k and v [N, kv_heads, D] (fp32 or bf16, rows may be parts of a joint
     projection's) to the paged cache, k turned by its position (``rotary``; inv_freq None: as it
     is), in one launch (``torch.ops.prunepath.kv_append`` and ``kv_append_q``).
@@ -409,23 +439,55 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
 
     q [N, heads, D]: turned as k is, returned as bf16 [N, heads, D] (in ``q_out``, which may be q
     itself, if given; other overlaps of what is written are refused). Rows behind cu_q[seqs] append
-    nothing; in a new result they are zeros, in q_out they stay. Inference only: arguments that require
-    a gradient are refused outside torch.no_grad(), tangents always."""
+    nothing; in a new result they are zeros, in q_out they stay.
+
+    q_weight and k_weight [D] (fp32, or k's dtype; k_weight alone without q): the heads of q and k are normed, as by
+    ``qk_norm_rotary``, before they are turned.
+
+    scales (``paged_cache8``): the cache is one of 8 bits. A block of 16 places and one head has one scale, the least power of
+    two whose 448-fold holds the call's values in it; where the sequence has earlier tokens in the block, at least
+    theirs, and if the scale grows they are brought to it in place (exactly, but for what falls below 2^-6 of it). Values are
+    rounded once, from fp32, to nearest even; one that is not finite is held as NaN and does not count in the scale. No two
+    sequences may share a block that the call writes, and what else reads those blocks is ordered with it.
+
+    Inference only: arguments that require a gradient are refused outside torch.no_grad(), tangents always."""
     ops = L.torch_ops()
+    cache, turn, s = (k_pages, v_pages, block_table, kv_lens, cu_q), (inv_freq, layout, mscale), scales or (None, None)
     if q is None:
-        if q_out is not None:
-            raise RuntimeError("prunepath.kv_append: q_out without q")
-        ops.kv_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+        if q_out is not None or q_weight is not None:
+            raise RuntimeError("prunepath.kv_append: q_out or q_weight without q")
+        ops.kv_append(k, v, *cache, *turn, k_weight, eps, *s)
         return None
     if q_out is None:
-        return ops.kv_append_q(q, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
-    ops.kv_append_q_into(q, q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, layout, mscale)
+        return ops.kv_append_q(q, k, v, *cache, *turn, q_weight, k_weight, eps, *s)
+    ops.kv_append_q_into(q, q_out, k, v, *cache, *turn, q_weight, k_weight, eps, *s)
     return q_out
+
+
+def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+            cu_q: torch.Tensor, rows: Optional[int] = None, scales: Scales = None,
+            out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v), each bf16 [rows, kv_heads, D], read back from a cache of either kind (``torch.ops.prunepath.kv_read``, or
+    ``kv_read_into`` writing ``out``): row i of sequence s, rows cu_q[s] .. cu_q[s + 1], is position
+    kv_lens[s] - (its rows) + i. So an append's cu_q reads what it wrote (keys as they are held, turned), and the running
+    sums of kv_lens read everything; rows, their number, is what the host gives (out's, if that is given). A value
+    of 8 bits times its scale is a bf16 number, so nothing is rounded. Rows whose place no page holds are zeros; rows behind
+    cu_q[seqs] are zero in new results and stay in out. Inference only, as ``kv_append``."""
+    ops, s = L.torch_ops(), scales or (None, None)
+    if out is None:
+        if rows is None:
+            raise RuntimeError("prunepath.kv_read: rows or out needed")
+        return ops.kv_read(k_pages, v_pages, block_table, kv_lens, cu_q, rows, *s)
+    if rows is not None and rows != out[0].shape[0]:
+        raise RuntimeError(f"prunepath.kv_read: {rows} rows into results of {out[0].shape[0]}")
+    ops.kv_read_into(k_pages, v_pages, block_table, kv_lens, cu_q, *out, *s)
+    return out
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                     kv_lens: torch.Tensor, cu_q: torch.Tensor, scale: Optional[float] = None,
-                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    out: Optional[torch.Tensor] = None, scales: Scales = None, window: Optional[int] = None,
+                    sinks: int = 0) -> torch.Tensor:
     """Attention of the new tokens (the ragged batch of ``kv_append``, appended before) over the
     paged cache: the token at position p attends the positions 0 .. p of its sequence, query head h
     the key head h // (heads / kv_heads). q bf16 [N, heads, D] -> bf16 [N, heads, D]
@@ -434,12 +496,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     -inf, is zero; an infinity in a value that a row attends gives that infinity. Rows behind cu_q[seqs]
     are zero in a new result and stay in ``out`` (which may be q itself; other overlaps are refused). Single
     tokens, chunks and whole prompts, in one call; lengths are read on the device, so a captured call serves
-    lengths that grow, in a table of any width. Inference only: arguments that require a gradient are
-    refused outside torch.no_grad(), tangents always."""
+    lengths that grow, in a table of any width.
+
+    scales (``paged_cache8``): the cache is one of 8 bits; the attention is that over the bf16 numbers which it stands for.
+    window: the token at position p attends only the positions from p - window + 1 on, and the sequence's first ``sinks`` (which
+    need a window). Pages that no row attends are not read, and their entries may be -1.
+
+    Inference only: arguments that require a gradient are refused outside torch.no_grad(), tangents always."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    ops = L.torch_ops()
+    if window is not None and window < 1:
+        raise RuntimeError(f"prunepath.paged_attention: a window of {window} tokens")
+    ops, extra = L.torch_ops(), (*(scales or (None, None)), window or 0, sinks)
     if out is None:
-        return ops.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale))
-    ops.paged_attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), out)
+        return ops.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), *extra)
+    ops.paged_attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), out, *extra)
     return out
