@@ -26,23 +26,12 @@ struct AppArgs {
   uint8_t *k_scales, *v_scales;
 };
 
-// The weights of a unit's channels.
-template <bool HALF>
-__device__ __forceinline__ void app_weights(const void* w, bool w32, int u, int nr, int per, int rd, float (&a)[8], float (&b)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int j = u < nr ? (HALF ? u * 8 + i : 2 * (u * 8 + i)) : rd + (u - nr) * 8 + i, l = HALF ? rd / 2 + u * 8 + i : j + 1;
-    a[i] = u >= per ? 0.0f : w32 ? ((const float*)w)[j] : bf16_to_f32(((const bf16_t*)w)[j]);
-    b[i] = u >= nr ? 0.0f : w32 ? ((const float*)w)[l] : bf16_to_f32(((const bf16_t*)w)[l]);
-  }
-}
-
 // A unit's values, normed (lgu: log2 of the lanes on a head, all of the wave's taking part) and weighted.
 template <typename T, bool HALF>
 __device__ __forceinline__ void app_norm(const float (&wa)[8], const float (&wb)[8], int D, float eps, int lgu, float (&p)[8], float (&q)[8]) {
   const float2 r = head_scale<8>(p, q, head_sum(rot_squares<8>(p, q), lgu), D, eps, lgu);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) p[i] = p[i] * r.y * r.x * wa[i], q[i] = q[i] * r.y * r.x * wb[i];
+  for (int i = 0; i < 8; ++i) p[i] = p[i] * r.x * wa[i], q[i] = q[i] * r.x * wb[i];
 }
 
 // nt tokens (rows from `row` on, at positions from p0 on) of the nh query (kind 0) or key heads from h0 on, turned to y:
@@ -65,7 +54,7 @@ __device__ __forceinline__ void app_turn(const AppArgs& a, int kind, float2* cs_
     for (int i = 0; i < 8; ++i) now.p.v[i] = now.q.v[i] = next.p.v[i] = next.q.v[i] = 0;
   }
   if (more) now.load(x + h * xs, w.u, nr, a.rd);
-  if constexpr (NORM) app_weights<HALF>(kind == 0 ? a.qw : a.kw, a.w32, w.u, nr, per, a.rd, wa, wb);
+  if constexpr (NORM) rot_weights<8, HALF>(kind == 0 ? a.qw : a.kw, a.w32, w.u, nr, per, a.rd, wa, wb);
   paged_asked();
   if (pair < half)
     for (int t = tid >> a.lgh; t < nt; t += APP_THREADS >> a.lgh) cs_s[t * half + pair] = rot_entry(p0 + t, freq, a.mscale, 1.0f);

@@ -54,12 +54,15 @@ __device__ __forceinline__ uint32_t c8_top(const float (&x)[N], bool& odd) {
   return top;
 }
 
+#define C8_BYTES 4  // new tokens of a block up to which its values go out byte by byte
+
 // The four of a block's value heads or key heads that the waves of a workgroup take.
 template <int D>
 struct C8Heads {
   static constexpr int V = D == 64 ? 2 : 1;  // value heads of a wave
 };
 
+#define QPER 8
 template <typename T, int D, bool HALF, bool FULL>
 __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
   constexpr int LGU = (D == 64 ? 2 : 3) + !FULL, SLOTS = 64 >> LGU, NP = APP_TOKENS / SLOTS;  // key items
@@ -123,15 +126,26 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     uint8_t* const scale = a.v_scales + to;
     uint4 was[2] = {};
     int old = FP8_LOW;
-    if (nt < APP_TOKENS) {  // the other places' bytes stay
-      was[0] = dst[0], was[1] = dst[1];
-      if (lo > 0) old = min(max((int)*scale, FP8_LOW), FP8_HIGH);
-    }
+    if (lo > 0) old = min(max((int)*scale, FP8_LOW), FP8_HIGH);
+    if (nt > C8_BYTES && nt < APP_TOKENS) was[0] = dst[0], was[1] = dst[1];  // the other places' bytes stay
     bool odd;
     const int byte = max(fp8_scale(c8_top<P>(x, odd)), old);
+    // A few tokens go out byte by byte, unless older ones change (256 single tokens of 12 heads 15.6 us, as whole words 16.1).
+    const bool bytes = nt <= C8_BYTES && __ballot(lo > 0 && byte > old) == 0;
+    if (nt <= C8_BYTES && !bytes) was[0] = dst[0], was[1] = dst[1];
     const float inv = fp8_inverse(byte), shrink = fp8_shrink(old, byte);
 #pragma unroll
     for (int i = 0; i < 2 * APP_TOKENS; ++i) x[i] = odd ? fp8_odd(x[i], inv) : x[i] * inv;
+    if (bytes) {
+#pragma unroll
+      for (int i = 0; i < APP_TOKENS; ++i)
+        if (on && i >= lo && i < hi) {
+          const uint32_t w = fp8_pack(x[i], x[APP_TOKENS + i], 0.0f, 0.0f);
+          ((uint8_t*)dst)[i] = (uint8_t)w, ((uint8_t*)(dst + 1))[i] = (uint8_t)(w >> 8);
+        }
+      if (on && l == 0 && (lo == 0 || byte > old)) *scale = (uint8_t)byte;
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       uint32_t w[4];
@@ -160,7 +174,8 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     return;
   }
   // keys
-  const int h = (block - a.nqb) * 4 + wave, u = lane & ((1 << LGU) - 1), slot = lane >> LGU;
+  const int u = lane & ((1 << LGU) - 1), slot = lane >> LGU;
+  const int h = (block - a.nqb) * 4 + wave;
   const bool on = h < a.Hkv;
   const int nr = half / 8, per = nr + (D - a.rd) / 8;
   RotUnit<T, 8, HALF> x[NP];
@@ -173,7 +188,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     if (on && n < nt && u < per) x[i].load(src + n * a.ks[0], u, nr, a.rd);
   }
   float wa[8], wb[8];
-  if (a.kw) app_weights<HALF>(a.kw, a.w32, u, nr, per, a.rd, wa, wb);
+  if (a.kw) rot_weights<8, HALF>(a.kw, a.w32, u, nr, per, a.rd, wa, wb);
   paged_asked();
   if (pair < half)
     for (int n = tid >> a.lgh; n < nt; n += APP_THREADS >> a.lgh) cs_s[n * half + pair] = rot_entry(p0 + lo + n, freq, a.mscale, 1.0f);
@@ -230,7 +245,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
 
 int app8_launch(const char* what, AppArgs& a, int dtype, int D, int layout, int64_t n_tokens, hipStream_t st) {
   const int vheads = 4 * (D == 64 ? 2 : 1);
-  a.per = n_tokens <= 4 * (int64_t)a.seqs.n_seqs ? 32 : 4;
+  a.per = n_tokens <= 4 * (int64_t)a.seqs.n_seqs ? 32 : QPER;
   a.nqb = (a.Hq + a.per - 1) / a.per, a.nkb = (a.Hkv + 3) / 4, a.nvb = (a.Hkv + vheads - 1) / vheads;
   const int64_t groups = (n_tokens >> 4) + 2 * ((int64_t)a.seqs.n_seqs + 1), items = groups * (a.nqb + a.nkb + a.nvb);
   PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld work items (at most 2^24 - 1)", what, (long long)items);

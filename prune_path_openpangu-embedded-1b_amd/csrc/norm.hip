@@ -14,7 +14,12 @@
 // dw: a thread meets the same channels in every head, so it adds them up in registers over all that its workgroup
 // takes, workgroups write one partial sum each, and a second launch adds those in order: the same bits every time.
 //
-// Memory bound: x and y once; x, dy and dx in the gradient.
+// Memory bound: x and y once; x, dy and dx in the gradient. Queries and keys are launched as two sets of workgroups, each with
+// its own weights (and their sums) in registers: with both sets in every thread, picked by the head, the backward took
+// 221 registers, two waves a SIMD and 58 us for 8192 tokens of 24 bf16 heads of 128 (151 MB) where it now takes 35 (4.3 TB/s),
+// the forward 26 where it takes 21 (101 MB, 4.8 TB/s, a large copy's rate), and the sums' launch 6.4 where it takes 4.0.
+// float32, 3333 tokens of 24 heads of 80: 12 and 21 us (4.3 and 3.6 TB/s). One token: 4.0 us, a launch, its chain of loads and
+// the sine.
 #include <algorithm>
 #include <cmath>
 
@@ -23,22 +28,26 @@
 #define NORM_THREADS ROT_THREADS
 #define NORM_MAX_D 256
 
+// One of q and k in a launch: its workgroups are those from `first` on, gx groups of tokens by gy of heads.
+struct NormSide {
+  const void *x, *dy, *w;
+  void* y;                // the result, or the gradient of x: [tokens][H][D]
+  float* part;            // workspace: [gx * gy][D], NULL: no gradient of w
+  int64_t xs[3], ds[3];   // strides of batch, token and head, in elements
+  int H, lgt;             // heads, log2 of the tokens of a group
+  uint32_t first, gx, gy;
+};
+
 struct NormArgs {
-  const void *x[2];       // q, k
-  const void *dy[2];
-  void *y[2];             // the results, or the gradients of x: [tokens][heads][D]
-  const void *w[2];
-  float* part;            // workspace: [workgroup][2][D], NULL: no gradient of w
+  NormSide side[2];
   const void* pos;
   const double* inv_freq;
-  int64_t xs[2][3], ds[2][3];  // strides of batch, token and head, in elements
   int64_t pb, pl;
   int64_t n;              // tokens
   uint32_t L;
-  int H[2];               // query and key heads
   int D, rd, pos64, w32;
   float mscale, eps;
-  int lgu, lgt, lgh;      // as in the rotation
+  int lgu, lgh;           // as in the rotation
 };
 
 // A lane's unit of a head. VEC: in 16-byte vectors; otherwise element by element, for any alignment and any even
@@ -52,6 +61,7 @@ struct NormUnit {
     const int j = u * V + i;
     return j >= half ? -1 : HALF ? j + (second ? half : 0) : 2 * j + second;
   }
+  // `on`: whether there is a head, at p
   __device__ __forceinline__ void load(const T* p, bool on, int u, int nr, int per, int half, int rd, int D) {
 #pragma unroll
     for (int i = 0; i < V; ++i) x.p.v[i] = x.q.v[i] = 0;
@@ -82,15 +92,24 @@ struct NormUnit {
         if (k >= 0) rot_store<1>(y + k, two);
       }
   }
-  // the unit's channels of a row of D floats or of elements like x's
+  // the unit's weights
   static __device__ __forceinline__ void weights(const void* w, bool w32, int u, int nr, int per, int half, int rd, int D,
                                                  float (&a)[V], float (&b)[V]) {
+    if constexpr (VEC) return rot_weights<V, HALF>(w, w32, u, nr, per, rd, a, b);
+    int j[V], k[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int j = u < per ? at(i, false, u, nr, half, rd, D) : -1, k = u < per ? at(i, true, u, nr, half, rd, D) : -1;
-      a[i] = j < 0 ? 0.0f : w32 ? ((const float*)w)[j] : bf16_to_f32(((const bf16_t*)w)[j]);
-      b[i] = k < 0 ? 0.0f : w32 ? ((const float*)w)[k] : bf16_to_f32(((const bf16_t*)w)[k]);
+      j[i] = u < per ? at(i, false, u, nr, half, rd, D) : -1, k[i] = u < per ? at(i, true, u, nr, half, rd, D) : -1;
     }
+    if (w32) {  // the loads of one kind or of the other, without a branch between them
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = ((const float*)w)[max(j[i], 0)], b[i] = ((const float*)w)[max(k[i], 0)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = bf16_to_f32(((const bf16_t*)w)[max(j[i], 0)]), b[i] = bf16_to_f32(((const bf16_t*)w)[max(k[i], 0)]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = j[i] < 0 ? 0.0f : a[i], b[i] = k[i] < 0 ? 0.0f : b[i];
   }
 };
 
@@ -100,194 +119,188 @@ __device__ __forceinline__ int64_t norm_position(const NormArgs& a, uint32_t n) 
   return a.pos64 ? ((const int64_t*)a.pos)[at] : (int64_t)((const int32_t*)a.pos)[at];
 }
 
+// What a workgroup has: a side, a group of tokens (the first of them, if it takes several) and a part of the heads.
+template <typename F>
+__device__ __forceinline__ void norm_work(const NormArgs& a, F f) {
+  if (blockIdx.x < a.side[1].first) f(a.side[0], blockIdx.x);  // (one side's arguments at a time, in scalar registers)
+  else f(a.side[1], blockIdx.x - a.side[1].first);
+}
+
 template <typename T, int V, bool HALF, bool VEC>
 __global__ __launch_bounds__(NORM_THREADS) void qk_norm_kernel(NormArgs a) {
   using Unit = NormUnit<T, V, HALF, VEC>;
   __shared__ float2 cs_s[ROT_TABLE + V];  // (a unit that is not full reads past its token's last entry)
   const int half = a.rd / 2, nr = (half + V - 1) / V, per = nr + (a.D - a.rd + V - 1) / V, D = a.D, rd = a.rd;
-  const uint32_t n0 = blockIdx.x << a.lgt;
-  const int nt = (int)min((uint32_t)1 << a.lgt, (uint32_t)a.n - n0);
-  const RotLanes w(threadIdx.x, a.lgu, a.lgt);
-  const int u = w.u, heads = a.H[0] + a.H[1], step = w.hstep * gridDim.y;
-  const bool there = w.i < nt, turned = u < nr;
-  const uint32_t n = n0 + (there ? w.i : 0), b = n / a.L, l = n - b * a.L;
-  auto from = [&](int h) {
-    const int which = h >= a.H[0];
-    return (const T*)a.x[which] + b * a.xs[which][0] + l * a.xs[which][1] + (h - which * a.H[0]) * a.xs[which][2];
-  };
-  int h = w.h + w.hstep * blockIdx.y;
-  Unit now, next;
-  now.load(there && h < heads ? from(h) : nullptr, there && h < heads, u, nr, per, half, rd, D);
-  float wa[2][V], wb[2][V];
+  norm_work(a, [&](const NormSide& s, uint32_t id) {
+    const uint32_t n0 = (id / s.gy) << s.lgt, gy = id % s.gy;
+    const int nt = (int)min((uint32_t)1 << s.lgt, (uint32_t)a.n - n0);
+    const RotLanes w(threadIdx.x, a.lgu, s.lgt);
+    const int u = w.u, step = w.hstep * s.gy;
+    const bool there = w.i < nt, turned = u < nr;
+    const uint32_t n = n0 + (there ? w.i : 0), b = n / a.L, l = n - b * a.L;
+    const T* const x = (const T*)s.x + b * s.xs[0] + l * s.xs[1];
+    T* const y = (T*)s.y + (int64_t)n * s.H * D;
+    int h = w.h + w.hstep * gy;
+    Unit now, next;
+    now.load(x + h * s.xs[2], there && h < s.H, u, nr, per, half, rd, D);
+    float wa[V], wb[V];
+    Unit::weights(s.w, a.w32, u, nr, per, half, rd, D, wa, wb);
+    paged_asked();
+    rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, 1.0f, [&](int t) { return norm_position(a, n0 + t); });
+    __syncthreads();
+    for (int h0 = w.hstep * gy; h0 < s.H; h0 += step, h += step) {  // (the folds need whole waves)
+      next.load(x + (h + step) * s.xs[2], there && h + step < s.H, u, nr, per, half, rd, D);
+      float p[V], q[V];
+      now.pairs(turned, p, q);
+      const float2 r = head_scale<V>(p, q, head_sum(rot_squares<V>(p, q), a.lgu), D, a.eps, a.lgu);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (a.H[k]) Unit::weights(a.w[k], a.w32, u, nr, per, half, rd, D, wa[k], wb[k]);
-  rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, 1.0f, [&](int t) { return norm_position(a, n0 + t); });
-  __syncthreads();
-  for (int h0 = w.hstep * blockIdx.y; h0 < heads; h0 += step, h += step) {  // (the folds need whole waves)
-    next.load(there && h + step < heads ? from(h + step) : nullptr, there && h + step < heads, u, nr, per, half, rd, D);
-    float p[V], q[V];
-    now.pairs(turned, p, q);
-    const float2 r = head_scale<V>(p, q, head_sum(rot_squares<V>(p, q), a.lgu), D, a.eps, a.lgu);
-    const bool key = h >= a.H[0];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      p[i] = p[i] * r.y * r.x * (key ? wa[1][i] : wa[0][i]);
-      q[i] = q[i] * r.y * r.x * (key ? wb[1][i] : wb[0][i]);
+      for (int i = 0; i < V; ++i) p[i] = p[i] * r.x * wa[i], q[i] = q[i] * r.x * wb[i];
+      if (there && h < s.H && u < per) {
+        if (turned) rot_turn<V>(cs_s + w.i * half + u * V, p, q);
+        Unit::put(y + h * D, p, q, u, nr, half, rd, D);
+      }
+      now = next;
     }
-    if (there && h < heads && u < per) {
-      if (turned) rot_turn<V>(cs_s + w.i * half + u * V, p, q);
-      Unit::put((T*)a.y[key] + ((int64_t)n * a.H[key] + h - (key ? a.H[0] : 0)) * D, p, q, u, nr, half, rd, D);
-    }
-    now = next;
-  }
+  });
 }
 
 template <typename T, int V, bool HALF, bool VEC>
-__global__ __launch_bounds__(NORM_THREADS) void qk_norm_bwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(NORM_THREADS, VEC ? 4 : 2) void qk_norm_bwd_kernel(NormArgs a) {
   using Unit = NormUnit<T, V, HALF, VEC>;
   __shared__ float2 cs_s[ROT_TABLE + V];
-  __shared__ float dw_s[NORM_THREADS / 64][2 * NORM_MAX_D];
+  __shared__ float dw_s[NORM_THREADS / 64][NORM_MAX_D];
   const int half = a.rd / 2, nr = (half + V - 1) / V, per = nr + (a.D - a.rd + V - 1) / V, D = a.D, rd = a.rd;
-  const RotLanes w(threadIdx.x, a.lgu, a.lgt);
-  const int u = w.u, heads = a.H[0] + a.H[1], step = w.hstep * gridDim.y;
-  const bool turned = u < nr;
-  const float inv = 1.0f / D;
-  float wa[2][V], wb[2][V], da[2][V], db[2][V];
+  norm_work(a, [&](const NormSide& side, uint32_t id) {
+    const uint32_t gy = id % side.gy;
+    const RotLanes w(threadIdx.x, a.lgu, side.lgt);
+    const int u = w.u, step = w.hstep * side.gy, H = side.H;
+    const bool turned = u < nr;
+    const float inv = 1.0f / D;
+    float wa[V], wb[V], da[V], db[V];
+    Unit::weights(side.w, a.w32, u, nr, per, half, rd, D, wa, wb);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (a.H[k]) Unit::weights(a.w[k], a.w32, u, nr, per, half, rd, D, wa[k], wb[k]);
+    for (int i = 0; i < V; ++i) da[i] = db[i] = 0.0f;
+    for (int64_t first = (int64_t)(id / side.gy) << side.lgt; first < a.n; first += (int64_t)side.gx << side.lgt) {
+      const uint32_t n0 = (uint32_t)first;
+      const int nt = (int)min((uint32_t)1 << side.lgt, (uint32_t)a.n - n0);
+      const bool there = w.i < nt;
+      const uint32_t n = n0 + (there ? w.i : 0), b = n / a.L, l = n - b * a.L;
+      const T* const xp = (const T*)side.x + b * side.xs[0] + l * side.xs[1];
+      const T* const gp = (const T*)side.dy + b * side.ds[0] + l * side.ds[1];
+      T* const y = (T*)side.y + (int64_t)n * H * D;
+      int h = w.h + w.hstep * gy;
+      // (the next head's loads ahead of the present one's sums: 32 registers more, one wave of four less on a SIMD, and
+      // 63 us instead of 60 for 8192 tokens of 24 heads with their forward)
+      Unit x, g;
+      auto load = [&](int h) {
+        x.load(xp + h * side.xs[2], there && h < H, u, nr, per, half, rd, D);
+        g.load(gp + h * side.ds[2], there && h < H, u, nr, per, half, rd, D);
+      };
+      load(h);
+      __syncthreads();  // every thread is done with the entries before
+      rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, -1.0f, [&](int t) { return norm_position(a, n0 + t); });
+      __syncthreads();
+      for (int h0 = w.hstep * gy; h0 < H; h0 += step, h += step) {
+        float p[V], q[V], s[V], t[V];
+        x.pairs(turned, p, q);
+        g.pairs(turned, s, t);
+        const bool on = there && h < H && u < per;
+        if (on && turned) rot_turn<V>(cs_s + w.i * half + u * V, s, t);
+        if constexpr (!VEC)  // what fills a unit up met no entry of its own
 #pragma unroll
-    for (int i = 0; i < V; ++i) da[k][i] = db[k][i] = 0.0f;
-  }
-  for (int64_t first = (int64_t)blockIdx.x << a.lgt; first < a.n; first += (int64_t)gridDim.x << a.lgt) {
-    const uint32_t n0 = (uint32_t)first;
-    const int nt = (int)min((uint32_t)1 << a.lgt, (uint32_t)a.n - n0);
-    const bool there = w.i < nt;
-    const uint32_t n = n0 + (there ? w.i : 0), b = n / a.L, l = n - b * a.L;
-    auto from = [&](const void* const* x, const int64_t (*s)[3], int h) {
-      const int which = h >= a.H[0];
-      return (const T*)x[which] + b * s[which][0] + l * s[which][1] + (h - which * a.H[0]) * s[which][2];
-    };
-    int h = w.h + w.hstep * blockIdx.y;
-    Unit x, g, nx, ng;
-    auto load = [&](Unit& x, Unit& g, int h) {
-      const bool on = there && h < heads;
-      x.load(on ? from(a.x, a.xs, h) : nullptr, on, u, nr, per, half, rd, D);
-      g.load(on ? from(a.dy, a.ds, h) : nullptr, on, u, nr, per, half, rd, D);
-    };
-    load(x, g, h);
-    __syncthreads();  // every thread is done with the entries before
-    rot_table(cs_s, a.inv_freq, half, a.lgh, nt, a.mscale, -1.0f, [&](int t) { return norm_position(a, n0 + t); });
-    __syncthreads();
-    for (int h0 = w.hstep * blockIdx.y; h0 < heads; h0 += step, h += step) {
-      load(nx, ng, h + step);
-      float p[V], q[V], s[V], t[V];
-      x.pairs(turned, p, q);
-      g.pairs(turned, s, t);
-      const bool on = there && h < heads && u < per, key = h >= a.H[0];
-      if (on && turned) rot_turn<V>(cs_s + w.i * half + u * V, s, t);
-      if constexpr (!VEC)  // what fills a unit up met no entry of its own
+          for (int i = 0; i < V; ++i)
+            if (turned && u * V + i >= half) s[i] = t[i] = 0.0f;
+        const float2 r = head_scale<V>(p, q, head_sum(rot_squares<V>(p, q), a.lgu), D, a.eps, a.lgu);
+        float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (turned && u * V + i >= half) s[i] = t[i] = 0.0f;
-      const float2 r = head_scale<V>(p, q, head_sum(rot_squares<V>(p, q), a.lgu), D, a.eps, a.lgu);
-      float m = 0.0f;
+        for (int i = 0; i < V; ++i) {
+          p[i] = on ? p[i] * r.x : 0.0f;
+          q[i] = on ? q[i] * r.x : 0.0f;
+          da[i] = __fmaf_rn(s[i], p[i], da[i]), db[i] = __fmaf_rn(t[i], q[i], db[i]);
+          s[i] *= wa[i], t[i] *= wb[i];
+          m = __fmaf_rn(s[i], p[i], __fmaf_rn(t[i], q[i], m));
+        }
+        m = head_sum(m, a.lgu) * inv;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        p[i] = on ? p[i] * r.y * r.x : 0.0f;
-        q[i] = on ? q[i] * r.y * r.x : 0.0f;
-        const float ga = s[i] * p[i], gb = t[i] * q[i];
-        da[0][i] += key ? 0.0f : ga, db[0][i] += key ? 0.0f : gb;
-        da[1][i] += key ? ga : 0.0f, db[1][i] += key ? gb : 0.0f;
-        s[i] *= key ? wa[1][i] : wa[0][i];
-        t[i] *= key ? wb[1][i] : wb[0][i];
-        m = __fmaf_rn(s[i], p[i], __fmaf_rn(t[i], q[i], m));
+        for (int i = 0; i < V; ++i) {
+          p[i] = __fmaf_rn(-p[i], m, s[i]) * r.x * r.y;
+          q[i] = __fmaf_rn(-q[i], m, t[i]) * r.x * r.y;
+        }
+        if (on) Unit::put(y + h * D, p, q, u, nr, half, rd, D);
+        load(h + step);
       }
-      m = head_sum(m, a.lgu) * inv;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        p[i] = __fmaf_rn(-p[i], m, s[i]) * r.x * r.y;
-        q[i] = __fmaf_rn(-q[i], m, t[i]) * r.x * r.y;
-      }
-      if (on) Unit::put((T*)a.y[key] + ((int64_t)n * a.H[key] + h - (key ? a.H[0] : 0)) * D, p, q, u, nr, half, rd, D);
-      x = nx, g = ng;
     }
-  }
-  if (!a.part) return;
-  // the sums of a wave's lanes that meet the same channels, then of the waves
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
+    if (!side.part) return;
+    // the sums of a wave's lanes that meet the same channels, then of the waves
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < V; ++i)
       for (int m = 1 << a.lgu; m < 64; m <<= 1) {
-        da[k][i] += __shfl_xor(da[k][i], m);
-        db[k][i] += __shfl_xor(db[k][i], m);
+        da[i] += __shfl_xor(da[i], m);
+        db[i] += __shfl_xor(db[i], m);
       }
-  if ((lane >> a.lgu) == 0 && u < per) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
+    if ((lane >> a.lgu) == 0 && u < per) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int j = Unit::at(i, false, u, nr, half, rd, D), l = Unit::at(i, true, u, nr, half, rd, D);
-        if (j >= 0) dw_s[wave][k * D + j] = da[k][i];
-        if (l >= 0) dw_s[wave][k * D + l] = db[k][i];
+        const int j = Unit::at(i, false, u, nr, half, rd, D), k = Unit::at(i, true, u, nr, half, rd, D);
+        if (j >= 0) dw_s[wave][j] = da[i];
+        if (k >= 0) dw_s[wave][k] = db[i];
       }
-  }
-  __syncthreads();
-  float* const to = a.part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * D;
-  for (int c = threadIdx.x; c < 2 * D; c += NORM_THREADS)
-    to[c] = (dw_s[0][c] + dw_s[1][c]) + (dw_s[2][c] + dw_s[3][c]);
+    }
+    __syncthreads();
+    float* const to = side.part + (int64_t)id * D;
+    for (int c = threadIdx.x; c < D; c += NORM_THREADS) to[c] = (dw_s[0][c] + dw_s[1][c]) + (dw_s[2][c] + dw_s[3][c]);
+  });
 }
 
-// The workgroups' partial sums added: 16 channels a workgroup (64 bytes of a row), 16 threads to each, which take
-// rows in turn.
+// The workgroups' partial sums of either side added: 16 channels a workgroup (64 bytes of a row), 16 threads to each,
+// which take rows in turn.
 #define NORM_COLS 16
-__global__ __launch_bounds__(NORM_THREADS) void qk_norm_join_kernel(const float* part, int rows, int D, int w32, void* dqw, void* dkw) {
-  constexpr int G = NORM_THREADS / NORM_COLS;
+struct NormJoin {
+  const float* part[2];
+  void* dw[2];
+  int rows[2];
+  int D, w32;
+};
+__global__ __launch_bounds__(NORM_THREADS) void qk_norm_join_kernel(NormJoin a) {
+  constexpr int G = NORM_THREADS / NORM_COLS, U = 8;
   __shared__ float sum_s[G][NORM_COLS];
-  const int c = blockIdx.x * NORM_COLS + threadIdx.x % NORM_COLS, g = threadIdx.x / NORM_COLS;
-  float s[4] = {};
-  if (c < 2 * D) {
-    int i = g;
-    for (; i + 3 * G < rows; i += 4 * G)
+  const int side = blockIdx.y, c = blockIdx.x * NORM_COLS + threadIdx.x % NORM_COLS, g = threadIdx.x / NORM_COLS, rows = a.rows[side];
+  const float* const part = a.part[side] + min(c, a.D - 1);
+  float s[U] = {};
+  int i = g;
+  for (; i + (U - 1) * G < rows; i += U * G)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] += part[(int64_t)(i + j * G) * 2 * D + c];
-    for (; i < rows; i += G) s[0] += part[(int64_t)i * 2 * D + c];
-  }
-  sum_s[g][threadIdx.x % NORM_COLS] = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int j = 0; j < U; ++j) s[j] += part[(int64_t)(i + j * G) * a.D];
+  for (; i < rows; i += G) s[0] += part[(int64_t)i * a.D];
+  sum_s[g][threadIdx.x % NORM_COLS] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
-  if (g || c >= 2 * D) return;
+  if (g || c >= a.D || !a.dw[side]) return;
   float t = 0.0f;
 #pragma unroll
-  for (int i = 0; i < G; ++i) t += sum_s[i][threadIdx.x];
-  void* const to = c < D ? dqw : dkw;
-  const int at = c < D ? c : c - D;
-  if (!to) return;
-  if (w32) ((float*)to)[at] = t;
-  else ((bf16_t*)to)[at] = f32_to_bf16(t);
+  for (int k = 0; k < G; ++k) t += sum_s[k][threadIdx.x];
+  if (a.w32) ((float*)a.dw[side])[c] = t;
+  else ((bf16_t*)a.dw[side])[c] = f32_to_bf16(t);
 }
 
 // ------------------------------------------------------------------ host
+// Sizes that the launch of one side, and the workspace of the gradient, go by.
 struct NormPlan {
-  bool vec;
-  int lgu, lgt, lgh;
+  int lgt;
   int64_t gx, gy;
 };
 
-// Sizes that the launch, and the workspace of the gradient, go by. `vec` changes neither.
-static NormPlan norm_plan(int64_t n, int heads, int D, int rd, int V, bool backward) {
+static NormPlan norm_plan(int64_t n, int H, int D, int rd, int V, bool backward) {
   NormPlan p = {};
-  const int half = rd / 2, per = (half + V - 1) / V + (D - rd + V - 1) / V;
+  if (H == 0) return p;
+  const int half = rd / 2, per = (half + V - 1) / V + (D - rd + V - 1) / V, lgu = rot_log2up(per);
   const int64_t cus = pp_device_cus();
-  p.lgu = rot_log2up(per), p.lgh = std::min(8, rot_log2up(half));
-  while (p.lgt < 4 && p.lgu + p.lgt < 8 && ((int64_t)heads * per << p.lgt) < 4 * NORM_THREADS &&
-         (n >> (p.lgt + 1)) >= 2 * cus && (half << (p.lgt + 1)) <= ROT_TABLE)
+  while (p.lgt < 4 && lgu + p.lgt < 8 && ((int64_t)H * per << p.lgt) < 4 * NORM_THREADS && (n >> (p.lgt + 1)) >= 2 * cus &&
+         (half << (p.lgt + 1)) <= ROT_TABLE)
     ++p.lgt;
-  const int64_t groups = (n + (1 << p.lgt) - 1) >> p.lgt, hstep = (NORM_THREADS >> p.lgu) >> p.lgt;
-  p.gx = backward ? std::min<int64_t>(groups, 4 * cus) : groups;
-  p.gy = std::max<int64_t>(1, std::min<int64_t>((heads + hstep - 1) / hstep, (2 * cus + p.gx - 1) / p.gx));
+  const int64_t groups = (n + (1 << p.lgt) - 1) >> p.lgt, hstep = (NORM_THREADS >> lgu) >> p.lgt;
+  p.gx = backward ? std::min<int64_t>(groups, 2 * cus) : groups;
+  p.gy = std::max<int64_t>(1, std::min<int64_t>((H + hstep - 1) / hstep, (2 * cus + p.gx - 1) / p.gx));
   return p;
 }
 
@@ -307,10 +320,17 @@ static int norm_unit(int dtype, int D, int rd) {
   return dtype == PP_DTYPE_F32 && (rd / 2 + 3) / 4 + (D - rd + 3) / 4 <= 64 ? 4 : 8;
 }
 
-static int norm_launch(const char* what, NormArgs& a, int dtype, int layout, bool backward, const NormPlan& p, int V, hipStream_t st) {
-  a.lgu = p.lgu, a.lgt = p.lgt, a.lgh = p.lgh;
-  PP_REQUIRE(p.gx <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld tokens of this head size", what, (long long)a.n);
-  const dim3 grid((unsigned)p.gx, (unsigned)p.gy);
+static int norm_launch(const char* what, NormArgs& a, int dtype, int layout, bool backward, bool vec, int V, hipStream_t st) {
+  int64_t groups = 0;
+  for (int i = 0; i < 2; ++i) {
+    const NormPlan p = norm_plan(a.n, a.side[i].H, a.D, a.rd, V, backward);
+    a.side[i].lgt = p.lgt, a.side[i].gx = (uint32_t)p.gx, a.side[i].gy = (uint32_t)std::max<int64_t>(p.gy, 1);
+    a.side[i].first = (uint32_t)groups;
+    groups += p.gx * p.gy;
+    PP_REQUIRE(groups <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld tokens of this head size", what, (long long)a.n);
+  }
+  a.lgu = rot_log2up((a.rd / 2 + V - 1) / V + (a.D - a.rd + V - 1) / V), a.lgh = std::min(8, rot_log2up(a.rd / 2));
+  const unsigned grid = (unsigned)groups;
 #define NORM(T, V_, HALF_, VEC_)                                                                 \
   do {                                                                                           \
     if (backward) qk_norm_bwd_kernel<T, V_, HALF_, VEC_><<<grid, NORM_THREADS, 0, st>>>(a);      \
@@ -322,11 +342,11 @@ static int norm_launch(const char* what, NormArgs& a, int dtype, int layout, boo
     else NORM(T, V_, false, VEC_);                         \
   } while (0)
   if (dtype == PP_DTYPE_F32) {
-    if (p.vec) NORM_LAYOUT(float, 4, true);
+    if (vec) NORM_LAYOUT(float, 4, true);
     else if (V == 4) NORM_LAYOUT(float, 4, false);
     else NORM_LAYOUT(float, 8, false);
   } else {
-    if (p.vec) NORM_LAYOUT(bf16_t, 8, true);
+    if (vec) NORM_LAYOUT(bf16_t, 8, true);
     else NORM_LAYOUT(bf16_t, 8, false);
   }
 #undef NORM_LAYOUT
@@ -342,7 +362,7 @@ static int norm_args(const char* what, NormArgs& a, int w_dtype, const void* pos
   PP_REQUIRE(eps >= 0.0f && std::isfinite(eps), PP_ERR_INVALID, "%s: eps %g", what, eps);
   PP_REQUIRE(positions && pos_strides && inv_freq, PP_ERR_INVALID, "%s: null pointer", what);
   a.pos = positions, a.pos64 = pos64, a.pb = pos_strides[0], a.pl = pos_strides[1];
-  a.inv_freq = inv_freq, a.n = batch * length, a.L = (uint32_t)length, a.H[0] = Hq, a.H[1] = Hk;
+  a.inv_freq = inv_freq, a.n = batch * length, a.L = (uint32_t)length, a.side[0].H = Hq, a.side[1].H = Hk;
   a.D = D, a.rd = rotary_dim, a.w32 = w_dtype == PP_DTYPE_F32, a.mscale = mscale, a.eps = eps;
   return PP_OK;
 }
@@ -366,21 +386,21 @@ extern "C" int pp_qk_norm_rotary(const void* q, const int64_t* q_strides, const 
   void* ys[2] = {q_out, k_out};
   const int64_t* ss[2] = {q_strides, k_strides};
   for (int i = 0; i < 2; ++i) {
-    if (a.H[i] == 0) continue;
-    a.x[i] = xs[i], a.y[i] = ys[i], a.w[i] = ws[i];
-    for (int j = 0; j < 3; ++j) a.xs[i][j] = ss[i][j];
-    vec = vec && rot_aligned(xs[i], ss[i], 3, bytes) && ((uintptr_t)ys[i] & 15) == 0;
+    NormSide& s = a.side[i];
+    if (s.H == 0) continue;
+    s.x = xs[i], s.y = ys[i], s.w = ws[i];
+    for (int j = 0; j < 3; ++j) s.xs[j] = ss[i][j];
+    vec = vec && ((uintptr_t)ws[i] & 15) == 0 && rot_aligned(xs[i], ss[i], 3, bytes) && ((uintptr_t)ys[i] & 15) == 0;
   }
-  NormPlan p = norm_plan(a.n, Hq + Hk, D, rotary_dim, V, false);
-  p.vec = vec;
-  return norm_launch(what, a, dtype, layout, false, p, V, (hipStream_t)stream);
+  return norm_launch(what, a, dtype, layout, false, vec, V, (hipStream_t)stream);
 }
 
 extern "C" size_t pp_qk_norm_rotary_workspace_bytes(int dtype, int64_t batch, int64_t length, int Hq, int Hk, int D, int rotary_dim) {
   if (norm_sizes("pp_qk_norm_rotary_bwd", dtype, batch, length, Hq, Hk, D, rotary_dim)) return 0;
   if (batch == 0 || length == 0 || Hq + Hk == 0) return 0;
-  const NormPlan p = norm_plan(batch * length, Hq + Hk, D, rotary_dim, norm_unit(dtype, D, rotary_dim), true);
-  return (size_t)(p.gx * p.gy) * 2 * D * 4;
+  const int V = norm_unit(dtype, D, rotary_dim);
+  const NormPlan p = norm_plan(batch * length, Hq, D, rotary_dim, V, true), q = norm_plan(batch * length, Hk, D, rotary_dim, V, true);
+  return (size_t)(p.gx * p.gy + q.gx * q.gy) * D * 4;
 }
 
 extern "C" int pp_qk_norm_rotary_bwd(const void* dq, const int64_t* dq_strides, const void* dk, const int64_t* dk_strides,
@@ -396,9 +416,10 @@ extern "C" int pp_qk_norm_rotary_bwd(const void* dq, const int64_t* dq_strides, 
   PP_REQUIRE(w_dtype == PP_DTYPE_F32 || w_dtype == PP_DTYPE_BF16, PP_ERR_INVALID, "%s: weights of dtype %d", what, w_dtype);
   const bool need = q_weight_grad || k_weight_grad;
   hipStream_t st = (hipStream_t)stream;
-  const int joins = (2 * D + NORM_COLS - 1) / NORM_COLS;
+  const dim3 joins((D + NORM_COLS - 1) / NORM_COLS, 2);
+  NormJoin join = {{nullptr, nullptr}, {q_weight_grad, k_weight_grad}, {0, 0}, D, w_dtype == PP_DTYPE_F32};
   if (batch == 0 || length == 0 || Hq + Hk == 0) {  // a sum of nothing
-    if (need) qk_norm_join_kernel<<<joins, NORM_THREADS, 0, st>>>(nullptr, 0, D, w_dtype == PP_DTYPE_F32, q_weight_grad, k_weight_grad);
+    if (need) qk_norm_join_kernel<<<joins, NORM_THREADS, 0, st>>>(join);
     return need ? pp_check_launch(what) : PP_OK;
   }
   NormArgs a = {};
@@ -413,19 +434,23 @@ extern "C" int pp_qk_norm_rotary_bwd(const void* dq, const int64_t* dq_strides, 
   void* ys[2] = {q_grad, k_grad};
   const int64_t *ss[2] = {q_strides, k_strides}, *ds[2] = {dq_strides, dk_strides};
   for (int i = 0; i < 2; ++i) {
-    if (a.H[i] == 0) continue;
-    a.x[i] = xs[i], a.dy[i] = gs[i], a.y[i] = ys[i], a.w[i] = ws[i];
-    for (int j = 0; j < 3; ++j) a.xs[i][j] = ss[i][j], a.ds[i][j] = ds[i][j];
-    vec = vec && rot_aligned(xs[i], ss[i], 3, bytes) && rot_aligned(gs[i], ds[i], 3, bytes) && ((uintptr_t)ys[i] & 15) == 0;
+    NormSide& s = a.side[i];
+    if (s.H == 0) continue;
+    s.x = xs[i], s.dy = gs[i], s.y = ys[i], s.w = ws[i];
+    for (int j = 0; j < 3; ++j) s.xs[j] = ss[i][j], s.ds[j] = ds[i][j];
+    vec = vec && ((uintptr_t)ws[i] & 15) == 0 && rot_aligned(xs[i], ss[i], 3, bytes) && rot_aligned(gs[i], ds[i], 3, bytes) && ((uintptr_t)ys[i] & 15) == 0;
   }
-  NormPlan p = norm_plan(a.n, Hq + Hk, D, rotary_dim, V, true);
-  p.vec = vec;
-  const size_t bytes_needed = need ? (size_t)(p.gx * p.gy) * 2 * D * 4 : 0;
+  const NormPlan p[2] = {norm_plan(a.n, Hq, D, rotary_dim, V, true), norm_plan(a.n, Hk, D, rotary_dim, V, true)};
+  for (int i = 0; i < 2; ++i) join.rows[i] = (int)(p[i].gx * p[i].gy);
+  const size_t bytes_needed = need ? (size_t)(join.rows[0] + join.rows[1]) * D * 4 : 0;
   PP_REQUIRE(bytes_needed == 0 || (workspace && workspace_bytes >= bytes_needed && ((uintptr_t)workspace & 15) == 0), PP_ERR_INVALID,
              "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes, bytes_needed);
-  a.part = need ? (float*)workspace : nullptr;
-  rc = norm_launch(what, a, dtype, layout, true, p, V, st);
+  if (need) {
+    a.side[0].part = (float*)workspace, a.side[1].part = a.side[0].part + (size_t)join.rows[0] * D;
+    join.part[0] = a.side[0].part, join.part[1] = a.side[1].part;
+  }
+  rc = norm_launch(what, a, dtype, layout, true, vec, V, st);
   if (rc || !need) return rc;
-  qk_norm_join_kernel<<<joins, NORM_THREADS, 0, st>>>(a.part, (int)(p.gx * p.gy), D, a.w32, q_weight_grad, k_weight_grad);
+  qk_norm_join_kernel<<<joins, NORM_THREADS, 0, st>>>(join);
   return pp_check_launch(what);
 }

@@ -133,6 +133,20 @@ __device__ __forceinline__ void rot_turn(const float2* cs, float (&a)[V], float 
 }
 
 // ------------------------------------------------------------------ norms of heads
+// The weights of a unit's channels, from a row that starts on a 16-byte boundary: float32, or bfloat16.
+template <int V, bool HALF>
+__device__ __forceinline__ void rot_weights(const void* w, bool w32, int u, int nr, int per, int rd, float (&a)[V], float (&b)[V]) {
+  const int at = min(u, per - 1);
+  if (w32) {
+    RotUnit<float, V, HALF> x;
+    x.load((const float*)w, at, nr, rd);
+    rot_pairs(x, at < nr, a, b);
+  } else if constexpr (V == 8) {
+    RotUnit<bf16_t, V, HALF> x;
+    x.load((const bf16_t*)w, at, nr, rd);
+    rot_pairs(x, at < nr, a, b);
+  }
+}
 // A reduction over the 2^lgu neighbours that hold a head, in every one of them; every lane of the wave takes part.
 template <typename F>
 __device__ __forceinline__ float head_fold(float v, int lgu, F f) {
@@ -158,14 +172,15 @@ __device__ __forceinline__ float rot_squares(const float (&a)[V], const float (&
   for (int i = 0; i < V; ++i) s = __fmaf_rn(a[i], a[i], __fmaf_rn(b[i], b[i], s));
   return s;
 }
-// 1 / sqrt(mean of squares + eps) of a head, as the two factors x and y of it: y is 1 unless the squares leave
-// float32's range, then it is what brings the head's largest value next to 1. ss: the head's sum of squares.
+// What a head's values are to be multiplied by: x of the result, 1 / sqrt(mean of squares + eps). ss: the head's sum of
+// squares. If the squares leave float32's range, the values are first multiplied, here, by what brings the largest of
+// them next to 1, y of the result, and x is that of these.
 template <int V>
-__device__ __forceinline__ float2 head_scale(const float (&a)[V], const float (&b)[V], float ss, int D, float eps, int lgu) {
+__device__ __forceinline__ float2 head_scale(float (&a)[V], float (&b)[V], float ss, int D, float eps, int lgu) {
   const float inv = 1.0f / D, mean = __fmaf_rn(ss, inv, eps);
   float r = rsqrtf(mean), pre = 1.0f;
   const bool odd = !(mean >= 0x1p-100f && ss <= 0x1p120f);
-  if (__ballot(odd)) {  // the whole wave: the folds below need its lanes
+  if (__builtin_expect(__ballot(odd) != 0, 0)) {  // the whole wave: the folds below need its lanes
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmaxf(top, fmaxf(fabsf(a[i]), fabsf(b[i])));
@@ -179,6 +194,8 @@ __device__ __forceinline__ float2 head_scale(const float (&a)[V], const float (&
     if (odd && top > 0.0f && top < __builtin_inff()) {
       pre = by;
       r = e2 < __builtin_inff() ? rsqrtf(__fmaf_rn(ss2, inv, e2)) : rsqrtf(eps) / by;
+#pragma unroll
+      for (int i = 0; i < V; ++i) a[i] = x[i], b[i] = y[i];
     }
   }
   return make_float2(r, pre);

@@ -283,6 +283,7 @@ static int append(const char* what, const void* q, const int64_t* q_strides, con
   if (k_weight) {
     PP_REQUIRE(w_dtype == PP_DTYPE_F32 || w_dtype == dtype, PP_ERR_INVALID, "%s: weights of dtype %d for heads of %d", what, w_dtype, dtype);
     PP_REQUIRE(eps >= 0.0f && std::isfinite(eps), PP_ERR_INVALID, "%s: eps %g", what, eps);
+    PP_REQUIRE((((uintptr_t)q_weight | (uintptr_t)k_weight) & 15) == 0, PP_ERR_INVALID, "%s: weights not 16-byte aligned", what);
   }
   if (n_tokens == 0) return PP_OK;
   PP_REQUIRE(k && v && k_strides && v_strides && (!q || (q_strides && q_out)), PP_ERR_INVALID, "%s: null pointer", what);

@@ -934,6 +934,8 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   kv_append_check(q ? &*q : nullptr, q ? &*q_out : nullptr, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, inv_freq, q_weight,
                   k_weight, k_scales, v_scales);
   auto given = [](const optional<Tensor>& t) { return t ? &*t : nullptr; };
+  // (a row of weights inside another tensor may start anywhere)
+  auto row = [](const optional<Tensor>& t) { return t && ((uintptr_t)t->data_ptr() & 15) ? optional<Tensor>(t->clone()) : t; };
   const Paged p = paged_sizes(name, k_pages, block_table, k.size(0), q ? q->size(1) : 0);
   need_gpu(name, k, {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, given(inv_freq), given(q_weight), given(k_weight),
                      given(k_scales), given(v_scales)});
@@ -974,11 +976,12 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   }
   const c10::DeviceGuard g(k.device());
   const int64_t ks[2] = {step(k, 0), step(k, 1)}, vs[2] = {step(v, 0), step(v, 1)};
+  const optional<Tensor> qw = row(q_weight), kw = row(k_weight);
   check_rc(pp_kv_append_with(q ? q->data_ptr() : nullptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, x_code(k, name), p.n,
                              (int)p.seqs, cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
                              block_table.data_ptr<int32_t>(), (int)p.max_pages, (int)p.pages, (int)p.page, (int)p.Hq,
                              (int)p.Hkv, (int)p.D, (const double*)ptr(inv_freq), inv_freq ? (int)(2 * inv_freq->numel()) : 0,
-                             lay, (float)mscale, ptr(q_weight), ptr(k_weight), k_weight ? w_code(*k_weight, name) : 0, (float)eps,
+                             lay, (float)mscale, ptr(qw), ptr(kw), kw ? w_code(*kw, name) : 0, (float)eps,
                              k_pages.data_ptr(), v_pages.data_ptr(), (void*)ptr(k_scales), (void*)ptr(v_scales),
                              q ? q_out->data_ptr() : nullptr, zero_tail, stream_of(k)),
            name);

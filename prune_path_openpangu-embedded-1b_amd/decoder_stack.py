@@ -20,13 +20,15 @@ Several sequences of different lengths are served through a paged cache instead
 (``PagedKV``, ``generate``): the new tokens of all of them are packed on one axis, each
 layer appends their keys and values with the rotation on the way (``ops.kv_append``) and
 attends over the pages (``ops.paged_attention``). Prompts go in in chunks, then one greedy
-step of the whole batch is captured and replayed.
+step of the whole batch is captured and replayed. The cache may be one of 8 bits; a stack may
+norm its query and key heads (``ops.qk_norm_rotary``, and on the way of the append) and attend a
+window and the first tokens only.
 """
 from __future__ import annotations
 
 import math
 import types
-from typing import Dict, List
+from typing import Dict, List, Optional
 
 import torch
 import torch.nn as nn
@@ -60,11 +62,18 @@ def rope(x: torch.Tensor, pos: torch.Tensor, base: float = 10000.0) -> torch.Ten
 
 
 class Attention(nn.Module):
-    def __init__(self, d: int, heads: int, max_len: int):
+    """``qk_norm``: the heads of queries and keys are normed before they are turned. ``window``: a token
+    attends the last ``window`` tokens, itself among them, and the first ``sinks``."""
+
+    def __init__(self, d: int, heads: int, max_len: int, qk_norm: bool = False, window: Optional[int] = None,
+                 sinks: int = 0):
         super().__init__()
         self.h, self.hd = heads, d // heads
         self.qkv = nn.Linear(d, 3 * d, bias=False)
         self.o = nn.Linear(d, d, bias=False)
+        self.q_norm, self.k_norm = (RMSNorm(self.hd), RMSNorm(self.hd)) if qk_norm else (None, None)
+        self.inv_freq = None
+        self.window, self.sinks = window, sinks
         self.max_len = max_len
         self.kt_cache = None  # [B, h, hd, max_len]: K kept transposed
         self.v_cache = None   # [B, h, max_len, hd]
@@ -75,20 +84,36 @@ class Attention(nn.Module):
         self.v_cache = torch.zeros(B, self.h, self.max_len, self.hd, device=device, dtype=dtype)
         self.len = 0
 
+    def turned(self, x, pos):
+        """q, k and v [B, h, L, hd] of x [B, L, D] at positions pos [L], q and k normed (if they are) and turned."""
+        B, L, _ = x.shape
+        qkv = self.qkv(x).view(B, L, 3, self.h, self.hd)
+        q, k, v = qkv.permute(2, 0, 3, 1, 4)
+        if self.q_norm is None:
+            return rope(q, pos), rope(k, pos), v
+        if self.inv_freq is None or self.inv_freq.device != x.device:  # (float64, which a buffer would not stay)
+            self.inv_freq, _ = ops.rotary_frequencies(self.hd, device=x.device)
+        q, k = ops.qk_norm_rotary(qkv[:, :, 0], qkv[:, :, 1], self.q_norm.weight, self.k_norm.weight, pos.expand(B, L),
+                                  self.inv_freq, eps=self.q_norm.eps)
+        return q.transpose(1, 2), k.transpose(1, 2), v
+
+    def visible(self, pos, places):
+        """Whether a token at ``pos`` attends a place, for tensors that broadcast."""
+        seen = places <= pos
+        return seen if self.window is None else seen & ((places > pos - self.window) | (places < self.sinks))
+
     def forward(self, x):
         """Eager: L new tokens at host position ``self.len``."""
         B, L, D = x.shape
-        q, k, v = self.qkv(x).view(B, L, 3, self.h, self.hd).permute(2, 0, 3, 1, 4)  # [B, h, L, hd] each
         pos = torch.arange(self.len, self.len + L, device=x.device)
-        q, k = rope(q, pos), rope(k, pos)
+        q, k, v = self.turned(x, pos)
         self.kt_cache[:, :, :, self.len:self.len + L] = k.transpose(-1, -2)
         self.v_cache[:, :, self.len:self.len + L] = v
         T = self.len + L
         kt = self.kt_cache[:, :, :, :T].contiguous()                    # [B, h, hd, T]
         s = torch.matmul(q.contiguous(), kt).float() / math.sqrt(self.hd)  # [B, h, L, T]
-        if L > 1:
-            causal = torch.ones(L, T, device=x.device, dtype=torch.bool).tril(T - L)
-            s = s.masked_fill(~causal, float("-inf"))
+        if L > 1 or self.window is not None:
+            s = s.masked_fill(~self.visible(pos[:, None], torch.arange(T, device=x.device)), float("-inf"))
         p = torch.softmax(s, -1).to(x.dtype)
         o = torch.matmul(p, self.v_cache[:, :, :T].contiguous())        # [B, h, L, hd]
         self.len = T
@@ -96,11 +121,10 @@ class Attention(nn.Module):
 
     def forward_static(self, x, pos_t, mask):
         """One token at device position ``pos_t`` ([1] int64), attending over the whole
-        cache with ``mask`` ([max_len]: 0 up to pos_t, -inf after): static shapes, so a
+        cache with ``mask`` ([max_len]: 0 where it attends, -inf elsewhere): static shapes, so a
         step can be captured in a graph."""
         B, L, D = x.shape
-        q, k, v = self.qkv(x).view(B, L, 3, self.h, self.hd).permute(2, 0, 3, 1, 4)  # [B, h, 1, hd]
-        q, k = rope(q, pos_t), rope(k, pos_t)
+        q, k, v = self.turned(x, pos_t)  # [B, h, 1, hd]
         self.kt_cache.index_copy_(3, pos_t, k.transpose(-1, -2).contiguous())
         self.v_cache.index_copy_(2, pos_t, v.contiguous())
         s = torch.matmul(q.contiguous(), self.kt_cache).float() / math.sqrt(self.hd)  # [B, h, 1, max_len]
@@ -113,32 +137,46 @@ class Attention(nn.Module):
         """The packed new tokens x [N, d] of ``kv``'s sequences (rows cu_q[s] .. cu_q[s + 1] of
         sequence s, already counted in ``kv.lens``) over the paged cache."""
         qkv = self.qkv(x).view(-1, 3, self.h, self.hd)
-        cache = (*kv.pages[layer], kv.table, kv.lens, cu_q)
-        q = ops.kv_append(qkv[:, 1], qkv[:, 2], *cache, inv_freq=kv.inv_freq, q=qkv[:, 0])
-        return self.o(ops.paged_attention(q, *cache).view(x.shape[0], -1))
+        cache, scales = (*kv.pages[layer], kv.table, kv.lens, cu_q), kv.scales[layer]
+        norm = {} if self.q_norm is None else dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=self.q_norm.eps)
+        q = ops.kv_append(qkv[:, 1], qkv[:, 2], *cache, inv_freq=kv.inv_freq, q=qkv[:, 0], scales=scales, **norm)
+        o = ops.paged_attention(q, *cache, scales=scales, window=self.window, sinks=self.sinks)
+        return self.o(o.view(x.shape[0], -1))
 
 
 class PagedKV:
     """The paged cache of every layer for ``seqs`` sequences of up to ``max_len`` tokens: pages of
     ``page_size`` tokens, a block table that gives each sequence its own (scattered, as an
-    allocator would leave them), and the lengths, all on the device."""
+    allocator would leave them), and the lengths, all on the device. ``bits`` 16 (bfloat16) or 8 (with
+    a scale for each block of 16 tokens and head)."""
 
     def __init__(self, layers: int, seqs: int, max_len: int, heads: int, head_dim: int, page_size: int = 16,
-                 device="cuda:0"):
+                 device="cuda:0", bits: int = 16):
+        if bits not in (8, 16):
+            raise ValueError(f"PagedKV: a cache of 8 or 16 bits (got {bits})")
         per = -(-max_len // page_size)
         self.max_len = max_len
         self.table = torch.arange(seqs * per, dtype=torch.int32, device=device).view(per, seqs).t().contiguous()
-        self.pages = [ops.paged_cache(seqs * per, page_size, heads, head_dim, device) for _ in range(layers)]
+        size = (seqs * per, page_size, heads, head_dim, device)
+        made = [ops.paged_cache8(*size) if bits == 8 else (ops.paged_cache(*size), None) for _ in range(layers)]
+        self.pages, self.scales = [p for p, _ in made], [s for _, s in made]
         self.lens = torch.zeros(seqs, dtype=torch.int32, device=device)
         self.one_each = torch.arange(seqs + 1, dtype=torch.int32, device=device)  # cu_q of a decode step
         self.inv_freq, _ = ops.rotary_frequencies(head_dim, device=device)
 
+    def read(self, layer: int):
+        """(k, v, offsets): a layer's keys and values of every token so far, bf16 [tokens, heads, head_dim], sequence s the
+        rows offsets[s] .. offsets[s + 1]. (Waits for the device: the number of rows is the lengths' sum.)"""
+        offsets = F.pad(self.lens.cumsum(0, dtype=torch.int32), (1, 0))
+        k, v = ops.kv_read(*self.pages[layer], self.table, self.lens, offsets, int(offsets[-1]), scales=self.scales[layer])
+        return k, v, offsets
+
 
 class Block(nn.Module):
-    def __init__(self, cfg, args, max_len: int):
+    def __init__(self, cfg, args, max_len: int, **attention):
         super().__init__()
         self.input_layernorm = RMSNorm(cfg.hidden_size)
-        self.self_attn = Attention(cfg.hidden_size, cfg.num_attention_heads, max_len)
+        self.self_attn = Attention(cfg.hidden_size, cfg.num_attention_heads, max_len, **attention)
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size)
         self.mlp = IntegratedOpenPanguMoEMLP(cfg, args)
         self.moe_events: List = []
@@ -168,13 +206,15 @@ class Block(nn.Module):
 
 class DecoderStack(nn.Module):
     def __init__(self, layers: int = 26, hidden: int = 1536, heads: int = 12, experts: int = 16,
-                 group: int = 384, tau: float = 0.70, vocab: int = VOCAB, max_len: int = 1152):
+                 group: int = 384, tau: float = 0.70, vocab: int = VOCAB, max_len: int = 1152, qk_norm: bool = False,
+                 window: Optional[int] = None, sinks: int = 0):
         super().__init__()
         self.cfg = types.SimpleNamespace(hidden_size=hidden, intermediate_size=experts * group,
                                          num_attention_heads=heads)
         self.args = types.SimpleNamespace(group_size=group, tau=tau)
         self.embed_tokens = nn.Embedding(vocab, hidden)
-        self.layers = nn.ModuleList([Block(self.cfg, self.args, max_len) for _ in range(layers)])
+        self.layers = nn.ModuleList([Block(self.cfg, self.args, max_len, qk_norm=qk_norm, window=window, sinks=sinks)
+                                     for _ in range(layers)])
         self.norm = RMSNorm(hidden)
         self.lm_head = nn.Linear(hidden, vocab, bias=False)
 
@@ -206,7 +246,7 @@ class DecoderStack(nn.Module):
         ``pos_t`` [1]; writes the next token into ``tok_t`` and advances ``pos_t``.
         ``finite_t`` ([1] bool, optional) is and-ed with "every logit is finite"."""
         ar = torch.arange(self.layers[0].self_attn.max_len, device=tok_t.device)
-        mask = torch.where(ar <= pos_t, 0.0, float("-inf")).to(torch.float32)
+        mask = torch.where(self.layers[0].self_attn.visible(pos_t, ar), 0.0, float("-inf")).to(torch.float32)
         x = self.embed_tokens(tok_t)
         for blk in self.layers:
             x = blk.forward_static(x, pos_t, mask, moe)
@@ -232,23 +272,25 @@ class DecoderStack(nn.Module):
 
 @torch.no_grad()
 def generate(model: DecoderStack, prompts: List[torch.Tensor], steps: int, chunk: int = 512, page_size: int = 16,
-             capture: bool = True) -> torch.Tensor:
+             capture: bool = True, bits: int = 16) -> torch.Tensor:
     """Greedy tokens [seqs, steps] for prompts (int64 id tensors [length >= 1]) of any lengths, served
     together: the prompts in calls of at most ``chunk`` tokens of each, then ``steps - 1`` decode
     steps of the batch (the step captured in a graph and replayed, or eager). ``model`` in eval mode,
-    reordered for inference, with attention heads of 64 or 128 channels."""
+    reordered for inference, with attention heads of 64 or 128 channels. ``bits``: of the cache, 16 or 8."""
     lengths = [int(p.numel()) for p in prompts]
     if steps < 1 or chunk < 1 or not prompts or min(lengths) < 1 or any(p.dim() != 1 for p in prompts):
         raise ValueError("generate: at least one step, chunks and 1-D prompts of at least one token")
+    if bits not in (8, 16):
+        raise ValueError(f"generate: a cache of 8 or 16 bits (got {bits})")
     dev = model.embed_tokens.weight.device
     with torch.cuda.device(dev):  # streams and the graph are the current device's
-        return _generate(model, prompts, lengths, steps, chunk, page_size, capture, dev)
+        return _generate(model, prompts, lengths, steps, chunk, page_size, capture, dev, bits)
 
 
 @torch.no_grad()
-def _generate(model, prompts, lengths, steps, chunk, page_size, capture, dev):
+def _generate(model, prompts, lengths, steps, chunk, page_size, capture, dev, bits):
     attn = model.layers[0].self_attn
-    kv = PagedKV(len(model.layers), len(prompts), max(lengths) + steps, attn.h, attn.hd, page_size, dev)
+    kv = PagedKV(len(model.layers), len(prompts), max(lengths) + steps, attn.h, attn.hd, page_size, dev, bits)
     tok_t = torch.zeros(len(prompts), dtype=torch.int64, device=dev)
     for at in range(0, max(lengths), chunk):
         new = [min(max(n - at, 0), chunk) for n in lengths]
