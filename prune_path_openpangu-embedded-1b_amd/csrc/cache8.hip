@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t c8_top(const float (&x)[N], bool& odd) {
   for (int i = 0; i < N; ++i) top = c8_max(top, c8_bits(x[i]));
   top = c8_fold<LANES>(top);
   odd = __ballot(top > FP8_TOP) != 0;
-  if (odd) {
+  if (__builtin_expect(odd, 0)) {
     top = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) top = c8_max(top, c8_bits(x[i]) < 0x7f800000u ? c8_bits(x[i]) : 0u);
@@ -54,7 +54,19 @@ __device__ __forceinline__ uint32_t c8_top(const float (&x)[N], bool& odd) {
   return top;
 }
 
-#define C8_BYTES 4  // new tokens of a block up to which its values go out byte by byte
+#define C8_FEW 4  // new tokens of a block up to which its values go out byte by byte
+
+// x * inv as the cache takes it; `odd`: some value of the wave is not finite or beyond the largest scale's 448.
+template <int N>
+__device__ __forceinline__ void c8_scale(float (&x)[N], float inv, bool odd) {
+  if (__builtin_expect(odd, 0)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fp8_odd(x[i], inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= inv;
+  }
+}
 
 // The four of a block's value heads or key heads that the waves of a workgroup take.
 template <int D>
@@ -111,6 +123,38 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     const int h = (block * 4 + wave) * HW + lane / P, l = lane % P;  // channels 2 l and 2 l + 1
     const bool on = h < a.Hkv;
     const T* const src = (const T*)a.v + row0 * a.vs[0] + (on ? h : 0) * a.vs[1] + 2 * l;
+    auto where = [&](int page) { return (((int64_t)page * a.Hkv + (on ? h : 0)) << lb) + (place >> 4); };
+    // A few tokens go out byte by byte, unless older ones change, and skip what the places of a whole block take
+    // (256 single tokens of 12 heads 11.5 us, as a block's whole words 14.5; one 4.2 and 5.1).
+    if (nt <= C8_FEW) {
+      float x[2 * C8_FEW];
+#pragma unroll
+      for (int i = 0; i < C8_FEW; ++i) {
+        const float2 w = c8_pair(src + min(i, nt - 1) * a.vs[0]);
+        x[2 * i] = on && i < nt ? w.x : 0.0f, x[2 * i + 1] = on && i < nt ? w.y : 0.0f;
+      }
+      paged_asked();
+      const int page = place_ok ? a.seqs.page(entry) : -1;
+      if (page < 0) return;
+      const int64_t to = where(page);
+      int old = FP8_LOW;
+      if (lo > 0) old = min(max((int)a.v_scales[to], FP8_LOW), FP8_HIGH);
+      bool odd;
+      const int byte = max(fp8_scale(c8_top<P>(x, odd)), old);
+      if (__ballot(lo > 0 && byte > old) == 0) {
+        const float inv = fp8_inverse(byte);
+        c8_scale(x, inv, odd);
+        uint8_t* const dst = a.v8 + to * (APP_TOKENS * D) + 32 * l + lo;
+#pragma unroll
+        for (int i = 0; i < C8_FEW; ++i)
+          if (on && i < nt) {
+            const uint32_t w = fp8_pack(x[2 * i], x[2 * i + 1], 0.0f, 0.0f);
+            dst[i] = (uint8_t)w, dst[i + 16] = (uint8_t)(w >> 8);
+          }
+        if (on && l == 0 && lo == 0) a.v_scales[to] = (uint8_t)byte;
+        return;
+      }
+    }
     float x[2 * APP_TOKENS];
 #pragma unroll
     for (int i = 0; i < APP_TOKENS; ++i) {
@@ -121,31 +165,17 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     paged_asked();
     const int page = place_ok ? a.seqs.page(entry) : -1;
     if (page < 0) return;
-    const int64_t to = (((int64_t)page * a.Hkv + (on ? h : 0)) << lb) + (place >> 4);
+    const int64_t to = where(page);
     uint4* const dst = (uint4*)(a.v8 + to * (APP_TOKENS * D)) + 2 * l;
     uint8_t* const scale = a.v_scales + to;
     uint4 was[2] = {};
     int old = FP8_LOW;
     if (lo > 0) old = min(max((int)*scale, FP8_LOW), FP8_HIGH);
-    if (nt > C8_BYTES && nt < APP_TOKENS) was[0] = dst[0], was[1] = dst[1];  // the other places' bytes stay
+    if (nt < APP_TOKENS) was[0] = dst[0], was[1] = dst[1];  // the other places' bytes stay
     bool odd;
     const int byte = max(fp8_scale(c8_top<P>(x, odd)), old);
-    // A few tokens go out byte by byte, unless older ones change (256 single tokens of 12 heads 15.6 us, as whole words 16.1).
-    const bool bytes = nt <= C8_BYTES && __ballot(lo > 0 && byte > old) == 0;
-    if (nt <= C8_BYTES && !bytes) was[0] = dst[0], was[1] = dst[1];
     const float inv = fp8_inverse(byte), shrink = fp8_shrink(old, byte);
-#pragma unroll
-    for (int i = 0; i < 2 * APP_TOKENS; ++i) x[i] = odd ? fp8_odd(x[i], inv) : x[i] * inv;
-    if (bytes) {
-#pragma unroll
-      for (int i = 0; i < APP_TOKENS; ++i)
-        if (on && i >= lo && i < hi) {
-          const uint32_t w = fp8_pack(x[i], x[APP_TOKENS + i], 0.0f, 0.0f);
-          ((uint8_t*)dst)[i] = (uint8_t)w, ((uint8_t*)(dst + 1))[i] = (uint8_t)(w >> 8);
-        }
-      if (on && l == 0 && (lo == 0 || byte > old)) *scale = (uint8_t)byte;
-      return;
-    }
+    c8_scale(x, inv, odd);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       uint32_t w[4];
@@ -182,6 +212,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
   const T* const src = (const T*)a.k + row0 * a.ks[0] + (on ? h : 0) * a.ks[1];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
+    if (i * SLOTS >= nt) break;
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[i].p.v[j] = x[i].q.v[j] = 0;
     const int n = i * SLOTS + slot;
@@ -194,15 +225,19 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     for (int n = tid >> a.lgh; n < nt; n += APP_THREADS >> a.lgh) cs_s[n * half + pair] = rot_entry(p0 + lo + n, freq, a.mscale, 1.0f);
   const int page = place_ok ? a.seqs.page(entry) : -1;
   if (page < 0) return;
+  const int64_t to = (((int64_t)page * a.Hkv + (on ? h : 0)) << lb) + (place >> 4);
+  const int held = lo > 0 ? a.k_scales[to] : FP8_LOW;
+  paged_asked();
   __syncthreads();
   if (!on) return;  // the whole wave
-  const int64_t to = (((int64_t)page * a.Hkv + h) << lb) + (place >> 4);
   uint8_t* const dst = a.k8 + to * (APP_TOKENS * D);
-  int old = FP8_LOW;
-  if (lo > 0) old = min(max((int)a.k_scales[to], FP8_LOW), FP8_HIGH);
+  const int old = min(max(held, FP8_LOW), FP8_HIGH);
   float y[2 * 8 * NP];
 #pragma unroll
+  for (int i = 0; i < 2 * 8 * NP; ++i) y[i] = 0.0f;
+#pragma unroll
   for (int i = 0; i < NP; ++i) {
+    if (i * SLOTS >= nt) break;
     float p[8], q[8];
     rot_pairs(x[i], u < nr, p, q);
     if (a.kw) app_norm<T, HALF>(wa, wb, D, a.eps, LGU, p, q);
@@ -222,11 +257,11 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
       ((uint4*)dst)[c] = make_uint4(fp8_rescale(w.x, shrink), fp8_rescale(w.y, shrink), fp8_rescale(w.z, shrink), fp8_rescale(w.w, shrink));
     }
   }
+  c8_scale(y, inv, odd);
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    float* const v = y + 16 * i;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = odd ? fp8_odd(v[j], inv) : v[j] * inv;
+    if (i * SLOTS >= nt) break;
+    const float* const v = y + 16 * i;
     const int n = i * SLOTS + slot;
     if (n >= nt || u >= per) continue;
     uint8_t* const row = dst + (lo + n) * D;
