@@ -19,10 +19,13 @@ struct AppArgs {
   int per, nqb, nkb;   // heads per block, blocks of query and of key heads
   int vper, nvb;       // the same of the value items
   uint32_t values;     // value items
+};
+// What only appends with norms, or to a cache of 8 bits, take besides.
+struct AppMore {
   const void *qw, *kw;  // weights of the norms, NULL: none
   int w32;
   float eps;
-  uint8_t *k8, *v8;     // an 8-bit cache's pages and scales (in place of k_pages and v_pages)
+  uint8_t *k8, *v8;     // the pages and scales (in place of k_pages and v_pages)
   uint8_t *k_scales, *v_scales;
 };
 
@@ -38,7 +41,7 @@ __device__ __forceinline__ void app_norm(const float (&wa)[8], const float (&wb)
 // token i, head h at y + i * yt + h * yh. `pair`, `freq`: the thread's pair of the table and its frequency, asked for
 // by the caller. drop(): whether the tokens have no place.
 template <typename T, int D, bool HALF, bool NORM, typename F>
-__device__ __forceinline__ void app_turn(const AppArgs& a, int kind, float2* cs_s, double freq, int pair, int half, int64_t row, int nt,
+__device__ __forceinline__ void app_turn(const AppArgs& a, const AppMore& e, int kind, float2* cs_s, double freq, int pair, int half, int64_t row, int nt,
                                          int h0, int nh, int64_t p0, bf16_t* y, int64_t yt, int64_t yh, F drop) {
   const int nr = half / 8, per = nr + (D - a.rd) / 8, tid = threadIdx.x;
   const RotLanes w(tid, a.lgu, 32 - __clz(nt - 1));  // as many tokens as there are
@@ -54,7 +57,7 @@ __device__ __forceinline__ void app_turn(const AppArgs& a, int kind, float2* cs_
     for (int i = 0; i < 8; ++i) now.p.v[i] = now.q.v[i] = next.p.v[i] = next.q.v[i] = 0;
   }
   if (more) now.load(x + h * xs, w.u, nr, a.rd);
-  if constexpr (NORM) rot_weights<8, HALF>(kind == 0 ? a.qw : a.kw, a.w32, w.u, nr, per, a.rd, wa, wb);
+  if constexpr (NORM) rot_weights<8, HALF>(kind == 0 ? e.qw : e.kw, e.w32, w.u, nr, per, a.rd, wa, wb);
   paged_asked();
   if (pair < half)
     for (int t = tid >> a.lgh; t < nt; t += APP_THREADS >> a.lgh) cs_s[t * half + pair] = rot_entry(p0 + t, freq, a.mscale, 1.0f);
@@ -68,7 +71,7 @@ __device__ __forceinline__ void app_turn(const AppArgs& a, int kind, float2* cs_
       if (more) next.load(x + h2 * xs, w.u, nr, a.rd);
       float p[8], q[8];
       rot_pairs(now, w.u < nr, p, q);
-      app_norm<T, HALF>(wa, wb, D, a.eps, a.lgu, p, q);
+      app_norm<T, HALF>(wa, wb, D, e.eps, a.lgu, p, q);
       if (mine) {
         if (w.u < nr) rot_turn<8>(cs_s + w.i * half + w.u * 8, p, q);
         rot_put<8, HALF>(y + h * yh, p, q, w.u, nr, a.rd);
@@ -87,4 +90,4 @@ __device__ __forceinline__ void app_turn(const AppArgs& a, int kind, float2* cs_
 }
 
 // Of cache8.hip: the launch of an append to a cache of 8 bits, whose arguments have been checked.
-int app8_launch(const char* what, AppArgs& a, int dtype, int D, int layout, int64_t n_tokens, hipStream_t stream);
+int app8_launch(const char* what, AppArgs& a, const AppMore& e, int dtype, int D, int layout, int64_t n_tokens, hipStream_t stream);

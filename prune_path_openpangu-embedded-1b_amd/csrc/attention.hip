@@ -939,7 +939,7 @@ static AttnPlan attn_plan(int64_t n_tokens, int n_seqs, int max_pages, int page_
                           int64_t sinks) {
   AttnPlan p = {};
   const int64_t rows = n_tokens * (Hq / Hkv), cus = pp_device_cus(), room = (int64_t)max_pages * page_size;
-  const int64_t capacity = window > 0 ? std::min(room, window + std::min(sinks, room) + 2 * ATTN_ROWS) : room;
+  const int64_t capacity = window > 0 ? std::min(room, std::min(window, room) + std::min(sinks, room) + 2 * ATTN_ROWS) : room;
   auto items = [&](int tile) { return std::max<int64_t>(1, (rows / tile + n_seqs) * Hkv); };
   // Tiles of 16 rows for single tokens and the like, for what does not fill the GPU, and for what is short
   // altogether: their steps cost four times as much for the same work (6 ns for 16 rows x 128 tokens of D = 128,

@@ -74,9 +74,8 @@ struct C8Heads {
   static constexpr int V = D == 64 ? 2 : 1;  // value heads of a wave
 };
 
-#define QPER 8
 template <typename T, int D, bool HALF, bool FULL>
-__global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
+__global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppMore more) {
   constexpr int LGU = (D == 64 ? 2 : 3) + !FULL, SLOTS = 64 >> LGU, NP = APP_TOKENS / SLOTS;  // key items
   constexpr int HW = C8Heads<D>::V, P = 64 / HW;                                              // value items
   __shared__ float2 cs_s[APP_TOKENS * D / 2];
@@ -110,8 +109,8 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     const int h0 = block * a.per;
     auto drop = [] { return false; };
     bf16_t* const to = a.q_out + row0 * a.Hq * D;
-    if (a.qw) app_turn<T, D, HALF, true>(a, 0, cs_s, freq, pair, half, row0, nt, h0, min(a.per, a.Hq - h0), p0 + lo, to, (int64_t)a.Hq * D, D, drop);
-    else app_turn<T, D, HALF, false>(a, 0, cs_s, freq, pair, half, row0, nt, h0, min(a.per, a.Hq - h0), p0 + lo, to, (int64_t)a.Hq * D, D, drop);
+    if (more.qw) app_turn<T, D, HALF, true>(a, more, 0, cs_s, freq, pair, half, row0, nt, h0, min(a.per, a.Hq - h0), p0 + lo, to, (int64_t)a.Hq * D, D, drop);
+    else app_turn<T, D, HALF, false>(a, more, 0, cs_s, freq, pair, half, row0, nt, h0, min(a.per, a.Hq - h0), p0 + lo, to, (int64_t)a.Hq * D, D, drop);
     return;
   }
   const int64_t at = p0 >> a.seqs.lp;
@@ -138,20 +137,20 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
       if (page < 0) return;
       const int64_t to = where(page);
       int old = FP8_LOW;
-      if (lo > 0) old = min(max((int)a.v_scales[to], FP8_LOW), FP8_HIGH);
+      if (lo > 0) old = min(max((int)more.v_scales[to], FP8_LOW), FP8_HIGH);
       bool odd;
       const int byte = max(fp8_scale(c8_top<P>(x, odd)), old);
       if (__ballot(lo > 0 && byte > old) == 0) {
         const float inv = fp8_inverse(byte);
         c8_scale(x, inv, odd);
-        uint8_t* const dst = a.v8 + to * (APP_TOKENS * D) + 32 * l + lo;
+        uint8_t* const dst = more.v8 + to * (APP_TOKENS * D) + 32 * l + lo;
 #pragma unroll
         for (int i = 0; i < C8_FEW; ++i)
           if (on && i < nt) {
             const uint32_t w = fp8_pack(x[2 * i], x[2 * i + 1], 0.0f, 0.0f);
             dst[i] = (uint8_t)w, dst[i + 16] = (uint8_t)(w >> 8);
           }
-        if (on && l == 0 && lo == 0) a.v_scales[to] = (uint8_t)byte;
+        if (on && l == 0 && lo == 0) more.v_scales[to] = (uint8_t)byte;
         return;
       }
     }
@@ -166,8 +165,8 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     const int page = place_ok ? a.seqs.page(entry) : -1;
     if (page < 0) return;
     const int64_t to = where(page);
-    uint4* const dst = (uint4*)(a.v8 + to * (APP_TOKENS * D)) + 2 * l;
-    uint8_t* const scale = a.v_scales + to;
+    uint4* const dst = (uint4*)(more.v8 + to * (APP_TOKENS * D)) + 2 * l;
+    uint8_t* const scale = more.v_scales + to;
     uint4 was[2] = {};
     int old = FP8_LOW;
     if (lo > 0) old = min(max((int)*scale, FP8_LOW), FP8_HIGH);
@@ -219,18 +218,18 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     if (on && n < nt && u < per) x[i].load(src + n * a.ks[0], u, nr, a.rd);
   }
   float wa[8], wb[8];
-  if (a.kw) rot_weights<8, HALF>(a.kw, a.w32, u, nr, per, a.rd, wa, wb);
+  if (more.kw) rot_weights<8, HALF>(more.kw, more.w32, u, nr, per, a.rd, wa, wb);
   paged_asked();
   if (pair < half)
     for (int n = tid >> a.lgh; n < nt; n += APP_THREADS >> a.lgh) cs_s[n * half + pair] = rot_entry(p0 + lo + n, freq, a.mscale, 1.0f);
   const int page = place_ok ? a.seqs.page(entry) : -1;
   if (page < 0) return;
   const int64_t to = (((int64_t)page * a.Hkv + (on ? h : 0)) << lb) + (place >> 4);
-  const int held = lo > 0 ? a.k_scales[to] : FP8_LOW;
+  const int held = lo > 0 ? more.k_scales[to] : FP8_LOW;
   paged_asked();
   __syncthreads();
   if (!on) return;  // the whole wave
-  uint8_t* const dst = a.k8 + to * (APP_TOKENS * D);
+  uint8_t* const dst = more.k8 + to * (APP_TOKENS * D);
   const int old = min(max(held, FP8_LOW), FP8_HIGH);
   float y[2 * 8 * NP];
 #pragma unroll
@@ -240,7 +239,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
     if (i * SLOTS >= nt) break;
     float p[8], q[8];
     rot_pairs(x[i], u < nr, p, q);
-    if (a.kw) app_norm<T, HALF>(wa, wb, D, a.eps, LGU, p, q);
+    if (more.kw) app_norm<T, HALF>(wa, wb, D, more.eps, LGU, p, q);
     const int n = i * SLOTS + slot;
     const bool mine = n < nt && u < per;
     if (mine && u < nr) rot_turn<8>(cs_s + n * half + u * 8, p, q);
@@ -275,12 +274,14 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a) {
                                            fp8_pack(v[4], v[12], v[5], v[13]), fp8_pack(v[6], v[14], v[7], v[15]));
     }
   }
-  if (lane == 0) a.k_scales[to] = (uint8_t)byte;
+  if (lane == 0) more.k_scales[to] = (uint8_t)byte;
 }
 
-int app8_launch(const char* what, AppArgs& a, int dtype, int D, int layout, int64_t n_tokens, hipStream_t st) {
+int app8_launch(const char* what, AppArgs& a, const AppMore& e, int dtype, int D, int layout, int64_t n_tokens, hipStream_t st) {
   const int vheads = 4 * (D == 64 ? 2 : 1);
-  a.per = n_tokens <= 4 * (int64_t)a.seqs.n_seqs ? 32 : QPER;
+  // Query heads of an item: as of the 16-bit cache for single tokens; 8 for chunks (8192 tokens of 12 heads 35.4 us, with 4
+  // heads 35.5, with 12 41.7; 4 chunks of 2048, 24 heads on 8, 37.2, 41.5, 41.7).
+  a.per = n_tokens <= 4 * (int64_t)a.seqs.n_seqs ? 32 : 8;
   a.nqb = (a.Hq + a.per - 1) / a.per, a.nkb = (a.Hkv + 3) / 4, a.nvb = (a.Hkv + vheads - 1) / vheads;
   const int64_t groups = (n_tokens >> 4) + 2 * ((int64_t)a.seqs.n_seqs + 1), items = groups * (a.nqb + a.nkb + a.nvb);
   PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld work items (at most 2^24 - 1)", what, (long long)items);
@@ -288,8 +289,8 @@ int app8_launch(const char* what, AppArgs& a, int dtype, int D, int layout, int6
   const unsigned grid = (unsigned)items;
 #define APP8_FULL(T, D_, HALF_)                                                                        \
   do {                                                                                                 \
-    if (a.rd == D_) kv_append8_kernel<T, D_, HALF_, true><<<grid, APP_THREADS, 0, st>>>(a);            \
-    else kv_append8_kernel<T, D_, HALF_, false><<<grid, APP_THREADS, 0, st>>>(a);                      \
+    if (a.rd == D_) kv_append8_kernel<T, D_, HALF_, true><<<grid, APP_THREADS, 0, st>>>(a, e);         \
+    else kv_append8_kernel<T, D_, HALF_, false><<<grid, APP_THREADS, 0, st>>>(a, e);                   \
   } while (0)
 #define APP8(T, D_)                                             \
   do {                                                          \

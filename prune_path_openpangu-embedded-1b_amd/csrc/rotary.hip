@@ -142,7 +142,7 @@ __device__ __forceinline__ uint32_t app_pair(const float* p) {
 __device__ __forceinline__ uint32_t app_pair(const bf16_t* p) { return *(const uint32_t*)p; }
 
 template <typename T, int D, bool HALF, bool NORM>
-__global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
+__global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a, AppMore norms) {
   __shared__ float2 cs_s[APP_TOKENS * D / 2];
   const int tid = threadIdx.x;
   // the grid: value items, whose way is the longest, then query and key items
@@ -230,9 +230,36 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append_kernel(AppArgs a) {
     }
     return;
   }
+  if constexpr (!NORM) {  // (by app_turn: 106 scalar registers instead of 84, so 7 waves a SIMD, and 8192 tokens 30.3 us, not 29.1)
+    const int nr = half / 8, per = nr + (D - a.rd) / 8;
+    const RotLanes w(tid, a.lgu, 32 - __clz(nt - 1));  // as many tokens as there are
+    const int64_t row = row0 + lo + w.i;
+    const T* const x = (const T*)(kind == 0 ? a.q : a.k) + row * (kind == 0 ? a.qs[0] : a.ks[0]);
+    const int64_t xs = kind == 0 ? a.qs[1] : a.ks[1];
+    bf16_t* const y = kind == 0 ? a.q_out + row * a.Hq * D
+                                : a.k_pages + (((int64_t)entry * a.Hkv << a.seqs.lp) + place + lo + w.i) * D;
+    const int64_t ys = kind == 0 ? D : (int64_t)D << a.seqs.lp;
+    int h = h0 + w.h;
+    bool more = w.i < nt && h < h0 + nh && w.u < per;
+    RotUnit<T, 8, HALF> now, next;
+    if (more) now.load(x + h * xs, w.u, nr, a.rd);
+    paged_asked();
+    if (pair < half)
+      for (int t = tid >> a.lgh; t < nt; t += APP_THREADS >> a.lgh) cs_s[t * half + pair] = rot_entry(p0 + lo + t, freq, a.mscale, 1.0f);
+    if (kind && no_page()) return;
+    __syncthreads();
+    while (more) {
+      const int h2 = h + w.hstep;
+      more = h2 < h0 + nh;
+      if (more) next.load(x + h2 * xs, w.u, nr, a.rd);
+      now.store(y + h * ys, cs_s + w.i * half, w.u, nr, a.rd);
+      now = next, h = h2;
+    }
+    return;
+  }
   bf16_t* const to = kind == 0 ? a.q_out + (int64_t)(row0 + lo) * a.Hq * D
                                : a.k_pages + (((int64_t)entry * a.Hkv << a.seqs.lp) + place + lo) * D;
-  app_turn<T, D, HALF, NORM>(a, kind, cs_s, freq, pair, half, row0 + lo, nt, h0, nh, p0 + lo, to,
+  app_turn<T, D, HALF, true>(a, norms, kind, cs_s, freq, pair, half, row0 + lo, nt, h0, nh, p0 + lo, to,
                              kind == 0 ? (int64_t)a.Hq * D : D, kind == 0 ? D : (int64_t)D << a.seqs.lp, [&] { return kind && no_page(); });
 }
 
@@ -297,11 +324,12 @@ static int append(const char* what, const void* q, const int64_t* q_strides, con
   for (int i = 0; i < 2; ++i) a.qs[i] = q ? q_strides[i] : 0, a.ks[i] = k_strides[i], a.vs[i] = v_strides[i];
   a.q_out = (bf16_t*)q_out, a.k_pages = (bf16_t*)k_pages, a.v_pages = (bf16_t*)v_pages;
   a.inv_freq = inv_freq, a.Hq = Hq, a.Hkv = Hkv, a.rd = rotary_dim, a.mscale = mscale, a.zero_tail = zero_tail;
-  a.qw = q_weight, a.kw = k_weight, a.w32 = w_dtype == PP_DTYPE_F32, a.eps = eps;
+  AppMore e = {};
+  e.qw = q_weight, e.kw = k_weight, e.w32 = w_dtype == PP_DTYPE_F32, e.eps = eps;
   a.lgu = rot_log2up(rotary_dim / 16 + (D - rotary_dim) / 8), a.lgh = rot_log2up(std::max(rotary_dim / 2, 1));
   if (k_scales) {
-    a.k8 = (uint8_t*)k_pages, a.v8 = (uint8_t*)v_pages, a.k_scales = (uint8_t*)k_scales, a.v_scales = (uint8_t*)v_scales;
-    return app8_launch(what, a, dtype, D, layout, n_tokens, (hipStream_t)stream);
+    e.k8 = (uint8_t*)k_pages, e.v8 = (uint8_t*)v_pages, e.k_scales = (uint8_t*)k_scales, e.v_scales = (uint8_t*)v_scales;
+    return app8_launch(what, a, e, dtype, D, layout, n_tokens, (hipStream_t)stream);
   }
   // Heads of an item. Single tokens: a group has one, so all the heads that the threads hold in one step
   // (32, value heads 4, or 16 where there are workgroups enough); 1, 64, 256 sequences of 12 heads 3.5,
@@ -309,7 +337,8 @@ static int append(const char* what, const void* q, const int64_t* q_strides, con
   // 8192 tokens (151 MB, from memory) 38 us, 8 or 12 heads 42 and 41. Between them, and where a chunk is among
   // single tokens, 4 value heads: 64 sequences of 4 and 16 tokens 8.7 and 16.6 us, with 16 13.4 and 27.5; 64
   // single tokens and 512 8.9 against 13.2, 255 and 3800 24 against 34 (with one 31).
-  a.per = n_tokens <= 4 * (int64_t)n_seqs ? 32 : 4;
+  // With norms 12 query or key heads in chunks, for the sake of the weights (8192 tokens 36.5 us, with 4 heads 40.7, with 8 42.7).
+  a.per = n_tokens <= 4 * (int64_t)n_seqs ? 32 : k_weight ? 12 : 4;
   a.vper = n_tokens > 16 * (int64_t)n_seqs ? 1 : n_seqs >= 64 && n_tokens <= 2 * (int64_t)n_seqs ? 16 : 4;
   a.nqb = (Hq + a.per - 1) / a.per, a.nkb = (Hkv + a.per - 1) / a.per, a.nvb = (Hkv + a.vper - 1) / a.vper;
   const int64_t values = ((n_tokens >> 6) + 2 * ((int64_t)n_seqs + 1)) * a.nvb;
@@ -320,8 +349,8 @@ static int append(const char* what, const void* q, const int64_t* q_strides, con
   hipStream_t st = (hipStream_t)stream;
 #define APP_NORM(T, D_, HALF_)                                                                           \
   do {                                                                                                   \
-    if (k_weight) kv_append_kernel<T, D_, HALF_, true><<<grid, APP_THREADS, 0, st>>>(a);                 \
-    else kv_append_kernel<T, D_, HALF_, false><<<grid, APP_THREADS, 0, st>>>(a);                         \
+    if (k_weight) kv_append_kernel<T, D_, HALF_, true><<<grid, APP_THREADS, 0, st>>>(a, e);              \
+    else kv_append_kernel<T, D_, HALF_, false><<<grid, APP_THREADS, 0, st>>>(a, e);                      \
   } while (0)
 #define APP(T, D_)                                                                                       \
   do {                                                                                                   \

@@ -66,7 +66,7 @@ def _append(**kw):
 
 @pytest.mark.parametrize("kw,code", BOTH + [(dict(dtype=3), 1), (dict(layout=5), 1), (dict(rd=24), 3), (dict(rd=144), 3), (dict(k=None), 1), (dict(v=None), 1),
                                             (dict(out=None), 1), (dict(ksc=None), 1), (dict(vsc=None), 1), (dict(qw=None), 1), (dict(kw=None), 1),
-                                            (dict(q=None, qw=None, n=0), 0), (dict(wd=2), 1), (dict(wd=1, dtype=0), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),
+                                            (dict(q=None, qw=None, n=0), 0), (dict(wd=2), 1), (dict(qw=ODD), 1), (dict(kw=ODD), 1), (dict(wd=1, dtype=0), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),
                                             (dict(vs=(ctypes.c_int64 * 2)(1 << 14, 130)), 1), (dict(n=0, cu=None), 0), (dict(seqs=1 << 20, Hkv=32, Hq=32), 3)])
 def test_append_refusals(kw, code):
     assert _append(**kw) == code
@@ -112,7 +112,8 @@ def test_workspace_of_windows():
             sizes = [b(n, seqs, maxp, 16, hq, hkv, 128, eight, 1000, 4) for maxp in (100, 1 << 10, 1 << 16)]
             assert sizes[1] == sizes[2] and all(x <= n * hq * (64 * 130 * 4 + 4) for x in sizes)
             assert b(n, seqs, 1 << 10, 16, hq, hkv, 128, eight, -1, 4) == 0
-            assert b(n, seqs, 1 << 10, 16, hq, hkv, 128, eight, 1 << 62, 1 << 62) <= n * hq * (64 * 130 * 4 + 4)
+            for most in (1 << 62, (1 << 63) - 1):  # as without a window, or less
+                assert b(n, seqs, 1 << 10, 16, hq, hkv, 128, eight, most, most) <= n * hq * (64 * 130 * 4 + 4)
 
 
 # ------------------------------------------------------------------ the windowed walk, restated

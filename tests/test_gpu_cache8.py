@@ -346,6 +346,42 @@ def test_read(pkg, new, total, page, kv_heads, dim, eight):
     assert pkg.ops.kv_read(*cache, 0, scales=scales)[0].shape == (0, kv_heads, dim)
 
 
+def test_read_of_every_value_at_every_scale(pkg):
+    """256 bytes times the 237 scales: bfloat16 numbers, from 2^-126 to 448 * 2^119, exactly."""
+    page, heads, dim = 16, 1, 128
+    pages = 237
+    byte = (torch.arange(16 * dim) % 256).to(torch.uint8).view(16, dim)
+    k = byte.expand(pages, heads, 16, dim).contiguous().view(E4)
+    v = byte.t().expand(pages, heads, 1, dim, 16).contiguous().view(E4)
+    s = torch.arange(10, 247, dtype=torch.uint8).view(pages, 1, 1)
+    table = torch.arange(pages, dtype=torch.int32).view(1, pages)
+    lens, cu = torch.tensor([pages * 16], dtype=torch.int32), torch.tensor([0, pages * 16], dtype=torch.int32)
+    got = pkg.ops.kv_read(*(t.to(dev()) for t in (k, v, table, lens, cu)), pages * 16, scales=(s.view(E8).to(dev()), s.clone().view(E8).to(dev())))
+    want = byte.view(E4).double()[None] * torch.exp2(s.double() - 127)
+    for x in got:
+        x = x.cpu().double().view(pages, 16, dim)
+        assert bool(((x == want) | (torch.isnan(x) & torch.isnan(want))).all())
+        assert int(torch.isnan(x).sum()) == int(torch.isnan(want).sum()) > 0
+
+
+@pytest.mark.parametrize("new,total", [([1, 1], [17, 40]), ([70, 3], [90, 3])])
+def test_append_onto_the_queries_with_norms(pkg, new, total):
+    """q_out = q, both caches: the bits of a result of its own; weights that start anywhere in another tensor."""
+    ops = pkg.ops
+    b = Batch8(new, total, 16, 2, 128, seed=2)
+    f = ops.rotary_frequencies(128)[0].to(dev())
+    w = (1 + 0.3 * torch.randn(3 * 128 + 1, generator=gen(1))).to(torch.bfloat16).to(dev())
+    q, k, v = (torch.randn(b.n + 1, h, 128, generator=gen(h)).to(torch.bfloat16).to(dev()) for h in (6, 2, 2))
+    for eight in (True, False):
+        cache, scales = b.cache() if eight else (b.gpu(), None)
+        more = dict(inv_freq=f, scales=scales, q_weight=w[1:129], k_weight=w[200:328])
+        want = ops.kv_append(k, v, *cache, q=q, **more)
+        again = dict(more, q_weight=w[1:129].clone(), k_weight=w[200:328].clone())
+        own = q.clone()
+        assert ops.kv_append(k, v, *cache, q=own, q_out=own, **again) is own
+        assert torch.equal(own[:b.n], want[:b.n]) and torch.equal(own[b.n:], q[b.n:])
+
+
 def test_append_then_read_over_long_tables(pkg):
     """A cache whose places lie beyond 2^31 bytes: the last pages of one."""
     pages, page, heads, dim = 1100, 4096, 4, 128  # 2.3e9 bytes of keys, as many of values

@@ -71,7 +71,7 @@ def close(got, want, big, factor, what):
 CASES = [  # leading shape, query heads, key heads, D, rotary_dim, first position
     ((1,), 12, 12, 128, 128, 1024), ((2, 33), 4, 2, 64, 64, 0), ((3, 7), 20, 4, 80, 32, 1000000), ((5,), 3, 1, 256, 256, 7),
     ((4,), 2, 1, 256, 2, 3), ((9,), 1, 3, 2, 2, 5), ((2, 3), 3, 3, 50, 50, 9), ((70,), 5, 5, 36, 16, 1 << 33), ((600,), 12, 4, 128, 64, -3),
-    ((13,), 0, 2, 64, 64, 1), ((13,), 2, 0, 64, 32, 1), ((700,), 2, 2, 18, 18, 0)]
+    ((11,), 3, 2, 7, 2, 4), ((5000,), 12, 2, 128, 128, 0), ((13,), 0, 2, 64, 64, 1), ((13,), 2, 0, 64, 32, 1), ((700,), 2, 2, 18, 18, 0)]
 
 
 def make(lead, hq, hk, D, rd, first, dtype, wdtype, seed=0):
@@ -268,6 +268,24 @@ def test_opcheck(pkg):
                      (t.qk_norm_rotary_bwd, (q, k, q, k, wq, wk, pos, f, "half", 1.0, 1e-6, False))):
         print(f"opcheck {op}", flush=True)
         opcheck(op, args)
+
+
+def test_compiled_training_step(pkg):
+    """Traced with its gradient: the same numbers as eager."""
+    q, k, wq, wk, pos = (x.to(dev()) for x in make((40,), 4, 2, 64, 32, 3, torch.bfloat16, torch.float32))
+    f = pkg.ops.rotary_frequencies(32)[0].to(dev())
+    t = pkg._lib.torch_ops()
+    dy = [torch.randn_like(q), torch.randn_like(k)]
+
+    def run(fn):
+        leaves = [x.clone().requires_grad_() for x in (q, k, wq, wk)]
+        y = fn(*leaves)
+        return (*y, *torch.autograd.grad(y, leaves, dy))
+
+    plain = lambda a, b, c, d: t.qk_norm_rotary(a, b, c, d, pos, f, "interleaved", 1.0, 1e-5)  # noqa: E731
+    torch._dynamo.reset()
+    for a, b in zip(run(torch.compile(plain, backend="aot_eager")), run(plain)):
+        assert torch.equal(a, b)
 
 
 def test_captured_with_its_backward(pkg):
