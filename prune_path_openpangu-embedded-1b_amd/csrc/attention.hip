@@ -14,6 +14,14 @@
 // channel's tokens next to each other ([page][head][channel][token]), so V^T operands are 16-byte
 // loads, like K's.
 //
+// A cache of 8 bits (fp8.h) is widened to bfloat16, its scales with it, on the way to the matrix cores: the products are those
+// over the bfloat16 numbers that it stands for, at half of their bytes from memory. (Products of 8-bit operands would run at
+// twice the rate, but take a query or a weight in parts of four bits: two hold a query exactly, while weights below
+// 2^-17 of a row's largest would be lost to two.)
+//
+// With a window, a tile walks the first tokens that stay visible, then the tokens from the group of 16 on in which its first
+// row's window begins (AttnTile::at); what lies between is not loaded. Rows mask what is not theirs of the tile's walk.
+//
 // A workgroup takes one tile of rows of one key head over one range of tokens. Where the tiles alone
 // do not fill the GPU, a tile's tokens are cut into ranges ("splits"); the ranges' (m, l, o) go to
 // the workspace and attn_join_kernel combines them in order. The cut depends on the tile's own tokens
@@ -254,6 +262,12 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // Measured, 12 heads of 128: one token on each of 64 sequences of 8192 557 us (3.2 GB, 5.8 TB/s, where a
 // large copy reaches 4.9), of 1 to 8192 tokens 270 us (5.6 TB/s); one sequence of 1152 tokens 8.9 us with
 // the join's 3.5, chains of offsets, table, K and join rather than bytes.
+// 8 bits: a lane's 16 bytes are 16 channels of a K row, two operands of it (the queries go the same way), and 16 tokens, a
+// block, of a V channel: steps of 64 tokens with the same registers in flight, one scale a lane for each of K and V.
+// 64 sequences of 8192 tokens 283 us (1.6 GB, 5.7 TB/s), of 1 to 8192 150, one of 1152 9.0 with the join. (219 registers, two
+// waves a SIMD: the widened operands of one piece at a time; all at once spilled.)
+// A window of 1000 and 4 first tokens, 32 sequences anywhere in 16384, 24 heads on 8: 23 us (64 MB of 8 bits: five steps a
+// wave behind the chain of loads; in two ranges 23 to 25).
 template <int D, bool EIGHT, bool WIN>
 __global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(AttnArgs a) {
   constexpr int R = 16, KS = D / 32, MB = D / 16, OS = D + 4;
@@ -541,6 +555,10 @@ __global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(A
 // four, one a SIMD (319), no priorities (232).
 // Measured: 12 heads of 128, a prompt of 8192 tokens 238 us (870 TFLOP/s; as much in pages of 64), of 4096 85 us
 // (605), of 2048 37 us, 7 of them the join's; 512 new tokens at 30000 131 us (730).
+// 8 bits: the next step's 16 bytes of K and V to each thread are asked for before the present step's products, widened and stored
+// to LDS behind them: 8192 tokens 237 us, 4096 84, 512 at 30000 127.
+// A window of 1024 and 4 first tokens, 8192 tokens: 87 us (550 TFLOP/s): 19 steps of 64 tokens a tile, four of them with
+// masked places, and three tiles a CU for two places.
 #define ATTN_ROWS 128
 
 // 16 bytes per lane from memory into LDS at lds + 16 lane, by the copy path that does not pass through

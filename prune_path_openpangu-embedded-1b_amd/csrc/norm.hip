@@ -16,10 +16,10 @@
 //
 // Memory bound: x and y once; x, dy and dx in the gradient. Queries and keys are launched as two sets of workgroups, each with
 // its own weights (and their sums) in registers: with both sets in every thread, picked by the head, the backward took
-// 221 registers, two waves a SIMD and 58 us for 8192 tokens of 24 bf16 heads of 128 (151 MB) where it now takes 35 (4.3 TB/s),
-// the forward 26 where it takes 21 (101 MB, 4.8 TB/s, a large copy's rate), and the sums' launch 6.4 where it takes 4.0.
-// float32, 3333 tokens of 24 heads of 80: 12 and 21 us (4.3 and 3.6 TB/s). One token: 4.0 us, a launch, its chain of loads and
-// the sine.
+// 221 registers, two waves a SIMD and 58 us for 8192 tokens of 24 bf16 heads of 128 (151 MB) where it now takes 32 (4.7 TB/s),
+// the forward 26 where it takes 21 (101 MB, 4.8 TB/s, a large copy's rate), and the sums' launch 6.4 where it takes 3.8.
+// float32, 3333 tokens of 24 heads of 80: 11.4 and 20.9 us (4.5 and 3.7 TB/s). One token: 3.4 us, a launch, its chain of
+// loads and the sine.
 #include <algorithm>
 #include <cmath>
 
