@@ -71,16 +71,10 @@ __device__ __forceinline__ void c8_scale(float (&x)[N], float inv, bool odd) {
   }
 }
 
-// The four of a block's value heads or key heads that the waves of a workgroup take.
-template <int D>
-struct C8Heads {
-  static constexpr int V = D == 64 ? 2 : 1;  // value heads of a wave
-};
-
 template <typename T, int D, bool HALF, bool FULL>
 __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppMore more) {
   constexpr int LGU = (D == 64 ? 2 : 3) + !FULL, SLOTS = 64 >> LGU, NP = APP_TOKENS / SLOTS;  // key items
-  constexpr int HW = C8Heads<D>::V, P = 64 / HW;                                              // value items
+  constexpr int P = D / 2, HW = 64 / P;                                                       // value items: lanes of a head, heads of a wave
   __shared__ float2 cs_s[APP_TOKENS * D / 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool value = blockIdx.x < a.values;
@@ -281,7 +275,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
 }
 
 int app8_launch(const char* what, AppArgs& a, const AppMore& e, int dtype, int D, int layout, int64_t n_tokens, hipStream_t st) {
-  const int vheads = 4 * (D == 64 ? 2 : 1);
+  const int vheads = 512 / D;
   // Query heads of an item: as of the 16-bit cache for single tokens; 8 for chunks (8192 tokens of 12 heads 35.4 us, with 4
   // heads 35.5, with 12 41.7; 4 chunks of 2048, 24 heads on 8, 37.2, 41.5, 41.7).
   a.per = n_tokens <= 4 * (int64_t)a.seqs.n_seqs ? 32 : 8;
@@ -326,7 +320,7 @@ struct ReadArgs {
 
 template <int D, bool EIGHT>
 __global__ __launch_bounds__(APP_THREADS) void kv_read_kernel(ReadArgs a) {
-  constexpr int HW = C8Heads<D>::V, P = 64 / HW;
+  constexpr int P = D / 2, HW = 64 / P;  // lanes of a value head, value heads of a wave
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t nb = a.nkb + a.nvb, block = blockIdx.x % nb, t = blockIdx.x / nb;
   const bool value = block >= (uint32_t)a.nkb;
@@ -421,7 +415,7 @@ extern "C" int pp_kv_read(const void* k_pages, const void* v_pages, const void* 
   a.seqs = {cu_q, kv_lens, block_table, (int)n_rows, n_seqs, max_pages, num_pages, paged_log2(page_size)};
   a.k = k_pages, a.v = v_pages, a.k_scales = (const uint8_t*)k_scales, a.v_scales = (const uint8_t*)v_scales;
   a.k_out = (bf16_t*)k_out, a.v_out = (bf16_t*)v_out, a.Hkv = Hkv, a.zero_tail = zero_tail;
-  const int vheads = 4 * (D == 64 ? 2 : 1);
+  const int vheads = 512 / D;
   a.nkb = (Hkv + 3) / 4, a.nvb = (Hkv + vheads - 1) / vheads;
   const int64_t items = ((n_rows >> 4) + 2 * ((int64_t)n_seqs + 1)) * (a.nkb + a.nvb);
   PP_REQUIRE(items <= 0xffffff, PP_ERR_UNSUPPORTED, "%s: %lld work items (at most 2^24 - 1)", what, (long long)items);
