@@ -106,13 +106,12 @@ __device__ __forceinline__ int attn_cut(const AttnArgs& a, int nt, int ranges) {
   return max(1, min(cut, a.splits));
 }
 
-// STEP: tokens of a step, which lie on one side of the gap.
+// Tile t, of the sequence f. STEP: tokens of a step, which lie on one side of the gap.
 template <int R, bool WIN, int STEP>
-__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, int64_t t, int split, int ranges) {
+__device__ __forceinline__ AttnTile attn_tile(const AttnArgs& a, const PagedSeq& f, int64_t t, int split, int ranges) {
   AttnTile w;
   const int g = a.group;
   auto first = [g](int c, int s) { return (int64_t)c * g / R + s; };
-  const PagedSeq f = paged_find(a.seqs, t, first);
   w.s = f.s, w.c0 = f.c0;
   const int len = f.rows;
   const int64_t r0 = (t - first(w.c0, w.s)) * R;
@@ -286,7 +285,8 @@ __global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(A
   const int items = (a.tiles - 1) * a.Hkv, most = items * a.splits, b = blockIdx.x;
   const int split = b < most ? b / items : (b - most) / a.Hkv, turn = split * (items - 4) & 7;
   const int item = b < most ? (b - split * items + turn) % items : items + (b - most) % a.Hkv, h = item % a.Hkv;
-  const AttnTile w = attn_tile<R, WIN, ST>(a, item / a.Hkv, split, a.base);
+  const PagedSeq seq = paged_find(a.seqs, item / a.Hkv, [&](int c, int s) { return (int64_t)c * a.group / R + s; });
+  const AttnTile w = attn_tile<R, WIN, ST>(a, seq, item / a.Hkv, split, a.base);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
     if (split == 0) attn_zero(a, w, h, D);
@@ -577,6 +577,54 @@ __device__ __forceinline__ void attn_landed() { asm volatile("s_waitcnt vmcnt(0)
 #define ATTN_KT 64
 #define ATTN_SLACK 8.0f
 
+// The u-th tile, -1: none, and its sequence: the last ones, which attend most, first. Of 2 to 64 sequences whose caches differ
+// by more than a quarter those with the longest first (a tile's walk is about as long as that), so that no long tile begins
+// when the others end: a lane has one sequence, and finds the tiles in front of its own; the rows of none come last.
+// (us in this order and in the reverse of the batch's, caches of 16 bits: nine sequences, chunks and single tokens, 84 / 88; 20
+// chunks of up to 600 at up to 4000 126 / 154; eight prompts of up to 3000 145 / 156; a chunk of 900 at 8000 and 63 single
+// tokens 213 / 280; 63 chunks of 64 at 1000, alike, 110 / 110, and 126 if they are sorted all the same.)
+__device__ __forceinline__ int attn_order(const AttnArgs& a, int u, PagedSeq& f) {
+  const int n = a.seqs.n_seqs, lane = threadIdx.x & 63;
+  auto first = [&](int c, int s) { return (int)((int64_t)c * a.group / ATTN_ROWS + s); };  // tile of row c of sequence s
+  int t = a.tiles - 1 - u;
+  if (t < 0) return -1;
+  if (n < 2 || n > 64) {
+    f = paged_find(a.seqs, t, first);
+    return t;
+  }
+  const int s = min(lane, n - 1);
+  const int this_q = a.seqs.cu_q[s], next_q = a.seqs.cu_q[s + 1], len = a.seqs.kv_lens[s], last_q = a.seqs.cu_q[n];
+  paged_asked();
+  auto row = [&](int c) { return min(max(c, 0), a.seqs.n_rows); };
+  const bool on = lane < n;
+  const int c = s == 0 ? 0 : row(this_q), rows = max(row(next_q) - c, 0), end = row(last_q), lo = first(c, s), tail = first(end, n);
+  const int tiles = on ? max((s + 1 < n ? first(row(next_q), s + 1) : tail) - lo, 0) : 0;
+  // by lengths (up to 2^25), then by numbers; 0: no rows
+  const uint32_t key = on && rows > 0 ? (uint32_t)min(max(len, 1), (1 << 25) - 1) << 6 | (63 - lane) : 0u;
+  uint64_t mine;
+  const uint32_t most = (uint32_t)wave_max((float)(key >> 6)), least = (uint32_t)-wave_max(key ? -(float)(key >> 6) : -0x1p26f);
+  if (most - least > most / 4 && most >= least) {
+    int before = 0;
+    for (int j = 0; j < n; ++j) {
+      const uint32_t k = __builtin_amdgcn_readlane(key, j);
+      const int m = __builtin_amdgcn_readlane(tiles, j);
+      before += k > key || (k == key && j < lane) ? m : 0;
+    }
+    mine = __ballot(on && u >= before && u < before + tiles);
+    if (mine != 0) t = __builtin_amdgcn_readlane(lo + tiles - 1 - (u - before), __builtin_ctzll(mine));
+    else t = a.tiles - 1 - (u - tail);  // (in front of the tail's are all the others', `tail` of them)
+  } else {
+    mine = __ballot(on && t >= lo && t < lo + tiles);
+  }
+  if (t < 0 || t >= a.tiles) return -1;
+  const int l = mine != 0 ? __builtin_ctzll(mine) : 0;
+  f.s = mine != 0 ? l : n;
+  f.c0 = mine != 0 ? __builtin_amdgcn_readlane(c, l) : __builtin_amdgcn_readfirstlane(end);
+  f.rows = mine != 0 ? __builtin_amdgcn_readlane(rows, l) : a.seqs.n_rows - f.c0;
+  f.len = mine != 0 ? __builtin_amdgcn_readlane(len, l) : 0;
+  return t;
+}
+
 template <int D, bool EIGHT, bool WIN>
 __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kernel(AttnArgs a) {
   constexpr int KC = D / 8, NK = ATTN_KT * KC / ATTN_THREADS, NV = D * (ATTN_KT / 8) / ATTN_THREADS, MB = D / 32;
@@ -584,15 +632,18 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   __shared__ a_u4 v_s[2][D * (ATTN_KT / 8)];
   __shared__ int bad_s[2];  // first token of the buffer's step if V there was not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, e = lane >> 5;
-  // Items are (tile, split, head): the last tiles, which attend most, first, and the heads fastest.
+  // Items are (tile, split, head): the tiles that attend most first, and the heads fastest.
   // Workgroup b runs on XCD b % 8, so an XCD meets only the key heads of one remainder (of 8, or of
   // what 8 and their number have in common), whose K and V its L2 then holds.
   // The ranges that the call does have are next to each other, those that it does not behind everything: among
   // them, they left half of the XCDs with most of the work (4096 tokens at 8000 458 us instead of 306).
   const int ranges = max(1, min(attn_ranges(a), a.splits));
-  const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % ranges, tile = a.tiles - 1 - rest / ranges;
+  const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % ranges, u = rest / ranges;
+  PagedSeq seq;
+  const int tile = __builtin_amdgcn_readfirstlane(attn_order(a, u, seq));
   if (tile < 0) return;
-  const AttnTile w = attn_tile<ATTN_ROWS, WIN, ATTN_KT>(a, tile, split, ranges);
+  for (int* v : {&seq.s, &seq.c0, &seq.rows, &seq.len}) *v = __builtin_amdgcn_readfirstlane(*v);
+  const AttnTile w = attn_tile<ATTN_ROWS, WIN, ATTN_KT>(a, seq, tile, split, ranges);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
     if (split == 0) attn_zero(a, w, h, D);

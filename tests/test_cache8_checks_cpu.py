@@ -148,6 +148,51 @@ def test_walk_over_a_window(step, rows, group):
             assert attended == {t for t in met if t <= limit and (t >= first or t < sinks)}
 
 
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_tiles_in_the_order_of_their_work(group):
+    """Every tile number once, whatever the lengths; where they differ, the sequences with rows by their lengths, each one's last
+    tiles first, the rows of none last; offsets out of order give numbers within the tiles or none."""
+    rng = random.Random(group)
+    for case in range(300):
+        n = rng.choice([2, 3, 9, 40, 63, 64])
+        new = [rng.choice([0, 1, 1, 5, 128, 300]) for _ in range(n)]
+        lens = [rng.choice([0, 7, 500, 500, 4000, 1 << 26]) if case % 3 else 900 + rng.randint(0, 100) for _ in range(n)]
+        cu = [sum(new[:i]) for i in range(n + 1)]
+        rows = cu[-1] + rng.choice([0, 3, 500])
+        if case % 4 == 3:
+            cu = [rng.randint(-5, rows + 5) for _ in cu]
+        tiles = rows * group // 128 + n + 1
+        row = lambda s: 0 if s == 0 else min(max(cu[s], 0), rows)  # noqa: E731
+        first = lambda s: row(s) * group // 128 + s  # noqa: E731
+        lo, tail = [first(s) for s in range(n)], first(n)
+        count = [max(first(s + 1) - lo[s], 0) for s in range(n)]
+        key = [min(max(lens[s], 1), (1 << 25) - 1) << 6 | (63 - s) if row(s + 1) > row(s) else 0 for s in range(n)]
+        before = [sum(count[j] for j in range(n) if key[j] > key[s] or (key[j] == key[s] and j < s)) for s in range(n)]
+        some = [k >> 6 for k in key if k]
+        by_length = bool(some) and max(some) - min(some) > max(some) // 4
+        got = []
+        for u in range(tiles):
+            t = tiles - 1 - u
+            if by_length:
+                mine = [s for s in range(n) if before[s] <= u < before[s] + count[s]]
+                t = lo[mine[0]] + count[mine[0]] - 1 - (u - before[mine[0]]) if mine else tiles - 1 - (u - tail)
+            else:
+                mine = [s for s in range(n) if lo[s] <= t < lo[s] + count[s]]
+            if not 0 <= t < tiles:
+                assert case % 4 == 3
+                continue
+            if case % 4 != 3:
+                assert len(mine) <= 1 and bool(mine) == (t < tail)
+                assert not mine or mine[0] == max(s for s in range(n) if lo[s] <= t)
+            got.append((t, mine[0] if mine else n))
+        if case % 4 == 3:
+            continue
+        assert sorted(t for t, _ in got) == list(range(tiles))
+        if by_length:
+            lengths = [key[s] >> 6 if s < n else 0 for _, s in got]
+            assert lengths == sorted(lengths, reverse=True)
+
+
 def test_bytes_of_scales():
     """The least scale whose 448-fold holds a magnitude, from its bits; and the ends of bfloat16."""
     import struct
