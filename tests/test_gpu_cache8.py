@@ -464,6 +464,28 @@ def test_attention(pkg, new, total, page, heads, kv_heads, dim, eight, window, s
     assert torch.equal(own[:b.n], got[:b.n]) and torch.equal(own[b.n:].cpu(), q[b.n:])
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+@pytest.mark.parametrize("eight", [True, False], ids=["8-bit", "16-bit"])
+@pytest.mark.parametrize("seqs,spread,dim", [(2, 900, 128), (3, 900, 64), (63, 400, 64), (64, 400, 64), (64, 10, 64), (65, 400, 64)])
+def test_tiles_in_the_order_of_their_work(pkg, seqs, spread, dim, eight, window, sinks):
+    """Up to 64 sequences, and one more, in tiles of 128 rows: lengths of all kinds and nearly equal ones, sequences without rows, at
+    the ends too, rows of no sequence behind."""
+    rnd = torch.randint(0, 1 << 30, (2, seqs), generator=gen(seqs + spread)).tolist()
+    new = [(300 if seqs < 4 else [0, 1, 5, 40, 130][x % 5]) for x in rnd[0]]
+    new[0], new[-1] = (0, new[-1]) if seqs % 2 else (new[0], 0)
+    total = [n + (0 if n == 0 and x % 3 == 0 else 150 - min(n, 150) + x % spread) for n, x in zip(new, rnd[1])]
+    b = Batch8(new, total, 16, 8, dim, seed=seqs)
+    cache, scales = b.cache() if eight else (b.gpu(), None)
+    if eight:
+        b.wide()
+    q = torch.randn(b.n + 5, 64, dim, generator=gen(1)).to(torch.bfloat16)
+    got = pkg.ops.paged_attention(q.to(dev()), *cache, scales=scales, window=window or None, sinks=sinks)
+    check_attention(got[:b.n], *attend(b, q[:b.n], window, sinks), False)
+    assert not bool(got[b.n:].any())
+    again = pkg.ops.paged_attention(q.to(dev()), *cache, scales=scales, window=window or None, sinks=sinks)
+    assert torch.equal(again, got)
+
+
 @pytest.mark.parametrize("eight", [True, False], ids=["8-bit", "16-bit"])
 @pytest.mark.parametrize("new,total,heads,kv_heads,dim", [([2, 1, 3], [300, 90, 41], 4, 2, 128), ([400, 70, 1], [700, 300, 90], 64, 8, 64),
                                                            ([400, 70], [700, 300], 48, 8, 128)])
