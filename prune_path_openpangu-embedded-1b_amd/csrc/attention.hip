@@ -265,8 +265,67 @@ __device__ __forceinline__ f32x16_t mfma32a(const a_u4 a, const a_u4 b, f32x16_t
 // block, of a V channel: steps of 64 tokens with the same registers in flight, one scale a lane for each of K and V.
 // 64 sequences of 8192 tokens 283 us (1.6 GB, 5.7 TB/s), of 1 to 8192 150, one of 1152 9.0 with the join. (219 registers, two
 // waves a SIMD: the widened operands of one piece at a time; all at once spilled.)
-// A window of 1000 and 4 first tokens, 32 sequences anywhere in 16384, 24 heads on 8: 23 us (64 MB of 8 bits: five steps a
-// wave behind the chain of loads; in two ranges 23 to 25).
+// A window of 1000 and 4 first tokens, 32 sequences anywhere in 16384, 24 heads on 8: 18.4 us (64 MB of 8 bits: five steps a
+// wave behind the chain of loads).
+// A lane's sequence of up to 64: its first row, its rows; and the first row of no sequence.
+struct AttnLane {
+  int c, rows, len, end;
+};
+__device__ __forceinline__ AttnLane attn_lane(const AttnArgs& a) {
+  const int n = a.seqs.n_seqs, lane = threadIdx.x & 63, s = min(lane, n - 1);
+  const int this_q = a.seqs.cu_q[s], next_q = a.seqs.cu_q[s + 1], len = a.seqs.kv_lens[s], last_q = a.seqs.cu_q[n];
+  paged_asked();
+  auto row = [&](int c) { return min(max(c, 0), a.seqs.n_rows); };
+  AttnLane x;
+  x.c = s == 0 ? 0 : row(this_q), x.end = row(last_q), x.len = len;
+  x.rows = lane < n ? max(row(next_q) - x.c, 0) : 0;
+  return x;
+}
+// The sequence of lane l, the rows of none if l < 0.
+__device__ __forceinline__ PagedSeq attn_of(const AttnArgs& a, const AttnLane& x, int l) {
+  PagedSeq f;
+  const int at = max(l, 0), end = __builtin_amdgcn_readfirstlane(x.end);
+  f.s = l < 0 ? a.seqs.n_seqs : l;
+  f.c0 = l < 0 ? end : __builtin_amdgcn_readlane(x.c, at);
+  f.rows = l < 0 ? a.seqs.n_rows - end : __builtin_amdgcn_readlane(x.rows, at);
+  f.len = l < 0 ? 0 : __builtin_amdgcn_readlane(x.len, at);
+  return f;
+}
+// The sum of v over the lanes up to this one.
+__device__ __forceinline__ int attn_scan(int v) {
+#define ATTN_SCAN(ctrl, rows) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false)
+  ATTN_SCAN(0x111, 0xf);
+  ATTN_SCAN(0x112, 0xf);
+  ATTN_SCAN(0x114, 0xf);
+  ATTN_SCAN(0x118, 0xf);
+  ATTN_SCAN(0x142, 0xa);
+  ATTN_SCAN(0x143, 0xc);
+#undef ATTN_SCAN
+  return v;
+}
+
+// Tile u of those that have rows, -1: none, and its sequence. The numbers of tiles have gaps (a sequence takes one more than it
+// may need); of up to 64 sequences those with rows come first, so that their workgroups are the first ones of the grid and
+// find a CU each where there are that many: workgroups of the gaps among them held places for the moment in which the last
+// ones were given out, two to a CU while others went idle (32 single tokens, 24 heads on 8, a window of 1000: 18.7 us instead of
+// 22.8 over 8 bits, 24.4 instead of 31.7 over 16; 64 of 500 tokens, 12 heads, 22.8 instead of 24.3).
+__device__ __forceinline__ int attn_filled(const AttnArgs& a, int u, PagedSeq& f) {
+  const int n = a.seqs.n_seqs;
+  if (n < 1 || n > 64) {
+    f = paged_find(a.seqs, u, [&](int c, int s) { return (int64_t)c * a.group / 16 + s; });
+    return u;
+  }
+  const AttnLane x = attn_lane(a);
+  auto first = [&](int c, int s) { return (int)((int64_t)c * a.group / 16 + s); };
+  const int tiles = (int)(((int64_t)x.rows * a.group + 15) / 16), upto = attn_scan(tiles);
+  const int all = __builtin_amdgcn_readlane(upto, 63);
+  const uint64_t mine = __ballot(u < upto && u >= upto - tiles);
+  const int l = mine != 0 ? __builtin_ctzll(mine) : -1;
+  f = attn_of(a, x, l);
+  if (l < 0) return first(f.c0, n) + u - all;  // (beyond its rows: a tile without any)
+  return first(f.c0, l) + u - __builtin_amdgcn_readlane(upto - tiles, l);
+}
+
 template <int D, bool EIGHT, bool WIN>
 __global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(AttnArgs a) {
   constexpr int R = 16, KS = D / 32, MB = D / 16, OS = D + 4;
@@ -285,8 +344,10 @@ __global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(A
   const int items = (a.tiles - 1) * a.Hkv, most = items * a.splits, b = blockIdx.x;
   const int split = b < most ? b / items : (b - most) / a.Hkv, turn = split * (items - 4) & 7;
   const int item = b < most ? (b - split * items + turn) % items : items + (b - most) % a.Hkv, h = item % a.Hkv;
-  const PagedSeq seq = paged_find(a.seqs, item / a.Hkv, [&](int c, int s) { return (int64_t)c * a.group / R + s; });
-  const AttnTile w = attn_tile<R, WIN, ST>(a, seq, item / a.Hkv, split, a.base);
+  PagedSeq seq;
+  const int tile = __builtin_amdgcn_readfirstlane(attn_filled(a, item / a.Hkv, seq));
+  for (int* v : {&seq.s, &seq.c0, &seq.rows, &seq.len}) *v = __builtin_amdgcn_readfirstlane(*v);
+  const AttnTile w = attn_tile<R, WIN, ST>(a, seq, tile, split, a.base);
   if (w.nr <= 0) return;
   if (w.ns == 0) {
     if (split == 0) attn_zero(a, w, h, D);
@@ -592,15 +653,12 @@ __device__ __forceinline__ int attn_order(const AttnArgs& a, int u, PagedSeq& f)
     f = paged_find(a.seqs, t, first);
     return t;
   }
-  const int s = min(lane, n - 1);
-  const int this_q = a.seqs.cu_q[s], next_q = a.seqs.cu_q[s + 1], len = a.seqs.kv_lens[s], last_q = a.seqs.cu_q[n];
-  paged_asked();
-  auto row = [&](int c) { return min(max(c, 0), a.seqs.n_rows); };
+  const AttnLane x = attn_lane(a);
   const bool on = lane < n;
-  const int c = s == 0 ? 0 : row(this_q), rows = max(row(next_q) - c, 0), end = row(last_q), lo = first(c, s), tail = first(end, n);
-  const int tiles = on ? max((s + 1 < n ? first(row(next_q), s + 1) : tail) - lo, 0) : 0;
+  const int s = min(lane, n - 1), lo = first(x.c, s), tail = first(x.end, n);
+  const int next = __shfl(lo, min(lane + 1, n - 1)), tiles = on ? max((s + 1 < n ? next : tail) - lo, 0) : 0;
   // by lengths (up to 2^25), then by numbers; 0: no rows
-  const uint32_t key = on && rows > 0 ? (uint32_t)min(max(len, 1), (1 << 25) - 1) << 6 | (63 - lane) : 0u;
+  const uint32_t key = on && x.rows > 0 ? (uint32_t)min(max(x.len, 1), (1 << 25) - 1) << 6 | (63 - lane) : 0u;
   uint64_t mine;
   const uint32_t most = (uint32_t)wave_max((float)(key >> 6)), least = (uint32_t)-wave_max(key ? -(float)(key >> 6) : -0x1p26f);
   if (most - least > most / 4 && most >= least) {
@@ -617,11 +675,7 @@ __device__ __forceinline__ int attn_order(const AttnArgs& a, int u, PagedSeq& f)
     mine = __ballot(on && t >= lo && t < lo + tiles);
   }
   if (t < 0 || t >= a.tiles) return -1;
-  const int l = mine != 0 ? __builtin_ctzll(mine) : 0;
-  f.s = mine != 0 ? l : n;
-  f.c0 = mine != 0 ? __builtin_amdgcn_readlane(c, l) : __builtin_amdgcn_readfirstlane(end);
-  f.rows = mine != 0 ? __builtin_amdgcn_readlane(rows, l) : a.seqs.n_rows - f.c0;
-  f.len = mine != 0 ? __builtin_amdgcn_readlane(len, l) : 0;
+  f = attn_of(a, x, mine != 0 ? __builtin_ctzll(mine) : -1);
   return t;
 }
 

@@ -193,6 +193,44 @@ def test_tiles_in_the_order_of_their_work(group):
             assert lengths == sorted(lengths, reverse=True)
 
 
+@pytest.mark.parametrize("group", [1, 3, 8, 16, 40])
+def test_tiles_with_rows_come_first(group):
+    """16-row tiles of up to 64 sequences: every row of a sequence, and of none, once; no tile without rows before one of a
+    sequence with some; offsets out of order stay inside."""
+    rng = random.Random(group)
+    for case in range(300):
+        n = rng.choice([1, 2, 9, 33, 63, 64])
+        new = [rng.choice([0, 1, 1, 1, 2, 17]) for _ in range(n)]
+        cu = [sum(new[:i]) for i in range(n + 1)]
+        N = cu[-1] + rng.choice([0, 1, 40])
+        if N == 0:
+            continue
+        if case % 4 == 3:
+            cu = [rng.randint(-5, N + 5) for _ in cu]
+        row = lambda s: 0 if s == 0 else min(max(cu[s], 0), N)  # noqa: E731
+        first = lambda c, s: c * group // 16 + s  # noqa: E731
+        rows = [max(row(s + 1) - row(s), 0) for s in range(n)]
+        tiles = [(r * group + 15) // 16 for r in rows]
+        upto = [sum(tiles[:s + 1]) for s in range(n)]
+        seen, empty = [], False
+        for u in range(N * group // 16 + n + 1):
+            mine = [s for s in range(n) if upto[s] - tiles[s] <= u < upto[s]]
+            s = mine[0] if mine else n
+            c0, length = (row(s), rows[s]) if mine else (row(n), N - row(n))
+            t = first(c0, s) + u - (upto[s] - tiles[s] if mine else upto[-1])
+            r0 = (t - first(c0, s)) * 16
+            nr = max(0, min(16, length * group - r0)) if r0 >= 0 else 0
+            for r in range(nr):
+                i, h = divmod(r0 + r, group)
+                assert 0 <= c0 + i < N
+                seen.append((c0 + i, h))
+            if case % 4 != 3:
+                assert not (empty and mine)
+                empty = empty or nr == 0 or not mine
+        if case % 4 != 3:
+            assert sorted(seen) == [(i, h) for i in range(N) for h in range(group)]
+
+
 def test_bytes_of_scales():
     """The least scale whose 448-fold holds a magnitude, from its bits; and the ends of bfloat16."""
     import struct
