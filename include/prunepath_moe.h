@@ -398,8 +398,8 @@ int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const i
 
 /* pp_kv_append with the norms of queries and keys on the way, into a cache of 16 or of 8 bits.
  *
- * q_weight, k_weight [D] (w_dtype: float32, or dtype; both NULL: no norms; q_weight NULL without q): every head is
- * normed as above before it is turned.
+ * q_weight, k_weight [D] (w_dtype: float32, or dtype; 16-byte aligned; both NULL: no norms; q_weight NULL without q): every
+ * head is normed as above before it is turned.
  *
  * k_scales, v_scales (both NULL: the bfloat16 cache): a cache of 8 bits. k_pages [num_pages][Hkv][page_size][D] and
  * v_pages [num_pages][Hkv][page_size / 16][D][16] hold e4m3 values, k_scales and v_scales
