@@ -406,7 +406,8 @@ int pp_kv_append(const void* q, const int64_t* q_strides, const void* k, const i
  * [num_pages][Hkv][page_size / 16] a power of two for each block of 16 places as its biased exponent (2^(byte - 127),
  * bytes 10 to 246). A block's scale is the least whose 448-fold holds the call's values in it; where the sequence has tokens
  * in the block in front of the call's (appended before), at least the scale that they have, and they are brought to
- * the new one. Each value is rounded once, from float32, to nearest even; what is not finite is held as NaN and
+ * the new one; a stored byte below 10 or above 246 (of a cache that was quantised elsewhere; 255: no number) is first brought
+ * to that range, what then exceeds 448 as 448, or NaN where bfloat16 has no room for it. Each value is rounded once, from float32, to nearest even; what is not finite is held as NaN and
  * does not count in the scale. No two sequences may share a block that the call writes. */
 int pp_kv_append_with(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                       const int64_t* v_strides, int dtype, int64_t n_tokens, int n_seqs, const int32_t* cu_q,

@@ -133,11 +133,10 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
       const int page = place_ok ? a.seqs.page(entry) : -1;
       if (page < 0) return;
       const int64_t to = where(page);
-      int old = FP8_LOW;
-      if (lo > 0) old = min(max((int)more.v_scales[to], FP8_LOW), FP8_HIGH);
+      const int held = lo > 0 ? more.v_scales[to] : FP8_LOW;
       bool odd;
-      const int byte = max(fp8_scale(c8_top<P>(x, odd)), old);
-      if (__ballot(lo > 0 && byte > old) == 0) {
+      const int byte = max(fp8_scale(c8_top<P>(x, odd)), min(max(held, FP8_LOW), FP8_HIGH));
+      if (__ballot(lo > 0 && byte != held) == 0) {
         const float inv = fp8_inverse(byte);
         c8_scale(x, inv, odd);
         uint8_t* const dst = more.v8 + to * (APP_TOKENS * D) + 32 * l + lo;
@@ -165,12 +164,11 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
     uint4* const dst = (uint4*)(more.v8 + to * (APP_TOKENS * D)) + 2 * l;
     uint8_t* const scale = more.v_scales + to;
     uint4 was[2] = {};
-    int old = FP8_LOW;
-    if (lo > 0) old = min(max((int)*scale, FP8_LOW), FP8_HIGH);
+    const int held = lo > 0 ? *scale : FP8_LOW;
     if (nt < APP_TOKENS) was[0] = dst[0], was[1] = dst[1];  // the other places' bytes stay
     bool odd;
-    const int byte = max(fp8_scale(c8_top<P>(x, odd)), old);
-    const float inv = fp8_inverse(byte), shrink = fp8_shrink(old, byte);
+    const int byte = max(fp8_scale(c8_top<P>(x, odd)), min(max(held, FP8_LOW), FP8_HIGH));
+    const float inv = fp8_inverse(byte), bring = fp8_step(held, byte);
     c8_scale(x, inv, odd);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -190,8 +188,8 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
             fresh |= 4 * j + i >= lo && 4 * j + i < hi ? 0xffu << (8 * i) : 0u;
             kept |= 4 * j + i < lo ? 0xffu << (8 * i) : 0u;
           }
-          const uint32_t held = byte > old ? (fp8_rescale(before[j], shrink) & kept) | (before[j] & ~kept) : before[j];
-          w[j] = (w[j] & fresh) | (held & ~fresh);
+          const uint32_t old = lo > 0 && byte != held ? (fp8_rescale(before[j], bring) & kept) | (before[j] & ~kept) : before[j];
+          w[j] = (w[j] & fresh) | (old & ~fresh);
         }
       }
       if (on) dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -227,7 +225,6 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
   __syncthreads();
   if (!on) return;  // the whole wave
   uint8_t* const dst = more.k8 + to * (APP_TOKENS * D);
-  const int old = min(max(held, FP8_LOW), FP8_HIGH);
   float y[2 * 8 * NP];
 #pragma unroll
   for (int i = 0; i < 2 * 8 * NP; ++i) y[i] = 0.0f;
@@ -244,13 +241,13 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
     for (int j = 0; j < 8; ++j) y[16 * i + j] = mine ? p[j] : 0.0f, y[16 * i + 8 + j] = mine ? q[j] : 0.0f;
   }
   bool odd;
-  const int byte = max(fp8_scale(c8_top<64>(y, odd)), old);
+  const int byte = max(fp8_scale(c8_top<64>(y, odd)), min(max(held, FP8_LOW), FP8_HIGH));
   const float inv = fp8_inverse(byte);
-  if (lo > 0 && byte > old) {
-    const float shrink = fp8_shrink(old, byte);
+  if (lo > 0 && byte != held) {  // (a block of elsewhere may have any scale)
+    const float bring = fp8_step(held, byte);
     for (int c = lane; c < lo * (D / 16); c += 64) {
       const uint4 w = ((const uint4*)dst)[c];
-      ((uint4*)dst)[c] = make_uint4(fp8_rescale(w.x, shrink), fp8_rescale(w.y, shrink), fp8_rescale(w.z, shrink), fp8_rescale(w.w, shrink));
+      ((uint4*)dst)[c] = make_uint4(fp8_rescale(w.x, bring), fp8_rescale(w.y, bring), fp8_rescale(w.z, bring), fp8_rescale(w.w, bring));
     }
   }
   c8_scale(y, inv, odd);

@@ -410,8 +410,8 @@ def paged_cache8(num_pages: int, page_size: int, kv_heads: int, head_dim: int, d
     """((k_pages, v_pages), scales): a cache of 8 bits, float8_e4m3fn, for ``kv_append``, ``kv_read`` and ``paged_attention``
     with ``scales=scales``. k_pages [num_pages, kv_heads, page_size, head_dim], v_pages [num_pages, kv_heads, page_size / 16,
     head_dim, 16] (a channel's 16 tokens next to each other), scales = (k_scales, v_scales), each [num_pages, kv_heads,
-    page_size / 16] float8_e8m0fnu: a power of two for each block of 16 tokens and head. Uninitialised, sizes as of
-    ``paged_cache``."""
+    page_size / 16] float8_e8m0fnu: a power of two for each block of 16 tokens and head, from 2^-117 to 2^119 as an append
+    writes them (bytes 10 to 246: a value times its scale is a bf16 number). Uninitialised, sizes as of ``paged_cache``."""
     blocks = page_size // 16
     k = torch.empty(num_pages, kv_heads, page_size, head_dim, dtype=torch.float8_e4m3fn, device=device)
     v = torch.empty(num_pages, kv_heads, blocks, head_dim, 16, dtype=torch.float8_e4m3fn, device=device)
@@ -446,7 +446,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
 
     scales (``paged_cache8``): the cache is one of 8 bits. A block of 16 places and one head has one scale, the least power of
     two whose 448-fold holds the call's values in it; where the sequence has earlier tokens in the block, at least
-    theirs, and if the scale grows they are brought to it in place (exactly, but for what falls below 2^-6 of it). Values are
+    theirs, and if the scale grows they are brought to it in place (exactly, but for what falls below 2^-6 of it); a scale
+    beyond 2^-117 to 2^119, of a cache that was quantised elsewhere, is brought between them in the same way (what exceeds 448 times the
+    largest becomes that, or NaN if bf16 has no room for it). Values are
     rounded once, from fp32, to nearest even; one that is not finite is held as NaN and does not count in the scale. No two
     sequences may share a block that the call writes, and what else reads those blocks is ordered with it.
 
