@@ -72,12 +72,25 @@ class Attention(nn.Module):
         self.qkv = nn.Linear(d, 3 * d, bias=False)
         self.o = nn.Linear(d, d, bias=False)
         self.q_norm, self.k_norm = (RMSNorm(self.hd), RMSNorm(self.hd)) if qk_norm else (None, None)
-        self.inv_freq = None
+        self.inv_freq = None  # float64, which a buffer would not stay
+        if qk_norm:
+            self.place_frequencies(self.qkv.weight.device)
         self.window, self.sinks = window, sinks
         self.max_len = max_len
         self.kt_cache = None  # [B, h, hd, max_len]: K kept transposed
         self.v_cache = None   # [B, h, max_len, hd]
         self.len = 0
+
+    def place_frequencies(self, device):
+        """The rotation's angles on ``device``, as an ordinary tensor whatever mode the caller is in: a backward may save it."""
+        with torch.inference_mode(False), torch.device("cpu"):
+            self.inv_freq = ops.rotary_frequencies(self.hd)[0].to(device)
+
+    def _apply(self, fn, *args, **kwargs):  # what moves or converts the layer moves them
+        super()._apply(fn, *args, **kwargs)
+        if self.inv_freq is not None:
+            self.place_frequencies(self.qkv.weight.device)
+        return self
 
     def reset(self, B: int, device, dtype):
         self.kt_cache = torch.zeros(B, self.h, self.hd, self.max_len, device=device, dtype=dtype)
@@ -91,8 +104,8 @@ class Attention(nn.Module):
         q, k, v = qkv.permute(2, 0, 3, 1, 4)
         if self.q_norm is None:
             return rope(q, pos), rope(k, pos), v
-        if self.inv_freq is None or self.inv_freq.device != x.device:  # (float64, which a buffer would not stay)
-            self.inv_freq, _ = ops.rotary_frequencies(self.hd, device=x.device)
+        if self.inv_freq.device != x.device:  # weights that were put in place from elsewhere
+            self.place_frequencies(x.device)
         q, k = ops.qk_norm_rotary(qkv[:, :, 0], qkv[:, :, 1], self.q_norm.weight, self.k_norm.weight, pos.expand(B, L),
                                   self.inv_freq, eps=self.q_norm.eps)
         return q.transpose(1, 2), k.transpose(1, 2), v
