@@ -856,6 +856,8 @@ void paged_check(const char* name, const Tensor& k_pages, const Tensor& v_pages,
   TORCH_CHECK(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && kv_lens.dim() == 1 &&
                   kv_lens.scalar_type() == at::kInt && cu_q.dim() == 1 && cu_q.scalar_type() == at::kInt,
               "prunepath.", name, ": block_table [seqs, max_pages], kv_lens [seqs] and cu_q [seqs + 1] must be int32");
+  for (const Tensor* t : {&k_pages, &v_pages, &block_table, &kv_lens, &cu_q, k_scales ? &*k_scales : &k_pages, v_scales ? &*v_scales : &v_pages})
+    TORCH_CHECK(t->is_contiguous(), "prunepath.", name, ": the cache, its scales, block_table, kv_lens and cu_q must be contiguous");
   const c10::SymInt seqs = kv_lens.sym_size(0), Hkv = k_pages.sym_size(1);
   TORCH_SYM_CHECK(block_table.sym_size(0).sym_eq(seqs).sym_and(cu_q.sym_size(0).sym_eq(seqs + 1)), "prunepath.", name,
                   ": block_table ", block_table.sym_sizes(), ", kv_lens ", kv_lens.sym_sizes(), " and cu_q ",
@@ -901,8 +903,8 @@ void kv_append_check(const Tensor* q, const Tensor* q_out, const Tensor& k, cons
   for (const optional<Tensor>* w : {&q_weight, &k_weight})
     if (*w) {
       TORCH_CHECK((*w)->dim() == 1 && ((*w)->scalar_type() == at::kFloat || (*w)->scalar_type() == k.scalar_type()) &&
-                      (*w)->scalar_type() == (*k_weight).scalar_type(),
-                  "prunepath.kv_append: weights must be [D], both float32 or both like k");
+                      (*w)->scalar_type() == (*k_weight).scalar_type() && (*w)->is_contiguous(),
+                  "prunepath.kv_append: weights must be contiguous [D], both float32 or both like k");
       TORCH_SYM_CHECK((*w)->sym_size(0).sym_eq(k.sym_size(2)), "prunepath.kv_append: ", (*w)->sym_size(0), " weights for heads of ",
                       k.sym_size(2), " channels");
     }
@@ -911,8 +913,8 @@ void kv_append_check(const Tensor* q, const Tensor* q_out, const Tensor& k, cons
   TORCH_SYM_CHECK(k.sym_stride(2).sym_eq(1).sym_and(v.sym_stride(2).sym_eq(1)),
                   "prunepath.kv_append: channels must be contiguous");
   if (inv_freq) {
-    TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1,
-                "prunepath.kv_append: inv_freq must be float64 [rotary_dim / 2]");
+    TORCH_CHECK(inv_freq->scalar_type() == at::kDouble && inv_freq->dim() == 1 && inv_freq->is_contiguous(),
+                "prunepath.kv_append: inv_freq must be contiguous float64 [rotary_dim / 2]");
     const c10::SymInt rd = inv_freq->sym_size(0) * 2;
     TORCH_SYM_CHECK(rd.sym_le(k.sym_size(2)).sym_and((rd % 16).sym_eq(0)), "prunepath.kv_append: rotary_dim ", rd,
                     " unsupported (a multiple of 16 up to the head size ", k.sym_size(2), ")");

@@ -395,3 +395,34 @@ def test_wrappers_refuse():
                 lambda: ops.kv_read(*cache, 3, scales=s, out=(x, x))):
         with pytest.raises(RuntimeError, match="prunepath"):
             bad()
+
+
+def test_fake_calls_refuse_strided_arguments():
+    """What a real call takes contiguous only, a traced one does too: the weights of an append's norms, the frequencies, the cache, its
+    scales and the batch's integers."""
+    import torch
+    t, q, k, v, c, s, f, w = _fake8()
+
+    def strided(x):  # its shape, every other element of a row
+        return torch.empty(*x.shape[:-1], 2 * x.shape[-1], dtype=x.dtype, device=x.device)[..., ::2]
+
+    def put(args, i, x):
+        return (*args[:i], x, *args[i + 1:])
+
+    calls = [lambda c=c, s=s, f=f, w=w: t.kv_append_q(q, k, v, *c, f, "half", 1.0, *w, 1e-6, *s),
+             lambda c=c, s=s, f=f, w=w: t.kv_append_q_into(q, torch.empty_like(q), k, v, *c, f, "half", 1.0, *w, 1e-6, *s),
+             lambda c=c, s=s, f=f, w=w: t.kv_append(k, v, *c, f, "half", 1.0, w[1], 1e-6, *s)]
+    reads = [lambda c=c, s=s: t.kv_read(*c, 5, *s), lambda c=c, s=s: t.kv_read_into(*c, torch.empty_like(k), torch.empty_like(v), *s),
+             lambda c=c, s=s: t.paged_attention(q, *c, 0.1, *s, 7, 1), lambda c=c, s=s: t.paged_attention_into(q, *c, 0.1, torch.empty_like(q), *s)]
+    bad = []
+    for call in calls:
+        call()
+        bad += [(call, dict(f=strided(f))), (call, dict(w=put(w, 1, strided(w[1]))))]
+    bad += [(call, dict(w=put(w, 0, strided(w[0])))) for call in calls[:2]]
+    for call in calls + reads:
+        call()
+        bad += [(call, dict(c=put(c, i, strided(c[i])))) for i in range(5)] + [(call, dict(s=put(s, i, strided(s[i])))) for i in range(2)]
+    for call, kw in bad:
+        with pytest.raises(RuntimeError, match="prunepath.*contiguous"):
+            call(**kw)
+            print("not refused:", list(kw))
