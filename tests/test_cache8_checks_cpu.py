@@ -426,3 +426,49 @@ def test_fake_calls_refuse_strided_arguments():
         with pytest.raises(RuntimeError, match="prunepath.*contiguous"):
             call(**kw)
             print("not refused:", list(kw))
+
+
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_gaps_come_behind_the_tiles_of_uneven_batches(group):
+    """128-row tiles of sequences whose lengths differ by more than a quarter, restated: every row of a sequence, and of none, once, the
+    longest sequences first, each one's last tiles first, no tile without rows before one of a sequence with some; the four waves' counts
+    together are those of one; offsets out of order stay inside."""
+    rng = random.Random(group)
+    for case in range(60):
+        n = rng.choice([2, 3, 9, 40, 63, 64])
+        new = [rng.choice([0, 1, 1, 5, 128, 200, 300]) for _ in range(n)]
+        lens = [rng.choice([0, 7, 500, 500, 4000, 1 << 26]) for _ in range(n)]
+        cu = [sum(new[:i]) for i in range(n + 1)]
+        N = cu[-1] + rng.choice([0, 3, 500])
+        if case % 4 == 3:
+            cu = [rng.randint(-5, N + 5) for _ in cu]
+        row = lambda s: 0 if s == 0 else min(max(cu[s], 0), N)  # noqa: E731
+        first = lambda c, s: c * group // 128 + s  # noqa: E731
+        rows = [max(row(s + 1) - row(s), 0) for s in range(n)] + [0] * (64 - n)
+        tiles = [-(-r * group // 128) for r in rows]
+        key = [((min(max(lens[s], 1), (1 << 25) - 1) << 6) if tiles[s] else 0) | (63 - s) for s in range(n)] + [63 - s for s in range(n, 64)]
+        assert len(set(key)) == 64
+        parts = [[sum(tiles[j] for j in range(16 * w, 16 * w + 16) if key[j] > key[s]) for s in range(64)] for w in range(4)]
+        before, total = [sum(p[s] for p in parts) for s in range(64)], sum(tiles)
+        seen, order, empty = [], [], False
+        for u in range(N * group // 128 + n + 1):
+            mine = [s for s in range(64) if before[s] <= u < before[s] + tiles[s]]
+            assert len(mine) <= 1
+            s = mine[0] if mine else n
+            c0, length = (row(s), rows[s]) if mine else (row(n), N - row(n))
+            t = first(c0, s) + (before[s] + tiles[s] - 1 - u if mine else u - total)
+            r0 = (t - first(c0, s)) * 128
+            assert r0 >= 0
+            nr = max(0, min(128, length * group - r0))
+            for r in range(nr):
+                i, h = divmod(r0 + r, group)
+                assert 0 <= c0 + i < N
+                seen.append((c0 + i, h))
+            if case % 4 != 3:
+                assert not (empty and mine) and (not mine or nr)
+                empty = empty or not mine
+                if mine:
+                    order.append((key[s], r0))
+        if case % 4 != 3:
+            assert sorted(seen) == [(i, h) for i in range(N) for h in range(group)]
+            assert order == sorted(order, reverse=True)

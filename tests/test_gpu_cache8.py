@@ -713,3 +713,31 @@ def test_refusals(pkg):
                 lambda: ops.kv_read(kb, vb, *c[2:], out=(kb.view(-1)[:256].view(2, 2, 64), out))):
         with pytest.raises(RuntimeError, match="prunepath"):
             bad()
+
+
+# ------------------------------------------------------------------ uneven batches
+@pytest.mark.parametrize("eight", [True, False], ids=["8-bit", "16-bit"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 4), (60, 0)])
+@pytest.mark.parametrize("seqs,kv_heads,group,dim", [(2, 8, 4, 128), (20, 8, 1, 64), (64, 8, 2, 64), (63, 8, 1, 128)])
+def test_uneven_batches_of_more_tiles_than_one(pkg, seqs, kv_heads, group, dim, window, sinks, eight):
+    """128-row tiles, up to five a sequence, of caches between one and a few thousand tokens: with gaps in the tiles' numbers, sequences
+    without rows, and rows of no sequence behind. In any order of the batch the same bits."""
+    rnd = torch.randint(0, 1 << 30, (2, seqs), generator=gen(seqs + dim)).tolist()
+    new = [(150 if seqs > 2 else 500) + x % 60 if x % 5 else 0 for x in rnd[0]]
+    new[0] = new[0] or 131
+    total = [n + (x % 2600 if x % 3 else x % 40) for n, x in zip(new, rnd[1])]
+    order = torch.randperm(seqs, generator=gen(4)).tolist()
+    b = Batch8(new, total, 16, kv_heads, dim, seed=seqs)
+    cache, scales = b.cache() if eight else (b.gpu(), None)
+    if eight:
+        b.wide()
+    q = torch.randn(b.n + 3, kv_heads * group, dim, generator=gen(1)).to(torch.bfloat16)
+    kw = dict(scales=scales, window=window or None, sinks=sinks)
+    got = pkg.ops.paged_attention(q.to(dev()), *cache, **kw)
+    check_attention(got[:b.n], *attend(b, q[:b.n], window, sinks), False)
+    assert not bool(got[b.n:].any())
+    rows = torch.cat([torch.arange(int(b.cu[s]), int(b.cu[s + 1])) for s in order])
+    cu = torch.tensor([0] + [new[s] for s in order]).cumsum(0).int().to(dev())
+    at = torch.tensor(order, device=dev())
+    other = pkg.ops.paged_attention(q[rows].to(dev()), *cache[:2], cache[2][at].contiguous(), cache[3][at].contiguous(), cu, **kw)
+    assert torch.equal(other, got[rows.to(dev())])
