@@ -638,16 +638,21 @@ __device__ __forceinline__ void attn_landed() { asm volatile("s_waitcnt vmcnt(0)
 #define ATTN_KT 64
 #define ATTN_SLACK 8.0f
 
-// The u-th tile, -1: none, and its sequence: the last ones, which attend most, first. Of 2 to 64 sequences whose caches differ
-// by more than a quarter those with the longest first (a tile's walk is about as long as that), so that no long tile begins
-// when the others end: a lane has one sequence, and finds the tiles in front of its own, each wave for 16 of the sequences (lds:
-// 256 numbers). There the tiles that have rows come before the gaps in the numbers, which otherwise hold places while the last
-// of them are given out: 30 chunks of 200 tokens at 1050 to 1500, 12 heads of 64, 60 us with the gaps in between, 46 without;
-// 49 in the batch's order. (Sorted in every wave for all the sequences, one at a time: 63 chunks of 64 at 670 to 1000, 12 heads of
-// 128, 86 us, like this 79, in the batch's order 80.)
-// (us in this order and in the reverse of the batch's, caches of 16 bits: nine sequences, chunks and single tokens, 84 / 88; 20
-// chunks of up to 600 at up to 4000 126 / 154; eight prompts of up to 3000 145 / 156; a chunk of 900 at 8000 and 63 single
-// tokens 213 / 280; 63 chunks of 64 at 1000, alike, 110 / 110, and 126 if they are sorted all the same.)
+// The u-th tile, -1: none, and its sequence: the last ones, which attend most, first. Of 2 to 64 sequences whose longest walks differ
+// by more than a quarter (as the caches do, or as a window and the first tokens leave of them) those with the longest first, so
+// that no long tile begins when the others end: a lane has one sequence, and finds the tiles in front of its own, each wave for
+// 16 of the sequences (lds: 256 numbers). There, and with a window, the tiles that have rows come before the gaps in the numbers,
+// which otherwise hold places while the last of them are given out: 30 chunks of 200 tokens at 1050 to 1500, 12 heads of 64,
+// 60 us with the gaps in between, 46 without; 49 in the batch's order. (Sorted in every wave for all the sequences, one at a
+// time: 63 chunks of 64 at 670 to 1000, 12 heads of 128, 86 us, like this 79, in the batch's order 80.) Without a window
+// sequences that are alike keep the order of the numbers: behind the tiles the gaps make 40 chunks of 128 at 1400 113 -> 81 us, but 63
+// of 64 at 4000 302 -> 314. With windows of 1024 and 4 first tokens, in this order, in that of the numbers, by the caches' lengths
+// with the gaps in between: 40 chunks of 100 at 800 to 8000, 12 heads of 64, 40, 49, 54 us; 63 of 64 at 2000 to 4000, 12 heads of
+// 128, 110, 107, 116, over 8 bits 84, 90, 100.
+// (us in this order and in the reverse of the batch's, caches of 16 bits, 12 heads of 128: nine sequences, chunks of up to 700 and
+// single tokens, 78 / 92; 20 chunks of up to 600 at up to 4000 160 / 176; eight prompts of up to 3000 62 / 72; a chunk of 900 at
+// 8000 and 63 single tokens 212 / 306 if the chunk is the batch's first, 211 / 211 if it is its last.)
+template <bool WIN>
 __device__ __forceinline__ int attn_order(const AttnArgs& a, int u, int* lds, PagedSeq& f) {
   const int n = a.seqs.n_seqs, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   auto first = [&](int c, int s) { return (int)((int64_t)c * a.group / ATTN_ROWS + s); };  // tile of row c of sequence s
@@ -659,26 +664,31 @@ __device__ __forceinline__ int attn_order(const AttnArgs& a, int u, int* lds, Pa
   }
   const AttnLane x = attn_lane(a);
   const int tiles = (int)(((int64_t)x.rows * a.group + ATTN_ROWS - 1) / ATTN_ROWS);
-  // by lengths (up to 2^25; 0: no rows), then by numbers: no two keys are the same
-  const uint32_t key = (tiles ? (uint32_t)min(max(x.len, 1), (1 << 25) - 1) << 6 : 0u) | (63 - lane);
+  // by walks (up to 2^25; 0: no rows), then by numbers: no two keys are the same
+  const int walk = WIN ? (int)min((int64_t)a.window + a.sinks + ATTN_ROWS, (int64_t)(1 << 25) - 1) : (1 << 25) - 1;
+  const uint32_t key = (tiles ? (uint32_t)min(max(x.len, 1), walk) << 6 : 0u) | (63 - lane);
   const uint32_t most = (uint32_t)wave_max((float)(key >> 6)), least = (uint32_t)-wave_max(tiles ? -(float)(key >> 6) : -0x1p26f);
-  if (most >= least && most - least > most / 4) {  // (the same in all waves: they meet at the barriers)
-    int part = 0;
+  const bool uneven = most >= least && most - least > most / 4;  // (the same in all waves: they meet at the barriers)
+  if (WIN || uneven) {
+    const int upto = attn_scan(tiles), all = __builtin_amdgcn_readlane(upto, 63);
+    int before = all - upto;  // tiles in front of the sequence's: of those behind it in the batch
+    if (uneven) {
+      int part = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t k = __builtin_amdgcn_readlane(key, 16 * wave + i);
-      const int m = __builtin_amdgcn_readlane(tiles, 16 * wave + i);
-      part += k > key ? m : 0;
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t k = __builtin_amdgcn_readlane(key, 16 * wave + i);
+        const int m = __builtin_amdgcn_readlane(tiles, 16 * wave + i);
+        part += k > key ? m : 0;
+      }
+      lds[64 * wave + lane] = part;
+      __syncthreads();
+      before = (lds[lane] + lds[64 + lane]) + (lds[128 + lane] + lds[192 + lane]);
+      __syncthreads();
     }
-    lds[64 * wave + lane] = part;
-    __syncthreads();
-    const int before = (lds[lane] + lds[64 + lane]) + (lds[128 + lane] + lds[192 + lane]);
-    __syncthreads();
     const uint64_t mine = __ballot(u >= before && u < before + tiles);
     const int l = mine != 0 ? __builtin_ctzll(mine) : -1;
     f = attn_of(a, x, l);
-    // behind all of them those of the rows of no sequence (beyond these: a tile without any)
-    if (l < 0) return first(f.c0, n) + u - __builtin_amdgcn_readlane(attn_scan(tiles), 63);
+    if (l < 0) return first(f.c0, n) + u - all;  // behind all of them the rows of no sequence (beyond these: a tile without any)
     return first(f.c0, l) + __builtin_amdgcn_readlane(before + tiles - 1, l) - u;
   }
   const int s = min(lane, n - 1), lo = first(x.c, s), tail = first(x.end, n);
@@ -703,7 +713,7 @@ __global__ __launch_bounds__(ATTN_THREADS, D == 64 ? 3 : 2) void attn_many_kerne
   const int ranges = max(1, min(attn_ranges(a), a.splits));
   const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % ranges, u = rest / ranges;
   PagedSeq seq;
-  const int tile = __builtin_amdgcn_readfirstlane(attn_order(a, u, (int*)k_s, seq));
+  const int tile = __builtin_amdgcn_readfirstlane(attn_order<WIN>(a, u, (int*)k_s, seq));
   if (tile < 0) return;
   for (int* v : {&seq.s, &seq.c0, &seq.rows, &seq.len}) *v = __builtin_amdgcn_readfirstlane(*v);
   const AttnTile w = attn_tile<ATTN_ROWS, WIN, ATTN_KT>(a, seq, tile, split, ranges);

@@ -472,3 +472,35 @@ def test_gaps_come_behind_the_tiles_of_uneven_batches(group):
         if case % 4 != 3:
             assert sorted(seen) == [(i, h) for i in range(N) for h in range(group)]
             assert order == sorted(order, reverse=True)
+
+
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_windowed_tiles_by_their_walks(group):
+    """With a window, restated: the key of the order is no less than what the sequence's longest tile walks beyond the window's start and
+    the first tokens, and not the cache's length; walks that are alike go from the batch's last sequence to its first, tiles with rows
+    before all gaps."""
+    rng = random.Random(group)
+    for case in range(80):
+        n = rng.choice([2, 9, 40, 64])
+        window, sinks = rng.choice([1, 60, 700, 1 << 30]), rng.choice([0, 4, 300])
+        new = [rng.choice([0, 1, 128, 200, 300]) for _ in range(n)]
+        lens = [r + rng.choice([0, 500, 4000, 20000]) for r in new]
+        cu = [sum(new[:i]) for i in range(n + 1)]
+        N = cu[-1] + rng.choice([0, 3])
+        walk = min(window + sinks + 128, (1 << 25) - 1)
+        tiles = [-(-r * group // 128) for r in new]
+        keys = [min(max(x, 1), walk) for x, k in zip(lens, tiles) if k]
+        for x, r in zip(lens, new):
+            for r0 in range(0, r * group, 128):  # what the tile's rows attend
+                last, start = x - r + (r0 + min(128, r * group - r0) - 1) // group, max(0, x - r + r0 // group - window + 1)
+                assert min(max(x, 1), walk) >= min(sinks, start) + last + 1 - start
+        if keys and max(keys) - min(keys) > max(keys) // 4:
+            continue  # sorted, as without a window
+        total, seen = sum(tiles), []
+        before = [total - sum(tiles[:s + 1]) for s in range(n)]
+        for u in range(N * group // 128 + n + 1):
+            mine = [s for s in range(n) if before[s] <= u < before[s] + tiles[s]]
+            assert len(mine) == (u < total)
+            if mine:
+                seen.append((mine[0], before[mine[0]] + tiles[mine[0]] - 1 - u))
+        assert seen == [(s, i) for s in range(n - 1, -1, -1) for i in range(tiles[s] - 1, -1, -1)]
