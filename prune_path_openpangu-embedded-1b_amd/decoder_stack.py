@@ -68,6 +68,9 @@ class Attention(nn.Module):
     def __init__(self, d: int, heads: int, max_len: int, qk_norm: bool = False, window: Optional[int] = None,
                  sinks: int = 0):
         super().__init__()
+        if sinks < 0 or (sinks > 0 if window is None else window < 1):
+            raise ValueError(f"Attention: a window of {window} tokens and {sinks} first ones (a window of at least 1, or none; first "
+                             "tokens only beside one)")
         self.h, self.hd = heads, d // heads
         self.qkv = nn.Linear(d, 3 * d, bias=False)
         self.o = nn.Linear(d, d, bias=False)

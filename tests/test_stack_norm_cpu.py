@@ -68,3 +68,15 @@ def test_conversions_moves_and_copies(stack):
     assert torch.equal(seen[-1], want)
     assert set(attn.state_dict()) == {"qkv.weight", "o.weight", "q_norm.weight", "k_norm.weight"}
     assert ds.Attention(256, 2, 16).inv_freq is None
+
+
+def test_windows_that_say_nothing(stack):
+    """A window of no token would leave rows that attend nothing, NaN in the plain path; first tokens without a window were ignored there
+    and refused by the paged one."""
+    ds, _ = stack
+    for window, sinks in ((0, 0), (-1, 0), (None, 2), (5, -1)):
+        with pytest.raises(ValueError, match="window"):
+            ds.Attention(256, 2, 16, window=window, sinks=sinks)
+        with pytest.raises(ValueError, match="window"):
+            ds.DecoderStack(layers=1, hidden=64, heads=1, experts=2, group=32, vocab=16, max_len=8, window=window, sinks=sinks)
+    assert ds.Attention(256, 2, 16, window=1, sinks=0).window == 1
