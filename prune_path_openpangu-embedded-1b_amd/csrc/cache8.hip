@@ -273,8 +273,9 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
 
 int app8_launch(const char* what, AppArgs& a, const AppMore& e, int dtype, int D, int layout, int64_t n_tokens, hipStream_t st) {
   const int vheads = 512 / D;
-  // Query heads of an item: as of the 16-bit cache for single tokens; 8 for chunks (8192 tokens of 12 heads 35.4 us, with 4
-  // heads 35.5, with 12 41.7; 4 chunks of 2048, 24 heads on 8, 37.2, 41.5, 41.7).
+  // Query heads of an item: as of the 16-bit cache for single tokens; 8 for chunks. us for 4, 8, 12 heads, 8192 tokens: 12 query and key
+  // heads 30.1, 29.7, 36.7 (with norms 30.2, 31.0, 38.3), 16 36.9, 34.4, 39.6 (38.1, 37.2, 42.3), 32 81, 74, 75; 20 on 4 23.3, 23.9, 23.9;
+  // 4 chunks of 2048, 24 on 8, 31.6, 29.8, 34.3 (33.4, 31.7, 36.5).
   a.per = n_tokens <= 4 * (int64_t)a.seqs.n_seqs ? 32 : 8;
   a.nqb = (a.Hq + a.per - 1) / a.per, a.nkb = (a.Hkv + 3) / 4, a.nvb = (a.Hkv + vheads - 1) / vheads;
   const int64_t groups = (n_tokens >> 4) + 2 * ((int64_t)a.seqs.n_seqs + 1), items = groups * (a.nqb + a.nkb + a.nvb);

@@ -337,8 +337,14 @@ static int append(const char* what, const void* q, const int64_t* q_strides, con
   // 8192 tokens (151 MB, from memory) 38 us, 8 or 12 heads 42 and 41. Between them, and where a chunk is among
   // single tokens, 4 value heads: 64 sequences of 4 and 16 tokens 8.7 and 16.6 us, with 16 13.4 and 27.5; 64
   // single tokens and 512 8.9 against 13.2, 255 and 3800 24 against 34 (with one 31).
-  // With norms 12 query or key heads in chunks, for the sake of the weights (8192 tokens 36.5 us, with 4 heads 40.7, with 8 42.7).
-  a.per = n_tokens <= 4 * (int64_t)n_seqs ? 32 : k_weight ? 12 : 4;
+  // With norms more heads in chunks, for the sake of the weights, if few are left over: of 12, 8 and 4 the most that leave least. us for
+  // 4, 8, 12 heads an item, 8192 tokens: 12 query and key heads 35.5, 37.2, 32.2; 16 43.1, 40.5, 47.3; 32 99, 91, 92; 20 on 4 27.6, 29.5,
+  // 28.8; 24 on 8 36.3, 34.6, 35.7; 40 on 8 47.1, 44.3, 45.9.
+  auto over = [&](int per) { return (per - Hq % per) % per + (per - Hkv % per) % per; };
+  int heads = 12;
+  for (int per : {8, 4})
+    if (over(per) < over(heads)) heads = per;
+  a.per = n_tokens <= 4 * (int64_t)n_seqs ? 32 : k_weight ? heads : 4;
   a.vper = n_tokens > 16 * (int64_t)n_seqs ? 1 : n_seqs >= 64 && n_tokens <= 2 * (int64_t)n_seqs ? 16 : 4;
   a.nqb = (Hq + a.per - 1) / a.per, a.nkb = (Hkv + a.per - 1) / a.per, a.nvb = (Hkv + a.vper - 1) / a.vper;
   const int64_t values = ((n_tokens >> 6) + 2 * ((int64_t)n_seqs + 1)) * a.nvb;
