@@ -945,7 +945,7 @@ void kv_append_into(const optional<Tensor>& q, const optional<Tensor>& q_out, bo
   const Span sk(k), sv(v), kp(k_pages), vp(v_pages), st(block_table), sl(kv_lens), sc(cu_q);
   auto span = [&](const optional<Tensor>& t) { return t ? Span(*t) : st; };
   const Span sf = span(inv_freq), sqw = span(q_weight), skw = span(k_weight);
-  std::vector<const Span*> reads = {&sk, &sv, &st, &sl, &sc, &sf, &sqw, &skw};
+  const Span* const reads[] = {&sk, &sv, &st, &sl, &sc, &sf, &sqw, &skw};
   for (const Span* in : reads) {
     apart(name, kp, *in);
     apart(name, vp, *in);

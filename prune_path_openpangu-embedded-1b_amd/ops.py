@@ -454,15 +454,20 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
 
     Inference only: arguments that require a gradient are refused outside torch.no_grad(), tangents always."""
     ops = L.torch_ops()
-    cache, turn, s = (k_pages, v_pages, block_table, kv_lens, cu_q), (inv_freq, layout, mscale), scales or (None, None)
+    # (what a call does not name is left to the operators' defaults: each argument costs a call some 30 ns)
+    turn = () if inv_freq is None and layout == "half" and mscale == 1.0 else (inv_freq, layout, mscale)
+    norm = scales is not None or q_weight is not None or k_weight is not None
+    s = scales or (None, None)
     if q is None:
         if q_out is not None or q_weight is not None:
             raise RuntimeError("prunepath.kv_append: q_out or q_weight without q")
-        ops.kv_append(k, v, *cache, *turn, k_weight, eps, *s)
+        more = (inv_freq, layout, mscale, k_weight, eps, *s) if norm else turn
+        ops.kv_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q, *more)
         return None
+    more = (inv_freq, layout, mscale, q_weight, k_weight, eps, *s) if norm else turn
     if q_out is None:
-        return ops.kv_append_q(q, k, v, *cache, *turn, q_weight, k_weight, eps, *s)
-    ops.kv_append_q_into(q, q_out, k, v, *cache, *turn, q_weight, k_weight, eps, *s)
+        return ops.kv_append_q(q, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, *more)
+    ops.kv_append_q_into(q, q_out, k, v, k_pages, v_pages, block_table, kv_lens, cu_q, *more)
     return q_out
 
 
@@ -509,7 +514,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         scale = q.shape[-1] ** -0.5
     if window is not None and window < 1:
         raise RuntimeError(f"prunepath.paged_attention: a window of {window} tokens")
-    ops, extra = L.torch_ops(), (*(scales or (None, None)), window or 0, sinks)
+    ops = L.torch_ops()
+    extra = () if scales is None and window is None and sinks == 0 else (*(scales or (None, None)), window or 0, sinks)
     if out is None:
         return ops.paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), *extra)
     ops.paged_attention_into(q, k_pages, v_pages, block_table, kv_lens, cu_q, float(scale), out, *extra)
