@@ -427,8 +427,9 @@ int pp_kv_read(const void* k_pages, const void* v_pages, const void* k_scales, c
 
 /* Attention of the new tokens over the cache that holds them: the token at position p attends the
  * positions 0 .. p, query head h the key head h / (Hq / Hkv). q [n_tokens][Hq][D] bfloat16 (strides
- * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous (q itself, if q is). Scores, softmax and sums
- * in float32. A row that attends nothing, or whose scores are all -inf, gives zeros; what a masked
+ * as above) -> out [n_tokens][Hq][D] bfloat16, contiguous (q itself, if q is). Scores, exponentials and
+ * sums in float32; the weights meet the values as one bfloat16 number each in tiles of many rows (their sum is that of the same
+ * numbers), as two in tiles of few. A row that attends nothing, or whose scores are all -inf, gives zeros; what a masked
  * place holds, NaN and infinities too, does not reach a row, and an infinity in a value that a row
  * attends gives that infinity (NaN beside its opposite, or where its token's weight underflows). Rows behind cu_q[n_seqs] are zeroed
  * if zero_tail, else left as they are. workspace: pp_paged_attention_workspace_bytes of the same
@@ -444,7 +445,7 @@ int pp_paged_attention(const void* q, const int64_t* q_strides, int64_t n_tokens
 
 /* pp_paged_attention over a cache of 16 or of 8 bits (k_scales, v_scales as above, both NULL: bfloat16), of a window and the
  * first tokens: with window > 0 the token at position p attends the positions t <= p with t > p - window or t < sinks
- * (window 0: all up to p, sinks without meaning). Pages that no row attends are not read. Over 8 bits: as over the
+ * (window 0: all up to p, sinks without meaning). What no row attends reaches no result: its entries may be -1. Over 8 bits: as over the
  * bfloat16 numbers that the cache stands for, NaN as there. workspace:
  * pp_paged_attention_with_workspace_bytes of the same sizes. */
 size_t pp_paged_attention_with_workspace_bytes(int64_t n_tokens, int n_seqs, int max_pages, int page_size, int Hq, int Hkv,

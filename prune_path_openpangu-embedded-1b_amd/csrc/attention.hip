@@ -618,8 +618,8 @@ __global__ __launch_bounds__(ATTN_THREADS, EIGHT ? 2 : 3) void attn_few_kernel(A
 // (605), of 2048 37 us, 7 of them the join's; 512 new tokens at 30000 131 us (730).
 // 8 bits: the next step's 16 bytes of K and V to each thread are asked for before the present step's products, widened and stored
 // to LDS behind them: 8192 tokens 237 us, 4096 84, 512 at 30000 127.
-// A window of 1024 and 4 first tokens, 8192 tokens: 87 us (550 TFLOP/s): 19 steps of 64 tokens a tile, four of them with
-// masked places, and three tiles a CU for two places.
+// A window of 1024 and 4 first tokens, 8192 tokens: 87 us (550 TFLOP/s): 19 steps of 64 tokens a tile, five of them with
+// masked places (three of a wave's), and three tiles a CU for two places.
 #define ATTN_ROWS 128
 
 // 16 bytes per lane from memory into LDS at lds + 16 lane, by the copy path that does not pass through

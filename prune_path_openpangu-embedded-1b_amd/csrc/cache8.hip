@@ -9,10 +9,11 @@
 // is the least that holds its values; where the block held tokens before (places in front of the call's first
 // token in it), at least the one that it had.
 //
-// Memory bound for chunks: 8192 tokens of 12 query, key and value heads (126 MB) 29.4 us, with the norms 33.2 (3.8 TB/s; 95
-// registers, five waves a SIMD: fewer spill, and four channels a lane instead of two, for wider loads of V, 38 us). The chain
-// offsets, table, rows and scale for single tokens: 4.3 us for one, 4.6 for 32 of them, 11.6 for 256. The read: 64 sequences
-// of 12 heads, 2.26 GB, 452 us (5.0 TB/s, a large copy's rate).
+// Memory bound for chunks: 8192 tokens of 12 query, key and value heads (126 MB) 29.0 us, with the norms 31.6 (4.0 TB/s; 95
+// registers, five waves a SIMD: fewer spill, and four channels a lane instead of two, for wider loads of V, 38 us); half of the
+// channels turned 38.9 (145 registers, three waves). The chain offsets, table, rows and scale for single tokens: 4.5 us for one,
+// 5.1 for 32 of them, 12.3 for 256 (with norms 4.8, 5.3, 12.7). The read: 64 sequences of 12 heads, 2.26 GB, 453 us (5.0 TB/s,
+// a large copy's rate).
 #include <algorithm>
 
 #include "append.h"
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(APP_THREADS) void kv_append8_kernel(AppArgs a, AppM
     const T* const src = (const T*)a.v + row0 * a.vs[0] + (on ? h : 0) * a.vs[1] + 2 * l;
     auto where = [&](int page) { return (((int64_t)page * a.Hkv + (on ? h : 0)) << lb) + (place >> 4); };
     // A few tokens go out byte by byte, unless older ones change, and skip what the places of a whole block take
-    // (256 single tokens of 12 heads 11.5 us, as a block's whole words 14.5; one 4.2 and 5.1).
+    // (256 single tokens of 12 heads 12.3 us, as a block's whole words 13.7; 32 5.1 and 5.5).
     if (nt <= C8_FEW) {
       float x[2 * C8_FEW];
 #pragma unroll

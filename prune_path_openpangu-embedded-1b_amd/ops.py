@@ -392,8 +392,9 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     ``rotary``, in one launch (``torch.ops.prunepath.qk_norm_rotary``). q [N, heads, D] and k [N, kv_heads, D], or
     [B, L, heads, D] and [B, L, kv_heads, D], fp32 or bf16, any strides (parts of a joint projection's rows); the weights
     [D], both fp32 or both of q's dtype; D from 2 to 256; positions and inv_freq as ``rotary`` takes them. Computed in fp32,
-    rounded once. New contiguous tensors of q's dtype; differentiable once, in q, k and the weights, whose gradients are
-    sums in a fixed order (capture a backward, as any, with no eager graph of the same leaves alive)."""
+    rounded once. New contiguous tensors of q's dtype; differentiable once, in q, k and the weights (a backward with
+    create_graph=True is refused, whether or not a second derivative is then taken), whose gradients are sums in a fixed order
+    (capture a backward, as any, with no eager graph of the same leaves alive)."""
     return L.torch_ops().qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, layout, mscale, eps)
 
 
@@ -499,7 +500,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     paged cache: the token at position p attends the positions 0 .. p of its sequence, query head h
     the key head h // (heads / kv_heads). q bf16 [N, heads, D] -> bf16 [N, heads, D]
     (``torch.ops.prunepath.paged_attention``, or ``paged_attention_into`` writing ``out``); scale
-    defaults to D^-0.5. Scores and softmax in fp32. A row that attends nothing, or whose scores are all
+    defaults to D^-0.5. Scores, exponentials and sums in fp32; the weights meet the values as one bf16 number each where the
+    call has many rows a sequence (their sum is that of the same numbers), as two where it has few. A row that attends nothing, or whose scores are all
     -inf, is zero; an infinity in a value that a row attends gives that infinity. Rows behind cu_q[seqs]
     are zero in a new result and stay in ``out`` (which may be q itself; other overlaps are refused). Single
     tokens, chunks and whole prompts, in one call; lengths are read on the device, so a captured call serves
@@ -507,7 +509,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     scales (``paged_cache8``): the cache is one of 8 bits; the attention is that over the bf16 numbers which it stands for.
     window: the token at position p attends only the positions from p - window + 1 on, and the sequence's first ``sinks`` (which
-    need a window). Pages that no row attends are not read, and their entries may be -1.
+    need a window). What no row attends reaches no result, whatever its pages hold, and their entries may be -1.
 
     Inference only: arguments that require a gradient are refused outside torch.no_grad(), tangents always."""
     if scale is None:
